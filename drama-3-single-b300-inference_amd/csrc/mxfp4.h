@@ -1,0 +1,68 @@
+// MXFP4 building blocks (OCP Microscaling Formats): e2m1 codes, two a byte
+// with the even element in the low nibble, and one e8m0 scale (a power of
+// two, code - 127 its exponent, code 255 NaN) per 32 elements of a row.
+#pragma once
+
+#include "common.h"
+#include "expert_tile.h"
+
+namespace d3 {
+
+constexpr int kMxBlock = 32;       // elements per scale
+constexpr int kMxRows = 64;        // weight rows of a packed row group (four 16-row MFMA tiles)
+constexpr int kMxStep = 256;       // contracted elements of a packed step (two MFMAs deep)
+constexpr int kMxStepCodes = kMxRows * kMxStep / 2;          // 8 KiB of codes per row group and step
+constexpr int kMxStepScales = kMxRows * kMxStep / kMxBlock;  // 512 bytes of scales
+constexpr int kMxLow = 4;  // the MFMA's format code of e2m1 operands
+
+// Row orders of a packed weight: which row of W the lanes of an MFMA's
+// output hold.  An output lane of group g holds rows 4 g + i (i < 4) of each
+// of the row group's tiles t.
+constexpr int kMxOrderPairs = 0;   // 32 (t / 2) + 8 g + 4 (t % 2) + i: 16 bytes of bf16 a lane and tile pair
+constexpr int kMxOrderGateUp = 1;  // tiles 0-1 gate, 2-3 up rows 32 rg + 8 g + 4 (t % 2) + i: a lane holds both
+constexpr int kMxOrderPlain = 2;   // 16 t + 4 g + i: 16 bytes of fp32 a lane and tile
+
+// Row of W that row m of tile t of row group rg holds; rows from n on are padding.
+__host__ __device__ __forceinline__ int mx_weight_row(int order, int n, int rg, int t, int m) {
+  const int g = m >> 2, i = m & 3;
+  if (order == kMxOrderPlain) return kMxRows * rg + 16 * t + m;
+  if (order == kMxOrderPairs) return kMxRows * rg + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i;
+  return (t >= 2 ? n / 2 : 0) + 32 * rg + 8 * g + 4 * (t & 1) + i;
+}
+
+// Scale code of a block whose largest magnitude has the fp32 bits `amax`
+// (sign bit clear): floor(log2 amax) - 2, so that the largest element lies in
+// [4, 8) scaled; 0 (2^-127) for zero blocks and those below 2^-124; 255 (NaN)
+// where an element is infinite or NaN, which the whole block then stands for.
+__device__ __forceinline__ uint32_t mx_scale_code(uint32_t amax) {
+  const uint32_t e = amax >> 23;
+  return e >= 255u ? 255u : (e > 2u ? e - 2u : 0u);
+}
+
+// 2^(127 - code), the reciprocal of a scale: exact for every code of
+// mx_scale_code (0 .. 252); 0 for 255, whose codes are then zeros.
+__device__ __forceinline__ float mx_inverse(uint32_t code) {
+  return code == 255u ? 0.0f : __uint_as_float((254u - code) << 23);
+}
+
+// Eight scaled values (magnitudes below 8) as e2m1 codes, v[0] in the low
+// nibble: the gfx950 conversion at scale 1, round to nearest even, above 6 to
+// 6.  The product by a power of two is exact (fp32 subnormals are kept), so
+// one rounding is made.  A block at scale NaN gets zero codes.
+__device__ __forceinline__ uint32_t mx_codes8(const float* v, float inverse) {
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[i] = v[i] * inverse;
+  uint32_t w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, s[0], s[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, s[2], s[3], 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, s[4], s[5], 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, s[6], s[7], 1.0f, 3);
+  return inverse == 0.0f ? 0u : w;
+}
+
+// Memory words at the alignment of their elements only: gfx950 takes wide
+// accesses at any address, so odd row strides cost no narrow path.
+struct __attribute__((packed, aligned(2))) MxWords4 { uint32_t w[4]; };
+struct __attribute__((packed, aligned(1))) MxWord { uint32_t w; };
+
+}  // namespace d3

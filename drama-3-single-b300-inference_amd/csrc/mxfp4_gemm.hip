@@ -1,0 +1,538 @@
+// Products of MXFP4 rows with packed MXFP4 weights: dense, grouped by expert
+// over ragged boundaries, and the two products of the routed SwiGLU experts.
+//
+// out[r, j] = sum_k a[r, k] w[j, k] on mfma_scale_f32_16x16x128_f8f6f4 with
+// both operands e2m1: a lane's operand is exactly one block of 32 elements,
+// so its e8m0 scale is the instruction's own scale operand and no rescaling
+// is left to the vector unit.  The products are exact and the sums fp32 (6e-8
+// of sum |products| measured over scales that differ by 2^40).  Weights are
+// the first operand: an output lane holds one row of a and four consecutive
+// weight rows of each 16-row tile, as the packed row orders place them.
+#include "mxfp4.h"
+#include "status.h"
+
+namespace d3 {
+namespace {
+
+constexpr int kMxWaves = 4;
+constexpr int kMxThreads = kMxWaves * kWave;
+
+enum MxEpilogue {
+  kMxBf16,  // bf16 rows at the item's rows (row order: pairs)
+  kMxAct,   // silu(gate) * up quantised to MXFP4 rows at the item's rows (gate-up order)
+  kMxF32,   // fp32 rows at sorted[row] (plain order)
+};
+
+struct MxGemm {
+  const uint8_t* w;  // packed codes [E][row groups][steps][8 KiB]
+  const uint8_t* ws;
+  int n;
+  int row_groups;
+  int steps;
+  const uint8_t* a;  // codes [rows][k_bytes]
+  const uint8_t* as;  // scales [rows][k_blocks]
+  int k_bytes;
+  int k_blocks;
+  const int4* items;  // {expert (-1: zero rows), first row, rows, -}; nullptr: one expert, `rows` in order
+  const int32_t* num_items;
+  int rows;
+  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxF32)
+  int top_k;
+  void* out;
+  int64_t out_stride;
+  uint8_t* out_scales;
+};
+
+// One MFMA with the scales in byte SA of `sa` and byte SB of `sb`.
+template <int SA, int SB>
+__device__ __forceinline__ floatx4 mfma_fp4(const int4& a, const int4& b, const floatx4& c, uint32_t sa, uint32_t sb) {
+  const int32x8 av = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
+  const int32x8 bv = {b.x, b.y, b.z, b.w, 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, kMxLow, kMxLow, SA, static_cast<int>(sa), SB,
+                                                          static_cast<int>(sb));
+}
+
+template <int SB>
+__device__ __forceinline__ void mfma_tiles(const int4 (&a)[4], const int4& b, floatx4 (&c)[4], uint32_t sa, uint32_t sb) {
+  c[0] = mfma_fp4<0, SB>(a[0], b, c[0], sa, sb);
+  c[1] = mfma_fp4<1, SB>(a[1], b, c[1], sa, sb);
+  c[2] = mfma_fp4<2, SB>(a[2], b, c[2], sa, sb);
+  c[3] = mfma_fp4<3, SB>(a[3], b, c[3], sa, sb);
+}
+
+__device__ __forceinline__ int4 mx_item(const MxGemm& g, int index, int item_rows) {
+  if (g.items == nullptr) {
+    const int start = index * item_rows;
+    return make_int4(0, start, min(item_rows, g.rows - start), 0);
+  }
+  if (index >= *g.num_items) return make_int4(0, 0, 0, 0);
+  return g.items[index];
+}
+
+// The four tiles of one row of `a` (this lane's row `row` of the item's list,
+// live or not) for row group rg.
+template <int kEpi>
+__device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4], int rg, int row, bool live, int group) {
+  if constexpr (kEpi == kMxBf16) {
+    if (!live) return;
+    uint16_t* out = static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.out_stride;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int f = kMxRows * rg + 32 * p + 8 * group;
+      const floatx4 &lo = c[2 * p], &hi = c[2 * p + 1];
+      const MxWords4 v = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                          pack_bf16x2(hi[2], hi[3])};
+      if (f + 8 <= g.n) {
+        *reinterpret_cast<MxWords4*>(out + f) = v;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (f + i < g.n) out[f + i] = static_cast<uint16_t>(v.w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  } else if constexpr (kEpi == kMxAct) {
+    // Gate (tiles 0, 1) and up (tiles 2, 3) of columns 32 rg + 8 group + i;
+    // the four groups of a row hold one block of 32.  Nothing is rounded
+    // between the products and the codes.
+    float gate[8], up[8], v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      gate[i] = c[i / 4][i % 4];
+      up[i] = c[2 + i / 4][i % 4];
+    }
+    swiglu_values<8>(gate, up, v);
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = MaxU32::apply(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+    amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16)));
+    amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
+    const uint32_t code = mx_scale_code(amax);
+    const uint32_t word = mx_codes8(v, mx_inverse(code));
+    if (!live) return;
+    const int64_t at = static_cast<int64_t>(row) * (g.out_stride / kMxBlock) + rg;
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.out) + at * (kMxBlock / 2) + 4 * group) = word;
+    if (group == 0) g.out_scales[at] = static_cast<uint8_t>(code);
+  } else {
+    if (!live) return;
+    float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride + kMxRows * rg + 4 * group;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) *reinterpret_cast<floatx4*>(out + 16 * t) = c[t];
+  }
+}
+
+__device__ __forceinline__ void mx_zero_rows(const MxGemm& g, const int4& item, int first, int count) {
+  for (int r = 0; r < item.z; ++r) {
+    uint16_t* out = static_cast<uint16_t*>(g.out) + static_cast<int64_t>(item.y + r) * g.out_stride;
+    for (int f = first + threadIdx.x; f < min(first + count, g.n); f += kMxThreads) out[f] = 0;
+  }
+}
+
+// Few rows an item (up to 16 kRT): the weights stream from memory once, each
+// wave a share of the contraction.  A workgroup's four waves are kMxWaves /
+// kSplit row groups by kSplit interleaved slices of the steps; the slices'
+// fp32 sums meet in LDS and are added in slice order.
+template <int kRT, int kEpi, int kSplit>
+__global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blocks) {
+  constexpr int kGroups = kMxWaves / kSplit;
+  __shared__ floatx4 part[kSplit > 1 ? kMxWaves * kRT * 4 * kWave : 1];
+  const int index = blockIdx.x / blocks, block = blockIdx.x - index * blocks;
+  const int4 item = mx_item(g, index, 16 * kRT);
+  if (item.z <= 0) return;  // uniform
+  if (kEpi == kMxBf16 && item.x < 0) {
+    mx_zero_rows(g, item, block * kGroups * kMxRows, kGroups * kMxRows);
+    return;
+  }
+  const int lane = lane_id(), row16 = lane & 15, group = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int slice = wave % kSplit;
+  const int rg = block * kGroups + wave / kSplit;
+  const int rg_read = min(rg, g.row_groups - 1);
+  const int count = min(item.z, 16 * kRT);
+
+  // Rows past the item read its last row; their sums are dropped.
+  const uint8_t* codes[kRT];
+  const uint8_t* scales[kRT];
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt) {
+    int64_t row = item.y + min(16 * rt + row16, count - 1);
+    if constexpr (kEpi == kMxAct) row = g.sorted[row] / g.top_k;
+    codes[rt] = g.a + row * g.k_bytes;
+    scales[rt] = g.as + row * g.k_blocks;
+  }
+  const int64_t base = static_cast<int64_t>(item.x) * g.row_groups + rg_read;
+  const int4* w = reinterpret_cast<const int4*>(g.w + base * g.steps * kMxStepCodes) + lane;
+  const uint2* ws = reinterpret_cast<const uint2*>(g.ws + base * g.steps * kMxStepScales) + lane;
+
+  floatx4 acc[kRT][4];
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[rt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  for (int step = slice; step < g.steps; step += kSplit) {
+    int4 wf[2][4];
+    const int4* wp = w + static_cast<int64_t>(step) * (kMxStepCodes / 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) wf[h][t] = wp[(4 * h + t) * kWave];
+    const uint2 wsc = ws[static_cast<int64_t>(step) * (kMxStepScales / 8)];
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // Blocks from K on (an odd multiple of 128) meet zero weights at
+        // scale 1: the lane reads its first half again, at scale 2^-127.
+        const int kblock = 8 * step + 4 * h + group;
+        const bool live = kblock < g.k_blocks;
+        const int at = live ? kblock : kblock - 4;
+        const int4 b = *reinterpret_cast<const int4*>(codes[rt] + 16 * at);
+        const uint32_t sb = live ? scales[rt][at] : 0u;
+        mfma_tiles<0>(wf[h], b, acc[rt], h ? wsc.y : wsc.x, sb);
+      }
+    }
+  }
+
+  if constexpr (kSplit > 1) {
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) part[((wave * kRT + rt) * 4 + t) * kWave + lane] = acc[rt][t];
+    __syncthreads();
+    const int first = wave - slice;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      if (rt % kSplit != slice) continue;
+      floatx4 sum[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        sum[t] = part[((first * kRT + rt) * 4 + t) * kWave + lane];
+#pragma unroll
+        for (int s = 1; s < kSplit; ++s) sum[t] += part[(((first + s) * kRT + rt) * 4 + t) * kWave + lane];
+      }
+      if (rg < g.row_groups)
+        mx_store<kEpi>(g, sum, rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
+    }
+  } else {
+    if (rg >= g.row_groups) return;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+      mx_store<kEpi>(g, acc[rt], rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
+  }
+}
+
+// Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
+// of item_rows; with `zero_rest` the rows before b[0] and from b[E] on as
+// items of expert -1.  Boundaries are clamped to [0, rows].
+constexpr int kItemThreads = 1024;
+__global__ __launch_bounds__(kItemThreads) void mx_items_kernel(const int32_t* __restrict__ bounds, int experts, int rows,
+                                                                int item_rows, int zero_rest, int max_items,
+                                                                int4* __restrict__ items, int32_t* __restrict__ num_items) {
+  __shared__ int wave_sum[kItemThreads / kWave];
+  __shared__ int base;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  if (tid == 0) base = 0;
+  const int entries = experts + (zero_rest ? 2 : 0);
+  for (int first = 0; first < entries; first += kItemThreads) {
+    const int e = first + tid;
+    int a = 0, b = 0, expert = e;
+    if (e < experts) {
+      a = min(max(bounds[e], 0), rows);
+      b = min(max(bounds[e + 1], 0), rows);
+    } else if (e < entries) {
+      expert = -1;
+      a = e == experts ? 0 : min(max(bounds[experts], 0), rows);
+      b = e == experts ? min(max(bounds[0], 0), rows) : rows;
+    }
+    const int count = b > a ? (b - a + item_rows - 1) / item_rows : 0;
+    int scan = count;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int other = __shfl_up(scan, d);
+      if (lane >= d) scan += other;
+    }
+    if (lane == kWave - 1) wave_sum[wave] = scan;
+    __syncthreads();
+    int at = base + scan - count;
+    for (int w = 0; w < wave; ++w) at += wave_sum[w];
+    for (int i = 0; i < count && at + i < max_items; ++i)
+      items[at + i] = make_int4(expert, a + i * item_rows, min(item_rows, b - a - i * item_rows), 0);
+    __syncthreads();
+    if (tid == 0) {
+      int total = 0;
+      for (int w = 0; w < kItemThreads / kWave; ++w) total += wave_sum[w];
+      base += total;
+    }
+    __syncthreads();
+  }
+  if (tid == 0) *num_items = min(base, max_items);
+}
+
+// out[t, :] = sum over ranks r of weights[t, r] * down[t * top_k + r, :] in
+// rank order (fp32, one FMA a rank), rounded to bf16 once.  Ranks whose id
+// names no expert add nothing (their down rows were never written).
+constexpr int kMxCombineColumns = kMxThreads * 4;
+template <int kTopK>  // 0: any
+__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ down, const void* __restrict__ ids,
+                                                                int ids_i64, const void* __restrict__ weights,
+                                                                int weights_f32, int any_top_k, int experts, int hidden,
+                                                                int slices, uint16_t* __restrict__ out) {
+  const int row = blockIdx.x / slices;
+  const int column = (blockIdx.x % slices) * kMxCombineColumns + threadIdx.x * 4;
+  if (column >= hidden) return;
+  const int top_k = kTopK ? kTopK : any_top_k;
+  const int64_t first = static_cast<int64_t>(row) * top_k;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int r = 0; r < top_k; ++r) {
+    const floatx4 y = __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(down + (first + r) * hidden + column));
+    const int64_t id = ids_i64 ? static_cast<const int64_t*>(ids)[first + r] : static_cast<const int32_t*>(ids)[first + r];
+    const bool live = id >= 0 && id < experts;
+    const float w = live ? route_weight(weights, weights_f32, first + r) : 0.0f;
+    acc.x = fmaf(w, live ? y[0] : 0.0f, acc.x);
+    acc.y = fmaf(w, live ? y[1] : 0.0f, acc.y);
+    acc.z = fmaf(w, live ? y[2] : 0.0f, acc.z);
+    acc.w = fmaf(w, live ? y[3] : 0.0f, acc.w);
+  }
+  *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row) * hidden + column) = pack_bf16x4(acc);
+}
+
+bool mx_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+
+int mx_ceil(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+template <int kRT, int kEpi>
+void launch_stream(const MxGemm& g, int items, hipStream_t s) {
+  // Slices of the contraction: as many as there are steps, up to the waves.
+  const int split = g.steps >= 4 ? 4 : (g.steps >= 2 ? 2 : 1);
+  const int blocks = mx_ceil(g.row_groups, kMxWaves / split);
+  const dim3 grid(static_cast<unsigned>(items) * blocks), block(kMxThreads);
+  if (split == 4)
+    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 4>), grid, block, 0, s, g, blocks);
+  else if (split == 2)
+    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 2>), grid, block, 0, s, g, blocks);
+  else
+    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 1>), grid, block, 0, s, g, blocks);
+}
+
+template <int kEpi>
+void launch_gemm(const MxGemm& g, int item_rows, int items, hipStream_t s) {
+  if (items <= 0) return;
+  if (item_rows <= 16)
+    launch_stream<1, kEpi>(g, items, s);
+  else if (item_rows <= 32)
+    launch_stream<2, kEpi>(g, items, s);
+  else
+    launch_stream<4, kEpi>(g, items, s);
+}
+
+// Rows per work item for groups of `mean` rows on average.
+int mx_item_rows(int64_t rows, int64_t groups) {
+  const int64_t mean = rows / groups;
+  return mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
+}
+
+// Byte arena of one call, carved in order at 256-byte boundaries.
+struct Arena {
+  uint8_t* base;
+  int64_t used = 0;
+  template <class T>
+  T* take(int64_t count) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += (count * static_cast<int64_t>(sizeof(T)) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+void set_weight(MxGemm& g, const uint8_t* w, const uint8_t* ws, int n, int k) {
+  g.w = w, g.ws = ws, g.n = n;
+  g.row_groups = mx_ceil(n, kMxRows), g.steps = mx_ceil(k, kMxStep);
+  g.k_bytes = k / 2, g.k_blocks = k / kMxBlock;
+}
+
+struct GroupedPlan {
+  int item_rows, max_items;
+  uint8_t *q, *qs;
+  int4* items;
+  int32_t* num_items;
+  int64_t bytes;
+};
+
+GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, int k) {
+  GroupedPlan p{};
+  p.item_rows = mx_item_rows(rows, experts);
+  // every group, and each of the two runs of rows in none, adds one partial item at most
+  p.max_items = static_cast<int>(rows / p.item_rows + (rows < experts + 2 ? rows : experts + 2));
+  Arena a{static_cast<uint8_t*>(arena)};
+  p.q = a.take<uint8_t>(rows * (k / 2));
+  p.qs = a.take<uint8_t>(rows * (k / kMxBlock));
+  p.items = a.take<int4>(p.max_items);
+  p.num_items = a.take<int32_t>(1);
+  p.bytes = a.used;
+  return p;
+}
+
+constexpr int kMxSortTile = 16;
+constexpr int kMxWidePairs = 8192;  // more (row, rank) pairs: the sort spread over many workgroups
+struct MoePlan {
+  int item_rows, max_items, max_rows;
+  int64_t pairs, scratch_ints;
+  uint8_t *q, *qs, *act, *acts;
+  float* down;
+  int32_t *counts, *starts, *total, *sorted, *expert_ids, *num_items, *scratch;
+  int4* items;
+  int64_t bytes;
+};
+
+MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, int inter) {
+  MoePlan p{};
+  p.pairs = rows * top_k;
+  p.item_rows = mx_item_rows(p.pairs, experts);
+  const int32_t pairs = static_cast<int32_t>(p.pairs);
+  p.max_rows = d3_max_sorted_rows(pairs, experts, kMxSortTile);
+  p.max_items = d3_max_items(pairs, experts, p.item_rows);
+  p.scratch_ints = p.pairs > kMxWidePairs ? d3_sort_wide_scratch_ints(static_cast<int32_t>(rows), top_k, experts) : 0;
+  Arena a{static_cast<uint8_t*>(arena)};
+  p.q = a.take<uint8_t>(rows * (hidden / 2));
+  p.qs = a.take<uint8_t>(rows * (hidden / kMxBlock));
+  p.act = a.take<uint8_t>(static_cast<int64_t>(p.max_rows) * (inter / 2));
+  p.acts = a.take<uint8_t>(static_cast<int64_t>(p.max_rows) * (inter / kMxBlock));
+  p.down = a.take<float>(p.pairs * hidden);
+  p.counts = a.take<int32_t>(experts);
+  p.starts = a.take<int32_t>(experts);
+  p.total = a.take<int32_t>(1);
+  p.sorted = a.take<int32_t>(p.max_rows);
+  p.expert_ids = a.take<int32_t>(p.max_rows / kMxSortTile);
+  p.items = a.take<int4>(p.max_items);
+  p.num_items = a.take<int32_t>(1);
+  p.scratch = a.take<int32_t>(p.scratch_ints);
+  p.bytes = a.used;
+  return p;
+}
+
+bool grouped_shape(int64_t rows, int experts, int n, int k) {
+  return rows >= 0 && rows < (int64_t{1} << 30) && experts > 0 && experts <= (1 << 16) && n > 0 && k > 0 &&
+         k % kGroup == 0;
+}
+bool moe_shape(int64_t rows, int top_k, int experts, int hidden, int inter) {
+  return rows >= 0 && top_k >= 1 && top_k <= 16 && rows * top_k < (int64_t{1} << 26) && experts >= 1 && experts <= 512 &&
+         hidden > 0 && inter > 0 && hidden % kGroup == 0 && inter % kGroup == 0;
+}
+
+}  // namespace
+}  // namespace d3
+
+using namespace d3;
+
+extern "C" int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t k) {
+  if (!grouped_shape(rows, num_experts, 1, k)) return -1;
+  return plan_grouped(nullptr, rows, num_experts, k).bytes;
+}
+
+extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t rows, const int32_t* boundaries,
+                                int32_t num_experts, const uint8_t* w, const uint8_t* ws, int32_t n, int32_t k,
+                                uint16_t* out, int64_t out_row_stride, int32_t zero_rest, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
+  D3_REQUIRE(k > 0 && k % kGroup == 0, "mxfp4_grouped: K=%d must be a multiple of %d", k, kGroup);
+  D3_REQUIRE(grouped_shape(rows, num_experts, n, k), "mxfp4_grouped: rows %lld, experts %d, N=%d",
+             static_cast<long long>(rows), num_experts, n);
+  D3_REQUIRE(boundaries != nullptr || num_experts == 1, "mxfp4_grouped: several experts need boundaries");
+  D3_REQUIRE(rows == 0 || (x && w && ws && out && workspace), "mxfp4_grouped: null pointer");
+  D3_REQUIRE(rows <= 1 || (x_row_stride >= 0 && out_row_stride >= n), "mxfp4_grouped: row strides");
+  D3_REQUIRE(mx_aligned(x, 2) && mx_aligned(w, 16) && mx_aligned(ws, 8) && mx_aligned(out, 2) && mx_aligned(workspace, 16),
+             "mxfp4_grouped: alignment");
+  if (rows == 0) {
+    clear_error();
+    return D3_OK;
+  }
+  const GroupedPlan p = plan_grouped(workspace, rows, num_experts, k);
+  D3_REQUIRE(workspace_bytes >= p.bytes, "mxfp4_grouped: workspace of %lld bytes < required %lld",
+             static_cast<long long>(workspace_bytes), static_cast<long long>(p.bytes));
+  D3_SUPPORTED(static_cast<int64_t>(p.max_items) * mx_ceil(n, kMxRows) < (int64_t{1} << 31),
+               "mxfp4_grouped: more than 2^31 workgroups");
+  hipStream_t s = as_stream(stream);
+  int status = d3_mxfp4_quantize(x, D3_DTYPE_BF16, x_row_stride, rows, k, p.q, p.qs, stream);
+  if (status != D3_OK) return status;
+  MxGemm g{};
+  set_weight(g, w, ws, n, k);
+  g.a = p.q, g.as = p.qs, g.rows = static_cast<int>(rows);
+  g.out = out, g.out_stride = out_row_stride;
+  int items = mx_ceil(rows, p.item_rows);
+  if (boundaries != nullptr) {
+    hipLaunchKernelGGL(mx_items_kernel, dim3(1), dim3(kItemThreads), 0, s, boundaries, num_experts,
+                       static_cast<int>(rows), p.item_rows, zero_rest, p.max_items, p.items, p.num_items);
+    g.items = p.items, g.num_items = p.num_items;
+    items = p.max_items;
+  }
+  launch_gemm<kMxBf16>(g, p.item_rows, items, s);
+  D3_LAUNCHED("mxfp4_grouped");
+}
+
+extern "C" int64_t d3_mxfp4_moe_workspace(int64_t rows, int32_t top_k, int32_t num_experts, int32_t hidden,
+                                          int32_t intermediate) {
+  if (!moe_shape(rows, top_k, num_experts, hidden, intermediate)) return -1;
+  return plan_moe(nullptr, rows, top_k, num_experts, hidden, intermediate).bytes;
+}
+
+extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t rows, const void* ids, int32_t ids_dtype,
+                            const void* weights, int32_t weights_dtype, int32_t top_k, const uint8_t* w13,
+                            const uint8_t* s13, const uint8_t* w2, const uint8_t* s2, int32_t num_experts,
+                            int32_t hidden, int32_t intermediate, uint16_t* out, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  D3_REQUIRE(hidden > 0 && intermediate > 0 && hidden % kGroup == 0 && intermediate % kGroup == 0,
+             "mxfp4_moe: hidden %d and intermediate %d must be multiples of %d", hidden, intermediate, kGroup);
+  D3_REQUIRE(moe_shape(rows, top_k, num_experts, hidden, intermediate),
+             "mxfp4_moe: rows %lld, top_k %d (1 to 16), experts %d (1 to 512), fewer than 2^26 (row, rank) pairs",
+             static_cast<long long>(rows), top_k, num_experts);
+  D3_REQUIRE(ids_dtype == D3_DTYPE_I32 || ids_dtype == D3_DTYPE_I64, "mxfp4_moe: ids must be int32 or int64");
+  D3_REQUIRE(weights_dtype == D3_DTYPE_BF16 || weights_dtype == D3_DTYPE_F32, "mxfp4_moe: weights must be bf16 or f32");
+  D3_REQUIRE(rows == 0 || (x && ids && weights && w13 && s13 && w2 && s2 && out && workspace), "mxfp4_moe: null pointer");
+  D3_REQUIRE(rows <= 1 || x_row_stride >= 0, "mxfp4_moe: negative row stride");
+  D3_REQUIRE(mx_aligned(x, 2) && mx_aligned(w13, 16) && mx_aligned(s13, 8) && mx_aligned(w2, 16) && mx_aligned(s2, 8) &&
+                 mx_aligned(out, 8) && mx_aligned(workspace, 16) &&
+                 mx_aligned(ids, ids_dtype == D3_DTYPE_I64 ? 8 : 4) &&
+                 mx_aligned(weights, weights_dtype == D3_DTYPE_F32 ? 4 : 2),
+             "mxfp4_moe: alignment");
+  if (rows == 0) {
+    clear_error();
+    return D3_OK;
+  }
+  const MoePlan p = plan_moe(workspace, rows, top_k, num_experts, hidden, intermediate);
+  D3_REQUIRE(workspace_bytes >= p.bytes, "mxfp4_moe: workspace of %lld bytes < required %lld",
+             static_cast<long long>(workspace_bytes), static_cast<long long>(p.bytes));
+  D3_SUPPORTED(static_cast<int64_t>(p.max_items) * (mx_ceil(2 * static_cast<int64_t>(intermediate), kMxRows) +
+                                                    mx_ceil(hidden, kMxRows)) < (int64_t{1} << 31),
+               "mxfp4_moe: more than 2^31 workgroups");
+  hipStream_t s = as_stream(stream);
+  int status = d3_mxfp4_quantize(x, D3_DTYPE_BF16, x_row_stride, rows, hidden, p.q, p.qs, stream);
+  if (status != D3_OK) return status;
+  const int32_t rows32 = static_cast<int32_t>(rows);
+  if (p.scratch_ints > 0)
+    status = d3_sort_routes_wide(ids, ids_dtype, rows32, nullptr, top_k, num_experts, kMxSortTile, p.counts, p.starts,
+                                 p.total, p.sorted, p.expert_ids, p.max_rows, nullptr, p.item_rows,
+                                 reinterpret_cast<int32_t*>(p.items), p.max_items, p.num_items, nullptr, p.scratch,
+                                 p.scratch_ints, stream);
+  else
+    status = d3_sort_routes(ids, ids_dtype, rows32, nullptr, top_k, num_experts, kMxSortTile, p.counts, p.starts, p.total,
+                            p.sorted, p.expert_ids, p.max_rows, nullptr, p.item_rows, reinterpret_cast<int32_t*>(p.items),
+                            p.max_items, p.num_items, nullptr, stream);
+  if (status != D3_OK) return status;
+  MxGemm g{};
+  set_weight(g, w13, s13, 2 * intermediate, hidden);
+  g.a = p.q, g.as = p.qs, g.items = p.items, g.num_items = p.num_items, g.sorted = p.sorted, g.top_k = top_k;
+  g.out = p.act, g.out_stride = intermediate, g.out_scales = p.acts;
+  launch_gemm<kMxAct>(g, p.item_rows, p.max_items, s);
+  set_weight(g, w2, s2, hidden, intermediate);
+  g.a = p.act, g.as = p.acts, g.out = p.down, g.out_stride = hidden, g.out_scales = nullptr;
+  launch_gemm<kMxF32>(g, p.item_rows, p.max_items, s);
+  const int slices = mx_ceil(hidden, kMxCombineColumns);
+  const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
+  const int i64 = ids_dtype == D3_DTYPE_I64, f32 = weights_dtype == D3_DTYPE_F32;
+  if (top_k == 8)
+    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.down, ids, i64, weights, f32, top_k, num_experts, hidden,
+                       slices, out);
+  else
+    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.down, ids, i64, weights, f32, top_k, num_experts, hidden,
+                       slices, out);
+  D3_LAUNCHED("mxfp4_moe");
+}

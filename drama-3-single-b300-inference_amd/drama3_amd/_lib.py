@@ -108,6 +108,17 @@ SIGNATURES = {
                              _p, _p, _p, _p, _p, _p]),
     "d3_requests_load": (_i32, [_p, _p, _p, _p, _i32, _i64, _i64, _p, _p, _p, _p]),
     "d3_requests_save": (_i32, [_p, _p, _p, _p, _p, _i32, _p, _i64, _i64, _p]),
+    "d3_mxfp4_quantize": (_i32, [_p, _i32, _i64, _i64, _i32, _p, _p, _p]),
+    "d3_mxfp4_dequantize": (_i32, [_p, _p, _i64, _i32, _p, _i32, _p]),
+    "d3_mxfp4_pack": (_i32, [_p, _p, _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "d3_mxfp4_packed_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "d3_mxfp4_grouped": (
+        _i32, [_p, _i64, _i64, _p, _i32, _p, _p, _i32, _i32, _p, _i64, _i32, _p, _i64, _p]),
+    "d3_mxfp4_grouped_workspace": (_i64, [_i64, _i32, _i32]),
+    "d3_mxfp4_moe": (
+        _i32, [_p, _i64, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p,
+               _i64, _p]),
+    "d3_mxfp4_moe_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32]),
 }
 
 _lib = None

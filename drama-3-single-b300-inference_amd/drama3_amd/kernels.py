@@ -14,6 +14,7 @@ import torch
 
 from . import _lib
 from ._lib import call, ptr
+from .mxfp4 import Mxfp4Experts, mxfp4_moe
 from .pipeline import (WIDE_SORT_PAIRS, MoEWorkspace, Shape, by_pair_suited,
                        dtype_code, fragment_weights, grouped_supported, require_cuda,
                        routed_suited, rows_in_view, small_suited)
@@ -99,6 +100,10 @@ def route(logits: torch.Tensor):
 def _routed(x, topk_ids, topk_weights, experts, block_m: int = 16):
     _check_rows(x)
     require_cuda(topk_ids, topk_weights)
+    if isinstance(experts, Mxfp4Experts):
+        if block_m not in (16, 32, 64, 128):
+            raise ValueError("block_m must be 16, 32, 64 or 128")
+        return mxfp4_moe(x, topk_ids, topk_weights, experts)
     e, h, i = check_experts(experts, x.shape[1])
     if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape or len(topk_ids) != len(x):
         raise ValueError("topk_ids / topk_weights must be [T, k] for the T rows of x")
@@ -276,7 +281,8 @@ def add_norm(x, residual, weight, epsilon):
 def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start=None):
     """``DramaModel.routed_moe`` (``model.py:520-583``) as a function of the
     layer's inputs: top-8 routing of ``router`` [T, E], the routed FP8 SwiGLU
-    experts and the weighted combine -> bf16 [T, H].
+    experts (or MXFP4 ones, ``Mxfp4Experts``) and the weighted combine -> bf16
+    [T, H].
 
     The reference dispatches three numerically different backends (Triton
     GEMV for <= 8 rows, Fish's sorted GEMM for native prefill, FlashInfer for
@@ -294,7 +300,11 @@ def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start
         raise TypeError("router must be bfloat16 or float32")
     if (row_slots is None) != (padding_start is None):
         raise ValueError("Reserved padding routing requires both row_slots and padding_start")
-    e, h, i = check_experts(experts, x.shape[1])
+    mxfp4 = isinstance(experts, Mxfp4Experts)
+    if mxfp4 and x.shape[1] != experts.hidden:
+        raise ValueError(f"expert hidden size {experts.hidden} != activation width {x.shape[1]}")
+    e, h, i = ((experts.num_experts, experts.hidden, experts.intermediate) if mxfp4
+               else check_experts(experts, x.shape[1]))
     if router.shape[1] != e:
         raise ValueError(f"router has {router.shape[1]} experts, weights have {e}")
     rows = len(x)
@@ -309,6 +319,13 @@ def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start
 
         _, _, logits = prepare_moe_input(x, router, row_slots=row_slots,
                                          padding_start=padding_start)
+    if mxfp4:  # bf16 routing weights whatever the router's type, as below
+        ids = torch.empty((rows, TOP_K), dtype=torch.int32, device=x.device)
+        weights = torch.empty((rows, TOP_K), dtype=torch.bfloat16, device=x.device)
+        call("d3_route", ptr(logits), dtype_code(logits.dtype), logits.stride(0), rows, e, TOP_K,
+             None, None, ptr(ids), None, ptr(weights), dtype_code(weights.dtype),
+             _lib.stream(x.device))
+        return mxfp4_moe(x, ids, weights, experts)
     if x.stride(0) % 8 or x.data_ptr() % 16:
         x = x.contiguous()
     # (at most 64 rows: no expert has more routes than the exact path takes)

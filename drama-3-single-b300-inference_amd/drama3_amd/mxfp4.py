@@ -1,0 +1,285 @@
+"""MXFP4 (OCP Microscaling, 4 bits): quantisation of rows, and the products of
+quantised rows with MXFP4 weights: one matrix, one per group of rows, and the
+routed SwiGLU experts.  No counterpart in the reference, whose experts are FP8
+in 128 x 128 blocks: MXFP4 experts take half their bytes, and gfx950 multiplies
+them at twice the FP8 rate.
+
+A row of K elements is ``K / 2`` bytes of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4,
+6, bit 3 the sign; the even element in the low nibble) and ``K / 32`` e8m0
+scales, one byte per 32 elements: ``2 ** (code - 127)``, 255 = NaN.  A block's
+scale is ``2 ** (floor(log2(amax)) - 2)`` (at least 2 ** -127), its elements
+``e2m1(x / scale)``, ties to the even code, magnitudes above 6 to 6; a block
+that holds an infinity or a NaN reads as NaN throughout.
+
+Weights are packed once (``prepare_mxfp4``, ``prepare_mxfp4_experts``); every
+product takes bf16 rows and quantises them itself, so a batch of any size has
+the same numerics: codes times codes summed in fp32, rounded to bf16 once.
+
+Every call allocates what it returns and its workspace from torch's allocator
+on the current stream: calls on different streams share nothing, and a
+captured graph keeps its own workspace.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import call, ptr
+from .pipeline import dtype_code, require_cuda
+
+BLOCK = 32  # elements per scale
+ORDER_ROWS, ORDER_GATE_UP, ORDER_DOWN = 0, 1, 2  # which product reads a packed weight
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """``call`` with the current stream of ``device`` appended, launched with
+    ``device`` current (a stream takes kernels of its own device only)."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, _lib.stream(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, _lib.stream(device))
+
+
+def _one_device(x: torch.Tensor, **others: torch.Tensor) -> None:
+    for name, t in others.items():
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, the rows on {x.device}")
+
+
+def _check_rows(x: torch.Tensor, dtypes=(torch.bfloat16,)) -> None:
+    require_cuda(x)
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError("x must be 2-D with unit column stride")
+    if x.dtype not in dtypes:
+        raise TypeError("x must be " + " or ".join(str(d).removeprefix("torch.") for d in dtypes))
+
+
+def _check_codes(codes: torch.Tensor, scales: torch.Tensor) -> None:
+    require_cuda(codes, scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise TypeError("codes and scales must be uint8")
+    if (codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1]
+            or codes.shape[-1] * 2 != scales.shape[-1] * BLOCK):
+        raise ValueError("codes [..., K / 2] and scales [..., K / 32] do not match")
+    _one_device(codes, scales=scales)
+
+
+def quantize_mxfp4(x: torch.Tensor):
+    """bf16 or f32 rows [T, K] (K a multiple of 32, any row stride) ->
+    ``(codes uint8 [T, K / 2], scales uint8 [T, K / 32])``."""
+    _check_rows(x, (torch.bfloat16, torch.float32))
+    rows, width = x.shape
+    if width == 0 or width % BLOCK:
+        raise ValueError(f"row width {width} must be a multiple of {BLOCK}")
+    codes = torch.empty((rows, width // 2), dtype=torch.uint8, device=x.device)
+    scales = torch.empty((rows, width // BLOCK), dtype=torch.uint8, device=x.device)
+    _call(x.device, "d3_mxfp4_quantize", ptr(x), dtype_code(x.dtype), x.stride(0), rows, width,
+          ptr(codes), ptr(scales))
+    return codes, scales
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
+                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values MXFP4 rows stand for: bf16 (exact) or f32 [T, K]."""
+    _check_codes(codes, scales)
+    if codes.dim() != 2 or codes.shape[1] == 0:
+        raise ValueError("codes must be [T, K / 2]")
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("dtype must be bfloat16 or float32")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    rows, width = len(codes), 2 * codes.shape[1]
+    out = torch.empty((rows, width), dtype=dtype, device=codes.device)
+    _call(codes.device, "d3_mxfp4_dequantize", ptr(codes), ptr(scales), rows, width, ptr(out),
+          dtype_code(dtype))
+    return out
+
+
+@dataclass(frozen=True)
+class Mxfp4Weight:
+    """Packed MXFP4 weights of one product: ``experts`` matrices [N, K]
+    (``prepare_mxfp4``); ``codes`` / ``scales`` are in the kernels' layout."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    experts: int
+    n: int
+    k: int
+    order: int = ORDER_ROWS
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+@dataclass(frozen=True)
+class Mxfp4Experts:
+    """Routed SwiGLU experts on MXFP4 weights (``prepare_mxfp4_experts``)."""
+
+    w13: Mxfp4Weight
+    w2: Mxfp4Weight
+
+    @property
+    def num_experts(self) -> int:
+        return self.w13.experts
+
+    @property
+    def hidden(self) -> int:
+        return self.w13.k
+
+    @property
+    def intermediate(self) -> int:
+        return self.w2.k
+
+
+def _prepare(codes: torch.Tensor, scales: torch.Tensor, order: int) -> Mxfp4Weight:
+    _check_codes(codes, scales)
+    if codes.dim() == 2:
+        codes, scales = codes[None], scales[None]
+    if codes.dim() != 3 or 0 in codes.shape:
+        raise ValueError("weights must be [N, K / 2] or [E, N, K / 2] codes")
+    experts, n, k = codes.shape[0], codes.shape[1], 2 * codes.shape[2]
+    if k % 128:
+        raise ValueError(f"K={k} must be a multiple of 128")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    lib = _lib.load()
+    u8 = dict(dtype=torch.uint8, device=codes.device)
+    packed = torch.empty(lib.d3_mxfp4_packed_bytes(experts, n, k, 0), **u8)
+    packed_scales = torch.empty(lib.d3_mxfp4_packed_bytes(experts, n, k, 1), **u8)
+    _call(codes.device, "d3_mxfp4_pack", ptr(codes), ptr(scales), experts, n, k, order, ptr(packed),
+          ptr(packed_scales))
+    return Mxfp4Weight(packed, packed_scales, experts, n, k, order)
+
+
+def prepare_mxfp4(codes: torch.Tensor, scales: torch.Tensor) -> Mxfp4Weight:
+    """Weights [N, K] or [E, N, K] as ``quantize_mxfp4`` gives them (K a
+    multiple of 128, any N) -> the packed weight of ``mxfp4_linear`` /
+    ``grouped_mxfp4``.  The arguments are not needed afterwards."""
+    return _prepare(codes, scales, ORDER_ROWS)
+
+
+def prepare_mxfp4_experts(w13_codes, w13_scales, w2_codes, w2_scales) -> Mxfp4Experts:
+    """``w13`` [E, 2I, H] (rows [gate; up]) and ``w2`` [E, H, I] as codes and
+    scales (H and I multiples of 128) -> the experts of ``mxfp4_moe``."""
+    if w13_codes.dim() != 3 or w2_codes.dim() != 3:
+        raise ValueError("expert weights must be [E, N, K / 2] codes")
+    experts, two_i, half_h = w13_codes.shape
+    if w2_codes.shape != (experts, 2 * half_h, two_i // 4) or two_i % 256 or half_h % 64:
+        raise ValueError("expert weights must be w13 [E, 2I, H], w2 [E, H, I], H and I multiples of 128")
+    _one_device(w13_codes, w2_codes=w2_codes)
+    return Mxfp4Experts(_prepare(w13_codes, w13_scales, ORDER_GATE_UP),
+                        _prepare(w2_codes, w2_scales, ORDER_DOWN))
+
+
+def quantize_experts_mxfp4(experts) -> Mxfp4Experts:
+    """FP8 block-scaled experts (``w13_weight``, ``w13_scale_inv``,
+    ``w2_weight``, ``w2_scale_inv``: the MoE operators' contract) rounded to
+    MXFP4, one expert at a time, at load time."""
+    packed = []
+    for weight, inverse, order in ((experts.w13_weight, experts.w13_scale_inv, ORDER_GATE_UP),
+                                   (experts.w2_weight, experts.w2_scale_inv, ORDER_DOWN)):
+        require_cuda(weight, inverse)
+        if weight.dim() != 3 or weight.dtype != torch.float8_e4m3fn:
+            raise TypeError("expert weights must be float8_e4m3fn [E, N, K]")
+        e, n, k = weight.shape
+        if n % 128 or k % 128 or inverse.shape != (e, n // 128, k // 128):
+            raise ValueError("expert weights do not follow the 128x128 block layout")
+        codes = torch.empty((e, n, k // 2), dtype=torch.uint8, device=weight.device)
+        scales = torch.empty((e, n, k // BLOCK), dtype=torch.uint8, device=weight.device)
+        for i in range(e):
+            blocks = weight[i].float().view(n // 128, 128, k // 128, 128)
+            values = (blocks * inverse[i].float()[:, None, :, None]).view(n, k)
+            codes[i], scales[i] = quantize_mxfp4(values)
+        packed.append(_prepare(codes, scales, order))
+    return Mxfp4Experts(*packed)
+
+
+def _product(x, boundaries, weight: Mxfp4Weight, out, zero_rest: bool) -> torch.Tensor:
+    _check_rows(x)
+    if weight.order != ORDER_ROWS:
+        raise ValueError("weight was packed for mxfp4_moe; pack it with prepare_mxfp4")
+    rows, k = x.shape
+    if k != weight.k:
+        raise ValueError(f"rows of width {k}, weight of K={weight.k}")
+    _one_device(x, weight=weight.codes)
+    if out is None:
+        out = torch.empty((rows, weight.n), dtype=torch.bfloat16, device=x.device)
+    size = _lib.load().d3_mxfp4_grouped_workspace(rows, weight.experts, k)
+    workspace = torch.empty(max(size, 0), dtype=torch.uint8, device=x.device)
+    _call(x.device, "d3_mxfp4_grouped", ptr(x), x.stride(0), rows, ptr(boundaries), weight.experts,
+          ptr(weight.codes), ptr(weight.scales), weight.n, k, ptr(out), out.stride(0),
+          int(zero_rest), ptr(workspace), size)
+    return out
+
+
+def mxfp4_linear(x: torch.Tensor, weight: Mxfp4Weight) -> torch.Tensor:
+    """``x`` bf16 [T, K], quantised to MXFP4, times the weight [N, K]
+    transposed -> bf16 [T, N]."""
+    if weight.experts != 1:
+        raise ValueError(f"mxfp4_linear takes one matrix, the weight holds {weight.experts}")
+    return _product(x, None, weight, None, False)
+
+
+def grouped_mxfp4(x: torch.Tensor, boundaries: torch.Tensor, weight: Mxfp4Weight,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows ``[boundaries[e], boundaries[e + 1])`` of ``x`` bf16 [T, K],
+    quantised to MXFP4, times matrix e of ``weight`` [E, N, K] transposed ->
+    bf16 [T, N].
+
+    ``boundaries`` int32 [E + 1], ascending, on the device (groups may be
+    empty; values are clamped to [0, T]).  Rows of no group are zeros, or left
+    as they were in a given ``out`` (bf16 [T, N], unit column stride)."""
+    _check_rows(x)
+    require_cuda(boundaries, out)
+    if boundaries.dtype != torch.int32:
+        raise TypeError("boundaries must be int32")
+    if boundaries.shape != (weight.experts + 1,) or boundaries.stride(0) != 1:
+        raise ValueError(f"boundaries must be contiguous [{weight.experts + 1}], one more than the experts")
+    _one_device(x, boundaries=boundaries)
+    if out is not None:
+        if out.dtype != torch.bfloat16:
+            raise TypeError("out must be bfloat16")
+        if out.shape != (len(x), weight.n) or (weight.n > 1 and out.stride(1) != 1) or (
+                len(x) > 1 and out.stride(0) < weight.n):
+            raise ValueError(f"out must be [{len(x)}, {weight.n}] with unit column stride")
+        _one_device(x, out=out)
+    return _product(x, boundaries, weight, out, out is None)
+
+
+def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor,
+              experts: Mxfp4Experts) -> torch.Tensor:
+    """Routed SwiGLU experts: for row t and rank r with expert e =
+    ``topk_ids[t, r]``, ``a = silu(G_e x) * (U_e x)`` and ``out[t] = sum_r
+    topk_weights[t, r] * W2_e a`` in rank order, with x and a quantised to
+    MXFP4 and everything else fp32, rounded to bf16 [T, H] once.
+
+    ``topk_ids`` int32 / int64 [T, k], k <= 16 (an id that names no expert
+    adds nothing), ``topk_weights`` bf16 / f32 of the same shape."""
+    _check_rows(x)
+    require_cuda(topk_ids, topk_weights)
+    if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape or len(topk_ids) != len(x):
+        raise ValueError("topk_ids / topk_weights must be [T, k] for the T rows of x")
+    if topk_ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError("topk_ids must be int32 or int64")
+    if topk_weights.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError("topk_weights must be bfloat16 or float32")
+    if x.shape[1] != experts.hidden:
+        raise ValueError(f"rows of width {x.shape[1]}, experts of hidden size {experts.hidden}")
+    w13, w2 = experts.w13, experts.w2
+    if w13.order != ORDER_GATE_UP or w2.order != ORDER_DOWN:
+        raise ValueError("experts must come from prepare_mxfp4_experts")
+    _one_device(x, topk_ids=topk_ids, topk_weights=topk_weights, experts=w13.codes)
+    ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
+    rows, top_k = ids.shape
+    out = torch.empty((rows, experts.hidden), dtype=torch.bfloat16, device=x.device)
+    size = _lib.load().d3_mxfp4_moe_workspace(rows, top_k, w13.experts, w13.k, w2.k)
+    workspace = torch.empty(max(size, 0), dtype=torch.uint8, device=x.device)
+    _call(x.device, "d3_mxfp4_moe", ptr(x), x.stride(0), rows, ptr(ids), dtype_code(ids.dtype),
+          ptr(weights), dtype_code(weights.dtype), top_k, ptr(w13.codes), ptr(w13.scales),
+          ptr(w2.codes), ptr(w2.scales), w13.experts, w13.k, w2.k, ptr(out), ptr(workspace), size)
+    return out

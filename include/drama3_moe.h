@@ -770,6 +770,86 @@ int d3_requests_save(int64_t *last, int64_t *history, int64_t *metadata, int64_t
                      const int64_t *slots, int32_t rows, const int64_t *output, int64_t eos,
                      int64_t limit, void *stream);
 
+/*
+ * MXFP4 (no counterpart in the reference): experts and projections in the
+ * OCP Microscaling format of 4 bits, half the weight bytes of FP8, and their
+ * products on the gfx950 block-scaled matrix instructions.
+ *
+ * A row of K elements is K / 2 bytes of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4,
+ * 6, bit 3 the sign; the even element in the low nibble) and K / 32 e8m0
+ * scales, one byte per 32 elements: 2^(code - 127), 255 = NaN.  Quantisation:
+ * scale = 2^(floor(log2 amax) - 2) (at least 2^-127), element = e2m1(x /
+ * scale) rounded to nearest even, magnitudes above 6 to 6; a block that holds
+ * an infinity or a NaN gets scale 255 and zero codes, and reads as NaN.
+ */
+
+/*
+ * Rows of MXFP4 from bf16 or f32: x [rows, width] (row stride in elements,
+ * unit column stride, aligned to its elements) -> codes [rows, width / 2],
+ * scales [rows, width / 32].  width % 32 == 0.
+ */
+int d3_mxfp4_quantize(const void *x, int32_t x_dtype, int64_t x_row_stride, int64_t rows,
+                      int32_t width, uint8_t *codes, uint8_t *scales, void *stream);
+
+/* The values MXFP4 rows stand for, bf16 (exact) or f32 [rows, width], 16-byte aligned. */
+int d3_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int32_t width,
+                        void *out, int32_t out_dtype, void *stream);
+
+/*
+ * MXFP4 weights [num_experts, n, k / 2] codes, [num_experts, n, k / 32]
+ * scales -> the packed layout the products read, once at load time.  Buffers
+ * of d3_mxfp4_packed_bytes bytes; k % 128 == 0, any n.  `order` says which
+ * product reads them:
+ *   0 d3_mxfp4_grouped (bf16 rows);
+ *   1 the gate and up product of d3_mxfp4_moe (rows [gate; up], n % 64 == 0);
+ *   2 its down product.
+ */
+int d3_mxfp4_pack(const uint8_t *codes, const uint8_t *scales, int32_t num_experts, int32_t n,
+                  int32_t k, int32_t order, uint8_t *packed, uint8_t *packed_scales,
+                  void *stream);
+
+/* Bytes of the packed codes (scales = 0) or scales (scales = 1) of [num_experts, n, k]. */
+int64_t d3_mxfp4_packed_bytes(int32_t num_experts, int32_t n, int32_t k, int32_t scales);
+
+/*
+ * Product of rows grouped by expert: rows [boundaries[e], boundaries[e + 1])
+ * of x bf16 [rows, k], quantised to MXFP4, times expert e's packed weight
+ * (order 0) transposed -> the same rows of out bf16 [rows, n] (fp32 sums, one
+ * rounding).  boundaries int32 [num_experts + 1] on the device, ascending,
+ * clamped to [0, rows]; NULL with one expert: every row.  Rows of no group
+ * are zeroed with zero_rest, else left as they were.  workspace: at least
+ * d3_mxfp4_grouped_workspace bytes, 16-byte aligned, this call's alone until
+ * it has run.
+ */
+int d3_mxfp4_grouped(const uint16_t *x, int64_t x_row_stride, int64_t rows,
+                     const int32_t *boundaries, int32_t num_experts, const uint8_t *w,
+                     const uint8_t *ws, int32_t n, int32_t k, uint16_t *out,
+                     int64_t out_row_stride, int32_t zero_rest, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes of d3_mxfp4_grouped (host-side arithmetic only; -1: not supported). */
+int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t k);
+
+/*
+ * Routed SwiGLU experts on MXFP4 weights: for every row t and rank r with
+ * expert e = ids[t, r], a = silu(G x) * (U x) with x quantised to MXFP4 and
+ * [G; U] = w13[e] (order 1), a quantised to MXFP4 from its fp32 values, and
+ *   out[t] = sum over r of weights[t, r] * (w2[e] (order 2) a)
+ * in rank order, fp32 throughout, rounded to bf16 once.  ids int32 or int64
+ * [rows, top_k] (an id outside [0, num_experts) adds nothing), weights bf16 or
+ * f32.  top_k <= 16, num_experts <= 512, hidden and intermediate multiples of
+ * 128.  workspace: d3_mxfp4_moe_workspace bytes, as for d3_mxfp4_grouped.
+ */
+int d3_mxfp4_moe(const uint16_t *x, int64_t x_row_stride, int64_t rows, const void *ids,
+                 int32_t ids_dtype, const void *weights, int32_t weights_dtype, int32_t top_k,
+                 const uint8_t *w13, const uint8_t *s13, const uint8_t *w2, const uint8_t *s2,
+                 int32_t num_experts, int32_t hidden, int32_t intermediate, uint16_t *out,
+                 void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes of d3_mxfp4_moe (host-side arithmetic only; -1: not supported). */
+int64_t d3_mxfp4_moe_workspace(int64_t rows, int32_t top_k, int32_t num_experts, int32_t hidden,
+                               int32_t intermediate);
+
 #ifdef __cplusplus
 }
 #endif
