@@ -13,6 +13,8 @@ constexpr int kMxRows = 64;        // weight rows of a packed row group (four 16
 constexpr int kMxStep = 256;       // contracted elements of a packed step (two MFMAs deep)
 constexpr int kMxStepCodes = kMxRows * kMxStep / 2;          // 8 KiB of codes per row group and step
 constexpr int kMxStepScales = kMxRows * kMxStep / kMxBlock;  // 512 bytes of scales
+constexpr int kMxOperandCodes = kMxStep / 2;         // a quantised row's codes per step
+constexpr int kMxOperandScales = kMxStep / kMxBlock;  // and scales
 constexpr int kMxLow = 4;  // the MFMA's format code of e2m1 operands
 
 // Row orders of a packed weight: which row of W the lanes of an MFMA's
@@ -29,6 +31,24 @@ __host__ __device__ __forceinline__ int mx_weight_row(int order, int n, int rg, 
   if (order == kMxOrderPairs) return kMxRows * rg + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i;
   return (t >= 2 ? n / 2 : 0) + 32 * rg + 8 * g + 4 * (t & 1) + i;
 }
+
+// Quantised rows as the products read them: codes in row order at a pitch of
+// whole steps, scales per step as byte 2 (block % 4) + (block / 4) of its 8
+// blocks, so that an MFMA lane (block % 4 is its group) finds the scales of
+// both halves of a step in one 16-bit word.  A row whose width is an odd
+// multiple of 128 has its last half step's scales zeroed here (the weights'
+// codes are zeros there, the row's are whatever the buffer holds: no e2m1 code
+// is an infinity or a NaN, but scale 255 would be).
+__device__ __forceinline__ void mx_operand_scale(uint8_t* row, uint32_t block, uint32_t blocks, uint32_t code) {
+  const uint32_t step = block >> 3;
+  uint8_t* at = row + step * kMxOperandScales + 2 * (block & 3) + ((block >> 2) & 1);
+  *at = static_cast<uint8_t>(code);
+  if (8 * step + 4 >= blocks) at[1] = 0;  // the last step's second half is padding
+}
+
+// bf16 rows to that layout (width % 128 == 0).
+void mx_quantize_operand(const uint16_t* x, int64_t stride, int64_t rows, int width, uint8_t* codes, uint8_t* scales,
+                         hipStream_t stream);
 
 // Scale code of a block whose largest magnitude has the fp32 bits `amax`
 // (sign bit clear): floor(log2 amax) - 2, so that the largest element lies in

@@ -8,6 +8,8 @@
 // of sum |products| measured over scales that differ by 2^40).  Weights are
 // the first operand: an output lane holds one row of a and four consecutive
 // weight rows of each 16-row tile, as the packed row orders place them.
+#include <type_traits>
+
 #include "mxfp4.h"
 #include "status.h"
 
@@ -29,31 +31,29 @@ struct MxGemm {
   int n;
   int row_groups;
   int steps;
-  const uint8_t* a;  // codes [rows][k_bytes]
-  const uint8_t* as;  // scales [rows][k_blocks]
-  int k_bytes;
-  int k_blocks;
+  const uint8_t* a;  // quantised rows (operand layout, `steps` steps)
+  const uint8_t* as;
   const int4* items;  // {expert (-1: zero rows), first row, rows, -}; nullptr: one expert, `rows` in order
   const int32_t* num_items;
   int rows;
   const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxF32)
   int top_k;
   void* out;
-  int64_t out_stride;
-  uint8_t* out_scales;
+  int64_t out_stride;  // elements (kMxAct: the row's width)
+  uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout
 };
 
 // One MFMA with the scales in byte SA of `sa` and byte SB of `sb`.
 template <int SA, int SB>
-__device__ __forceinline__ floatx4 mfma_fp4(const int4& a, const int4& b, const floatx4& c, uint32_t sa, uint32_t sb) {
-  const int32x8 av = {a.x, a.y, a.z, a.w, 0, 0, 0, 0};
-  const int32x8 bv = {b.x, b.y, b.z, b.w, 0, 0, 0, 0};
+__device__ __forceinline__ floatx4 mfma_fp4(const int32x4& a, const int32x4& b, const floatx4& c, uint32_t sa, uint32_t sb) {
+  const int32x8 av = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
+  const int32x8 bv = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, kMxLow, kMxLow, SA, static_cast<int>(sa), SB,
                                                           static_cast<int>(sb));
 }
 
 template <int SB>
-__device__ __forceinline__ void mfma_tiles(const int4 (&a)[4], const int4& b, floatx4 (&c)[4], uint32_t sa, uint32_t sb) {
+__device__ __forceinline__ void mfma_tiles(const int32x4 (&a)[4], const int32x4& b, floatx4 (&c)[4], uint32_t sa, uint32_t sb) {
   c[0] = mfma_fp4<0, SB>(a[0], b, c[0], sa, sb);
   c[1] = mfma_fp4<1, SB>(a[1], b, c[1], sa, sb);
   c[2] = mfma_fp4<2, SB>(a[2], b, c[2], sa, sb);
@@ -85,9 +85,13 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4],
       if (f + 8 <= g.n) {
         *reinterpret_cast<MxWords4*>(out + f) = v;
       } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (f + i < g.n) out[f + i] = static_cast<uint16_t>(v.w[i / 2] >> (16 * (i & 1)));
+        uint64_t lo8 = v.w[0] | (static_cast<uint64_t>(v.w[1]) << 32), hi8 = v.w[2] | (static_cast<uint64_t>(v.w[3]) << 32);
+#pragma unroll 1
+        for (int i = f; i < g.n; ++i) {
+          out[i] = static_cast<uint16_t>(lo8);
+          lo8 = (lo8 >> 16) | (hi8 << 48);
+          hi8 >>= 16;
+        }
       }
     }
   } else if constexpr (kEpi == kMxAct) {
@@ -109,9 +113,10 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4],
     const uint32_t code = mx_scale_code(amax);
     const uint32_t word = mx_codes8(v, mx_inverse(code));
     if (!live) return;
-    const int64_t at = static_cast<int64_t>(row) * (g.out_stride / kMxBlock) + rg;
-    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.out) + at * (kMxBlock / 2) + 4 * group) = word;
-    if (group == 0) g.out_scales[at] = static_cast<uint8_t>(code);
+    const uint32_t blocks = static_cast<uint32_t>(g.out_stride) / kMxBlock;
+    const int64_t first = static_cast<int64_t>(row) * ((blocks + 7) / 8);  // in steps
+    *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.out) + first * kMxOperandCodes + rg * (kMxBlock / 2) + 4 * group) = word;
+    if (group == 0) mx_operand_scale(g.out_scales + first * kMxOperandScales, rg, blocks, code);
   } else {
     if (!live) return;
     float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride + kMxRows * rg + 4 * group;
@@ -156,11 +161,11 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
   for (int rt = 0; rt < kRT; ++rt) {
     int64_t row = item.y + min(16 * rt + row16, count - 1);
     if constexpr (kEpi == kMxAct) row = g.sorted[row] / g.top_k;
-    codes[rt] = g.a + row * g.k_bytes;
-    scales[rt] = g.as + row * g.k_blocks;
+    codes[rt] = g.a + row * g.steps * kMxOperandCodes + 16 * group;
+    scales[rt] = g.as + row * g.steps * kMxOperandScales + 2 * group;
   }
   const int64_t base = static_cast<int64_t>(item.x) * g.row_groups + rg_read;
-  const int4* w = reinterpret_cast<const int4*>(g.w + base * g.steps * kMxStepCodes) + lane;
+  const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * g.steps * kMxStepCodes) + lane;
   const uint2* ws = reinterpret_cast<const uint2*>(g.ws + base * g.steps * kMxStepScales) + lane;
 
   floatx4 acc[kRT][4];
@@ -170,8 +175,8 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
     for (int t = 0; t < 4; ++t) acc[rt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 
   for (int step = slice; step < g.steps; step += kSplit) {
-    int4 wf[2][4];
-    const int4* wp = w + static_cast<int64_t>(step) * (kMxStepCodes / 16);
+    int32x4 wf[2][4];
+    const int32x4* wp = w + static_cast<int64_t>(step) * (kMxStepCodes / 16);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -179,17 +184,10 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
     const uint2 wsc = ws[static_cast<int64_t>(step) * (kMxStepScales / 8)];
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        // Blocks from K on (an odd multiple of 128) meet zero weights at
-        // scale 1: the lane reads its first half again, at scale 2^-127.
-        const int kblock = 8 * step + 4 * h + group;
-        const bool live = kblock < g.k_blocks;
-        const int at = live ? kblock : kblock - 4;
-        const int4 b = *reinterpret_cast<const int4*>(codes[rt] + 16 * at);
-        const uint32_t sb = live ? scales[rt][at] : 0u;
-        mfma_tiles<0>(wf[h], b, acc[rt], h ? wsc.y : wsc.x, sb);
-      }
+      const uint32_t sb = *reinterpret_cast<const uint16_t*>(scales[rt] + kMxOperandScales * step);
+      const int32x4* b = reinterpret_cast<const int32x4*>(codes[rt] + kMxOperandCodes * step);
+      mfma_tiles<0>(wf[0], b[0], acc[rt], wsc.x, sb);
+      mfma_tiles<1>(wf[1], b[4], acc[rt], wsc.y, sb);
     }
   }
 
@@ -219,6 +217,170 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
     for (int rt = 0; rt < kRT; ++rt)
       mx_store<kEpi>(g, acc[rt], rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
   }
+}
+
+// Contraction-sized items (up to 128 rows).  A workgroup owns (item, 256
+// weight rows); each of its four waves one row group of 64 and every row of
+// the item, so that an operand read from LDS feeds four MFMAs and a weight
+// operand every row tile.  Weights go straight from memory into operands (the
+// packed layout is theirs); the item's quantised rows are staged through a
+// two-slot LDS ring in operand order ([row tile][half][lane][16 bytes]: each
+// ds_read_b128 of a wave is 1 KiB of consecutive memory), one step of 256
+// elements at a time, the next step's loads in flight while the current one
+// is multiplied.  An item is multiplied in the smallest of four bodies (2, 4,
+// 6, 8 row tiles) that holds it.
+constexpr int kMxTiledRows = 128;
+constexpr int kMxSlotCodes = kMxTiledRows * kMxOperandCodes;    // 16 KiB
+constexpr int kMxSlotScales = kMxTiledRows * kMxOperandScales;  // 1 KiB
+constexpr int kMxXcds = 8;
+
+struct MxTiles {
+  int n_tiles;  // 256-row weight tiles
+  int run;      // consecutive items whose tiles one XCD takes together
+};
+
+template <int kRT, int kEpi>
+__device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t (*ring)[kMxSlotCodes],
+                                              uint8_t (*ring_scales)[kMxSlotScales]) {
+  constexpr int kCopies = kRT / 2;  // 16-byte parts a thread stages per step
+  const int tid = threadIdx.x, lane = lane_id(), row16 = lane & 15, group = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int rg = n_tile * kMxWaves + wave;
+  const int rg_read = min(rg, g.row_groups - 1);
+  const int count = min(item.z, 16 * kRT);
+  const int steps = g.steps;
+
+  auto source_row = [&](int r) -> int64_t {  // rows past the item: its last row
+    const int at = item.y + min(r, count - 1);
+    if constexpr (kEpi == kMxAct) return g.sorted[at] / g.top_k;
+    return at;
+  };
+  // Wave w stages operands (row tile, half) w, w + 4, ..: a row tile's halves
+  // are consecutive, so copy i of this wave is row tile (w + 4 i) / 2.
+  const uint8_t* src[kCopies];
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i) {
+    const int unit = wave + kMxWaves * i;
+    src[i] = g.a + source_row(16 * (unit >> 1) + row16) * steps * kMxOperandCodes + 64 * (unit & 1) + 16 * group;
+  }
+  // and a thread four of the eight scales of row tid / 2.
+  const uint8_t* scale_src = g.as + source_row(tid >> 1) * steps * kMxOperandScales + 4 * (tid & 1);
+
+  const int64_t base = (static_cast<int64_t>(item.x) * g.row_groups + rg_read) * steps;
+  const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * kMxStepCodes) + lane;
+  const uint32_t* ws = reinterpret_cast<const uint32_t*>(g.ws + base * kMxStepScales) + 2 * lane;
+
+  int32x4 wf[2][4], copy[kCopies];
+  uint32_t wsc[2];
+  uint32_t copy_scale;
+  auto load_weights = [&](int step, auto half) {
+    constexpr int kHalf = decltype(half)::value;
+    const int32x4* wp = w + static_cast<int64_t>(step) * (kMxStepCodes / 16) + kHalf * 4 * kWave;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) wf[kHalf][t] = wp[t * kWave];
+    wsc[kHalf] = ws[static_cast<int64_t>(step) * (kMxStepScales / 4) + kHalf];
+  };
+  auto load_rows = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i) copy[i] = *reinterpret_cast<const int32x4*>(src[i] + step * kMxOperandCodes);
+    copy_scale = *reinterpret_cast<const uint32_t*>(scale_src + step * kMxOperandScales);
+  };
+  auto store_rows = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < kCopies; ++i)
+      *reinterpret_cast<int32x4*>(&ring[slot][((wave + kMxWaves * i) * kWave + lane) * 16]) = copy[i];
+    *reinterpret_cast<uint32_t*>(&ring_scales[slot][tid * 4]) = copy_scale;
+  };
+
+  floatx4 acc[kRT][4];
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[rt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  uint32_t sb[kRT];
+  auto multiply = [&](int slot, auto half) {
+    constexpr int kHalf = decltype(half)::value;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      if constexpr (kHalf == 0)
+        sb[rt] = *reinterpret_cast<const uint16_t*>(&ring_scales[slot][(16 * rt + row16) * kMxOperandScales + 2 * group]);
+      const int32x4 b = *reinterpret_cast<const int32x4*>(&ring[slot][((2 * rt + kHalf) * kWave + lane) * 16]);
+      mfma_tiles<kHalf>(wf[kHalf], b, acc[rt], wsc[kHalf], sb[rt]);
+    }
+  };
+  // Issue order of a half step: operand reads two row tiles ahead of their
+  // MFMAs (all at once they would take registers that the sums leave no room
+  // for), the half's loads from memory among the first MFMAs; nothing moves
+  // into another half.
+  auto issue_order = [&](auto reads, auto loads) {
+    constexpr int kReads = decltype(reads)::value, kLoads = decltype(loads)::value;
+    constexpr int kVmem = 0x020, kMfma = 0x008, kDsRead = 0x100, kAhead = kRT < 2 ? kRT : 2;
+    __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead * kReads, 0);
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) {
+      __builtin_amdgcn_sched_group_barrier(kVmem, (kLoads + kRT - 1) / kRT, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(kDsRead, kReads, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  using Half0 = std::integral_constant<int, 0>;
+  using Half1 = std::integral_constant<int, 1>;
+  // Step s is multiplied from slot s % 2 while step s + 1 loads: its rows
+  // first (their store to LDS then waits for no weights), each half's weights
+  // into the registers that half leaves.  The rows go to the slot that step
+  // s - 1 used, which every wave left before the last barrier.
+  load_rows(0);
+  load_weights(0, Half0{});
+  load_weights(0, Half1{});
+  store_rows(0);
+  lds_barrier();
+  for (int step = 0; step < steps; ++step) {
+    const int next = min(step + 1, steps - 1);  // the last step loads its own operands again, for nobody
+    load_rows(next);
+    multiply(step & 1, Half0{});
+    issue_order(std::integral_constant<int, 2>{}, std::integral_constant<int, kCopies + 1>{});
+    load_weights(next, Half0{});
+    multiply(step & 1, Half1{});
+    issue_order(std::integral_constant<int, 1>{}, std::integral_constant<int, 5>{});
+    load_weights(next, Half1{});
+    store_rows((step & 1) ^ 1);
+    lds_barrier();
+  }
+  if (rg >= g.row_groups) return;
+#pragma unroll
+  for (int rt = 0; rt < kRT; ++rt)
+    mx_store<kEpi>(g, acc[rt], rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
+}
+
+template <int kEpi>
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2))) void mx_tiled_kernel(MxGemm g,
+                                                                                                      MxTiles tiles) {
+  __shared__ __attribute__((aligned(16))) uint8_t ring[2][kMxSlotCodes];
+  __shared__ __attribute__((aligned(16))) uint8_t ring_scales[2][kMxSlotScales];
+  // Runs of consecutive items go to the XCDs in turn (workgroup b runs on XCD
+  // b % 8): a run's tiles share its rows, and an expert's consecutive items
+  // its weights, in that XCD's L2.
+  const int per_run = tiles.run * tiles.n_tiles;
+  const int j = blockIdx.x / kMxXcds;
+  const int in_run = j % per_run;
+  const int index = ((j / per_run) * kMxXcds + blockIdx.x % kMxXcds) * tiles.run + in_run % tiles.run;
+  const int n_tile = in_run / tiles.run;
+  const int4 item = mx_item(g, index, kMxTiledRows);
+  if (item.z <= 0) return;  // uniform
+  if (kEpi == kMxBf16 && item.x < 0) {
+    mx_zero_rows(g, item, n_tile * kMxWaves * kMxRows, kMxWaves * kMxRows);
+    return;
+  }
+  if (item.z > 96)
+    mx_tiled_body<8, kEpi>(g, item, n_tile, ring, ring_scales);
+  else if (item.z > 64)
+    mx_tiled_body<6, kEpi>(g, item, n_tile, ring, ring_scales);
+  else if (item.z > 32)
+    mx_tiled_body<4, kEpi>(g, item, n_tile, ring, ring_scales);
+  else
+    mx_tiled_body<2, kEpi>(g, item, n_tile, ring, ring_scales);
 }
 
 // Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
@@ -318,18 +480,24 @@ void launch_stream(const MxGemm& g, int items, hipStream_t s) {
 template <int kEpi>
 void launch_gemm(const MxGemm& g, int item_rows, int items, hipStream_t s) {
   if (items <= 0) return;
-  if (item_rows <= 16)
+  if (item_rows <= 16) {
     launch_stream<1, kEpi>(g, items, s);
-  else if (item_rows <= 32)
+  } else if (item_rows <= 32) {
     launch_stream<2, kEpi>(g, items, s);
-  else
+  } else if (item_rows <= 64) {
     launch_stream<4, kEpi>(g, items, s);
+  } else {
+    const MxTiles tiles{mx_ceil(g.row_groups, kMxWaves), 2};
+    const int runs = mx_ceil(items, kMxXcds * tiles.run) * kMxXcds;
+    hipLaunchKernelGGL(mx_tiled_kernel<kEpi>, dim3(static_cast<unsigned>(runs) * tiles.run * tiles.n_tiles),
+                       dim3(kMxThreads), 0, s, g, tiles);
+  }
 }
 
 // Rows per work item for groups of `mean` rows on average.
 int mx_item_rows(int64_t rows, int64_t groups) {
   const int64_t mean = rows / groups;
-  return mean <= 16 ? 16 : (mean <= 32 ? 32 : 64);
+  return mean <= 16 ? 16 : (mean <= 32 ? 32 : (mean <= 64 ? 64 : kMxTiledRows));
 }
 
 // Byte arena of one call, carved in order at 256-byte boundaries.
@@ -347,7 +515,6 @@ struct Arena {
 void set_weight(MxGemm& g, const uint8_t* w, const uint8_t* ws, int n, int k) {
   g.w = w, g.ws = ws, g.n = n;
   g.row_groups = mx_ceil(n, kMxRows), g.steps = mx_ceil(k, kMxStep);
-  g.k_bytes = k / 2, g.k_blocks = k / kMxBlock;
 }
 
 struct GroupedPlan {
@@ -364,8 +531,8 @@ GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, int k) {
   // every group, and each of the two runs of rows in none, adds one partial item at most
   p.max_items = static_cast<int>(rows / p.item_rows + (rows < experts + 2 ? rows : experts + 2));
   Arena a{static_cast<uint8_t*>(arena)};
-  p.q = a.take<uint8_t>(rows * (k / 2));
-  p.qs = a.take<uint8_t>(rows * (k / kMxBlock));
+  p.q = a.take<uint8_t>(rows * mx_ceil(k, kMxStep) * kMxOperandCodes);
+  p.qs = a.take<uint8_t>(rows * mx_ceil(k, kMxStep) * kMxOperandScales);
   p.items = a.take<int4>(p.max_items);
   p.num_items = a.take<int32_t>(1);
   p.bytes = a.used;
@@ -393,10 +560,11 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
   p.max_items = d3_max_items(pairs, experts, p.item_rows);
   p.scratch_ints = p.pairs > kMxWidePairs ? d3_sort_wide_scratch_ints(static_cast<int32_t>(rows), top_k, experts) : 0;
   Arena a{static_cast<uint8_t*>(arena)};
-  p.q = a.take<uint8_t>(rows * (hidden / 2));
-  p.qs = a.take<uint8_t>(rows * (hidden / kMxBlock));
-  p.act = a.take<uint8_t>(static_cast<int64_t>(p.max_rows) * (inter / 2));
-  p.acts = a.take<uint8_t>(static_cast<int64_t>(p.max_rows) * (inter / kMxBlock));
+  const int64_t x_steps = mx_ceil(hidden, kMxStep), act_steps = mx_ceil(inter, kMxStep);
+  p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
+  p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
+  p.act = a.take<uint8_t>(p.max_rows * act_steps * kMxOperandCodes);
+  p.acts = a.take<uint8_t>(p.max_rows * act_steps * kMxOperandScales);
   p.down = a.take<float>(p.pairs * hidden);
   p.counts = a.take<int32_t>(experts);
   p.starts = a.take<int32_t>(experts);
@@ -451,8 +619,7 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
   D3_SUPPORTED(static_cast<int64_t>(p.max_items) * mx_ceil(n, kMxRows) < (int64_t{1} << 31),
                "mxfp4_grouped: more than 2^31 workgroups");
   hipStream_t s = as_stream(stream);
-  int status = d3_mxfp4_quantize(x, D3_DTYPE_BF16, x_row_stride, rows, k, p.q, p.qs, stream);
-  if (status != D3_OK) return status;
+  mx_quantize_operand(x, x_row_stride, rows, k, p.q, p.qs, s);
   MxGemm g{};
   set_weight(g, w, ws, n, k);
   g.a = p.q, g.as = p.qs, g.rows = static_cast<int>(rows);
@@ -504,8 +671,8 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
                                                     mx_ceil(hidden, kMxRows)) < (int64_t{1} << 31),
                "mxfp4_moe: more than 2^31 workgroups");
   hipStream_t s = as_stream(stream);
-  int status = d3_mxfp4_quantize(x, D3_DTYPE_BF16, x_row_stride, rows, hidden, p.q, p.qs, stream);
-  if (status != D3_OK) return status;
+  mx_quantize_operand(x, x_row_stride, rows, hidden, p.q, p.qs, s);
+  int status;
   const int32_t rows32 = static_cast<int32_t>(rows);
   if (p.scratch_ints > 0)
     status = d3_sort_routes_wide(ids, ids_dtype, rows32, nullptr, top_k, num_experts, kMxSortTile, p.counts, p.starts,
