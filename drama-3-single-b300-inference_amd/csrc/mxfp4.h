@@ -80,6 +80,32 @@ __device__ __forceinline__ uint32_t mx_codes8(const float* v, float inverse) {
   return inverse == 0.0f ? 0u : w;
 }
 
+// 2^(code - 127): a subnormal for code 0, NaN for 255.
+__device__ __forceinline__ float mx_scale(uint32_t code) {
+  return __uint_as_float(code == 255u ? 0x7fc00000u : (code ? code << 23 : 0x00400000u));
+}
+
+typedef uint16_t uint16x2 __attribute__((ext_vector_type(2)));
+
+// Largest magnitude of bf16 pairs as bf16 bits in each half.
+template <int N>
+__device__ __forceinline__ uint16x2 mx_amax_bf16(const uint32_t* w) {
+  uint16x2 amax = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i) amax = __builtin_elementwise_max(amax, __builtin_bit_cast(uint16x2, w[i] & 0x7fff7fffu));
+  return amax;
+}
+
+// mx_codes8 of four words of bf16 pairs: the conversion divides by the scale
+// itself (the same codes for every bf16 value and every scale, 2^-127
+// included: compared on the device).
+__device__ __forceinline__ uint32_t mx_codes8_bf16(const uint32_t* w, float scale) {
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(0u, __builtin_bit_cast(bf16x2, w[0]), scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[1]), scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[2]), scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
+}
+
 // Memory words at the alignment of their elements only: gfx950 takes wide
 // accesses at any address, so odd row strides cost no narrow path.
 struct __attribute__((packed, aligned(2))) MxWords4 { uint32_t w[4]; };

@@ -48,19 +48,23 @@ __global__ __launch_bounds__(kRowThreads) void quantize_kernel(const void* __res
 #pragma unroll
   for (int j = 0; j < kRowUnits; ++j) {
     const uint64_t u = first + static_cast<uint64_t>(j) * kRowThreads;
-    float v[8];
+    uint32_t code, word;
+    if constexpr (kF32) {
+      float v[8];
+      uint32_t amax = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (kF32)
+      for (int i = 0; i < 8; ++i) {
         v[i] = __uint_as_float(raw[j][i / 4].w[i % 4]);
-      else
-        v[i] = (i & 1) ? bf16_hi(raw[j][0].w[i / 2]) : bf16_lo(raw[j][0].w[i / 2]);
+        amax = MaxU32::apply(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+      }
+      code = mx_scale_code(quad_max(amax));
+      word = mx_codes8(v, mx_inverse(code));
+    } else {
+      const uint16x2 amax = mx_amax_bf16<4>(raw[j][0].w);
+      code = mx_scale_code(quad_max(MaxU32::apply(amax[0], amax[1])) << 16);
+      word = mx_codes8_bf16(raw[j][0].w, mx_scale(code));
+      if (code == 255u) word = 0;
     }
-    uint32_t amax = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) amax = MaxU32::apply(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-    const uint32_t code = mx_scale_code(quad_max(amax));
-    const uint32_t word = mx_codes8(v, mx_inverse(code));
     if (u >= units) continue;
     if constexpr (kOperand) {
       *reinterpret_cast<uint32_t*>(codes + row[j] * steps * kMxOperandCodes + 4 * static_cast<uint64_t>(unit[j])) = word;
@@ -90,8 +94,7 @@ __global__ __launch_bounds__(kRowThreads) void dequantize_kernel(const uint8_t* 
   for (int j = 0; j < kRowUnits; ++j) {
     const uint64_t u = first + static_cast<uint64_t>(j) * kRowThreads;
     if (u >= units) return;
-    // 2^(code - 127): a subnormal for code 0, NaN for 255.
-    const float scale = __uint_as_float(code[j] == 255u ? 0x7fc00000u : (code[j] ? code[j] << 23 : 0x00400000u));
+    const float scale = mx_scale(code[j]);
     float v[8];
     const floatx2_hw p0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[j], 1.0f, 0);
     const floatx2_hw p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[j], 1.0f, 1);

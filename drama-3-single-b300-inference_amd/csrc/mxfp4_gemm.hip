@@ -33,11 +33,19 @@ struct MxGemm {
   int steps;
   const uint8_t* a;  // quantised rows (operand layout, `steps` steps)
   const uint8_t* as;
+  const uint16_t* x;  // or the rows themselves, bf16 [rows][k], quantised by the wave that multiplies them
+  int64_t x_stride;
+  int k_blocks;       // k / 32
   const int4* items;  // {expert (-1: zero rows), first row, rows, -}; nullptr: one expert, `rows` in order
   const int32_t* num_items;
   int rows;
-  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxF32)
-  int top_k;
+  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxF32);
+  int top_k;              // nullptr: the identity
+  const void* ids;        // kMxPairs: expert of each (row, rank) pair
+  int ids_i64;
+  int experts;
+  const int32_t* bounds;  // kMxGroups: the groups' boundaries
+  int zero_rest;
   void* out;
   int64_t out_stride;  // elements (kMxAct: the row's width)
   uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout
@@ -119,7 +127,8 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4],
     if (group == 0) mx_operand_scale(g.out_scales + first * kMxOperandScales, rg, blocks, code);
   } else {
     if (!live) return;
-    float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride + kMxRows * rg + 4 * group;
+    float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride +
+                 kMxRows * rg + 4 * group;
 #pragma unroll
     for (int t = 0; t < 4; ++t) *reinterpret_cast<floatx4*>(out + 16 * t) = c[t];
   }
@@ -132,21 +141,39 @@ __device__ __forceinline__ void mx_zero_rows(const MxGemm& g, const int4& item, 
   }
 }
 
+// One lane's operand (one block of 32) of a bf16 row: no other lane's values
+// are needed for its scale.
+struct MxOperand {
+  int32x4 codes;
+  uint32_t scale;
+};
+__device__ __forceinline__ MxOperand mx_operand_bf16(const uint16_t* x) {
+  MxWords4 raw[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) raw[i] = reinterpret_cast<const MxWords4*>(x)[i];
+  const uint16x2 amax = mx_amax_bf16<16>(&raw[0].w[0]);
+  MxOperand op;
+  op.scale = mx_scale_code(MaxU32::apply(amax[0], amax[1]) << 16);
+  const float scale = mx_scale(op.scale);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) op.codes[i] = static_cast<int>(mx_codes8_bf16(raw[i].w, scale));
+  return op;
+}
+
+__device__ __forceinline__ int64_t mx_pair_expert(const MxGemm& g, int64_t pair) {
+  return g.ids_i64 ? static_cast<const int64_t*>(g.ids)[pair] : static_cast<const int32_t*>(g.ids)[pair];
+}
+
 // Few rows an item (up to 16 kRT): the weights stream from memory once, each
 // wave a share of the contraction.  A workgroup's four waves are kMxWaves /
 // kSplit row groups by kSplit interleaved slices of the steps; the slices'
-// fp32 sums meet in LDS and are added in slice order.
-template <int kRT, int kEpi, int kSplit>
-__global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blocks) {
+// fp32 sums meet in LDS (`part`) and are added in slice order.
+// kDirect: the rows are bf16 and every wave quantises the operands it
+// multiplies: about 50 vector instructions an operand against a launch of
+// its own, which pays up to two row tiles.
+template <int kRT, int kEpi, int kSplit, bool kDirect>
+__device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item, int block, floatx4* part) {
   constexpr int kGroups = kMxWaves / kSplit;
-  __shared__ floatx4 part[kSplit > 1 ? kMxWaves * kRT * 4 * kWave : 1];
-  const int index = blockIdx.x / blocks, block = blockIdx.x - index * blocks;
-  const int4 item = mx_item(g, index, 16 * kRT);
-  if (item.z <= 0) return;  // uniform
-  if (kEpi == kMxBf16 && item.x < 0) {
-    mx_zero_rows(g, item, block * kGroups * kMxRows, kGroups * kMxRows);
-    return;
-  }
   const int lane = lane_id(), row16 = lane & 15, group = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int slice = wave % kSplit;
@@ -160,9 +187,13 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt) {
     int64_t row = item.y + min(16 * rt + row16, count - 1);
-    if constexpr (kEpi == kMxAct) row = g.sorted[row] / g.top_k;
-    codes[rt] = g.a + row * g.steps * kMxOperandCodes + 16 * group;
-    scales[rt] = g.as + row * g.steps * kMxOperandScales + 2 * group;
+    if constexpr (kEpi == kMxAct) row = (g.sorted ? g.sorted[row] : static_cast<int>(row)) / g.top_k;
+    if constexpr (kDirect) {
+      codes[rt] = reinterpret_cast<const uint8_t*>(g.x + row * g.x_stride);
+    } else {
+      codes[rt] = g.a + row * g.steps * kMxOperandCodes + 16 * group;
+      scales[rt] = g.as + row * g.steps * kMxOperandScales + 2 * group;
+    }
   }
   const int64_t base = static_cast<int64_t>(item.x) * g.row_groups + rg_read;
   const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * g.steps * kMxStepCodes) + lane;
@@ -184,10 +215,21 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
     const uint2 wsc = ws[static_cast<int64_t>(step) * (kMxStepScales / 8)];
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
-      const uint32_t sb = *reinterpret_cast<const uint16_t*>(scales[rt] + kMxOperandScales * step);
-      const int32x4* b = reinterpret_cast<const int32x4*>(codes[rt] + kMxOperandCodes * step);
-      mfma_tiles<0>(wf[0], b[0], acc[rt], wsc.x, sb);
-      mfma_tiles<1>(wf[1], b[4], acc[rt], wsc.y, sb);
+      if constexpr (kDirect) {
+        // The padded half of the last step reads the first half again, at
+        // scale 2^-127 (the weights are zeros there).
+        const bool more = 8 * step + 4 < g.k_blocks;  // uniform
+        const uint16_t* x = reinterpret_cast<const uint16_t*>(codes[rt]) + kMxStep * step + kMxBlock * group;
+        const MxOperand lo = mx_operand_bf16(x);
+        MxOperand hi = mx_operand_bf16(more ? x + 4 * kMxBlock : x);
+        mfma_tiles<0>(wf[0], lo.codes, acc[rt], wsc.x, lo.scale);
+        mfma_tiles<0>(wf[1], hi.codes, acc[rt], wsc.y, more ? hi.scale : 0u);
+      } else {
+        const uint32_t sb = *reinterpret_cast<const uint16_t*>(scales[rt] + kMxOperandScales * step);
+        const int32x4* b = reinterpret_cast<const int32x4*>(codes[rt] + kMxOperandCodes * step);
+        mfma_tiles<0>(wf[0], b[0], acc[rt], wsc.x, sb);
+        mfma_tiles<1>(wf[1], b[4], acc[rt], wsc.y, sb);
+      }
     }
   }
 
@@ -217,6 +259,105 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
     for (int rt = 0; rt < kRT; ++rt)
       mx_store<kEpi>(g, acc[rt], rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
   }
+}
+
+// Where a streaming workgroup's rows come from.
+enum MxSource {
+  kMxList,   // the work items (or the rows in order)
+  kMxPairs,  // an item per (row, rank) pair: few pairs, no route sort
+  kMxGroups, // the groups of the boundaries, one or two row tiles at a time
+};
+
+template <int kRT, int kEpi, int kSplit, bool kDirect, int kSource>
+__global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blocks) {
+  constexpr int kGroups = kMxWaves / kSplit;
+  __shared__ floatx4 part[kSplit > 1 ? kMxWaves * kRT * 4 * kWave : 1];
+  const int index = blockIdx.x / blocks, block = blockIdx.x - index * blocks;
+  if constexpr (kSource == kMxGroups) {
+    static_assert(kEpi == kMxBf16 && kRT == 2, "groups: bf16 rows, up to two row tiles");
+    if (index == g.experts) {  // the rows of no group
+      if (!g.zero_rest) return;
+      const int first = min(max(g.bounds[0], 0), g.rows), last = min(max(g.bounds[g.experts], 0), g.rows);
+      mx_zero_rows(g, make_int4(-1, 0, first, 0), block * kGroups * kMxRows, kGroups * kMxRows);
+      mx_zero_rows(g, make_int4(-1, last, g.rows - last, 0), block * kGroups * kMxRows, kGroups * kMxRows);
+      return;
+    }
+    const int end = min(max(g.bounds[index + 1], 0), g.rows);
+    for (int at = min(max(g.bounds[index], 0), g.rows); at < end; at += 16 * kRT) {  // uniform
+      const int4 item = make_int4(index, at, min(16 * kRT, end - at), 0);
+      if (item.z > 16)
+        mx_stream_item<2, kEpi, kSplit, kDirect>(g, item, block, part);
+      else
+        mx_stream_item<1, kEpi, kSplit, kDirect>(g, item, block, part);
+      if (kSplit > 1) __syncthreads();  // `part` is read before the next tiles write it
+    }
+  } else {
+    int4 item;
+    if constexpr (kSource == kMxPairs) {
+      const int64_t expert = mx_pair_expert(g, index);
+      if (expert < 0 || expert >= g.experts) return;  // uniform
+      item = make_int4(static_cast<int>(expert), index, 1, 0);
+    } else {
+      item = mx_item(g, index, 16 * kRT);
+      if (item.z <= 0) return;  // uniform
+    }
+    if (kEpi == kMxBf16 && item.x < 0) {
+      mx_zero_rows(g, item, block * kGroups * kMxRows, kGroups * kMxRows);
+      return;
+    }
+    mx_stream_item<kRT, kEpi, kSplit, kDirect>(g, item, block, part);
+  }
+}
+
+// Down product and combine of few rows in one launch: a workgroup owns one
+// row and 64 outputs; its waves take the row's ranks in turn, each one row
+// group of its expert's matrix times the rank's activations, and the ranks'
+// fp32 results meet in LDS and are added in rank order.
+constexpr int kMxMaxTopK = 16;
+__global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, const void* __restrict__ weights,
+                                                                     int weights_f32) {
+  __shared__ float result[kMxMaxTopK][kMxRows];
+  const int row = blockIdx.x / g.row_groups, rg = blockIdx.x - row * g.row_groups;
+  const int lane = lane_id(), group = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  for (int r = wave; r < g.top_k; r += kMxWaves) {
+    const int64_t pair = static_cast<int64_t>(row) * g.top_k + r;
+    const int64_t expert = mx_pair_expert(g, pair);
+    if (expert < 0 || expert >= g.experts) continue;
+    // Every column of the MFMA's second operand is the pair's row; column 0 is kept.
+    const uint8_t* codes = g.a + pair * g.steps * kMxOperandCodes + 16 * group;
+    const uint8_t* scales = g.as + pair * g.steps * kMxOperandScales + 2 * group;
+    const int64_t base = expert * g.row_groups + rg;
+    const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * g.steps * kMxStepCodes) + lane;
+    const uint2* ws = reinterpret_cast<const uint2*>(g.ws + base * g.steps * kMxStepScales) + lane;
+    floatx4 acc[4] = {};
+    for (int step = 0; step < g.steps; ++step) {
+      int32x4 wf[2][4];
+      const int32x4* wp = w + static_cast<int64_t>(step) * (kMxStepCodes / 16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) wf[h][t] = wp[(4 * h + t) * kWave];
+      const uint2 wsc = ws[static_cast<int64_t>(step) * (kMxStepScales / 8)];
+      const uint32_t sb = *reinterpret_cast<const uint16_t*>(scales + kMxOperandScales * step);
+      const int32x4* b = reinterpret_cast<const int32x4*>(codes + kMxOperandCodes * step);
+      mfma_tiles<0>(wf[0], b[0], acc, wsc.x, sb);
+      mfma_tiles<1>(wf[1], b[4], acc, wsc.y, sb);
+    }
+    if ((lane & 15) == 0) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) *reinterpret_cast<floatx4*>(&result[r][16 * t + 4 * group]) = acc[t];
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x >= kMxRows) return;
+  float sum = 0.0f;
+  for (int r = 0; r < g.top_k; ++r) {
+    const int64_t pair = static_cast<int64_t>(row) * g.top_k + r;
+    const int64_t expert = mx_pair_expert(g, pair);
+    if (expert >= 0 && expert < g.experts) sum = fmaf(route_weight(weights, weights_f32, pair), result[r][threadIdx.x], sum);
+  }
+  static_cast<uint16_t*>(g.out)[static_cast<int64_t>(row) * g.out_stride + kMxRows * rg + threadIdx.x] = f32_to_bf16(sum);
 }
 
 // Contraction-sized items (up to 128 rows).  A workgroup owns (item, 256
@@ -463,29 +604,39 @@ bool mx_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintp
 
 int mx_ceil(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-template <int kRT, int kEpi>
+template <int kRT, int kEpi, bool kDirect, int kSource>
 void launch_stream(const MxGemm& g, int items, hipStream_t s) {
   // Slices of the contraction: as many as there are steps, up to the waves.
   const int split = g.steps >= 4 ? 4 : (g.steps >= 2 ? 2 : 1);
   const int blocks = mx_ceil(g.row_groups, kMxWaves / split);
   const dim3 grid(static_cast<unsigned>(items) * blocks), block(kMxThreads);
   if (split == 4)
-    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 4>), grid, block, 0, s, g, blocks);
+    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 4, kDirect, kSource>), grid, block, 0, s, g, blocks);
   else if (split == 2)
-    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 2>), grid, block, 0, s, g, blocks);
+    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 2, kDirect, kSource>), grid, block, 0, s, g, blocks);
   else
-    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 1>), grid, block, 0, s, g, blocks);
+    hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 1, kDirect, kSource>), grid, block, 0, s, g, blocks);
+}
+
+// Items of up to kMxDirectRows rows whose bf16 rows are at hand.
+constexpr int kMxDirectRows = 32;
+template <int kEpi>
+void launch_direct(const MxGemm& g, int item_rows, int items, hipStream_t s) {
+  if (item_rows <= 16)
+    launch_stream<1, kEpi, true, kMxList>(g, items, s);
+  else
+    launch_stream<2, kEpi, true, kMxList>(g, items, s);
 }
 
 template <int kEpi>
 void launch_gemm(const MxGemm& g, int item_rows, int items, hipStream_t s) {
   if (items <= 0) return;
   if (item_rows <= 16) {
-    launch_stream<1, kEpi>(g, items, s);
+    launch_stream<1, kEpi, false, kMxList>(g, items, s);
   } else if (item_rows <= 32) {
-    launch_stream<2, kEpi>(g, items, s);
+    launch_stream<2, kEpi, false, kMxList>(g, items, s);
   } else if (item_rows <= 64) {
-    launch_stream<4, kEpi>(g, items, s);
+    launch_stream<4, kEpi, false, kMxList>(g, items, s);
   } else {
     const MxTiles tiles{mx_ceil(g.row_groups, kMxWaves), 2};
     const int runs = mx_ceil(items, kMxXcds * tiles.run) * kMxXcds;
@@ -514,10 +665,17 @@ struct Arena {
 
 void set_weight(MxGemm& g, const uint8_t* w, const uint8_t* ws, int n, int k) {
   g.w = w, g.ws = ws, g.n = n;
-  g.row_groups = mx_ceil(n, kMxRows), g.steps = mx_ceil(k, kMxStep);
+  g.row_groups = mx_ceil(n, kMxRows), g.steps = mx_ceil(k, kMxStep), g.k_blocks = k / kMxBlock;
 }
 
+// A grouped product takes one of three ways:
+//   direct   one group of few rows, or few rows over many groups: one launch
+//            that quantises the rows itself and, with boundaries, walks each
+//            group's row tiles (no work items);
+//   else     quantised rows, work items from the boundaries, the product.
+constexpr int kMxWalkRows = 512;  // most rows of groups walked by their own workgroups: one busy group is walked alone
 struct GroupedPlan {
+  bool direct;
   int item_rows, max_items;
   uint8_t *q, *qs;
   int4* items;
@@ -525,9 +683,11 @@ struct GroupedPlan {
   int64_t bytes;
 };
 
-GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, int k) {
+GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, bool bounded, int k) {
   GroupedPlan p{};
   p.item_rows = mx_item_rows(rows, experts);
+  p.direct = bounded ? rows <= kMxWalkRows && rows <= 16 * static_cast<int64_t>(experts) : rows <= kMxDirectRows;
+  if (p.direct) return p;
   // every group, and each of the two runs of rows in none, adds one partial item at most
   p.max_items = static_cast<int>(rows / p.item_rows + (rows < experts + 2 ? rows : experts + 2));
   Arena a{static_cast<uint8_t*>(arena)};
@@ -541,7 +701,9 @@ GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, int k) {
 
 constexpr int kMxSortTile = 16;
 constexpr int kMxWidePairs = 8192;  // more (row, rank) pairs: the sort spread over many workgroups
+constexpr int kMxFewPairs = 64;    // up to so many pairs each is an item of its own
 struct MoePlan {
+  bool few, direct;  // few: no sort, down product and combine in one launch; direct: FC1 quantises its rows itself
   int item_rows, max_items, max_rows;
   int64_t pairs, scratch_ints;
   uint8_t *q, *qs, *act, *acts;
@@ -561,19 +723,26 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
   p.scratch_ints = p.pairs > kMxWidePairs ? d3_sort_wide_scratch_ints(static_cast<int32_t>(rows), top_k, experts) : 0;
   Arena a{static_cast<uint8_t*>(arena)};
   const int64_t x_steps = mx_ceil(hidden, kMxStep), act_steps = mx_ceil(inter, kMxStep);
-  p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
-  p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
+  p.few = p.pairs <= kMxFewPairs;
+  p.direct = p.few || p.item_rows <= kMxDirectRows;
+  if (p.few) p.max_rows = pairs;
   p.act = a.take<uint8_t>(p.max_rows * act_steps * kMxOperandCodes);
   p.acts = a.take<uint8_t>(p.max_rows * act_steps * kMxOperandScales);
-  p.down = a.take<float>(p.pairs * hidden);
-  p.counts = a.take<int32_t>(experts);
-  p.starts = a.take<int32_t>(experts);
-  p.total = a.take<int32_t>(1);
-  p.sorted = a.take<int32_t>(p.max_rows);
-  p.expert_ids = a.take<int32_t>(p.max_rows / kMxSortTile);
-  p.items = a.take<int4>(p.max_items);
-  p.num_items = a.take<int32_t>(1);
-  p.scratch = a.take<int32_t>(p.scratch_ints);
+  if (!p.direct) {
+    p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
+    p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
+  }
+  if (!p.few) {
+    p.down = a.take<float>(p.pairs * hidden);
+    p.counts = a.take<int32_t>(experts);
+    p.starts = a.take<int32_t>(experts);
+    p.total = a.take<int32_t>(1);
+    p.sorted = a.take<int32_t>(p.max_rows);
+    p.expert_ids = a.take<int32_t>(p.max_rows / kMxSortTile);
+    p.items = a.take<int4>(p.max_items);
+    p.num_items = a.take<int32_t>(1);
+    p.scratch = a.take<int32_t>(p.scratch_ints);
+  }
   p.bytes = a.used;
   return p;
 }
@@ -592,9 +761,9 @@ bool moe_shape(int64_t rows, int top_k, int experts, int hidden, int inter) {
 
 using namespace d3;
 
-extern "C" int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t k) {
+extern "C" int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bounded, int32_t k) {
   if (!grouped_shape(rows, num_experts, 1, k)) return -1;
-  return plan_grouped(nullptr, rows, num_experts, k).bytes;
+  return plan_grouped(nullptr, rows, num_experts, bounded != 0, k).bytes;
 }
 
 extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t rows, const int32_t* boundaries,
@@ -605,7 +774,7 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
   D3_REQUIRE(grouped_shape(rows, num_experts, n, k), "mxfp4_grouped: rows %lld, experts %d, N=%d",
              static_cast<long long>(rows), num_experts, n);
   D3_REQUIRE(boundaries != nullptr || num_experts == 1, "mxfp4_grouped: several experts need boundaries");
-  D3_REQUIRE(rows == 0 || (x && w && ws && out && workspace), "mxfp4_grouped: null pointer");
+  D3_REQUIRE(rows == 0 || (x && w && ws && out), "mxfp4_grouped: null pointer");
   D3_REQUIRE(rows <= 1 || (x_row_stride >= 0 && out_row_stride >= n), "mxfp4_grouped: row strides");
   D3_REQUIRE(mx_aligned(x, 2) && mx_aligned(w, 16) && mx_aligned(ws, 8) && mx_aligned(out, 2) && mx_aligned(workspace, 16),
              "mxfp4_grouped: alignment");
@@ -613,17 +782,26 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
     clear_error();
     return D3_OK;
   }
-  const GroupedPlan p = plan_grouped(workspace, rows, num_experts, k);
-  D3_REQUIRE(workspace_bytes >= p.bytes, "mxfp4_grouped: workspace of %lld bytes < required %lld",
-             static_cast<long long>(workspace_bytes), static_cast<long long>(p.bytes));
-  D3_SUPPORTED(static_cast<int64_t>(p.max_items) * mx_ceil(n, kMxRows) < (int64_t{1} << 31),
-               "mxfp4_grouped: more than 2^31 workgroups");
+  const GroupedPlan p = plan_grouped(workspace, rows, num_experts, boundaries != nullptr, k);
+  D3_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes),
+             "mxfp4_grouped: workspace of %lld bytes < required %lld", static_cast<long long>(workspace_bytes),
+             static_cast<long long>(p.bytes));
+  const int64_t most = p.direct ? num_experts + 1 : p.max_items;
+  D3_SUPPORTED(most * mx_ceil(n, kMxRows) < (int64_t{1} << 31), "mxfp4_grouped: more than 2^31 workgroups");
   hipStream_t s = as_stream(stream);
-  mx_quantize_operand(x, x_row_stride, rows, k, p.q, p.qs, s);
   MxGemm g{};
   set_weight(g, w, ws, n, k);
-  g.a = p.q, g.as = p.qs, g.rows = static_cast<int>(rows);
+  g.a = p.q, g.as = p.qs, g.x = x, g.x_stride = x_row_stride, g.rows = static_cast<int>(rows);
+  g.experts = num_experts, g.bounds = boundaries, g.zero_rest = zero_rest;
   g.out = out, g.out_stride = out_row_stride;
+  if (p.direct) {
+    if (boundaries != nullptr)
+      launch_stream<2, kMxBf16, true, kMxGroups>(g, num_experts + 1, s);
+    else
+      launch_direct<kMxBf16>(g, static_cast<int>(rows), 1, s);
+    D3_LAUNCHED("mxfp4_grouped");
+  }
+  mx_quantize_operand(x, x_row_stride, rows, k, p.q, p.qs, s);
   int items = mx_ceil(rows, p.item_rows);
   if (boundaries != nullptr) {
     hipLaunchKernelGGL(mx_items_kernel, dim3(1), dim3(kItemThreads), 0, s, boundaries, num_experts,
@@ -671,7 +849,24 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
                                                     mx_ceil(hidden, kMxRows)) < (int64_t{1} << 31),
                "mxfp4_moe: more than 2^31 workgroups");
   hipStream_t s = as_stream(stream);
-  mx_quantize_operand(x, x_row_stride, rows, hidden, p.q, p.qs, s);
+  const int i64 = ids_dtype == D3_DTYPE_I64, f32 = weights_dtype == D3_DTYPE_F32;
+  MxGemm up{}, down{};  // the two products
+  set_weight(up, w13, s13, 2 * intermediate, hidden);
+  up.x = x, up.x_stride = x_row_stride, up.a = p.q, up.as = p.qs;
+  up.out = p.act, up.out_stride = intermediate, up.out_scales = p.acts;
+  set_weight(down, w2, s2, hidden, intermediate);
+  down.a = p.act, down.as = p.acts, down.out_stride = hidden;
+  for (MxGemm* g : {&up, &down}) {
+    g->items = p.items, g->num_items = p.num_items, g->sorted = p.sorted, g->top_k = top_k;
+    g->ids = ids, g->ids_i64 = i64, g->experts = num_experts;
+  }
+  if (p.few) {
+    launch_stream<1, kMxAct, true, kMxPairs>(up, static_cast<int>(p.pairs), s);
+    down.out = out;
+    hipLaunchKernelGGL(mx_down_combine_kernel, dim3(static_cast<unsigned>(rows) * down.row_groups), dim3(kMxThreads), 0, s,
+                       down, weights, f32);
+    D3_LAUNCHED("mxfp4_moe");
+  }
   int status;
   const int32_t rows32 = static_cast<int32_t>(rows);
   if (p.scratch_ints > 0)
@@ -684,17 +879,16 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
                             p.sorted, p.expert_ids, p.max_rows, nullptr, p.item_rows, reinterpret_cast<int32_t*>(p.items),
                             p.max_items, p.num_items, nullptr, stream);
   if (status != D3_OK) return status;
-  MxGemm g{};
-  set_weight(g, w13, s13, 2 * intermediate, hidden);
-  g.a = p.q, g.as = p.qs, g.items = p.items, g.num_items = p.num_items, g.sorted = p.sorted, g.top_k = top_k;
-  g.out = p.act, g.out_stride = intermediate, g.out_scales = p.acts;
-  launch_gemm<kMxAct>(g, p.item_rows, p.max_items, s);
-  set_weight(g, w2, s2, hidden, intermediate);
-  g.a = p.act, g.as = p.acts, g.out = p.down, g.out_stride = hidden, g.out_scales = nullptr;
-  launch_gemm<kMxF32>(g, p.item_rows, p.max_items, s);
+  if (p.direct) {
+    launch_direct<kMxAct>(up, p.item_rows, p.max_items, s);
+  } else {
+    mx_quantize_operand(x, x_row_stride, rows, hidden, p.q, p.qs, s);
+    launch_gemm<kMxAct>(up, p.item_rows, p.max_items, s);
+  }
+  down.out = p.down;
+  launch_gemm<kMxF32>(down, p.item_rows, p.max_items, s);
   const int slices = mx_ceil(hidden, kMxCombineColumns);
   const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
-  const int i64 = ids_dtype == D3_DTYPE_I64, f32 = weights_dtype == D3_DTYPE_F32;
   if (top_k == 8)
     hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.down, ids, i64, weights, f32, top_k, num_experts, hidden,
                        slices, out);

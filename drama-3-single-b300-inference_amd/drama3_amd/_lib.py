@@ -114,7 +114,7 @@ SIGNATURES = {
     "d3_mxfp4_packed_bytes": (_i64, [_i32, _i32, _i32, _i32]),
     "d3_mxfp4_grouped": (
         _i32, [_p, _i64, _i64, _p, _i32, _p, _p, _i32, _i32, _p, _i64, _i32, _p, _i64, _p]),
-    "d3_mxfp4_grouped_workspace": (_i64, [_i64, _i32, _i32]),
+    "d3_mxfp4_grouped_workspace": (_i64, [_i64, _i32, _i32, _i32]),
     "d3_mxfp4_moe": (
         _i32, [_p, _i64, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p,
                _i64, _p]),
@@ -145,11 +145,14 @@ def load() -> ctypes.CDLL:
 def call(name: str, *args) -> None:
     """Call an entry point and map its status to the reference's exceptions:
     contract violations -> ValueError, HIP failures -> RuntimeError."""
-    lib = load()
-    status = getattr(lib, name)(*args)
-    if status == D3_OK:
-        return
-    message = lib.d3_last_error().decode(errors="replace")
+    status = getattr(load(), name)(*args)
+    if status != D3_OK:
+        fail(status)
+
+
+def fail(status: int) -> None:
+    """Raise the exception of an entry point's status (this thread's last call)."""
+    message = load().d3_last_error().decode(errors="replace")
     if status in (D3_ERR_INVALID_ARGUMENT, D3_ERR_UNSUPPORTED):
         raise ValueError(message)
     raise RuntimeError(message)

@@ -22,32 +22,59 @@ captured graph keeps its own workspace.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import call, ptr
-from .pipeline import dtype_code, require_cuda
+from ._lib import ptr
+from .pipeline import require_cuda
 
 BLOCK = 32  # elements per scale
 ORDER_ROWS, ORDER_GATE_UP, ORDER_DOWN = 0, 1, 2  # which product reads a packed weight
+_FLOAT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_INT = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
+
+
+# The current stream's handle without building a torch.cuda.Stream (1.7 us of
+# the 6 us a call of one launch costs the host).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _raw_stream is None:
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+
+@functools.cache
+def _entry(name: str):
+    return getattr(_lib.load(), name)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
-    """``call`` with the current stream of ``device`` appended, launched with
-    ``device`` current (a stream takes kernels of its own device only)."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, _lib.stream(device))
+    """``_lib.call`` with the current stream of ``device`` appended, launched
+    with ``device`` current (a stream takes kernels of its own device only)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = _entry(name)(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, _lib.stream(device))
+            status = _entry(name)(*args, _raw_stream(index))
+    if status:
+        _lib.fail(status)
 
 
-def _one_device(x: torch.Tensor, **others: torch.Tensor) -> None:
-    for name, t in others.items():
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, the rows on {x.device}")
+def _same_device(x: torch.Tensor, t: torch.Tensor, name: str) -> None:
+    if t.device != x.device:
+        raise ValueError(f"{name} is on {t.device}, the rows on {x.device}")
+
+
+def _workspace(size: int, x: torch.Tensor):
+    """(the tensor to hold on to, its address) of a call's workspace; sizes
+    below 1 need none, or are refused by the call itself."""
+    if size <= 0:
+        return None, None
+    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    return workspace, workspace.data_ptr()
 
 
 def _check_rows(x: torch.Tensor, dtypes=(torch.bfloat16,)) -> None:
@@ -65,19 +92,19 @@ def _check_codes(codes: torch.Tensor, scales: torch.Tensor) -> None:
     if (codes.dim() != scales.dim() or codes.shape[:-1] != scales.shape[:-1]
             or codes.shape[-1] * 2 != scales.shape[-1] * BLOCK):
         raise ValueError("codes [..., K / 2] and scales [..., K / 32] do not match")
-    _one_device(codes, scales=scales)
+    _same_device(codes, scales, "scales")
 
 
 def quantize_mxfp4(x: torch.Tensor):
     """bf16 or f32 rows [T, K] (K a multiple of 32, any row stride) ->
     ``(codes uint8 [T, K / 2], scales uint8 [T, K / 32])``."""
-    _check_rows(x, (torch.bfloat16, torch.float32))
+    _check_rows(x, _FLOAT)
     rows, width = x.shape
     if width == 0 or width % BLOCK:
         raise ValueError(f"row width {width} must be a multiple of {BLOCK}")
     codes = torch.empty((rows, width // 2), dtype=torch.uint8, device=x.device)
     scales = torch.empty((rows, width // BLOCK), dtype=torch.uint8, device=x.device)
-    _call(x.device, "d3_mxfp4_quantize", ptr(x), dtype_code(x.dtype), x.stride(0), rows, width,
+    _call(x.device, "d3_mxfp4_quantize", ptr(x), _FLOAT[x.dtype], x.stride(0), rows, width,
           ptr(codes), ptr(scales))
     return codes, scales
 
@@ -88,13 +115,13 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
     _check_codes(codes, scales)
     if codes.dim() != 2 or codes.shape[1] == 0:
         raise ValueError("codes must be [T, K / 2]")
-    if dtype not in (torch.bfloat16, torch.float32):
+    if dtype not in _FLOAT:
         raise TypeError("dtype must be bfloat16 or float32")
     codes, scales = codes.contiguous(), scales.contiguous()
     rows, width = len(codes), 2 * codes.shape[1]
     out = torch.empty((rows, width), dtype=dtype, device=codes.device)
     _call(codes.device, "d3_mxfp4_dequantize", ptr(codes), ptr(scales), rows, width, ptr(out),
-          dtype_code(dtype))
+          _FLOAT[dtype])
     return out
 
 
@@ -147,10 +174,10 @@ def _prepare(codes: torch.Tensor, scales: torch.Tensor, order: int) -> Mxfp4Weig
     codes, scales = codes.contiguous(), scales.contiguous()
     if codes.data_ptr() % 16:
         codes = codes.clone()
-    lib = _lib.load()
+    size = _entry("d3_mxfp4_packed_bytes")
     u8 = dict(dtype=torch.uint8, device=codes.device)
-    packed = torch.empty(lib.d3_mxfp4_packed_bytes(experts, n, k, 0), **u8)
-    packed_scales = torch.empty(lib.d3_mxfp4_packed_bytes(experts, n, k, 1), **u8)
+    packed = torch.empty(size(experts, n, k, 0), **u8)
+    packed_scales = torch.empty(size(experts, n, k, 1), **u8)
     _call(codes.device, "d3_mxfp4_pack", ptr(codes), ptr(scales), experts, n, k, order, ptr(packed),
           ptr(packed_scales))
     return Mxfp4Weight(packed, packed_scales, experts, n, k, order)
@@ -171,7 +198,7 @@ def prepare_mxfp4_experts(w13_codes, w13_scales, w2_codes, w2_scales) -> Mxfp4Ex
     experts, two_i, half_h = w13_codes.shape
     if w2_codes.shape != (experts, 2 * half_h, two_i // 4) or two_i % 256 or half_h % 64:
         raise ValueError("expert weights must be w13 [E, 2I, H], w2 [E, H, I], H and I multiples of 128")
-    _one_device(w13_codes, w2_codes=w2_codes)
+    _same_device(w13_codes, w2_codes, "w2_codes")
     return Mxfp4Experts(_prepare(w13_codes, w13_scales, ORDER_GATE_UP),
                         _prepare(w2_codes, w2_scales, ORDER_DOWN))
 
@@ -206,14 +233,14 @@ def _product(x, boundaries, weight: Mxfp4Weight, out, zero_rest: bool) -> torch.
     rows, k = x.shape
     if k != weight.k:
         raise ValueError(f"rows of width {k}, weight of K={weight.k}")
-    _one_device(x, weight=weight.codes)
+    _same_device(x, weight.codes, "weight")
     if out is None:
         out = torch.empty((rows, weight.n), dtype=torch.bfloat16, device=x.device)
-    size = _lib.load().d3_mxfp4_grouped_workspace(rows, weight.experts, k)
-    workspace = torch.empty(max(size, 0), dtype=torch.uint8, device=x.device)
+    size = _entry("d3_mxfp4_grouped_workspace")(rows, weight.experts, boundaries is not None, k)
+    workspace, at = _workspace(size, x)
     _call(x.device, "d3_mxfp4_grouped", ptr(x), x.stride(0), rows, ptr(boundaries), weight.experts,
           ptr(weight.codes), ptr(weight.scales), weight.n, k, ptr(out), out.stride(0),
-          int(zero_rest), ptr(workspace), size)
+          zero_rest, at, size)
     return out
 
 
@@ -240,14 +267,14 @@ def grouped_mxfp4(x: torch.Tensor, boundaries: torch.Tensor, weight: Mxfp4Weight
         raise TypeError("boundaries must be int32")
     if boundaries.shape != (weight.experts + 1,) or boundaries.stride(0) != 1:
         raise ValueError(f"boundaries must be contiguous [{weight.experts + 1}], one more than the experts")
-    _one_device(x, boundaries=boundaries)
+    _same_device(x, boundaries, "boundaries")
     if out is not None:
         if out.dtype != torch.bfloat16:
             raise TypeError("out must be bfloat16")
         if out.shape != (len(x), weight.n) or (weight.n > 1 and out.stride(1) != 1) or (
                 len(x) > 1 and out.stride(0) < weight.n):
             raise ValueError(f"out must be [{len(x)}, {weight.n}] with unit column stride")
-        _one_device(x, out=out)
+        _same_device(x, out, "out")
     return _product(x, boundaries, weight, out, out is None)
 
 
@@ -264,22 +291,24 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     require_cuda(topk_ids, topk_weights)
     if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape or len(topk_ids) != len(x):
         raise ValueError("topk_ids / topk_weights must be [T, k] for the T rows of x")
-    if topk_ids.dtype not in (torch.int32, torch.int64):
+    if topk_ids.dtype not in _INT:
         raise TypeError("topk_ids must be int32 or int64")
-    if topk_weights.dtype not in (torch.bfloat16, torch.float32):
+    if topk_weights.dtype not in _FLOAT:
         raise TypeError("topk_weights must be bfloat16 or float32")
     if x.shape[1] != experts.hidden:
         raise ValueError(f"rows of width {x.shape[1]}, experts of hidden size {experts.hidden}")
+    ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
     w13, w2 = experts.w13, experts.w2
     if w13.order != ORDER_GATE_UP or w2.order != ORDER_DOWN:
         raise ValueError("experts must come from prepare_mxfp4_experts")
-    _one_device(x, topk_ids=topk_ids, topk_weights=topk_weights, experts=w13.codes)
-    ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
+    _same_device(x, ids, "topk_ids")
+    _same_device(x, weights, "topk_weights")
+    _same_device(x, w13.codes, "experts")
     rows, top_k = ids.shape
     out = torch.empty((rows, experts.hidden), dtype=torch.bfloat16, device=x.device)
-    size = _lib.load().d3_mxfp4_moe_workspace(rows, top_k, w13.experts, w13.k, w2.k)
-    workspace = torch.empty(max(size, 0), dtype=torch.uint8, device=x.device)
-    _call(x.device, "d3_mxfp4_moe", ptr(x), x.stride(0), rows, ptr(ids), dtype_code(ids.dtype),
-          ptr(weights), dtype_code(weights.dtype), top_k, ptr(w13.codes), ptr(w13.scales),
-          ptr(w2.codes), ptr(w2.scales), w13.experts, w13.k, w2.k, ptr(out), ptr(workspace), size)
+    size = _entry("d3_mxfp4_moe_workspace")(rows, top_k, w13.experts, w13.k, w2.k)
+    workspace, at = _workspace(size, x)
+    _call(x.device, "d3_mxfp4_moe", ptr(x), x.stride(0), rows, ptr(ids), _INT[ids.dtype],
+          ptr(weights), _FLOAT[weights.dtype], top_k, ptr(w13.codes), ptr(w13.scales),
+          ptr(w2.codes), ptr(w2.scales), w13.experts, w13.k, w2.k, ptr(out), at, size)
     return out

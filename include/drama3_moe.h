@@ -818,8 +818,8 @@ int64_t d3_mxfp4_packed_bytes(int32_t num_experts, int32_t n, int32_t k, int32_t
  * rounding).  boundaries int32 [num_experts + 1] on the device, ascending,
  * clamped to [0, rows]; NULL with one expert: every row.  Rows of no group
  * are zeroed with zero_rest, else left as they were.  workspace: at least
- * d3_mxfp4_grouped_workspace bytes, 16-byte aligned, this call's alone until
- * it has run.
+ * d3_mxfp4_grouped_workspace bytes (NULL where that is 0), 16-byte aligned,
+ * this call's alone until it has run.
  */
 int d3_mxfp4_grouped(const uint16_t *x, int64_t x_row_stride, int64_t rows,
                      const int32_t *boundaries, int32_t num_experts, const uint8_t *w,
@@ -827,8 +827,9 @@ int d3_mxfp4_grouped(const uint16_t *x, int64_t x_row_stride, int64_t rows,
                      int64_t out_row_stride, int32_t zero_rest, void *workspace,
                      int64_t workspace_bytes, void *stream);
 
-/* Workspace bytes of d3_mxfp4_grouped (host-side arithmetic only; -1: not supported). */
-int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t k);
+/* Workspace bytes of d3_mxfp4_grouped (host-side arithmetic only; 0: none is
+ * needed; -1: not supported).  bounded: whether boundaries are given. */
+int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bounded, int32_t k);
 
 /*
  * Routed SwiGLU experts on MXFP4 weights: for every row t and rank r with

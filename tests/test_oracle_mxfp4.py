@@ -97,7 +97,8 @@ def test_c_entries_refuse_before_launching(lib):
     refused("null", "d3_mxfp4_grouped", grouped, a0=None)
     refused("row strides", "d3_mxfp4_grouped", grouped, a10=63)
     refused("alignment", "d3_mxfp4_grouped", grouped, a5=24)
-    refused("workspace of 100", "d3_mxfp4_grouped", grouped, a13=100)
+    refused("workspace of 100", "d3_mxfp4_grouped", grouped, a2=4000, a13=100)
+    refused("workspace of", "d3_mxfp4_grouped", grouped, a2=4000, a12=None)
     refused("experts 0", "d3_mxfp4_grouped", grouped, a4=0)
     refused("rows -1", "d3_mxfp4_grouped", grouped, a2=-1)
     moe = [16, 256, 40, 16, 3, 16, 0, 8, 16, 16, 16, 16, 16, 256, 128, 16, 16, 1 << 30, None]
@@ -112,7 +113,7 @@ def test_c_entries_refuse_before_launching(lib):
     refused("pairs", "d3_mxfp4_moe", moe, a2=1 << 24)
     lib_ = lib.load()
     assert lib_.d3_mxfp4_moe_workspace(4, 8, 513, 256, 128) == -1
-    assert lib_.d3_mxfp4_grouped_workspace(4, 8, 100) == -1
+    assert lib_.d3_mxfp4_grouped_workspace(4, 8, 1, 100) == -1
     assert lib_.d3_mxfp4_packed_bytes(0, 64, 256, 0) == -1
     # padded to whole row groups of 64 and steps of 256
     assert lib_.d3_mxfp4_packed_bytes(3, 65, 384, 0) == 3 * 128 * 512 // 2
