@@ -33,17 +33,18 @@ __host__ __device__ __forceinline__ int mx_weight_row(int order, int n, int rg, 
 }
 
 // Quantised rows as the products read them: codes in row order at a pitch of
-// whole steps, scales per step as byte 2 (block % 4) + (block / 4) of its 8
-// blocks, so that an MFMA lane (block % 4 is its group) finds the scales of
-// both halves of a step in one 16-bit word.  A row whose width is an odd
-// multiple of 128 has its last half step's scales zeroed here (the weights'
-// codes are zeros there, the row's are whatever the buffer holds: no e2m1 code
-// is an infinity or a NaN, but scale 255 would be).
+// whole steps, scales per step as byte 4 (block % 2) + block / 2 of its 8
+// blocks: a lane of the 32x32x64 MFMA (block % 2 is its half of the wave) finds
+// the scales of a step's four MFMAs in one word, one of the 16x16x128 MFMA
+// (block % 4 is its group) both of its scales in one word, two bytes apart.
+// A row whose width is an odd multiple of 128 has its last half step's scales
+// zeroed here (the weights' codes are zeros there, the row's are whatever the
+// buffer holds: no e2m1 code is an infinity or a NaN, but scale 255 would be).
 __device__ __forceinline__ void mx_operand_scale(uint8_t* row, uint32_t block, uint32_t blocks, uint32_t code) {
   const uint32_t step = block >> 3;
-  uint8_t* at = row + step * kMxOperandScales + 2 * (block & 3) + ((block >> 2) & 1);
+  uint8_t* at = row + step * kMxOperandScales + 4 * (block & 1) + ((block & 7) >> 1);
   *at = static_cast<uint8_t>(code);
-  if (8 * step + 4 >= blocks) at[1] = 0;  // the last step's second half is padding
+  if (8 * step + 4 >= blocks) at[2] = 0;  // the last step's second half is padding
 }
 
 // bf16 rows to that layout (width % 128 == 0).

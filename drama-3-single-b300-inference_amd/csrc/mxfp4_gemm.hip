@@ -77,6 +77,21 @@ __device__ __forceinline__ int4 mx_item(const MxGemm& g, int index, int item_row
   return g.items[index];
 }
 
+// Eight bf16 values at columns f .. of a row of n.
+__device__ __forceinline__ void mx_store_bf16(uint16_t* out, int f, int n, const MxWords4& v) {
+  if (f + 8 <= n) {
+    *reinterpret_cast<MxWords4*>(out + f) = v;
+    return;
+  }
+  uint64_t lo = v.w[0] | (static_cast<uint64_t>(v.w[1]) << 32), hi = v.w[2] | (static_cast<uint64_t>(v.w[3]) << 32);
+#pragma unroll 1
+  for (int i = f; i < n; ++i) {
+    out[i] = static_cast<uint16_t>(lo);
+    lo = (lo >> 16) | (hi << 48);
+    hi >>= 16;
+  }
+}
+
 // The four tiles of one row of `a` (this lane's row `row` of the item's list,
 // live or not) for row group rg.
 template <int kEpi>
@@ -88,19 +103,9 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4],
     for (int p = 0; p < 2; ++p) {
       const int f = kMxRows * rg + 32 * p + 8 * group;
       const floatx4 &lo = c[2 * p], &hi = c[2 * p + 1];
-      const MxWords4 v = {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
-                          pack_bf16x2(hi[2], hi[3])};
-      if (f + 8 <= g.n) {
-        *reinterpret_cast<MxWords4*>(out + f) = v;
-      } else {
-        uint64_t lo8 = v.w[0] | (static_cast<uint64_t>(v.w[1]) << 32), hi8 = v.w[2] | (static_cast<uint64_t>(v.w[3]) << 32);
-#pragma unroll 1
-        for (int i = f; i < g.n; ++i) {
-          out[i] = static_cast<uint16_t>(lo8);
-          lo8 = (lo8 >> 16) | (hi8 << 48);
-          hi8 >>= 16;
-        }
-      }
+      mx_store_bf16(out, f, g.n,
+                    {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
+                     pack_bf16x2(hi[2], hi[3])});
     }
   } else if constexpr (kEpi == kMxAct) {
     // Gate (tiles 0, 1) and up (tiles 2, 3) of columns 32 rg + 8 group + i;
@@ -192,7 +197,7 @@ __device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item
       codes[rt] = reinterpret_cast<const uint8_t*>(g.x + row * g.x_stride);
     } else {
       codes[rt] = g.a + row * g.steps * kMxOperandCodes + 16 * group;
-      scales[rt] = g.as + row * g.steps * kMxOperandScales + 2 * group;
+      scales[rt] = g.as + row * g.steps * kMxOperandScales + 4 * (group & 1);
     }
   }
   const int64_t base = static_cast<int64_t>(item.x) * g.row_groups + rg_read;
@@ -225,10 +230,11 @@ __device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item
         mfma_tiles<0>(wf[0], lo.codes, acc[rt], wsc.x, lo.scale);
         mfma_tiles<0>(wf[1], hi.codes, acc[rt], wsc.y, more ? hi.scale : 0u);
       } else {
-        const uint32_t sb = *reinterpret_cast<const uint16_t*>(scales[rt] + kMxOperandScales * step);
+        const uint32_t sb =
+            *reinterpret_cast<const uint32_t*>(scales[rt] + kMxOperandScales * step) >> (8 * (group >> 1));
         const int32x4* b = reinterpret_cast<const int32x4*>(codes[rt] + kMxOperandCodes * step);
         mfma_tiles<0>(wf[0], b[0], acc[rt], wsc.x, sb);
-        mfma_tiles<1>(wf[1], b[4], acc[rt], wsc.y, sb);
+        mfma_tiles<2>(wf[1], b[4], acc[rt], wsc.y, sb);
       }
     }
   }
@@ -326,7 +332,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
     if (expert < 0 || expert >= g.experts) continue;
     // Every column of the MFMA's second operand is the pair's row; column 0 is kept.
     const uint8_t* codes = g.a + pair * g.steps * kMxOperandCodes + 16 * group;
-    const uint8_t* scales = g.as + pair * g.steps * kMxOperandScales + 2 * group;
+    const uint8_t* scales = g.as + pair * g.steps * kMxOperandScales + 4 * (group & 1);
     const int64_t base = expert * g.row_groups + rg;
     const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * g.steps * kMxStepCodes) + lane;
     const uint2* ws = reinterpret_cast<const uint2*>(g.ws + base * g.steps * kMxStepScales) + lane;
@@ -339,10 +345,10 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
 #pragma unroll
         for (int t = 0; t < 4; ++t) wf[h][t] = wp[(4 * h + t) * kWave];
       const uint2 wsc = ws[static_cast<int64_t>(step) * (kMxStepScales / 8)];
-      const uint32_t sb = *reinterpret_cast<const uint16_t*>(scales + kMxOperandScales * step);
+      const uint32_t sb = *reinterpret_cast<const uint32_t*>(scales + kMxOperandScales * step) >> (8 * (group >> 1));
       const int32x4* b = reinterpret_cast<const int32x4*>(codes + kMxOperandCodes * step);
       mfma_tiles<0>(wf[0], b[0], acc, wsc.x, sb);
-      mfma_tiles<1>(wf[1], b[4], acc, wsc.y, sb);
+      mfma_tiles<2>(wf[1], b[4], acc, wsc.y, sb);
     }
     if ((lane & 15) == 0) {
 #pragma unroll
@@ -362,14 +368,16 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
 
 // Contraction-sized items (up to 128 rows).  A workgroup owns (item, 256
 // weight rows); each of its four waves one row group of 64 and every row of
-// the item, so that an operand read from LDS feeds four MFMAs and a weight
-// operand every row tile.  Weights go straight from memory into operands (the
-// packed layout is theirs); the item's quantised rows are staged through a
-// two-slot LDS ring in operand order ([row tile][half][lane][16 bytes]: each
-// ds_read_b128 of a wave is 1 KiB of consecutive memory), one step of 256
-// elements at a time, the next step's loads in flight while the current one
-// is multiplied.  An item is multiplied in the smallest of four bodies (2, 4,
-// 6, 8 row tiles) that holds it.
+// the item, on the 32x32x64 MFMA (measured in registers alone 8.6 PFLOP/s with
+// two waves a SIMD; the 16x16x128 one, whose operands are the same size for
+// half the products, 6.2).  Weights go straight from memory into operands:
+// the packed layout's 256-byte runs of 16 rows at one block serve both
+// shapes.  The item's quantised rows are staged through a two-slot LDS ring,
+// one step of 256 elements at a time: 128 bytes a row, its 16-byte part p at
+// p ^ (row % 8), so that neither the stores (eight lanes a row) nor the reads
+// (a lane a row) meet in a bank.  An item is multiplied in the smallest of
+// four bodies (1 to 4 tiles of 32 rows) that holds it.
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 constexpr int kMxTiledRows = 128;
 constexpr int kMxSlotCodes = kMxTiledRows * kMxOperandCodes;    // 16 KiB
 constexpr int kMxSlotScales = kMxTiledRows * kMxOperandScales;  // 1 KiB
@@ -380,15 +388,76 @@ struct MxTiles {
   int run;      // consecutive items whose tiles one XCD takes together
 };
 
+template <int SA, int SB>
+__device__ __forceinline__ floatx16 mfma_fp4_32(const int32x4& a, const int32x4& b, const floatx16& c, uint32_t sa,
+                                                uint32_t sb) {
+  const int32x8 av = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
+  const int32x8 bv = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, kMxLow, kMxLow, SA, static_cast<int>(sa), SB,
+                                                         static_cast<int>(sb));
+}
+
+// A row's 64 sums of row group rg in the 32x32 output layout: lane half hl
+// holds rows 8 j + 4 hl + i (element 4 j + i) of each 32-row half u of the
+// group; in the pair orders those are columns 16 (j % 2) + 8 hl + 4 (j / 2) + i.
+template <int kEpi>
+__device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[2], int rg, int row, bool live, int hl) {
+  if constexpr (kEpi == kMxBf16) {
+    if (!live) return;
+    uint16_t* out = static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.out_stride;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int f = kMxRows * rg + 32 * u + 16 * j + 8 * hl;
+        const floatx16& v = c[u];
+        mx_store_bf16(out, f, g.n,
+                      {pack_bf16x2(v[4 * j], v[4 * j + 1]), pack_bf16x2(v[4 * j + 2], v[4 * j + 3]),
+                       pack_bf16x2(v[4 * j + 8], v[4 * j + 9]), pack_bf16x2(v[4 * j + 10], v[4 * j + 11])});
+      }
+  } else if constexpr (kEpi == kMxAct) {
+    float gate[16], up[16], v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = 4 * (i / 8 + 2 * (i / 4 % 2)) + i % 4;  // columns 16 (i / 8) + 8 hl + i % 8
+      gate[i] = c[0][e];
+      up[i] = c[1][e];
+    }
+    swiglu_values<16>(gate, up, v);
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) amax = MaxU32::apply(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+    amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
+    const uint32_t code = mx_scale_code(amax);
+    const float inverse = mx_inverse(code);
+    const uint32_t lo = mx_codes8(v, inverse), hi = mx_codes8(v + 8, inverse);
+    if (!live) return;
+    const uint32_t blocks = static_cast<uint32_t>(g.out_stride) / kMxBlock;
+    const int64_t first = static_cast<int64_t>(row) * ((blocks + 7) / 8);  // in steps
+    uint8_t* codes = static_cast<uint8_t*>(g.out) + first * kMxOperandCodes + rg * (kMxBlock / 2) + 4 * hl;
+    *reinterpret_cast<uint32_t*>(codes) = lo;
+    *reinterpret_cast<uint32_t*>(codes + 8) = hi;
+    if (hl == 0) mx_operand_scale(g.out_scales + first * kMxOperandScales, rg, blocks, code);
+  } else {
+    if (!live) return;
+    float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride + kMxRows * rg + 4 * hl;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<floatx4*>(out + 32 * u + 8 * j) =
+            floatx4{c[u][4 * j], c[u][4 * j + 1], c[u][4 * j + 2], c[u][4 * j + 3]};
+  }
+}
+
 template <int kRT, int kEpi>
 __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t (*ring)[kMxSlotCodes],
                                               uint8_t (*ring_scales)[kMxSlotScales]) {
-  constexpr int kCopies = kRT / 2;  // 16-byte parts a thread stages per step
-  const int tid = threadIdx.x, lane = lane_id(), row16 = lane & 15, group = lane >> 4;
+  const int tid = threadIdx.x, lane = lane_id(), col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rg = n_tile * kMxWaves + wave;
   const int rg_read = min(rg, g.row_groups - 1);
-  const int count = min(item.z, 16 * kRT);
+  const int count = min(item.z, 32 * kRT);
   const int steps = g.steps;
 
   auto source_row = [&](int r) -> int64_t {  // rows past the item: its last row
@@ -396,64 +465,79 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
     if constexpr (kEpi == kMxAct) return g.sorted[at] / g.top_k;
     return at;
   };
-  // Wave w stages operands (row tile, half) w, w + 4, ..: a row tile's halves
-  // are consecutive, so copy i of this wave is row tile (w + 4 i) / 2.
-  const uint8_t* src[kCopies];
+  // A thread stages part lane % 8 of rows 32 i + 8 wave + lane / 8,
+  const int stage_row = 8 * wave + (lane >> 3), part = lane & 7;
+  const uint8_t* src[kRT];
 #pragma unroll
-  for (int i = 0; i < kCopies; ++i) {
-    const int unit = wave + kMxWaves * i;
-    src[i] = g.a + source_row(16 * (unit >> 1) + row16) * steps * kMxOperandCodes + 64 * (unit & 1) + 16 * group;
-  }
-  // and a thread four of the eight scales of row tid / 2.
+  for (int i = 0; i < kRT; ++i) src[i] = g.a + source_row(32 * i + stage_row) * steps * kMxOperandCodes + 16 * part;
+  const int stage_at = stage_row * kMxOperandCodes + 16 * (part ^ (stage_row & 7));
+  // and four of the eight scales of row tid / 2.
   const uint8_t* scale_src = g.as + source_row(tid >> 1) * steps * kMxOperandScales + 4 * (tid & 1);
 
+  // Weight operand (half u, slice q) of a step: row 32 u + col, block 2 q + hl,
+  // which is tile 2 u + col / 16, half q / 2, group 2 (q % 2) + hl of the
+  // packed layout; its scale is byte 2 u of `wsc[q]` once that lane's odd tiles
+  // are shifted down.
   const int64_t base = (static_cast<int64_t>(item.x) * g.row_groups + rg_read) * steps;
-  const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * kMxStepCodes) + lane;
-  const uint32_t* ws = reinterpret_cast<const uint32_t*>(g.ws + base * kMxStepScales) + 2 * lane;
+  const uint8_t* w = g.w + base * kMxStepCodes + (col >> 4) * 1024 + hl * 256 + (col & 15) * 16;
+  const uint8_t* ws = g.ws + base * kMxStepScales + (hl * 16 + (col & 15)) * 8;
+  const int odd = 8 * (col >> 4);
 
-  int32x4 wf[2][4], copy[kCopies];
-  uint32_t wsc[2];
+  int32x4 wf[4][2], copy[kRT];
+  uint2 wraw[2];
   uint32_t copy_scale;
-  auto load_weights = [&](int step, auto half) {
-    constexpr int kHalf = decltype(half)::value;
-    const int32x4* wp = w + static_cast<int64_t>(step) * (kMxStepCodes / 16) + kHalf * 4 * kWave;
+  auto load_weights = [&](int step, auto slice) {
+    constexpr int q = decltype(slice)::value;
+    const uint8_t* wp = w + static_cast<int64_t>(step) * kMxStepCodes + (q / 2) * 4096 + (q % 2) * 512;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) wf[kHalf][t] = wp[t * kWave];
-    wsc[kHalf] = ws[static_cast<int64_t>(step) * (kMxStepScales / 4) + kHalf];
+    for (int u = 0; u < 2; ++u) wf[q][u] = *reinterpret_cast<const int32x4*>(wp + 2048 * u);
+  };
+  auto load_scales = [&](int step) {
+    const uint8_t* wp = ws + static_cast<int64_t>(step) * kMxStepScales;
+    wraw[0] = *reinterpret_cast<const uint2*>(wp);
+    wraw[1] = *reinterpret_cast<const uint2*>(wp + 256);
   };
   auto load_rows = [&](int step) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) copy[i] = *reinterpret_cast<const int32x4*>(src[i] + step * kMxOperandCodes);
+    for (int i = 0; i < kRT; ++i) copy[i] = *reinterpret_cast<const int32x4*>(src[i] + step * kMxOperandCodes);
     copy_scale = *reinterpret_cast<const uint32_t*>(scale_src + step * kMxOperandScales);
   };
   auto store_rows = [&](int slot) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i)
-      *reinterpret_cast<int32x4*>(&ring[slot][((wave + kMxWaves * i) * kWave + lane) * 16]) = copy[i];
+    for (int i = 0; i < kRT; ++i)
+      *reinterpret_cast<int32x4*>(&ring[slot][stage_at + 32 * i * kMxOperandCodes]) = copy[i];
     *reinterpret_cast<uint32_t*>(&ring_scales[slot][tid * 4]) = copy_scale;
   };
 
-  floatx4 acc[kRT][4];
+  floatx16 acc[kRT][2];
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) acc[rt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[rt][u][i] = 0.0f;
 
-  uint32_t sb[kRT];
-  auto multiply = [&](int slot, auto half) {
-    constexpr int kHalf = decltype(half)::value;
+  uint32_t sb[kRT], wsc[4];
+  auto multiply = [&](int slot, auto slice) {
+    constexpr int q = decltype(slice)::value;
+    if constexpr (q == 0) {
+      wsc[0] = wraw[0].x >> odd, wsc[1] = wraw[1].x >> odd, wsc[2] = wraw[0].y >> odd, wsc[3] = wraw[1].y >> odd;
+    }
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
-      if constexpr (kHalf == 0)
-        sb[rt] = *reinterpret_cast<const uint16_t*>(&ring_scales[slot][(16 * rt + row16) * kMxOperandScales + 2 * group]);
-      const int32x4 b = *reinterpret_cast<const int32x4*>(&ring[slot][((2 * rt + kHalf) * kWave + lane) * 16]);
-      mfma_tiles<kHalf>(wf[kHalf], b, acc[rt], wsc[kHalf], sb[rt]);
+      const int row = 32 * rt + col;
+      if constexpr (q == 0)
+        sb[rt] = *reinterpret_cast<const uint32_t*>(&ring_scales[slot][row * kMxOperandScales + 4 * hl]);
+      const int32x4 b =
+          *reinterpret_cast<const int32x4*>(&ring[slot][row * kMxOperandCodes + 16 * ((2 * q + hl) ^ (row & 7))]);
+      acc[rt][0] = mfma_fp4_32<0, q>(wf[q][0], b, acc[rt][0], wsc[q], sb[rt]);
+      acc[rt][1] = mfma_fp4_32<2, q>(wf[q][1], b, acc[rt][1], wsc[q], sb[rt]);
     }
   };
-  // Issue order of a half step: operand reads two row tiles ahead of their
-  // MFMAs (all at once they would take registers that the sums leave no room
-  // for), the half's loads from memory among the first MFMAs; nothing moves
-  // into another half.
+  // Issue order of a slice: operand reads one row tile ahead of their MFMAs,
+  // the slice's loads from memory among them; nothing moves into another
+  // slice (a step's operand reads all at once would take registers that the
+  // sums leave no room for).
   auto issue_order = [&](auto reads, auto loads) {
     constexpr int kReads = decltype(reads)::value, kLoads = decltype(loads)::value;
     constexpr int kVmem = 0x020, kMfma = 0x008, kDsRead = 0x100, kAhead = kRT < 2 ? kRT : 2;
@@ -461,38 +545,51 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
       __builtin_amdgcn_sched_group_barrier(kVmem, (kLoads + kRT - 1) / kRT, 0);
-      __builtin_amdgcn_sched_group_barrier(kMfma, 4, 0);
+      __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
       __builtin_amdgcn_sched_group_barrier(kDsRead, kReads, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
   };
-  using Half0 = std::integral_constant<int, 0>;
-  using Half1 = std::integral_constant<int, 1>;
+  using Q0 = std::integral_constant<int, 0>;
+  using Q1 = std::integral_constant<int, 1>;
+  using Q2 = std::integral_constant<int, 2>;
+  using Q3 = std::integral_constant<int, 3>;
   // Step s is multiplied from slot s % 2 while step s + 1 loads: its rows
-  // first (their store to LDS then waits for no weights), each half's weights
-  // into the registers that half leaves.  The rows go to the slot that step
+  // first (their store to LDS then waits for no weights), each slice's weights
+  // into the registers that slice leaves.  The rows go to the slot that step
   // s - 1 used, which every wave left before the last barrier.
   load_rows(0);
-  load_weights(0, Half0{});
-  load_weights(0, Half1{});
+  load_scales(0);
+  load_weights(0, Q0{});
+  load_weights(0, Q1{});
+  load_weights(0, Q2{});
+  load_weights(0, Q3{});
   store_rows(0);
   lds_barrier();
   for (int step = 0; step < steps; ++step) {
     const int next = min(step + 1, steps - 1);  // the last step loads its own operands again, for nobody
+    const int slot = step & 1;
     load_rows(next);
-    multiply(step & 1, Half0{});
-    issue_order(std::integral_constant<int, 2>{}, std::integral_constant<int, kCopies + 1>{});
-    load_weights(next, Half0{});
-    multiply(step & 1, Half1{});
-    issue_order(std::integral_constant<int, 1>{}, std::integral_constant<int, 5>{});
-    load_weights(next, Half1{});
-    store_rows((step & 1) ^ 1);
+    multiply(slot, Q0{});
+    issue_order(std::integral_constant<int, 2>{}, std::integral_constant<int, kRT + 1>{});
+    load_scales(next);
+    load_weights(next, Q0{});
+    multiply(slot, Q1{});
+    issue_order(Q1{}, std::integral_constant<int, 4>{});
+    load_weights(next, Q1{});
+    multiply(slot, Q2{});
+    issue_order(Q1{}, Q2{});
+    load_weights(next, Q2{});
+    multiply(slot, Q3{});
+    issue_order(Q1{}, Q2{});
+    load_weights(next, Q3{});
+    store_rows(slot ^ 1);
     lds_barrier();
   }
   if (rg >= g.row_groups) return;
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt)
-    mx_store<kEpi>(g, acc[rt], rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
+    mx_store32<kEpi>(g, acc[rt], rg, item.y + 32 * rt + col, 32 * rt + col < count, hl);
 }
 
 template <int kEpi>
@@ -515,13 +612,13 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
     return;
   }
   if (item.z > 96)
-    mx_tiled_body<8, kEpi>(g, item, n_tile, ring, ring_scales);
-  else if (item.z > 64)
-    mx_tiled_body<6, kEpi>(g, item, n_tile, ring, ring_scales);
-  else if (item.z > 32)
     mx_tiled_body<4, kEpi>(g, item, n_tile, ring, ring_scales);
-  else
+  else if (item.z > 64)
+    mx_tiled_body<3, kEpi>(g, item, n_tile, ring, ring_scales);
+  else if (item.z > 32)
     mx_tiled_body<2, kEpi>(g, item, n_tile, ring, ring_scales);
+  else
+    mx_tiled_body<1, kEpi>(g, item, n_tile, ring, ring_scales);
 }
 
 // Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
