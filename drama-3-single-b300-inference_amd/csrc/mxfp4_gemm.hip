@@ -9,6 +9,7 @@
 // the first operand: an output lane holds one row of a and four consecutive
 // weight rows of each 16-row tile, as the packed row orders place them.
 #include <type_traits>
+#include <utility>
 
 #include "mxfp4.h"
 #include "status.h"
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
 // two waves a SIMD; the 16x16x128 one, whose operands are the same size for
 // half the products, 6.2).  Weights go straight from memory into operands:
 // the packed layout's 256-byte runs of 16 rows at one block serve both
-// shapes.  The item's quantised rows are staged through a two-slot LDS ring,
+// shapes.  The item's quantised rows are staged through a three-slot LDS ring,
 // one step of 256 elements at a time: 128 bytes a row, its 16-byte part p at
 // p ^ (row % 8), so that neither the stores (eight lanes a row) nor the reads
 // (a lane a row) meet in a bank.  An item is multiplied in the smallest of
@@ -380,8 +381,18 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 constexpr int kMxTiledRows = 128;
 constexpr int kMxSlotCodes = kMxTiledRows * kMxOperandCodes;    // 16 KiB
-constexpr int kMxSlotScales = kMxTiledRows * kMxOperandScales;  // 1 KiB
+constexpr int kMxSlot = kMxSlotCodes + kMxTiledRows * kMxOperandScales;  // and 1 KiB of scales
 constexpr int kMxXcds = 8;
+
+// f(integral_constant 0), .., f(integral_constant N - 1).
+template <class F, int... I>
+__device__ __forceinline__ void mx_each_of(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void mx_each(F&& f) {
+  mx_each_of(f, std::make_integer_sequence<int, N>{});
+}
 
 struct MxTiles {
   int n_tiles;  // 256-row weight tiles
@@ -451,8 +462,7 @@ __device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[
 }
 
 template <int kRT, int kEpi>
-__device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t (*ring)[kMxSlotCodes],
-                                              uint8_t (*ring_scales)[kMxSlotScales]) {
+__device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t* ring) {
   const int tid = threadIdx.x, lane = lane_id(), col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rg = n_tile * kMxWaves + wave;
@@ -479,34 +489,46 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   // packed layout; its scale is byte 2 u of `wsc[q]` once that lane's odd tiles
   // are shifted down.
   const int64_t base = (static_cast<int64_t>(item.x) * g.row_groups + rg_read) * steps;
-  const uint8_t* w = g.w + base * kMxStepCodes + (col >> 4) * 1024 + hl * 256 + (col & 15) * 16;
-  const uint8_t* ws = g.ws + base * kMxStepScales + (hl * 16 + (col & 15)) * 8;
+  const __amdgpu_buffer_rsrc_t w = BufferView(g.w + base * kMxStepCodes, steps * kMxStepCodes).rsrc;
+  const __amdgpu_buffer_rsrc_t ws = BufferView(g.ws + base * kMxStepScales, steps * kMxStepScales).rsrc;
+  const int w_lane = (col >> 4) * 1024 + hl * 256 + (col & 15) * 16;
+  const int ws_lane = (hl * 16 + (col & 15)) * 8;
   const int odd = 8 * (col >> 4);
 
-  int32x4 wf[4][2], copy[kRT];
-  uint2 wraw[2];
-  uint32_t copy_scale;
-  auto load_weights = [&](int step, auto slice) {
-    constexpr int q = decltype(slice)::value;
-    const uint8_t* wp = w + static_cast<int64_t>(step) * kMxStepCodes + (q / 2) * 4096 + (q % 2) * 512;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) wf[q][u] = *reinterpret_cast<const int32x4*>(wp + 2048 * u);
+  int32x4 wf[4][2], copy[kRT], operand[4];
+  floatx2_hw wraw[2];
+  uint32_t copy_scale, sb[kRT], sb_next[kRT], wsc[4];
+  auto load_weight = [&](int step, auto slice, auto half) {  // past the last step: zeros, nothing read
+    constexpr int q = decltype(slice)::value, u = decltype(half)::value;
+    wf[q][u] = __builtin_amdgcn_raw_buffer_load_b128(w, w_lane + (q / 2) * 4096 + (q % 2) * 512 + 2048 * u,
+                                                     step * kMxStepCodes, 0);
   };
-  auto load_scales = [&](int step) {
-    const uint8_t* wp = ws + static_cast<int64_t>(step) * kMxStepScales;
-    wraw[0] = *reinterpret_cast<const uint2*>(wp);
-    wraw[1] = *reinterpret_cast<const uint2*>(wp + 256);
+  auto load_scales = [&](int step, auto part) {
+    constexpr int i = decltype(part)::value;
+    wraw[i] = __builtin_bit_cast(floatx2_hw, __builtin_amdgcn_raw_buffer_load_b64(ws, ws_lane + 256 * i,
+                                                                                  step * kMxStepScales, 0));
   };
-  auto load_rows = [&](int step) {
-#pragma unroll
-    for (int i = 0; i < kRT; ++i) copy[i] = *reinterpret_cast<const int32x4*>(src[i] + step * kMxOperandCodes);
-    copy_scale = *reinterpret_cast<const uint32_t*>(scale_src + step * kMxOperandScales);
+  auto load_row = [&](int step, auto copies) {
+    constexpr int i = decltype(copies)::value;
+    const int at = min(step, steps - 1);
+    if constexpr (i < kRT)
+      copy[i] = *reinterpret_cast<const int32x4*>(src[i] + at * kMxOperandCodes);
+    else
+      copy_scale = *reinterpret_cast<const uint32_t*>(scale_src + at * kMxOperandScales);
   };
-  auto store_rows = [&](int slot) {
+  auto store_rows = [&](uint8_t* slot) {
 #pragma unroll
-    for (int i = 0; i < kRT; ++i)
-      *reinterpret_cast<int32x4*>(&ring[slot][stage_at + 32 * i * kMxOperandCodes]) = copy[i];
-    *reinterpret_cast<uint32_t*>(&ring_scales[slot][tid * 4]) = copy_scale;
+    for (int i = 0; i < kRT; ++i) *reinterpret_cast<int32x4*>(slot + stage_at + 32 * i * kMxOperandCodes) = copy[i];
+    *reinterpret_cast<uint32_t*>(slot + kMxSlotCodes + tid * 4) = copy_scale;
+  };
+  auto read_operand = [&](const uint8_t* slot, auto unit) {
+    constexpr int i = decltype(unit)::value, q = i / kRT, rt = i % kRT;
+    operand[i % 4] = *reinterpret_cast<const int32x4*>(slot + (32 * rt + col) * kMxOperandCodes +
+                                                       16 * ((2 * q + hl) ^ (col & 7)));
+  };
+  auto read_scale = [&](const uint8_t* slot, auto tile) {
+    constexpr int rt = decltype(tile)::value;
+    sb_next[rt] = *reinterpret_cast<const uint32_t*>(slot + kMxSlotCodes + (32 * rt + col) * kMxOperandScales + 4 * hl);
   };
 
   floatx16 acc[kRT][2];
@@ -517,74 +539,71 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[rt][u][i] = 0.0f;
 
-  uint32_t sb[kRT], wsc[4];
-  auto multiply = [&](int slot, auto slice) {
-    constexpr int q = decltype(slice)::value;
-    if constexpr (q == 0) {
-      wsc[0] = wraw[0].x >> odd, wsc[1] = wraw[1].x >> odd, wsc[2] = wraw[0].y >> odd, wsc[3] = wraw[1].y >> odd;
-    }
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      const int row = 32 * rt + col;
-      if constexpr (q == 0)
-        sb[rt] = *reinterpret_cast<const uint32_t*>(&ring_scales[slot][row * kMxOperandScales + 4 * hl]);
-      const int32x4 b =
-          *reinterpret_cast<const int32x4*>(&ring[slot][row * kMxOperandCodes + 16 * ((2 * q + hl) ^ (row & 7))]);
-      acc[rt][0] = mfma_fp4_32<0, q>(wf[q][0], b, acc[rt][0], wsc[q], sb[rt]);
-      acc[rt][1] = mfma_fp4_32<2, q>(wf[q][1], b, acc[rt][1], wsc[q], sb[rt]);
-    }
-  };
-  // Issue order of a slice: operand reads one row tile ahead of their MFMAs,
-  // the slice's loads from memory among them; nothing moves into another
-  // slice (a step's operand reads all at once would take registers that the
-  // sums leave no room for).
-  auto issue_order = [&](auto reads, auto loads) {
-    constexpr int kReads = decltype(reads)::value, kLoads = decltype(loads)::value;
-    constexpr int kVmem = 0x020, kMfma = 0x008, kDsRead = 0x100, kAhead = kRT < 2 ? kRT : 2;
-    __builtin_amdgcn_sched_group_barrier(kDsRead, kAhead * kReads, 0);
-#pragma unroll
-    for (int rt = 0; rt < kRT; ++rt) {
-      __builtin_amdgcn_sched_group_barrier(kVmem, (kLoads + kRT - 1) / kRT, 0);
-      __builtin_amdgcn_sched_group_barrier(kMfma, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(kDsRead, kReads, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  using Q0 = std::integral_constant<int, 0>;
-  using Q1 = std::integral_constant<int, 1>;
-  using Q2 = std::integral_constant<int, 2>;
-  using Q3 = std::integral_constant<int, 3>;
-  // Step s is multiplied from slot s % 2 while step s + 1 loads: its rows
-  // first (their store to LDS then waits for no weights), each slice's weights
-  // into the registers that slice leaves.  The rows go to the slot that step
-  // s - 1 used, which every wave left before the last barrier.
-  load_rows(0);
-  load_scales(0);
-  load_weights(0, Q0{});
-  load_weights(0, Q1{});
-  load_weights(0, Q2{});
-  load_weights(0, Q3{});
-  store_rows(0);
+  // A step is 4 kRT units (slice, row tile) of one operand read and two
+  // MFMAs, in this order and not the compiler's: the reads run kAhead units
+  // ahead, across slices and into the next step; one load from memory goes
+  // with each unit, a slice's weights once its registers are free, so that
+  // loads that wait to be issued have MFMAs in flight before them.  Rows pass
+  // through three slots: step s reads slot s % 3 and, in its last units, slot
+  // (s + 1) % 3, which was stored in step s - 1 before the barrier in the
+  // middle of step s; after that barrier nobody reads slot (s + 2) % 3, where
+  // the rows of step s + 2 go, loaded since the middle of step s - 1.
+  // (The barrier lies before the first read of the next slot.)
+  constexpr int kUnits = 4 * kRT, kAhead = 3;
+  constexpr int kBarrier = kUnits / 2 <= kUnits - kAhead ? kUnits / 2 : kUnits - kAhead;
+  using std::integral_constant;
+  mx_each<kRT + 1>([&](auto i) { load_row(0, i); });
+  mx_each<2>([&](auto i) { load_scales(0, i); });
+  mx_each<3>([&](auto q) {
+    load_weight(0, q, integral_constant<int, 0>{});
+    load_weight(0, q, integral_constant<int, 1>{});
+  });
+  store_rows(ring);
+  mx_each<kRT + 1>([&](auto i) { load_row(1, i); });
+  store_rows(ring + kMxSlot);
+  mx_each<kRT + 1>([&](auto i) { load_row(2, i); });
   lds_barrier();
+  mx_each<kAhead>([&](auto i) { read_operand(ring, i); });
+  mx_each<kRT>([&](auto i) { read_scale(ring, i); });
+  const uint8_t* slot = ring;
+  const uint8_t* slot_next = ring + kMxSlot;
+  uint8_t* slot_free = ring + 2 * kMxSlot;
   for (int step = 0; step < steps; ++step) {
-    const int next = min(step + 1, steps - 1);  // the last step loads its own operands again, for nobody
-    const int slot = step & 1;
-    load_rows(next);
-    multiply(slot, Q0{});
-    issue_order(std::integral_constant<int, 2>{}, std::integral_constant<int, kRT + 1>{});
-    load_scales(next);
-    load_weights(next, Q0{});
-    multiply(slot, Q1{});
-    issue_order(Q1{}, std::integral_constant<int, 4>{});
-    load_weights(next, Q1{});
-    multiply(slot, Q2{});
-    issue_order(Q1{}, Q2{});
-    load_weights(next, Q2{});
-    multiply(slot, Q3{});
-    issue_order(Q1{}, Q2{});
-    load_weights(next, Q3{});
-    store_rows(slot ^ 1);
-    lds_barrier();
+    wsc[0] = __float_as_uint(wraw[0][0]) >> odd, wsc[1] = __float_as_uint(wraw[1][0]) >> odd;
+    wsc[2] = __float_as_uint(wraw[0][1]) >> odd, wsc[3] = __float_as_uint(wraw[1][1]) >> odd;
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt) sb[rt] = sb_next[rt];
+    mx_each<kUnits>([&](auto unit) {
+      constexpr int i = decltype(unit)::value, q = i / kRT, rt = i % kRT;
+      if constexpr (i == kBarrier) {
+        lds_barrier();
+        store_rows(slot_free);
+      }
+      if constexpr (i + kAhead < kUnits)
+        read_operand(slot, integral_constant<int, i + kAhead>{});
+      else
+        read_operand(slot_next, integral_constant<int, i + kAhead - kUnits>{});
+      if constexpr (q == 2) read_scale(slot_next, integral_constant<int, rt>{});
+      // this step's slice 3, then the next step's slices 0 to 2 as they end
+      constexpr int kSlice = (q + 3) % 4;
+      const int of = q == 0 ? step : step + 1;
+      if constexpr (rt == 0) load_weight(of, integral_constant<int, kSlice>{}, integral_constant<int, 0>{});
+      if constexpr (rt == (kRT > 1 ? 1 : 0))
+        load_weight(of, integral_constant<int, kSlice>{}, integral_constant<int, 1>{});
+      if constexpr (q == 1 && rt == kRT - 1) {
+        load_scales(step + 1, integral_constant<int, 0>{});
+        load_scales(step + 1, integral_constant<int, 1>{});
+      }
+      if constexpr (q == 2 && rt == kRT - 1) load_row(step + 3, integral_constant<int, kRT>{});
+      if constexpr (q == 3) load_row(step + 3, integral_constant<int, rt>{});
+      acc[rt][0] = mfma_fp4_32<0, q>(wf[q][0], operand[i % 4], acc[rt][0], wsc[q], sb[rt]);
+      acc[rt][1] = mfma_fp4_32<2, q>(wf[q][1], operand[i % 4], acc[rt][1], wsc[q], sb[rt]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    const uint8_t* done = slot;
+    slot = slot_next;
+    slot_next = slot_free;
+    slot_free = const_cast<uint8_t*>(done);
   }
   if (rg >= g.row_groups) return;
 #pragma unroll
@@ -595,8 +614,7 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
 template <int kEpi>
 __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2))) void mx_tiled_kernel(MxGemm g,
                                                                                                       MxTiles tiles) {
-  __shared__ __attribute__((aligned(16))) uint8_t ring[2][kMxSlotCodes];
-  __shared__ __attribute__((aligned(16))) uint8_t ring_scales[2][kMxSlotScales];
+  __shared__ __attribute__((aligned(16))) uint8_t ring[3 * kMxSlot];
   // Runs of consecutive items go to the XCDs in turn (workgroup b runs on XCD
   // b % 8): a run's tiles share its rows, and an expert's consecutive items
   // its weights, in that XCD's L2.
@@ -612,13 +630,13 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
     return;
   }
   if (item.z > 96)
-    mx_tiled_body<4, kEpi>(g, item, n_tile, ring, ring_scales);
+    mx_tiled_body<4, kEpi>(g, item, n_tile, ring);
   else if (item.z > 64)
-    mx_tiled_body<3, kEpi>(g, item, n_tile, ring, ring_scales);
+    mx_tiled_body<3, kEpi>(g, item, n_tile, ring);
   else if (item.z > 32)
-    mx_tiled_body<2, kEpi>(g, item, n_tile, ring, ring_scales);
+    mx_tiled_body<2, kEpi>(g, item, n_tile, ring);
   else
-    mx_tiled_body<1, kEpi>(g, item, n_tile, ring, ring_scales);
+    mx_tiled_body<1, kEpi>(g, item, n_tile, ring);
 }
 
 // Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
