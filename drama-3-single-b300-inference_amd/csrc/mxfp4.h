@@ -17,19 +17,17 @@ constexpr int kMxOperandCodes = kMxStep / 2;         // a quantised row's codes 
 constexpr int kMxOperandScales = kMxStep / kMxBlock;  // and scales
 constexpr int kMxLow = 4;  // the MFMA's format code of e2m1 operands
 
-// Row orders of a packed weight: which row of W the lanes of an MFMA's
-// output hold.  An output lane of group g holds rows 4 g + i (i < 4) of each
-// of the row group's tiles t.
-constexpr int kMxOrderPairs = 0;   // 32 (t / 2) + 8 g + 4 (t % 2) + i: 16 bytes of bf16 a lane and tile pair
+// Row orders of a packed weight: which row of W row m = 4 g + i (i < 4) of
+// tile t of a row group holds.  The MFMAs' output lanes hold rows 4 g + i of
+// every tile; with these orders a pair of tiles is eight consecutive columns.
+constexpr int kMxOrderRows = 0;    // 32 (t / 2) + 8 g + 4 (t % 2) + i
 constexpr int kMxOrderGateUp = 1;  // tiles 0-1 gate, 2-3 up rows 32 rg + 8 g + 4 (t % 2) + i: a lane holds both
-constexpr int kMxOrderPlain = 2;   // 16 t + 4 g + i: 16 bytes of fp32 a lane and tile
 
 // Row of W that row m of tile t of row group rg holds; rows from n on are padding.
 __host__ __device__ __forceinline__ int mx_weight_row(int order, int n, int rg, int t, int m) {
-  const int g = m >> 2, i = m & 3;
-  if (order == kMxOrderPlain) return kMxRows * rg + 16 * t + m;
-  if (order == kMxOrderPairs) return kMxRows * rg + 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i;
-  return (t >= 2 ? n / 2 : 0) + 32 * rg + 8 * g + 4 * (t & 1) + i;
+  const int in_pair = 8 * (m >> 2) + 4 * (t & 1) + (m & 3);
+  if (order == kMxOrderRows) return kMxRows * rg + 32 * (t >> 1) + in_pair;
+  return (t >= 2 ? n / 2 : 0) + 32 * rg + in_pair;
 }
 
 // Quantised rows as the products read them: codes in row order at a pitch of
@@ -105,6 +103,30 @@ __device__ __forceinline__ uint32_t mx_codes8_bf16(const uint32_t* w, float scal
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[1]), scale, 1);
   c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[2]), scale, 2);
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
+}
+
+// Eight fp32 values as scaled fp16 and back: a route's down row is kept in 16
+// bits between the product and the combine, with one power of two per 64
+// columns that brings their largest finite magnitude into [2^14, 2^15).  Its
+// rounding (2^-11 relative, fp16's half step, down to 2^-29 of the largest) is
+// an eighth of the bf16 rounding of the result, and the rows' traffic, the
+// largest of a prefill's down product and combine, is halved.
+// `exponent`: of the largest finite magnitude, biased, 15 .. 254; the factor is
+// 2^(141 - exponent), its inverse 2^(exponent - 141).
+__device__ __forceinline__ uint32_t mx_half_exponent(uint32_t amax) {
+  const uint32_t e = amax >> 23;
+  return e < 15u ? 15u : e;
+}
+__device__ __forceinline__ float mx_half_factor(uint32_t exponent) { return __uint_as_float((268u - exponent) << 23); }
+__device__ __forceinline__ float mx_half_inverse(uint32_t exponent) { return __uint_as_float((exponent - 14u) << 23); }
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t mx_pack_half(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, halfx2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+}
+// The larger of two magnitudes' bits, leaving out infinities and NaN.
+__device__ __forceinline__ uint32_t mx_max_finite(uint32_t amax, float v) {
+  const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
+  return MaxU32::apply(amax, bits < 0x7f800000u ? bits : 0u);
 }
 
 // Memory words at the alignment of their elements only: gfx950 takes wide

@@ -225,7 +225,7 @@ extern "C" int d3_mxfp4_pack(const uint8_t* codes, const uint8_t* scales, int32_
   D3_REQUIRE(codes && scales && packed && packed_scales, "mxfp4_pack: null pointer");
   D3_REQUIRE(num_experts > 0 && n > 0 && k > 0 && k % kGroup == 0, "mxfp4_pack: K=%d must be a multiple of %d", k,
              kGroup);
-  D3_REQUIRE(order >= kMxOrderPairs && order <= kMxOrderPlain, "mxfp4_pack: row order %d", order);
+  D3_REQUIRE(order == kMxOrderRows || order == kMxOrderGateUp, "mxfp4_pack: row order %d", order);
   D3_REQUIRE(order != kMxOrderGateUp || n % kMxRows == 0,
              "mxfp4_pack: gate and up need N=%d to be a multiple of %d", n, kMxRows);
   D3_REQUIRE(mx_aligned(codes, 16) && mx_aligned(packed, 16) && mx_aligned(packed_scales, 8),

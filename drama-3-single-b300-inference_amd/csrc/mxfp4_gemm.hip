@@ -21,9 +21,9 @@ constexpr int kMxWaves = 4;
 constexpr int kMxThreads = kMxWaves * kWave;
 
 enum MxEpilogue {
-  kMxBf16,  // bf16 rows at the item's rows (row order: pairs)
+  kMxBf16,  // bf16 rows at the item's rows
   kMxAct,   // silu(gate) * up quantised to MXFP4 rows at the item's rows (gate-up order)
-  kMxF32,   // fp32 rows at sorted[row] (plain order)
+  kMxHalf,  // scaled fp16 rows at sorted[row]
 };
 
 struct MxGemm {
@@ -40,7 +40,7 @@ struct MxGemm {
   const int4* items;  // {expert (-1: zero rows), first row, rows, -}; nullptr: one expert, `rows` in order
   const int32_t* num_items;
   int rows;
-  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxF32);
+  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxHalf);
   int top_k;              // nullptr: the identity
   const void* ids;        // kMxPairs: expert of each (row, rank) pair
   int ids_i64;
@@ -49,7 +49,7 @@ struct MxGemm {
   int zero_rest;
   void* out;
   int64_t out_stride;  // elements (kMxAct: the row's width)
-  uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout
+  uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout; kMxHalf: exponents [rows][row groups]
 };
 
 // One MFMA with the scales in byte SA of `sa` and byte SB of `sb`.
@@ -78,8 +78,18 @@ __device__ __forceinline__ int4 mx_item(const MxGemm& g, int index, int item_row
   return g.items[index];
 }
 
-// Eight bf16 values at columns f .. of a row of n.
-__device__ __forceinline__ void mx_store_bf16(uint16_t* out, int f, int n, const MxWords4& v) {
+// Eight values as bf16, or as the fp16 of kMxHalf.
+template <int kEpi>
+__device__ __forceinline__ MxWords4 mx_pack8(const float* v) {
+  MxWords4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w.w[i] = kEpi == kMxHalf ? mx_pack_half(v[2 * i], v[2 * i + 1]) : pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  return w;
+}
+
+// Eight 16-bit values at columns f .. of a row of n.
+__device__ __forceinline__ void mx_store16(uint16_t* out, int f, int n, const MxWords4& v) {
   if (f + 8 <= n) {
     *reinterpret_cast<MxWords4*>(out + f) = v;
     return;
@@ -97,16 +107,32 @@ __device__ __forceinline__ void mx_store_bf16(uint16_t* out, int f, int n, const
 // live or not) for row group rg.
 template <int kEpi>
 __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4], int rg, int row, bool live, int group) {
-  if constexpr (kEpi == kMxBf16) {
+  if constexpr (kEpi == kMxBf16 || kEpi == kMxHalf) {
+    int64_t to = row;
+    float factor = 1.0f;
+    if constexpr (kEpi == kMxHalf) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) amax = mx_max_finite(amax, c[t][i]);
+      amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16)));
+      amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
+      const uint32_t exponent = mx_half_exponent(amax);
+      factor = mx_half_factor(exponent);
+      if (live) {
+        to = g.sorted[row];
+        if (group == 0) g.out_scales[to * g.row_groups + rg] = static_cast<uint8_t>(exponent);
+      }
+    }
     if (!live) return;
-    uint16_t* out = static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.out_stride;
+    uint16_t* out = static_cast<uint16_t*>(g.out) + to * g.out_stride;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int f = kMxRows * rg + 32 * p + 8 * group;
-      const floatx4 &lo = c[2 * p], &hi = c[2 * p + 1];
-      mx_store_bf16(out, f, g.n,
-                    {pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]),
-                     pack_bf16x2(hi[2], hi[3])});
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c[2 * p + i / 4][i % 4] * factor;
+      mx_store16(out, kMxRows * rg + 32 * p + 8 * group, g.n, mx_pack8<kEpi>(v));
     }
   } else if constexpr (kEpi == kMxAct) {
     // Gate (tiles 0, 1) and up (tiles 2, 3) of columns 32 rg + 8 group + i;
@@ -131,12 +157,6 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4],
     const int64_t first = static_cast<int64_t>(row) * ((blocks + 7) / 8);  // in steps
     *reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(g.out) + first * kMxOperandCodes + rg * (kMxBlock / 2) + 4 * group) = word;
     if (group == 0) mx_operand_scale(g.out_scales + first * kMxOperandScales, rg, blocks, code);
-  } else {
-    if (!live) return;
-    float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride +
-                 kMxRows * rg + 4 * group;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) *reinterpret_cast<floatx4*>(out + 16 * t) = c[t];
   }
 }
 
@@ -353,7 +373,8 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
     }
     if ((lane & 15) == 0) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) *reinterpret_cast<floatx4*>(&result[r][16 * t + 4 * group]) = acc[t];
+      for (int t = 0; t < 4; ++t)
+        *reinterpret_cast<floatx4*>(&result[r][32 * (t >> 1) + 8 * group + 4 * (t & 1)]) = acc[t];
     }
   }
   __syncthreads();
@@ -408,25 +429,22 @@ __device__ __forceinline__ floatx16 mfma_fp4_32(const int32x4& a, const int32x4&
                                                          static_cast<int>(sb));
 }
 
-// A row's 64 sums of row group rg in the 32x32 output layout: lane half hl
-// holds rows 8 j + 4 hl + i (element 4 j + i) of each 32-row half u of the
-// group; in the pair orders those are columns 16 (j % 2) + 8 hl + 4 (j / 2) + i.
+// The sums of 32 rows for row group rg in the 32x32 output layout: lane half
+// hl holds rows 8 j + 4 hl + i (element 4 j + i) of each 32-row half u of the
+// group, columns 16 (j % 2) + 8 hl + 4 (j / 2) + i of it.
+// 16-bit rows pass through the wave's own LDS, 144 bytes a row, so that a store
+// writes eight whole 128-byte pieces instead of 32 bytes of 32 rows: a quarter
+// of the lines to look up (4096 x 2048 x 1281, whose rows start anywhere in a
+// line: 17.8 -> 13.6 us).
+constexpr int kMxStoreRow = 2 * kMxRows + 16;
+constexpr int kMxStoreArea = 32 * kMxStoreRow;
 template <int kEpi>
-__device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[2], int rg, int row, bool live, int hl) {
-  if constexpr (kEpi == kMxBf16) {
-    if (!live) return;
-    uint16_t* out = static_cast<uint16_t*>(g.out) + static_cast<int64_t>(row) * g.out_stride;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int f = kMxRows * rg + 32 * u + 16 * j + 8 * hl;
-        const floatx16& v = c[u];
-        mx_store_bf16(out, f, g.n,
-                      {pack_bf16x2(v[4 * j], v[4 * j + 1]), pack_bf16x2(v[4 * j + 2], v[4 * j + 3]),
-                       pack_bf16x2(v[4 * j + 8], v[4 * j + 9]), pack_bf16x2(v[4 * j + 10], v[4 * j + 11])});
-      }
-  } else if constexpr (kEpi == kMxAct) {
+__device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[2], int rg, const int4& item, int first,
+                                           int count, const int32_t* targets, uint8_t* area) {
+  const int lane = lane_id(), col = lane & 31, hl = lane >> 5;
+  const int row = item.y + first + col;
+  const bool live = first + col < count;
+  if constexpr (kEpi == kMxAct) {
     float gate[16], up[16], v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -444,25 +462,52 @@ __device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[
     const uint32_t lo = mx_codes8(v, inverse), hi = mx_codes8(v + 8, inverse);
     if (!live) return;
     const uint32_t blocks = static_cast<uint32_t>(g.out_stride) / kMxBlock;
-    const int64_t first = static_cast<int64_t>(row) * ((blocks + 7) / 8);  // in steps
-    uint8_t* codes = static_cast<uint8_t*>(g.out) + first * kMxOperandCodes + rg * (kMxBlock / 2) + 4 * hl;
+    const int64_t at = static_cast<int64_t>(row) * ((blocks + 7) / 8);  // in steps
+    uint8_t* codes = static_cast<uint8_t*>(g.out) + at * kMxOperandCodes + rg * (kMxBlock / 2) + 4 * hl;
     *reinterpret_cast<uint32_t*>(codes) = lo;
     *reinterpret_cast<uint32_t*>(codes + 8) = hi;
-    if (hl == 0) mx_operand_scale(g.out_scales + first * kMxOperandScales, rg, blocks, code);
+    if (hl == 0) mx_operand_scale(g.out_scales + at * kMxOperandScales, rg, blocks, code);
   } else {
-    if (!live) return;
-    float* out = static_cast<float*>(g.out) + static_cast<int64_t>(g.sorted[row]) * g.out_stride + kMxRows * rg + 4 * hl;
+    float factor = 1.0f;
+    if constexpr (kEpi == kMxHalf) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = mx_max_finite(amax, c[u][i]);
+      amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
+      const uint32_t exponent = mx_half_exponent(amax);
+      factor = mx_half_factor(exponent);
+      if (live && hl == 0)
+        g.out_scales[static_cast<int64_t>(targets[first + col]) * g.row_groups + rg] = static_cast<uint8_t>(exponent);
+    }
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *reinterpret_cast<floatx4*>(out + 32 * u + 8 * j) =
-            floatx4{c[u][4 * j], c[u][4 * j + 1], c[u][4 * j + 2], c[u][4 * j + 3]};
+      for (int j = 0; j < 2; ++j) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c[u][4 * j + 8 * (i / 4) + i % 4] * factor;
+        *reinterpret_cast<int32x4*>(area + col * kMxStoreRow + 64 * u + 32 * j + 16 * hl) =
+            __builtin_bit_cast(int32x4, mx_pack8<kEpi>(v));
+      }
+    const int part = lane & 7;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = 8 * k + (lane >> 3);
+      const MxWords4 w = __builtin_bit_cast(MxWords4, *reinterpret_cast<const int32x4*>(area + r * kMxStoreRow + 16 * part));
+      if (first + r < count) {
+        int64_t to = item.y + first + r;
+        if constexpr (kEpi == kMxHalf) to = targets[first + r];
+        mx_store16(static_cast<uint16_t*>(g.out) + to * g.out_stride, kMxRows * rg + 8 * part, g.n, w);
+      }
+    }
   }
 }
 
 template <int kRT, int kEpi>
-__device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t* ring) {
+__device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t* ring,
+                                              int32_t* targets) {
   const int tid = threadIdx.x, lane = lane_id(), col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rg = n_tile * kMxWaves + wave;
@@ -530,6 +575,10 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
     constexpr int rt = decltype(tile)::value;
     sb_next[rt] = *reinterpret_cast<const uint32_t*>(slot + kMxSlotCodes + (32 * rt + col) * kMxOperandScales + 4 * hl);
   };
+
+  // Where the item's rows go, for the stores (written before the first barrier).
+  if constexpr (kEpi == kMxHalf)
+    if (tid < kMxTiledRows) targets[tid] = g.sorted[item.y + min(tid, count - 1)];
 
   floatx16 acc[kRT][2];
 #pragma unroll
@@ -605,16 +654,20 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
     slot_next = slot_free;
     slot_free = const_cast<uint8_t*>(done);
   }
+  lds_barrier();
   if (rg >= g.row_groups) return;
+  // Every wave has left the ring: two areas of it a wave take turns.
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt)
-    mx_store32<kEpi>(g, acc[rt], rg, item.y + 32 * rt + col, 32 * rt + col < count, hl);
+    mx_store32<kEpi>(g, acc[rt], rg, item, 32 * rt, count, targets, ring + (2 * wave + rt % 2) * kMxStoreArea);
 }
 
 template <int kEpi>
 __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2))) void mx_tiled_kernel(MxGemm g,
                                                                                                       MxTiles tiles) {
   __shared__ __attribute__((aligned(16))) uint8_t ring[3 * kMxSlot];
+  static_assert(2 * kMxWaves * kMxStoreArea <= 3 * kMxSlot, "the waves' store areas fit the ring");
+  __shared__ int32_t targets[kEpi == kMxHalf ? kMxTiledRows : 1];
   // Runs of consecutive items go to the XCDs in turn (workgroup b runs on XCD
   // b % 8): a run's tiles share its rows, and an expert's consecutive items
   // its weights, in that XCD's L2.
@@ -630,13 +683,13 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
     return;
   }
   if (item.z > 96)
-    mx_tiled_body<4, kEpi>(g, item, n_tile, ring);
+    mx_tiled_body<4, kEpi>(g, item, n_tile, ring, targets);
   else if (item.z > 64)
-    mx_tiled_body<3, kEpi>(g, item, n_tile, ring);
+    mx_tiled_body<3, kEpi>(g, item, n_tile, ring, targets);
   else if (item.z > 32)
-    mx_tiled_body<2, kEpi>(g, item, n_tile, ring);
+    mx_tiled_body<2, kEpi>(g, item, n_tile, ring, targets);
   else
-    mx_tiled_body<1, kEpi>(g, item, n_tile, ring);
+    mx_tiled_body<1, kEpi>(g, item, n_tile, ring, targets);
 }
 
 // Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
@@ -688,31 +741,51 @@ __global__ __launch_bounds__(kItemThreads) void mx_items_kernel(const int32_t* _
 
 // out[t, :] = sum over ranks r of weights[t, r] * down[t * top_k + r, :] in
 // rank order (fp32, one FMA a rank), rounded to bf16 once.  Ranks whose id
-// names no expert add nothing (their down rows were never written).
-constexpr int kMxCombineColumns = kMxThreads * 4;
+// names no expert add nothing (their down rows were never written).  A thread
+// has eight columns; every rank's row piece is loaded before the first sum.
+constexpr int kMxCombineColumns = kMxThreads * 8;
 template <int kTopK>  // 0: any
-__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ down, const void* __restrict__ ids,
-                                                                int ids_i64, const void* __restrict__ weights,
-                                                                int weights_f32, int any_top_k, int experts, int hidden,
-                                                                int slices, uint16_t* __restrict__ out) {
+__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint16_t* __restrict__ down,
+                                                                const uint8_t* __restrict__ exponents,
+                                                                const void* __restrict__ ids, int ids_i64,
+                                                                const void* __restrict__ weights, int weights_f32,
+                                                                int any_top_k, int experts, int hidden, int slices,
+                                                                uint16_t* __restrict__ out) {
   const int row = blockIdx.x / slices;
-  const int column = (blockIdx.x % slices) * kMxCombineColumns + threadIdx.x * 4;
+  const int column = (blockIdx.x % slices) * kMxCombineColumns + threadIdx.x * 8;
   if (column >= hidden) return;
   const int top_k = kTopK ? kTopK : any_top_k;
   const int64_t first = static_cast<int64_t>(row) * top_k;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  constexpr int kBatch = kTopK ? kTopK : 4;
+  float acc[8] = {};
+  for (int r0 = 0; r0 < top_k; r0 += kBatch) {
+    int32x4 y[kBatch];
+    float scale[kBatch];
 #pragma unroll
-  for (int r = 0; r < top_k; ++r) {
-    const floatx4 y = __builtin_nontemporal_load(reinterpret_cast<const floatx4*>(down + (first + r) * hidden + column));
-    const int64_t id = ids_i64 ? static_cast<const int64_t*>(ids)[first + r] : static_cast<const int32_t*>(ids)[first + r];
-    const bool live = id >= 0 && id < experts;
-    const float w = live ? route_weight(weights, weights_f32, first + r) : 0.0f;
-    acc.x = fmaf(w, live ? y[0] : 0.0f, acc.x);
-    acc.y = fmaf(w, live ? y[1] : 0.0f, acc.y);
-    acc.z = fmaf(w, live ? y[2] : 0.0f, acc.z);
-    acc.w = fmaf(w, live ? y[3] : 0.0f, acc.w);
+    for (int k = 0; k < kBatch; ++k) {
+      const int64_t pair = first + min(r0 + k, top_k - 1);
+      y[k] = __builtin_nontemporal_load(reinterpret_cast<const int32x4*>(down + pair * hidden + column));
+      scale[k] = mx_half_inverse(exponents[pair * (hidden / kMxRows) + column / kMxRows]);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int64_t pair = first + min(r0 + k, top_k - 1);
+      const int64_t id = ids_i64 ? static_cast<const int64_t*>(ids)[pair] : static_cast<const int32_t*>(ids)[pair];
+      const bool live = id >= 0 && id < experts && r0 + k < top_k;  // uniform
+      const float w = route_weight(weights, weights_f32, pair);
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int word = y[k][i / 2];  // (a bit_cast of the element itself reads the vector's first)
+          const halfx2 h = __builtin_bit_cast(halfx2, word);
+          acc[i] = fmaf(w, static_cast<float>(h[i % 2]) * scale[k], acc[i]);
+        }
+      }
+    }
   }
-  *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row) * hidden + column) = pack_bf16x4(acc);
+  *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * hidden + column) =
+      make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
+                 pack_bf16x2(acc[6], acc[7]));
 }
 
 bool mx_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
@@ -822,7 +895,8 @@ struct MoePlan {
   int item_rows, max_items, max_rows;
   int64_t pairs, scratch_ints;
   uint8_t *q, *qs, *act, *acts;
-  float* down;
+  uint16_t* down;
+  uint8_t* exponents;
   int32_t *counts, *starts, *total, *sorted, *expert_ids, *num_items, *scratch;
   int4* items;
   int64_t bytes;
@@ -848,7 +922,8 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
     p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
   }
   if (!p.few) {
-    p.down = a.take<float>(p.pairs * hidden);
+    p.down = a.take<uint16_t>(p.pairs * hidden);
+    p.exponents = a.take<uint8_t>(p.pairs * (hidden / kMxRows));
     p.counts = a.take<int32_t>(experts);
     p.starts = a.take<int32_t>(experts);
     p.total = a.take<int32_t>(1);
@@ -949,7 +1024,7 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   D3_REQUIRE(rows == 0 || (x && ids && weights && w13 && s13 && w2 && s2 && out && workspace), "mxfp4_moe: null pointer");
   D3_REQUIRE(rows <= 1 || x_row_stride >= 0, "mxfp4_moe: negative row stride");
   D3_REQUIRE(mx_aligned(x, 2) && mx_aligned(w13, 16) && mx_aligned(s13, 8) && mx_aligned(w2, 16) && mx_aligned(s2, 8) &&
-                 mx_aligned(out, 8) && mx_aligned(workspace, 16) &&
+                 mx_aligned(out, 16) && mx_aligned(workspace, 16) &&
                  mx_aligned(ids, ids_dtype == D3_DTYPE_I64 ? 8 : 4) &&
                  mx_aligned(weights, weights_dtype == D3_DTYPE_F32 ? 4 : 2),
              "mxfp4_moe: alignment");
@@ -1000,15 +1075,15 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
     mx_quantize_operand(x, x_row_stride, rows, hidden, p.q, p.qs, s);
     launch_gemm<kMxAct>(up, p.item_rows, p.max_items, s);
   }
-  down.out = p.down;
-  launch_gemm<kMxF32>(down, p.item_rows, p.max_items, s);
+  down.out = p.down, down.out_scales = p.exponents;
+  launch_gemm<kMxHalf>(down, p.item_rows, p.max_items, s);
   const int slices = mx_ceil(hidden, kMxCombineColumns);
   const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
   if (top_k == 8)
-    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.down, ids, i64, weights, f32, top_k, num_experts, hidden,
+    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.down, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
                        slices, out);
   else
-    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.down, ids, i64, weights, f32, top_k, num_experts, hidden,
+    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.down, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
                        slices, out);
   D3_LAUNCHED("mxfp4_moe");
 }

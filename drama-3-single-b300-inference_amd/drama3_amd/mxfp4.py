@@ -32,7 +32,7 @@ from ._lib import ptr
 from .pipeline import require_cuda
 
 BLOCK = 32  # elements per scale
-ORDER_ROWS, ORDER_GATE_UP, ORDER_DOWN = 0, 1, 2  # which product reads a packed weight
+ORDER_ROWS, ORDER_GATE_UP = 0, 1  # row order of a packed weight
 _FLOAT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 _INT = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
@@ -200,7 +200,7 @@ def prepare_mxfp4_experts(w13_codes, w13_scales, w2_codes, w2_scales) -> Mxfp4Ex
         raise ValueError("expert weights must be w13 [E, 2I, H], w2 [E, H, I], H and I multiples of 128")
     _same_device(w13_codes, w2_codes, "w2_codes")
     return Mxfp4Experts(_prepare(w13_codes, w13_scales, ORDER_GATE_UP),
-                        _prepare(w2_codes, w2_scales, ORDER_DOWN))
+                        _prepare(w2_codes, w2_scales, ORDER_ROWS))
 
 
 def quantize_experts_mxfp4(experts) -> Mxfp4Experts:
@@ -209,7 +209,7 @@ def quantize_experts_mxfp4(experts) -> Mxfp4Experts:
     MXFP4, one expert at a time, at load time."""
     packed = []
     for weight, inverse, order in ((experts.w13_weight, experts.w13_scale_inv, ORDER_GATE_UP),
-                                   (experts.w2_weight, experts.w2_scale_inv, ORDER_DOWN)):
+                                   (experts.w2_weight, experts.w2_scale_inv, ORDER_ROWS)):
         require_cuda(weight, inverse)
         if weight.dim() != 3 or weight.dtype != torch.float8_e4m3fn:
             raise TypeError("expert weights must be float8_e4m3fn [E, N, K]")
@@ -229,7 +229,7 @@ def quantize_experts_mxfp4(experts) -> Mxfp4Experts:
 def _product(x, boundaries, weight: Mxfp4Weight, out, zero_rest: bool) -> torch.Tensor:
     _check_rows(x)
     if weight.order != ORDER_ROWS:
-        raise ValueError("weight was packed for mxfp4_moe; pack it with prepare_mxfp4")
+        raise ValueError("weight holds gate and up rows; pack it with prepare_mxfp4")
     rows, k = x.shape
     if k != weight.k:
         raise ValueError(f"rows of width {k}, weight of K={weight.k}")
@@ -283,7 +283,9 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     """Routed SwiGLU experts: for row t and rank r with expert e =
     ``topk_ids[t, r]``, ``a = silu(G_e x) * (U_e x)`` and ``out[t] = sum_r
     topk_weights[t, r] * W2_e a`` in rank order, with x and a quantised to
-    MXFP4 and everything else fp32, rounded to bf16 [T, H] once.
+    MXFP4 and fp32 sums, rounded to bf16 [T, H] once.  (Above 64 pairs the
+    ranks' rows are held as scaled fp16 in between, whose rounding is an
+    eighth of bf16's.)
 
     ``topk_ids`` int32 / int64 [T, k], k <= 16 (an id that names no expert
     adds nothing), ``topk_weights`` bf16 / f32 of the same shape."""
@@ -299,7 +301,7 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
         raise ValueError(f"rows of width {x.shape[1]}, experts of hidden size {experts.hidden}")
     ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
     w13, w2 = experts.w13, experts.w2
-    if w13.order != ORDER_GATE_UP or w2.order != ORDER_DOWN:
+    if w13.order != ORDER_GATE_UP or w2.order != ORDER_ROWS:
         raise ValueError("experts must come from prepare_mxfp4_experts")
     _same_device(x, ids, "topk_ids")
     _same_device(x, weights, "topk_weights")

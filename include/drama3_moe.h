@@ -800,9 +800,8 @@ int d3_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t row
  * scales -> the packed layout the products read, once at load time.  Buffers
  * of d3_mxfp4_packed_bytes bytes; k % 128 == 0, any n.  `order` says which
  * product reads them:
- *   0 d3_mxfp4_grouped (bf16 rows);
- *   1 the gate and up product of d3_mxfp4_moe (rows [gate; up], n % 64 == 0);
- *   2 its down product.
+ *   0 d3_mxfp4_grouped and the down product of d3_mxfp4_moe;
+ *   1 the gate and up product of d3_mxfp4_moe (rows [gate; up], n % 64 == 0).
  */
 int d3_mxfp4_pack(const uint8_t *codes, const uint8_t *scales, int32_t num_experts, int32_t n,
                   int32_t k, int32_t order, uint8_t *packed, uint8_t *packed_scales,
@@ -835,8 +834,10 @@ int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bo
  * Routed SwiGLU experts on MXFP4 weights: for every row t and rank r with
  * expert e = ids[t, r], a = silu(G x) * (U x) with x quantised to MXFP4 and
  * [G; U] = w13[e] (order 1), a quantised to MXFP4 from its fp32 values, and
- *   out[t] = sum over r of weights[t, r] * (w2[e] (order 2) a)
- * in rank order, fp32 throughout, rounded to bf16 once.  ids int32 or int64
+ *   out[t] = sum over r of weights[t, r] * (w2[e] (order 0) a)
+ * in rank order, the sums fp32, rounded to bf16 once (above 64 pairs each
+ * rank's row is first rounded to a scaled fp16, an eighth of bf16's step).
+ * ids int32 or int64
  * [rows, top_k] (an id outside [0, num_experts) adds nothing), weights bf16 or
  * f32.  top_k <= 16, num_experts <= 512, hidden and intermediate multiples of
  * 128.  workspace: d3_mxfp4_moe_workspace bytes, as for d3_mxfp4_grouped.

@@ -82,7 +82,7 @@ def test_c_entries_refuse_before_launching(lib):
     with pytest.raises(ValueError, match="multiple of 64"):
         call("d3_mxfp4_pack", 16, 16, 1, 96, 256, 1, 16, 16, None)
     with pytest.raises(ValueError, match="order"):
-        call("d3_mxfp4_pack", 16, 16, 1, 64, 256, 3, 16, 16, None)
+        call("d3_mxfp4_pack", 16, 16, 1, 64, 256, 2, 16, 16, None)
     grouped = [16, 256, 40, 16, 4, 16, 16, 64, 256, 16, 64, 0, 16, 1 << 30, None]
 
     def refused(match, entry, args, **changes):
