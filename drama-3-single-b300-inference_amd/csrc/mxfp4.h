@@ -45,10 +45,6 @@ __device__ __forceinline__ void mx_operand_scale(uint8_t* row, uint32_t block, u
   if (8 * step + 4 >= blocks) at[2] = 0;  // the last step's second half is padding
 }
 
-// bf16 rows to that layout (width % 128 == 0).
-void mx_quantize_operand(const uint16_t* x, int64_t stride, int64_t rows, int width, uint8_t* codes, uint8_t* scales,
-                         hipStream_t stream);
-
 // Scale code of a block whose largest magnitude has the fp32 bits `amax`
 // (sign bit clear): floor(log2 amax) - 2, so that the largest element lies in
 // [4, 8) scaled; 0 (2^-127) for zero blocks and those below 2^-124; 255 (NaN)
@@ -133,5 +129,77 @@ __device__ __forceinline__ uint32_t mx_max_finite(uint32_t amax, float v) {
 // accesses at any address, so odd row strides cost no narrow path.
 struct __attribute__((packed, aligned(2))) MxWords4 { uint32_t w[4]; };
 struct __attribute__((packed, aligned(1))) MxWord { uint32_t w; };
+
+// Rows -> codes: a lane takes 8 consecutive elements, four lanes a block of
+// 32.  The block's largest magnitude is an integer maximum of the values' bits
+// (which orders NaN above infinity above every number), exchanged inside the
+// quad with two DPP moves.  kOperand: the layout the products read, `steps`
+// steps a row; else plain rows.
+struct MxQuantize {
+  const void* x;
+  int64_t stride;
+  uint64_t units;    // of 8 elements
+  uint32_t per_row;  // units a row
+  int steps;
+  uint8_t* codes;
+  uint8_t* scales;
+};
+constexpr int kMxQuantizeUnits = 4;  // units a thread has in flight
+
+__device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
+  v = MaxU32::apply(v, dpp_move<kDppQuad1032>(v, 0u));
+  return MaxU32::apply(v, dpp_move<kDppQuad2301>(v, 0u));
+}
+
+template <bool kF32, bool kOperand, int kThreads>
+__device__ __forceinline__ void mx_quantize_units(const MxQuantize& q, uint32_t block) {
+  constexpr int kUnits = kMxQuantizeUnits;
+  const uint64_t first = static_cast<uint64_t>(block) * (kThreads * kUnits) + threadIdx.x;
+  MxWords4 raw[kUnits][kF32 ? 2 : 1];
+  uint64_t row[kUnits];
+  uint32_t unit[kUnits];
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    const uint64_t u = first + static_cast<uint64_t>(j) * kThreads;
+    const uint64_t at = u < q.units ? u : q.units - 1;
+    row[j] = (at >> 32) == 0 ? static_cast<uint32_t>(at) / q.per_row : at / q.per_row;
+    unit[j] = static_cast<uint32_t>(at - row[j] * q.per_row);
+    const int64_t element = static_cast<int64_t>(row[j]) * q.stride + 8 * static_cast<int64_t>(unit[j]);
+    const MxWords4* p = reinterpret_cast<const MxWords4*>(static_cast<const uint8_t*>(q.x) + element * (kF32 ? 4 : 2));
+#pragma unroll
+    for (int h = 0; h < (kF32 ? 2 : 1); ++h) raw[j][h] = p[h];
+  }
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    const uint64_t u = first + static_cast<uint64_t>(j) * kThreads;
+    uint32_t code, word;
+    if constexpr (kF32) {
+      float v[8];
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = __uint_as_float(raw[j][i / 4].w[i % 4]);
+        amax = MaxU32::apply(amax, __float_as_uint(v[i]) & 0x7fffffffu);
+      }
+      code = mx_scale_code(mx_quad_max(amax));
+      word = mx_codes8(v, mx_inverse(code));
+    } else {
+      const uint16x2 amax = mx_amax_bf16<4>(raw[j][0].w);
+      code = mx_scale_code(mx_quad_max(MaxU32::apply(amax[0], amax[1])) << 16);
+      word = mx_codes8_bf16(raw[j][0].w, mx_scale(code));
+      if (code == 255u) word = 0;
+    }
+    if (u >= q.units) continue;
+    if constexpr (kOperand) {
+      *reinterpret_cast<uint32_t*>(q.codes + row[j] * q.steps * kMxOperandCodes + 4 * static_cast<uint64_t>(unit[j])) =
+          word;
+      if ((unit[j] & 3) == 0)
+        mx_operand_scale(q.scales + row[j] * q.steps * kMxOperandScales, unit[j] >> 2, q.per_row >> 2, code);
+    } else {
+      reinterpret_cast<MxWord*>(q.codes)[u].w = word;
+      if ((u & 3) == 0) q.scales[u >> 2] = static_cast<uint8_t>(code);
+    }
+  }
+}
 
 }  // namespace d3

@@ -1,11 +1,7 @@
 // MXFP4 quantisation of rows, the way back, and the packed weight layout of
 // the MXFP4 products.
 //
-// Rows -> codes: a lane takes 8 consecutive elements, four lanes a block of
-// 32.  The block's largest magnitude is an integer maximum of the fp32 bits
-// (which orders NaN above infinity above every number), exchanged inside the
-// quad with two DPP moves.  Reads 2 (or 4) bytes and writes 17/32 of a byte
-// an element: bound by HBM.
+// Both directions read and write every element once and are bound by HBM.
 #include "mxfp4.h"
 #include "status.h"
 
@@ -13,68 +9,11 @@ namespace d3 {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowUnits = 4;  // 8-element units a thread has in flight
+constexpr int kRowUnits = kMxQuantizeUnits;
 
-__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
-  v = MaxU32::apply(v, dpp_move<kDppQuad1032>(v, 0u));
-  return MaxU32::apply(v, dpp_move<kDppQuad2301>(v, 0u));
-}
-
-// Row and unit in the row of unit u.
-__device__ __forceinline__ void unit_row(uint64_t u, uint32_t per_row, uint64_t* row, uint32_t* unit) {
-  *row = (u >> 32) == 0 ? static_cast<uint32_t>(u) / per_row : u / per_row;
-  *unit = static_cast<uint32_t>(u - *row * per_row);
-}
-
-// kOperand: the layout the products read (mx_operand_*), else plain rows.
-template <bool kF32, bool kOperand>
-__global__ __launch_bounds__(kRowThreads) void quantize_kernel(const void* __restrict__ x, int64_t stride,
-                                                               uint64_t units, uint32_t per_row, int steps,
-                                                               uint8_t* __restrict__ codes,
-                                                               uint8_t* __restrict__ scales) {
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * (kRowThreads * kRowUnits) + threadIdx.x;
-  MxWords4 raw[kRowUnits][kF32 ? 2 : 1];
-  uint64_t row[kRowUnits];
-  uint32_t unit[kRowUnits];
-#pragma unroll
-  for (int j = 0; j < kRowUnits; ++j) {
-    const uint64_t u = first + static_cast<uint64_t>(j) * kRowThreads;
-    unit_row(u < units ? u : units - 1, per_row, &row[j], &unit[j]);
-    const int64_t at = static_cast<int64_t>(row[j]) * stride + 8 * static_cast<int64_t>(unit[j]);
-    const MxWords4* p = reinterpret_cast<const MxWords4*>(static_cast<const uint8_t*>(x) + at * (kF32 ? 4 : 2));
-#pragma unroll
-    for (int h = 0; h < (kF32 ? 2 : 1); ++h) raw[j][h] = p[h];
-  }
-#pragma unroll
-  for (int j = 0; j < kRowUnits; ++j) {
-    const uint64_t u = first + static_cast<uint64_t>(j) * kRowThreads;
-    uint32_t code, word;
-    if constexpr (kF32) {
-      float v[8];
-      uint32_t amax = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = __uint_as_float(raw[j][i / 4].w[i % 4]);
-        amax = MaxU32::apply(amax, __float_as_uint(v[i]) & 0x7fffffffu);
-      }
-      code = mx_scale_code(quad_max(amax));
-      word = mx_codes8(v, mx_inverse(code));
-    } else {
-      const uint16x2 amax = mx_amax_bf16<4>(raw[j][0].w);
-      code = mx_scale_code(quad_max(MaxU32::apply(amax[0], amax[1])) << 16);
-      word = mx_codes8_bf16(raw[j][0].w, mx_scale(code));
-      if (code == 255u) word = 0;
-    }
-    if (u >= units) continue;
-    if constexpr (kOperand) {
-      *reinterpret_cast<uint32_t*>(codes + row[j] * steps * kMxOperandCodes + 4 * static_cast<uint64_t>(unit[j])) = word;
-      if ((unit[j] & 3) == 0)
-        mx_operand_scale(scales + row[j] * steps * kMxOperandScales, unit[j] >> 2, per_row >> 2, code);
-    } else {
-      reinterpret_cast<MxWord*>(codes)[u].w = word;
-      if ((u & 3) == 0) scales[u >> 2] = static_cast<uint8_t>(code);
-    }
-  }
+template <bool kF32>
+__global__ __launch_bounds__(kRowThreads) void quantize_kernel(MxQuantize q) {
+  mx_quantize_units<kF32, false, kRowThreads>(q, blockIdx.x);
 }
 
 template <bool kF32>
@@ -160,14 +99,6 @@ unsigned row_blocks(uint64_t units) {
 
 }  // namespace
 
-void mx_quantize_operand(const uint16_t* x, int64_t stride, int64_t rows, int width, uint8_t* codes, uint8_t* scales,
-                         hipStream_t stream) {
-  const uint32_t per_row = static_cast<uint32_t>(width) / 8;
-  const uint64_t units = static_cast<uint64_t>(rows) * per_row;
-  hipLaunchKernelGGL((quantize_kernel<false, true>), dim3(row_blocks(units)), dim3(kRowThreads), 0, stream, x, stride,
-                     units, per_row, (width + kMxStep - 1) / kMxStep, codes, scales);
-}
-
 }  // namespace d3
 
 using namespace d3;
@@ -188,13 +119,12 @@ extern "C" int d3_mxfp4_quantize(const void* x, int32_t x_dtype, int64_t x_row_s
   const uint32_t per_row = static_cast<uint32_t>(width) / 8;
   D3_SUPPORTED(rows <= (int64_t{1} << 40) / per_row, "mxfp4_quantize: more than 2^43 elements");
   const uint64_t units = static_cast<uint64_t>(rows) * per_row;
+  const MxQuantize q{x, x_row_stride, units, per_row, 0, codes, scales};
   const dim3 grid(row_blocks(units)), block(kRowThreads);
   if (f32)
-    hipLaunchKernelGGL((quantize_kernel<true, false>), grid, block, 0, as_stream(stream), x, x_row_stride, units,
-                       per_row, 0, codes, scales);
+    hipLaunchKernelGGL(quantize_kernel<true>, grid, block, 0, as_stream(stream), q);
   else
-    hipLaunchKernelGGL((quantize_kernel<false, false>), grid, block, 0, as_stream(stream), x, x_row_stride, units,
-                       per_row, 0, codes, scales);
+    hipLaunchKernelGGL(quantize_kernel<false>, grid, block, 0, as_stream(stream), q);
   D3_LAUNCHED("mxfp4_quantize");
 }
 

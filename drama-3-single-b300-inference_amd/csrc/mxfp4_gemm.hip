@@ -418,6 +418,7 @@ __device__ __forceinline__ void mx_each(F&& f) {
 struct MxTiles {
   int n_tiles;  // 256-row weight tiles
   int run;      // consecutive items whose tiles one XCD takes together
+  int item_rows;
 };
 
 template <int SA, int SB>
@@ -676,7 +677,7 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
   const int in_run = j % per_run;
   const int index = ((j / per_run) * kMxXcds + blockIdx.x % kMxXcds) * tiles.run + in_run % tiles.run;
   const int n_tile = in_run / tiles.run;
-  const int4 item = mx_item(g, index, kMxTiledRows);
+  const int4 item = mx_item(g, index, tiles.item_rows);
   if (item.z <= 0) return;  // uniform
   if (kEpi == kMxBf16 && item.x < 0) {
     mx_zero_rows(g, item, n_tile * kMxWaves * kMxRows, kMxWaves * kMxRows);
@@ -692,51 +693,215 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
     mx_tiled_body<1, kEpi>(g, item, n_tile, ring, targets);
 }
 
-// Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
-// of item_rows; with `zero_rest` the rows before b[0] and from b[E] on as
-// items of expert -1.  Boundaries are clamped to [0, rows].
-constexpr int kItemThreads = 1024;
-__global__ __launch_bounds__(kItemThreads) void mx_items_kernel(const int32_t* __restrict__ bounds, int experts, int rows,
-                                                                int item_rows, int zero_rest, int max_items,
-                                                                int4* __restrict__ items, int32_t* __restrict__ num_items) {
-  __shared__ int wave_sum[kItemThreads / kWave];
-  __shared__ int base;
-  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
-  if (tid == 0) base = 0;
-  const int entries = experts + (zero_rest ? 2 : 0);
-  for (int first = 0; first < entries; first += kItemThreads) {
-    const int e = first + tid;
-    int a = 0, b = 0, expert = e;
-    if (e < experts) {
-      a = min(max(bounds[e], 0), rows);
-      b = min(max(bounds[e + 1], 0), rows);
-    } else if (e < entries) {
-      expert = -1;
-      a = e == experts ? 0 : min(max(bounds[experts], 0), rows);
-      b = e == experts ? min(max(bounds[0], 0), rows) : rows;
-    }
-    const int count = b > a ? (b - a + item_rows - 1) / item_rows : 0;
-    int scan = count;
+// What a product needs first, in one launch: its rows quantised, and (by the
+// first workgroup) its work items, from the groups' boundaries or from the
+// routes' ids.
+constexpr int kPrepareThreads = 1024;
+constexpr int kMxSortExperts = 512;
+enum MxPrepareWhat {
+  kMxRowsOnly,
+  kMxBounds,
+  kMxRoutes,       // few enough pairs for one workgroup
+  kMxRouteChunks,  // a workgroup per chunk of pairs counts, mx_place_kernel places
+};
+struct MxPrepare {
+  MxQuantize rows;
+  const int32_t* bounds;  // kMxBounds
+  int groups;             // groups or experts
+  int count;              // rows or (row, rank) pairs
+  int zero_rest;
+  const void* ids;  // kMxRoutes, kMxRouteChunks
+  int ids_i64;
+  int32_t* sorted;
+  int chunks;
+  int32_t* chunk_counts;  // [chunks][groups]
+  int32_t* ranks;         // of a pair among its chunk's pairs of its expert
+  int item_rows;
+  int max_items;
+  int4* items;
+  int32_t* num_items;
+};
+
+// Exclusive scan over the workgroup; *total is the sum.  `sums` is LDS of one
+// int a wave, free again at the next barrier.
+__device__ __forceinline__ int mx_scan(int v, int* sums, int* total) {
+  const int wave = threadIdx.x / kWave, lane = lane_id();
+  int scan = v;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int other = __shfl_up(scan, d);
-      if (lane >= d) scan += other;
-    }
-    if (lane == kWave - 1) wave_sum[wave] = scan;
-    __syncthreads();
-    int at = base + scan - count;
-    for (int w = 0; w < wave; ++w) at += wave_sum[w];
-    for (int i = 0; i < count && at + i < max_items; ++i)
-      items[at + i] = make_int4(expert, a + i * item_rows, min(item_rows, b - a - i * item_rows), 0);
-    __syncthreads();
-    if (tid == 0) {
-      int total = 0;
-      for (int w = 0; w < kItemThreads / kWave; ++w) total += wave_sum[w];
-      base += total;
-    }
-    __syncthreads();
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int other = __shfl_up(scan, d);
+    if (lane >= d) scan += other;
   }
-  if (tid == 0) *num_items = min(base, max_items);
+  if (lane == kWave - 1) sums[wave] = scan;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kPrepareThreads / kWave; ++w) {
+    if (w == wave) before = all;
+    all += sums[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + scan - v;
+}
+
+__device__ __forceinline__ void mx_write_items(const MxPrepare& p, int at, int expert, int first, int count) {
+  for (int i = 0; i * p.item_rows < count && at + i < p.max_items; ++i)
+    p.items[at + i] = make_int4(expert, first + i * p.item_rows, min(p.item_rows, count - i * p.item_rows), 0);
+}
+
+// Work items of ragged boundaries: group e's rows [b[e], b[e + 1]) in chunks
+// of item_rows; with zero_rest the rows before b[0] and from b[E] on as items
+// of expert -1.  Boundaries are clamped to [0, rows].
+__device__ __forceinline__ void mx_items_of_bounds(const MxPrepare& p, int* sums) {
+  const int entries = p.groups + (p.zero_rest ? 2 : 0);
+  auto bound = [&](int e) { return min(max(p.bounds[e], 0), p.count); };
+  int base = 0;
+  for (int from = 0; from < entries; from += kPrepareThreads) {
+    const int e = from + threadIdx.x;
+    int first = 0, last = 0, expert = -1;
+    if (e < p.groups)
+      first = bound(e), last = bound(e + 1), expert = e;
+    else if (e == p.groups && e < entries)
+      last = bound(0);
+    else if (e < entries)
+      first = bound(p.groups), last = p.count;
+    const int count = max(last - first, 0);
+    int total;
+    const int at = base + mx_scan((count + p.item_rows - 1) / p.item_rows, sums, &total);
+    mx_write_items(p, at, expert, first, count);
+    base += total;
+  }
+  if (threadIdx.x == 0) *p.num_items = min(base, p.max_items);
+}
+
+// Routes grouped by expert: sorted[] holds the pairs of expert 0, 1, ..; ids
+// that name no expert are left out.  A counting sort of one workgroup with
+// LDS atomics: the order of an expert's pairs may differ from call to call,
+// which no result depends on (a pair's row is multiplied by itself wherever it
+// stands, and its results are stored by pair).  kBatch pairs a thread are
+// loaded at once, so that up to 1024 kBatch pairs cost one round trip.
+template <int kBatch>
+__device__ __forceinline__ void mx_items_of_routes(const MxPrepare& p, int* cursor, int* sums) {
+  const int tid = threadIdx.x;
+  int expert[kBatch];
+  auto load = [&](int from) {
+    int64_t id[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int64_t at = min(from + j * kPrepareThreads + tid, p.count - 1);
+      id[j] = p.ids_i64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<const int32_t*>(p.ids)[at];
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      expert[j] = from + j * kPrepareThreads + tid < p.count && id[j] >= 0 && id[j] < p.groups ? static_cast<int>(id[j]) : -1;
+  };
+  constexpr int kRound = kPrepareThreads * kBatch;
+  const bool once = p.count <= kRound;  // uniform
+  if (tid < kMxSortExperts) cursor[tid] = 0;
+  load(0);
+  __syncthreads();
+  for (int from = 0; from < p.count; from += kRound) {
+    if (from > 0) load(from);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (expert[j] >= 0) atomicAdd(&cursor[expert[j]], 1);
+  }
+  __syncthreads();
+  const int count = tid < p.groups ? cursor[tid] : 0;
+  int total;
+  const int first = mx_scan(count, sums, &total);
+  if (tid < p.groups) cursor[tid] = first;
+  const int at = mx_scan((count + p.item_rows - 1) / p.item_rows, sums, &total);
+  mx_write_items(p, at, tid, first, count);
+  if (tid == 0) *p.num_items = min(total, p.max_items);
+  for (int from = 0; from < p.count; from += kRound) {
+    if (!once) load(from);
+    int place[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) place[j] = expert[j] >= 0 ? atomicAdd(&cursor[expert[j]], 1) : -1;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (place[j] >= 0) p.sorted[place[j]] = from + j * kPrepareThreads + tid;
+  }
+}
+
+// The same spread over workgroups of kChunkPairs pairs, for batches whose LDS
+// atomics one workgroup would be long at (29,344 pairs over 128 experts 26 us):
+// each ranks its pairs and counts its experts' beside the rows' quantisation,
+// then each sums the counts before its own and places its pairs.
+constexpr int kChunkPairs = 2 * kPrepareThreads;
+constexpr int kMxMaxChunks = 32;
+
+__device__ __forceinline__ int mx_route_expert(const MxPrepare& p, int pair) {
+  const int64_t at = min(pair, p.count - 1);
+  const int64_t id = p.ids_i64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<const int32_t*>(p.ids)[at];
+  return pair < p.count && id >= 0 && id < p.groups ? static_cast<int>(id) : -1;
+}
+
+__device__ __forceinline__ void mx_count_chunk(const MxPrepare& p, int chunk, int* counts) {
+  const int tid = threadIdx.x, first = chunk * kChunkPairs + tid;
+  const int e0 = mx_route_expert(p, first), e1 = mx_route_expert(p, first + kPrepareThreads);
+  if (tid < kMxSortExperts) counts[tid] = 0;
+  __syncthreads();
+  if (e0 >= 0) p.ranks[first] = atomicAdd(&counts[e0], 1);
+  if (e1 >= 0) p.ranks[first + kPrepareThreads] = atomicAdd(&counts[e1], 1);
+  __syncthreads();
+  if (tid < p.groups) p.chunk_counts[chunk * p.groups + tid] = counts[tid];
+}
+
+__global__ __launch_bounds__(kPrepareThreads) void mx_place_kernel(MxPrepare p) {
+  __shared__ int place[kMxSortExperts];
+  __shared__ int sums[kPrepareThreads / kWave];
+  const int tid = threadIdx.x, first = blockIdx.x * kChunkPairs + tid;
+  int expert[2], rank[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int pair = first + j * kPrepareThreads;
+    expert[j] = mx_route_expert(p, pair);
+    rank[j] = p.ranks[min(pair, p.count - 1)];  // (of a pair of no expert: not used)
+  }
+  int all = 0, before = 0;
+  if (tid < p.groups) {
+#pragma unroll 8
+    for (int c = 0; c < p.chunks; ++c) {
+      const int n = p.chunk_counts[c * p.groups + tid];
+      before += c < static_cast<int>(blockIdx.x) ? n : 0;
+      all += n;
+    }
+  }
+  int total;
+  const int start = mx_scan(all, sums, &total);
+  if (tid < p.groups) place[tid] = start + before;
+  const int at = mx_scan((all + p.item_rows - 1) / p.item_rows, sums, &total);
+  if (blockIdx.x == 0) {
+    mx_write_items(p, at, tid, start, all);
+    if (tid == 0) *p.num_items = min(total, p.max_items);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (expert[j] >= 0) p.sorted[place[expert[j]] + rank[j]] = first + j * kPrepareThreads;
+}
+
+template <int kWhat, int kBatch = 1>
+__global__ __launch_bounds__(kPrepareThreads) void mx_prepare_kernel(MxPrepare p) {
+  uint32_t block = blockIdx.x;
+  if constexpr (kWhat != kMxRowsOnly) {
+    __shared__ int cursor[kMxSortExperts];
+    __shared__ int sums[kPrepareThreads / kWave];
+    const uint32_t others = kWhat == kMxRouteChunks ? p.chunks : 1;
+    if (block < others) {
+      if constexpr (kWhat == kMxBounds)
+        mx_items_of_bounds(p, sums);
+      else if constexpr (kWhat == kMxRoutes)
+        mx_items_of_routes<kBatch>(p, cursor, sums);
+      else
+        mx_count_chunk(p, block, cursor);
+      return;
+    }
+    block -= others;
+  }
+  mx_quantize_units<false, true, kPrepareThreads>(p.rows, block);
 }
 
 // out[t, :] = sum over ranks r of weights[t, r] * down[t * top_k + r, :] in
@@ -806,37 +971,71 @@ void launch_stream(const MxGemm& g, int items, hipStream_t s) {
     hipLaunchKernelGGL((mx_stream_kernel<kRT, kEpi, 1, kDirect, kSource>), grid, block, 0, s, g, blocks);
 }
 
-// Items of up to kMxDirectRows rows whose bf16 rows are at hand.
-constexpr int kMxDirectRows = 32;
-template <int kEpi>
-void launch_direct(const MxGemm& g, int item_rows, int items, hipStream_t s) {
-  if (item_rows <= 16)
-    launch_stream<1, kEpi, true, kMxList>(g, items, s);
-  else
-    launch_stream<2, kEpi, true, kMxList>(g, items, s);
-}
+// How a product runs: streaming (16 rows an item, or 32; the rows bf16 where
+// they are at hand) or tiled (32, 64 or 128).
+struct MxChoice {
+  bool tiled;
+  int item_rows;
+};
 
 template <int kEpi>
-void launch_gemm(const MxGemm& g, int item_rows, int items, hipStream_t s) {
+void launch_gemm(const MxGemm& g, MxChoice c, int items, hipStream_t s) {
   if (items <= 0) return;
-  if (item_rows <= 16) {
-    launch_stream<1, kEpi, false, kMxList>(g, items, s);
-  } else if (item_rows <= 32) {
-    launch_stream<2, kEpi, false, kMxList>(g, items, s);
-  } else if (item_rows <= 64) {
-    launch_stream<4, kEpi, false, kMxList>(g, items, s);
-  } else {
-    const MxTiles tiles{mx_ceil(g.row_groups, kMxWaves), 2};
+  if (c.tiled) {
+    const MxTiles tiles{mx_ceil(g.row_groups, kMxWaves), 2, c.item_rows};
     const int runs = mx_ceil(items, kMxXcds * tiles.run) * kMxXcds;
     hipLaunchKernelGGL(mx_tiled_kernel<kEpi>, dim3(static_cast<unsigned>(runs) * tiles.run * tiles.n_tiles),
                        dim3(kMxThreads), 0, s, g, tiles);
+  } else if constexpr (kEpi == kMxBf16) {
+    if (c.item_rows <= 16)
+      launch_stream<1, kEpi, true, kMxList>(g, items, s);
+    else
+      launch_stream<2, kEpi, true, kMxList>(g, items, s);
+  } else {
+    launch_stream<1, kEpi, kEpi == kMxAct, kMxList>(g, items, s);
   }
 }
 
-// Rows per work item for groups of `mean` rows on average.
-int mx_item_rows(int64_t rows, int64_t groups) {
-  const int64_t mean = rows / groups;
-  return mean <= 16 ? 16 : (mean <= 32 ? 32 : (mean <= 64 ? 64 : kMxTiledRows));
+// Tiled items: as many rows as leave three quarters of the CUs a workgroup
+// (`partial`: items that groups end early), for a larger item reads the weights
+// less often.  Us at 32 / 64 / 128 rows an item, K and N 4096: 512 rows 19.5 /
+// 19.5 / 23.7, 1024 rows 26.8 / 21.5 / 26.8, 2048 rows 49 / 35 / 30; K 2048 N
+// 1281: 1024 rows 12.0 / 12.8 / 16.3, 4096 rows 22.4 / 20.4 / 20.1.
+constexpr int kMxEnoughTiles = 192;
+MxChoice choose_tiled(int64_t rows, int64_t partial, int64_t n) {
+  const int64_t n_tiles = mx_ceil(n, kMxRows * kMxWaves);
+  for (int item_rows = kMxTiledRows; item_rows > 32; item_rows /= 2)
+    if (((rows + item_rows - 1) / item_rows + partial) * n_tiles >= kMxEnoughTiles) return {true, item_rows};
+  return {true, 32};
+}
+
+int64_t stream_blocks(int64_t n, int64_t k) {
+  const int64_t split = k > 3 * kMxStep ? 4 : (k > kMxStep ? 2 : 1);
+  return mx_ceil(mx_ceil(n, kMxRows), kMxWaves / split);
+}
+
+// One matrix, every row: streaming while its workgroups are one round of the
+// CUs.  Us, streaming 16 / 32 rows an item against tiled: K 2048 N 1281, 192
+// rows 7.1 / 8.6 / 11.1, 384 rows 9.7 / 9.3 / 11.3, 512 rows 12.1 / 13.8 /
+// 11.5; K and N 4096, 64 rows 8.9 / 12.0 / 16.6, 128 rows 13.9 / 12.7 / 17.3,
+// 384 rows 33 / 29 / 18.5.
+constexpr int kMxCus = 256;
+MxChoice choose_linear(int64_t rows, int64_t n, int64_t k) {
+  const int64_t blocks = stream_blocks(n, k);
+  if (((rows + 15) / 16) * blocks <= kMxCus) return {false, 16};
+  if (((rows + 31) / 32) * blocks <= kMxCus) return {false, 32};
+  return choose_tiled(rows, 0, n);
+}
+
+// Rows grouped by expert.  Routed experts stream up to 8 rows an expert, or
+// while that is a few rounds of workgroups.  Us, streaming / tiled: E256 H2048
+// I512, 8 rows an expert 98.7 / 105, 16 rows 122 / 108; E16 H1024 I256, 32 rows
+// an expert 20.1 / 22.9, 96 rows 25.0 / 25.6, 128 rows 28.1 / 26.6.
+constexpr int kMxFewGroups = 832;
+MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n, int64_t k) {
+  const int64_t partial = (pairs < experts ? pairs : experts) / 2;
+  if (pairs <= 8 * experts || (pairs / 16 + partial) * stream_blocks(n, k) <= kMxFewGroups) return {false, 16};
+  return choose_tiled(pairs, partial, n);
 }
 
 // Byte arena of one call, carved in order at 256-byte boundaries.
@@ -857,45 +1056,68 @@ void set_weight(MxGemm& g, const uint8_t* w, const uint8_t* ws, int n, int k) {
 }
 
 // A grouped product takes one of three ways:
-//   direct   one group of few rows, or few rows over many groups: one launch
-//            that quantises the rows itself and, with boundaries, walks each
-//            group's row tiles (no work items);
+//   walk     few rows over many groups: one launch that walks each group's row
+//            tiles and quantises them itself (no work items);
+//   direct   few rows of one matrix: one launch that quantises them itself;
 //   else     quantised rows, work items from the boundaries, the product.
 constexpr int kMxWalkRows = 512;  // most rows of groups walked by their own workgroups: one busy group is walked alone
 struct GroupedPlan {
-  bool direct;
-  int item_rows, max_items;
+  bool walk;
+  MxChoice how;
+  int max_items;
   uint8_t *q, *qs;
   int4* items;
   int32_t* num_items;
   int64_t bytes;
 };
 
-GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, bool bounded, int k) {
+GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, bool bounded, int n, int k) {
   GroupedPlan p{};
-  p.item_rows = mx_item_rows(rows, experts);
-  p.direct = bounded ? rows <= kMxWalkRows && rows <= 16 * static_cast<int64_t>(experts) : rows <= kMxDirectRows;
-  if (p.direct) return p;
+  p.walk = bounded && rows <= kMxWalkRows && rows <= 16 * static_cast<int64_t>(experts);
+  if (p.walk) return p;
+  const int64_t partial = rows < experts ? rows : experts;
+  p.how = bounded ? choose_tiled(rows, partial / 2, n) : choose_linear(rows, n, k);
   // every group, and each of the two runs of rows in none, adds one partial item at most
-  p.max_items = static_cast<int>(rows / p.item_rows + (rows < experts + 2 ? rows : experts + 2));
+  p.max_items = bounded ? static_cast<int>(rows / p.how.item_rows + (rows < experts + 2 ? rows : experts + 2))
+                        : mx_ceil(rows, p.how.item_rows);
+  if (!p.how.tiled) return p;
   Arena a{static_cast<uint8_t*>(arena)};
   p.q = a.take<uint8_t>(rows * mx_ceil(k, kMxStep) * kMxOperandCodes);
   p.qs = a.take<uint8_t>(rows * mx_ceil(k, kMxStep) * kMxOperandScales);
-  p.items = a.take<int4>(p.max_items);
-  p.num_items = a.take<int32_t>(1);
+  if (bounded) {
+    p.items = a.take<int4>(p.max_items);
+    p.num_items = a.take<int32_t>(1);
+  }
   p.bytes = a.used;
   return p;
 }
 
-constexpr int kMxSortTile = 16;
-constexpr int kMxWidePairs = 8192;  // more (row, rank) pairs: the sort spread over many workgroups
-constexpr int kMxFewPairs = 64;    // up to so many pairs each is an item of its own
+MxQuantize operand_rows(const uint16_t* x, int64_t stride, int64_t rows, int k, uint8_t* codes, uint8_t* scales) {
+  const uint32_t per_row = static_cast<uint32_t>(k) / 8;
+  return {x, stride, static_cast<uint64_t>(rows) * per_row, per_row, mx_ceil(k, kMxStep), codes, scales};
+}
+
+unsigned prepare_blocks(const MxQuantize& q) {
+  constexpr uint64_t kPerBlock = kPrepareThreads * kMxQuantizeUnits;
+  return static_cast<unsigned>((q.units + kPerBlock - 1) / kPerBlock);
+}
+
+// Up to so many pairs each is an item of its own, whatever their experts:
+// E256 H2048 I512, 64 / 128 / 192 / 256 pairs 23.9 / 36.3 / 49.7 / 61.8 us
+// against 32.3 / 42.9 / 53.2 / 61.1 with the routes grouped; E128 I768, 64 /
+// 128 / 192 pairs 30.9 / 46.7 / 62.9 against 38.8 / 48.7 / 55.8.
+constexpr int kMxFewPairs = 128;
+// Up to so many pairs are grouped by one workgroup, up to kMxMaxChunks chunks by
+// a workgroup a chunk, more by the route sort over many workgroups.
+constexpr int kMxOnePairs = 8 * kPrepareThreads;
 struct MoePlan {
-  bool few, direct;  // few: no sort, down product and combine in one launch; direct: FC1 quantises its rows itself
-  int item_rows, max_items, max_rows;
+  bool few;   // no grouping, down product and combine in one launch
+  int chunks;  // 0: one workgroup groups the pairs; above kMxMaxChunks: the route sort
+  MxChoice how;
+  int max_items;
   int64_t pairs, scratch_ints;
   uint8_t *q, *qs, *act, *acts;
-  uint16_t* down;
+  uint16_t* rows;  // down rows
   uint8_t* exponents;
   int32_t *counts, *starts, *total, *sorted, *expert_ids, *num_items, *scratch;
   int4* items;
@@ -905,33 +1127,35 @@ struct MoePlan {
 MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, int inter) {
   MoePlan p{};
   p.pairs = rows * top_k;
-  p.item_rows = mx_item_rows(p.pairs, experts);
-  const int32_t pairs = static_cast<int32_t>(p.pairs);
-  p.max_rows = d3_max_sorted_rows(pairs, experts, kMxSortTile);
-  p.max_items = d3_max_items(pairs, experts, p.item_rows);
-  p.scratch_ints = p.pairs > kMxWidePairs ? d3_sort_wide_scratch_ints(static_cast<int32_t>(rows), top_k, experts) : 0;
+  p.few = p.pairs <= kMxFewPairs;
+  p.chunks = p.pairs <= kMxOnePairs ? 0 : mx_ceil(p.pairs, kChunkPairs);
+  p.how = choose_routed(p.pairs, experts, 2 * static_cast<int64_t>(inter), hidden);
+  p.max_items = d3_max_items(static_cast<int32_t>(p.pairs), experts, p.how.item_rows);
   Arena a{static_cast<uint8_t*>(arena)};
   const int64_t x_steps = mx_ceil(hidden, kMxStep), act_steps = mx_ceil(inter, kMxStep);
-  p.few = p.pairs <= kMxFewPairs;
-  p.direct = p.few || p.item_rows <= kMxDirectRows;
-  if (p.few) p.max_rows = pairs;
-  p.act = a.take<uint8_t>(p.max_rows * act_steps * kMxOperandCodes);
-  p.acts = a.take<uint8_t>(p.max_rows * act_steps * kMxOperandScales);
-  if (!p.direct) {
-    p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
-    p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
-  }
+  p.act = a.take<uint8_t>(p.pairs * act_steps * kMxOperandCodes);
+  p.acts = a.take<uint8_t>(p.pairs * act_steps * kMxOperandScales);
   if (!p.few) {
-    p.down = a.take<uint16_t>(p.pairs * hidden);
+    if (p.how.tiled) {
+      p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
+      p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
+    }
+    p.rows = a.take<uint16_t>(p.pairs * hidden);
     p.exponents = a.take<uint8_t>(p.pairs * (hidden / kMxRows));
-    p.counts = a.take<int32_t>(experts);
-    p.starts = a.take<int32_t>(experts);
-    p.total = a.take<int32_t>(1);
-    p.sorted = a.take<int32_t>(p.max_rows);
-    p.expert_ids = a.take<int32_t>(p.max_rows / kMxSortTile);
+    p.sorted = a.take<int32_t>(p.pairs);
     p.items = a.take<int4>(p.max_items);
     p.num_items = a.take<int32_t>(1);
-    p.scratch = a.take<int32_t>(p.scratch_ints);
+    if (p.chunks > 0 && p.chunks <= kMxMaxChunks) {
+      p.counts = a.take<int32_t>(static_cast<int64_t>(p.chunks) * experts);
+      p.scratch = a.take<int32_t>(p.pairs);
+    } else if (p.chunks > 0) {
+      p.scratch_ints = d3_sort_wide_scratch_ints(static_cast<int32_t>(rows), top_k, experts);
+      p.counts = a.take<int32_t>(experts);
+      p.starts = a.take<int32_t>(experts);
+      p.total = a.take<int32_t>(1);
+      p.expert_ids = a.take<int32_t>(p.pairs);
+      p.scratch = a.take<int32_t>(p.scratch_ints);
+    }
   }
   p.bytes = a.used;
   return p;
@@ -951,9 +1175,10 @@ bool moe_shape(int64_t rows, int top_k, int experts, int hidden, int inter) {
 
 using namespace d3;
 
-extern "C" int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bounded, int32_t k) {
-  if (!grouped_shape(rows, num_experts, 1, k)) return -1;
-  return plan_grouped(nullptr, rows, num_experts, bounded != 0, k).bytes;
+extern "C" int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bounded, int32_t n,
+                                              int32_t k) {
+  if (!grouped_shape(rows, num_experts, n, k)) return -1;
+  return plan_grouped(nullptr, rows, num_experts, bounded != 0, n, k).bytes;
 }
 
 extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t rows, const int32_t* boundaries,
@@ -972,11 +1197,11 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
     clear_error();
     return D3_OK;
   }
-  const GroupedPlan p = plan_grouped(workspace, rows, num_experts, boundaries != nullptr, k);
+  const GroupedPlan p = plan_grouped(workspace, rows, num_experts, boundaries != nullptr, n, k);
   D3_REQUIRE(p.bytes == 0 || (workspace != nullptr && workspace_bytes >= p.bytes),
              "mxfp4_grouped: workspace of %lld bytes < required %lld", static_cast<long long>(workspace_bytes),
              static_cast<long long>(p.bytes));
-  const int64_t most = p.direct ? num_experts + 1 : p.max_items;
+  const int64_t most = p.walk ? num_experts + 1 : p.max_items;
   D3_SUPPORTED(most * mx_ceil(n, kMxRows) < (int64_t{1} << 31), "mxfp4_grouped: more than 2^31 workgroups");
   hipStream_t s = as_stream(stream);
   MxGemm g{};
@@ -984,22 +1209,24 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
   g.a = p.q, g.as = p.qs, g.x = x, g.x_stride = x_row_stride, g.rows = static_cast<int>(rows);
   g.experts = num_experts, g.bounds = boundaries, g.zero_rest = zero_rest;
   g.out = out, g.out_stride = out_row_stride;
-  if (p.direct) {
-    if (boundaries != nullptr)
-      launch_stream<2, kMxBf16, true, kMxGroups>(g, num_experts + 1, s);
-    else
-      launch_direct<kMxBf16>(g, static_cast<int>(rows), 1, s);
+  if (p.walk) {
+    launch_stream<2, kMxBf16, true, kMxGroups>(g, num_experts + 1, s);
     D3_LAUNCHED("mxfp4_grouped");
   }
-  mx_quantize_operand(x, x_row_stride, rows, k, p.q, p.qs, s);
-  int items = mx_ceil(rows, p.item_rows);
-  if (boundaries != nullptr) {
-    hipLaunchKernelGGL(mx_items_kernel, dim3(1), dim3(kItemThreads), 0, s, boundaries, num_experts,
-                       static_cast<int>(rows), p.item_rows, zero_rest, p.max_items, p.items, p.num_items);
+  if (p.how.tiled) {
+    MxPrepare prepare{};
+    prepare.rows = operand_rows(x, x_row_stride, rows, k, p.q, p.qs);
+    prepare.bounds = boundaries, prepare.groups = num_experts, prepare.count = static_cast<int>(rows);
+    prepare.zero_rest = zero_rest, prepare.item_rows = p.how.item_rows, prepare.max_items = p.max_items;
+    prepare.items = p.items, prepare.num_items = p.num_items;
+    const unsigned blocks = prepare_blocks(prepare.rows);
+    if (boundaries != nullptr)
+      hipLaunchKernelGGL(mx_prepare_kernel<kMxBounds>, dim3(blocks + 1), dim3(kPrepareThreads), 0, s, prepare);
+    else
+      hipLaunchKernelGGL(mx_prepare_kernel<kMxRowsOnly>, dim3(blocks), dim3(kPrepareThreads), 0, s, prepare);
     g.items = p.items, g.num_items = p.num_items;
-    items = p.max_items;
   }
-  launch_gemm<kMxBf16>(g, p.item_rows, items, s);
+  launch_gemm<kMxBf16>(g, p.how, p.max_items, s);
   D3_LAUNCHED("mxfp4_grouped");
 }
 
@@ -1057,33 +1284,46 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
                        down, weights, f32);
     D3_LAUNCHED("mxfp4_moe");
   }
-  int status;
-  const int32_t rows32 = static_cast<int32_t>(rows);
-  if (p.scratch_ints > 0)
-    status = d3_sort_routes_wide(ids, ids_dtype, rows32, nullptr, top_k, num_experts, kMxSortTile, p.counts, p.starts,
-                                 p.total, p.sorted, p.expert_ids, p.max_rows, nullptr, p.item_rows,
-                                 reinterpret_cast<int32_t*>(p.items), p.max_items, p.num_items, nullptr, p.scratch,
-                                 p.scratch_ints, stream);
-  else
-    status = d3_sort_routes(ids, ids_dtype, rows32, nullptr, top_k, num_experts, kMxSortTile, p.counts, p.starts, p.total,
-                            p.sorted, p.expert_ids, p.max_rows, nullptr, p.item_rows, reinterpret_cast<int32_t*>(p.items),
-                            p.max_items, p.num_items, nullptr, stream);
-  if (status != D3_OK) return status;
-  if (p.direct) {
-    launch_direct<kMxAct>(up, p.item_rows, p.max_items, s);
-  } else {
-    mx_quantize_operand(x, x_row_stride, rows, hidden, p.q, p.qs, s);
-    launch_gemm<kMxAct>(up, p.item_rows, p.max_items, s);
+  MxPrepare prepare{};
+  unsigned blocks = 0;
+  if (p.how.tiled) {
+    prepare.rows = operand_rows(x, x_row_stride, rows, hidden, p.q, p.qs);
+    blocks = prepare_blocks(prepare.rows);
   }
-  down.out = p.down, down.out_scales = p.exponents;
-  launch_gemm<kMxHalf>(down, p.item_rows, p.max_items, s);
+  if (p.chunks > kMxMaxChunks) {
+    const int status = d3_sort_routes_wide(
+        ids, ids_dtype, static_cast<int32_t>(rows), nullptr, top_k, num_experts, 1, p.counts, p.starts, p.total, p.sorted,
+        p.expert_ids, static_cast<int32_t>(p.pairs), nullptr, p.how.item_rows, reinterpret_cast<int32_t*>(p.items),
+        p.max_items, p.num_items, nullptr, p.scratch, p.scratch_ints, stream);
+    if (status != D3_OK) return status;
+    if (blocks > 0)
+      hipLaunchKernelGGL(mx_prepare_kernel<kMxRowsOnly>, dim3(blocks), dim3(kPrepareThreads), 0, s, prepare);
+  } else {
+    prepare.groups = num_experts, prepare.count = static_cast<int>(p.pairs);
+    prepare.ids = ids, prepare.ids_i64 = i64, prepare.sorted = p.sorted;
+    prepare.item_rows = p.how.item_rows, prepare.max_items = p.max_items;
+    prepare.items = p.items, prepare.num_items = p.num_items;
+    prepare.chunks = p.chunks, prepare.chunk_counts = p.counts, prepare.ranks = p.scratch;
+    const dim3 block(kPrepareThreads);
+    if (p.chunks > 0) {
+      hipLaunchKernelGGL(mx_prepare_kernel<kMxRouteChunks>, dim3(blocks + p.chunks), block, 0, s, prepare);
+      hipLaunchKernelGGL(mx_place_kernel, dim3(p.chunks), block, 0, s, prepare);
+    } else if (p.pairs <= kPrepareThreads) {
+      hipLaunchKernelGGL((mx_prepare_kernel<kMxRoutes, 1>), dim3(blocks + 1), block, 0, s, prepare);
+    } else {
+      hipLaunchKernelGGL((mx_prepare_kernel<kMxRoutes, 8>), dim3(blocks + 1), block, 0, s, prepare);
+    }
+  }
+  launch_gemm<kMxAct>(up, p.how, p.max_items, s);
+  down.out = p.rows, down.out_scales = p.exponents;
+  launch_gemm<kMxHalf>(down, p.how, p.max_items, s);
   const int slices = mx_ceil(hidden, kMxCombineColumns);
   const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
   if (top_k == 8)
-    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.down, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
+    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
                        slices, out);
   else
-    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.down, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
+    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
                        slices, out);
   D3_LAUNCHED("mxfp4_moe");
 }

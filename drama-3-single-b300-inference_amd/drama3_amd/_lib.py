@@ -114,7 +114,7 @@ SIGNATURES = {
     "d3_mxfp4_packed_bytes": (_i64, [_i32, _i32, _i32, _i32]),
     "d3_mxfp4_grouped": (
         _i32, [_p, _i64, _i64, _p, _i32, _p, _p, _i32, _i32, _p, _i64, _i32, _p, _i64, _p]),
-    "d3_mxfp4_grouped_workspace": (_i64, [_i64, _i32, _i32, _i32]),
+    "d3_mxfp4_grouped_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32]),
     "d3_mxfp4_moe": (
         _i32, [_p, _i64, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p,
                _i64, _p]),

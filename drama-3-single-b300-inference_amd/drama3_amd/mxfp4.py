@@ -236,7 +236,8 @@ def _product(x, boundaries, weight: Mxfp4Weight, out, zero_rest: bool) -> torch.
     _same_device(x, weight.codes, "weight")
     if out is None:
         out = torch.empty((rows, weight.n), dtype=torch.bfloat16, device=x.device)
-    size = _entry("d3_mxfp4_grouped_workspace")(rows, weight.experts, boundaries is not None, k)
+    size = _entry("d3_mxfp4_grouped_workspace")(rows, weight.experts, boundaries is not None,
+                                                  weight.n, k)
     workspace, at = _workspace(size, x)
     _call(x.device, "d3_mxfp4_grouped", ptr(x), x.stride(0), rows, ptr(boundaries), weight.experts,
           ptr(weight.codes), ptr(weight.scales), weight.n, k, ptr(out), out.stride(0),
@@ -283,7 +284,7 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     """Routed SwiGLU experts: for row t and rank r with expert e =
     ``topk_ids[t, r]``, ``a = silu(G_e x) * (U_e x)`` and ``out[t] = sum_r
     topk_weights[t, r] * W2_e a`` in rank order, with x and a quantised to
-    MXFP4 and fp32 sums, rounded to bf16 [T, H] once.  (Above 64 pairs the
+    MXFP4 and fp32 sums, rounded to bf16 [T, H] once.  (Above 128 pairs the
     ranks' rows are held as scaled fp16 in between, whose rounding is an
     eighth of bf16's.)
 

@@ -828,14 +828,15 @@ int d3_mxfp4_grouped(const uint16_t *x, int64_t x_row_stride, int64_t rows,
 
 /* Workspace bytes of d3_mxfp4_grouped (host-side arithmetic only; 0: none is
  * needed; -1: not supported).  bounded: whether boundaries are given. */
-int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bounded, int32_t k);
+int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bounded, int32_t n,
+                                   int32_t k);
 
 /*
  * Routed SwiGLU experts on MXFP4 weights: for every row t and rank r with
  * expert e = ids[t, r], a = silu(G x) * (U x) with x quantised to MXFP4 and
  * [G; U] = w13[e] (order 1), a quantised to MXFP4 from its fp32 values, and
  *   out[t] = sum over r of weights[t, r] * (w2[e] (order 0) a)
- * in rank order, the sums fp32, rounded to bf16 once (above 64 pairs each
+ * in rank order, the sums fp32, rounded to bf16 once (above 128 pairs each
  * rank's row is first rounded to a scaled fp16, an eighth of bf16's step).
  * ids int32 or int64
  * [rows, top_k] (an id outside [0, num_experts) adds nothing), weights bf16 or

@@ -340,17 +340,21 @@ def test_moe_repeated_experts_and_nan_rows(device):
     assert torch.equal(out[keep], clean[keep])
 
 
-def test_moe_many_pairs(device):
-    """More pairs than one workgroup sorts."""
+@pytest.mark.parametrize("rows, id_type", [(1000, torch.int32), (1500, torch.int64), (8192, torch.int32),
+                                           (9000, torch.int64)])
+def test_moe_many_pairs(device, rows, id_type):
+    """More pairs than one workgroup has threads, than it groups, and than
+    workgroups by chunk do; now and then an id that names no expert."""
     from drama3_amd.mxfp4 import mxfp4_moe
 
     rng = np.random.default_rng(19)
     packed, v13, v2 = make_experts(rng, 24, 128, 128, device)
-    x = rows_of(rng, 1500, 128)
-    ids, weights = make_routes(rng, 1500, 24, 8, 0.7)
-    weights = weights.to(torch.bfloat16)
+    x = rows_of(rng, rows, 128)
+    ids, weights = make_routes(rng, rows, 24, 8, 0.7)
+    ids[rng.random(ids.shape) < 0.02] = -5
+    ids, weights = ids.to(id_type), weights.to(torch.bfloat16)
     out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
-    pick = rng.choice(1500, 150, replace=False)
+    pick = rng.choice(rows, 150, replace=False)
     want, bound = om.moe(f64(x)[pick], ids.numpy()[pick], f64(weights)[pick], v13, v2)
     within(out[torch.from_numpy(pick).to(device)], want, bound)
 

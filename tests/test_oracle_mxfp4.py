@@ -113,7 +113,7 @@ def test_c_entries_refuse_before_launching(lib):
     refused("pairs", "d3_mxfp4_moe", moe, a2=1 << 24)
     lib_ = lib.load()
     assert lib_.d3_mxfp4_moe_workspace(4, 8, 513, 256, 128) == -1
-    assert lib_.d3_mxfp4_grouped_workspace(4, 8, 1, 100) == -1
+    assert lib_.d3_mxfp4_grouped_workspace(4, 8, 1, 64, 100) == -1
     assert lib_.d3_mxfp4_packed_bytes(0, 64, 256, 0) == -1
     # padded to whole row groups of 64 and steps of 256
     assert lib_.d3_mxfp4_packed_bytes(3, 65, 384, 0) == 3 * 128 * 512 // 2
