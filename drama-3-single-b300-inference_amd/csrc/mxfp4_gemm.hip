@@ -33,12 +33,14 @@ struct MxGemm {
   int row_groups;
   int steps;
   const uint8_t* a;  // quantised rows (operand layout, `steps` steps)
+  int64_t a_rows;
   const uint8_t* as;
   const uint16_t* x;  // or the rows themselves, bf16 [rows][k], quantised by the wave that multiplies them
   int64_t x_stride;
   int k_blocks;       // k / 32
   const int4* items;  // {expert (-1: zero rows), first row, rows, -}; nullptr: one expert, `rows` in order
   const int32_t* num_items;
+  int max_items;
   int rows;
   const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxHalf);
   int top_k;              // nullptr: the identity
@@ -74,8 +76,10 @@ __device__ __forceinline__ int4 mx_item(const MxGemm& g, int index, int item_row
     const int start = index * item_rows;
     return make_int4(0, start, min(item_rows, g.rows - start), 0);
   }
-  if (index >= *g.num_items) return make_int4(0, 0, 0, 0);
-  return g.items[index];
+  // Read with the count, not after it: every index below max_items is in the list.
+  const int live = *g.num_items;
+  const int4 item = g.items[min(index, g.max_items - 1)];
+  return index < live ? item : make_int4(0, 0, 0, 0);
 }
 
 // Eight values as bf16, or as the fp16 of kMxHalf.
@@ -401,9 +405,11 @@ __global__ __launch_bounds__(kMxThreads) void mx_down_combine_kernel(MxGemm g, c
 // four bodies (1 to 4 tiles of 32 rows) that holds it.
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 constexpr int kMxTiledRows = 128;
-constexpr int kMxSlotCodes = kMxTiledRows * kMxOperandCodes;    // 16 KiB
-constexpr int kMxSlot = kMxSlotCodes + kMxTiledRows * kMxOperandScales;  // and 1 KiB of scales
+constexpr int kMxSlotScales = kMxThreads * 4;  // (a word a thread)
+constexpr int mx_slot_codes(int tiles) { return 32 * tiles * kMxOperandCodes; }
+constexpr int mx_slot(int tiles) { return mx_slot_codes(tiles) + kMxSlotScales; }
 constexpr int kMxXcds = 8;
+constexpr uint32_t kMxNowhere = 0xfffffff0u;  // an offset past every view
 
 // f(integral_constant 0), .., f(integral_constant N - 1).
 template <class F, int... I>
@@ -506,9 +512,10 @@ __device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[
   }
 }
 
-template <int kRT, int kEpi>
+template <int kRT, int kEpi, int kMax>
 __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item, int n_tile, uint8_t* ring,
                                               int32_t* targets) {
+  constexpr int kSlotCodes = mx_slot_codes(kMax), kSlot = mx_slot(kMax);
   const int tid = threadIdx.x, lane = lane_id(), col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int rg = n_tile * kMxWaves + wave;
@@ -516,19 +523,32 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   const int count = min(item.z, 32 * kRT);
   const int steps = g.steps;
 
-  auto source_row = [&](int r) -> int64_t {  // rows past the item: its last row
-    const int at = item.y + min(r, count - 1);
-    if constexpr (kEpi == kMxAct) return g.sorted[at] / g.top_k;
-    return at;
+  // A thread stages part lane % 8 of rows 32 i + 8 wave + lane / 8, and four of
+  // the eight scales of row tid / 2; rows past the item: its last row.  Offsets
+  // are from the first quantised row (gathered rows; the host keeps them within
+  // 32 bits) or from the item's first.
+  const uint32_t pitch = static_cast<uint32_t>(steps) * kMxOperandCodes;
+  const uint32_t scale_pitch = static_cast<uint32_t>(steps) * kMxOperandScales;
+  constexpr bool kGather = kEpi == kMxAct;
+  const int64_t first_row = kGather ? 0 : item.y;
+  const int64_t view_rows = kGather ? g.a_rows : count;
+  const __amdgpu_buffer_rsrc_t rows = BufferView(g.a + first_row * pitch, static_cast<uint32_t>(view_rows * pitch)).rsrc;
+  const __amdgpu_buffer_rsrc_t row_scales =
+      BufferView(g.as + first_row * scale_pitch, static_cast<uint32_t>(view_rows * scale_pitch)).rsrc;
+  auto source_row = [&](int r) -> uint32_t {
+    const int at = min(r, count - 1);
+    return kGather ? static_cast<uint32_t>(g.sorted[item.y + at]) / static_cast<uint32_t>(g.top_k)
+                   : static_cast<uint32_t>(at);
   };
-  // A thread stages part lane % 8 of rows 32 i + 8 wave + lane / 8,
   const int stage_row = 8 * wave + (lane >> 3), part = lane & 7;
-  const uint8_t* src[kRT];
+  uint32_t src[kRT + 1];
 #pragma unroll
-  for (int i = 0; i < kRT; ++i) src[i] = g.a + source_row(32 * i + stage_row) * steps * kMxOperandCodes + 16 * part;
+  for (int i = 0; i < kRT; ++i) src[i] = source_row(32 * i + stage_row);
+  src[kRT] = source_row(tid >> 1);
+#pragma unroll
+  for (int i = 0; i < kRT; ++i) src[i] = src[i] * pitch + 16 * part;
+  src[kRT] = src[kRT] * scale_pitch + 4 * (tid & 1);
   const int stage_at = stage_row * kMxOperandCodes + 16 * (part ^ (stage_row & 7));
-  // and four of the eight scales of row tid / 2.
-  const uint8_t* scale_src = g.as + source_row(tid >> 1) * steps * kMxOperandScales + 4 * (tid & 1);
 
   // Weight operand (half u, slice q) of a step: row 32 u + col, block 2 q + hl,
   // which is tile 2 u + col / 16, half q / 2, group 2 (q % 2) + hl of the
@@ -541,31 +561,37 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   const int ws_lane = (hl * 16 + (col & 15)) * 8;
   const int odd = 8 * (col >> 4);
 
-  int32x4 wf[4][2], copy[kRT], operand[4];
+  struct Rows {  // a step's rows on their way to LDS
+    int32x4 codes[kRT];
+    uint32_t scales;
+  };
+  int32x4 wf[4][2], operand[4];
   floatx2_hw wraw[2];
-  uint32_t copy_scale, sb[kRT], sb_next[kRT], wsc[4];
-  auto load_weight = [&](int step, auto slice, auto half) {  // past the last step: zeros, nothing read
+  uint32_t sb[kRT], sb_next[kRT], wsc[4];
+  // Past the last step these read nothing: out of their views' range.
+  auto load_weight = [&](int step, auto slice, auto half) {
     constexpr int q = decltype(slice)::value, u = decltype(half)::value;
-    wf[q][u] = __builtin_amdgcn_raw_buffer_load_b128(w, w_lane + (q / 2) * 4096 + (q % 2) * 512 + 2048 * u,
-                                                     step * kMxStepCodes, 0);
+    wf[q][u] = __builtin_amdgcn_raw_buffer_load_b128(
+        w, w_lane + step * kMxStepCodes + (q / 2) * 4096 + (q % 2) * 512 + 2048 * u, 0, 0);
   };
-  auto load_scales = [&](int step, auto part) {
-    constexpr int i = decltype(part)::value;
-    wraw[i] = __builtin_bit_cast(floatx2_hw, __builtin_amdgcn_raw_buffer_load_b64(ws, ws_lane + 256 * i,
-                                                                                  step * kMxStepScales, 0));
+  auto load_scales = [&](int step, auto index) {
+    constexpr int i = decltype(index)::value;
+    wraw[i] = __builtin_bit_cast(
+        floatx2_hw, __builtin_amdgcn_raw_buffer_load_b64(ws, ws_lane + step * kMxStepScales + 256 * i, 0, 0));
   };
-  auto load_row = [&](int step, auto copies) {
-    constexpr int i = decltype(copies)::value;
-    const int at = min(step, steps - 1);
+  auto load_row = [&](Rows& to, int step, auto index) {
+    constexpr int i = decltype(index)::value;
+    const bool live = step < steps;  // uniform
     if constexpr (i < kRT)
-      copy[i] = *reinterpret_cast<const int32x4*>(src[i] + at * kMxOperandCodes);
+      to.codes[i] = __builtin_amdgcn_raw_buffer_load_b128(rows, live ? src[i] + step * kMxOperandCodes : kMxNowhere, 0, 0);
     else
-      copy_scale = *reinterpret_cast<const uint32_t*>(scale_src + at * kMxOperandScales);
+      to.scales = __builtin_amdgcn_raw_buffer_load_b32(row_scales, live ? src[i] + step * kMxOperandScales : kMxNowhere, 0, 0);
   };
-  auto store_rows = [&](uint8_t* slot) {
+  auto store_rows = [&](uint8_t* slot, const Rows& from) {
 #pragma unroll
-    for (int i = 0; i < kRT; ++i) *reinterpret_cast<int32x4*>(slot + stage_at + 32 * i * kMxOperandCodes) = copy[i];
-    *reinterpret_cast<uint32_t*>(slot + kMxSlotCodes + tid * 4) = copy_scale;
+    for (int i = 0; i < kRT; ++i)
+      *reinterpret_cast<int32x4*>(slot + stage_at + 32 * i * kMxOperandCodes) = from.codes[i];
+    *reinterpret_cast<uint32_t*>(slot + kSlotCodes + tid * 4) = from.scales;
   };
   auto read_operand = [&](const uint8_t* slot, auto unit) {
     constexpr int i = decltype(unit)::value, q = i / kRT, rt = i % kRT;
@@ -574,12 +600,12 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   };
   auto read_scale = [&](const uint8_t* slot, auto tile) {
     constexpr int rt = decltype(tile)::value;
-    sb_next[rt] = *reinterpret_cast<const uint32_t*>(slot + kMxSlotCodes + (32 * rt + col) * kMxOperandScales + 4 * hl);
+    sb_next[rt] = *reinterpret_cast<const uint32_t*>(slot + kSlotCodes + (32 * rt + col) * kMxOperandScales + 4 * hl);
   };
 
   // Where the item's rows go, for the stores (written before the first barrier).
   if constexpr (kEpi == kMxHalf)
-    if (tid < kMxTiledRows) targets[tid] = g.sorted[item.y + min(tid, count - 1)];
+    if (tid < 32 * kRT) targets[tid] = g.sorted[item.y + min(tid, count - 1)];
 
   floatx16 acc[kRT][2];
 #pragma unroll
@@ -602,22 +628,26 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   constexpr int kUnits = 4 * kRT, kAhead = 3;
   constexpr int kBarrier = kUnits / 2 <= kUnits - kAhead ? kUnits / 2 : kUnits - kAhead;
   using std::integral_constant;
-  mx_each<kRT + 1>([&](auto i) { load_row(0, i); });
-  mx_each<2>([&](auto i) { load_scales(0, i); });
-  mx_each<3>([&](auto q) {
-    load_weight(0, q, integral_constant<int, 0>{});
-    load_weight(0, q, integral_constant<int, 1>{});
-  });
-  store_rows(ring);
-  mx_each<kRT + 1>([&](auto i) { load_row(1, i); });
-  store_rows(ring + kMxSlot);
-  mx_each<kRT + 1>([&](auto i) { load_row(2, i); });
+  Rows next;
+  {
+    Rows now;
+    mx_each<kRT + 1>([&](auto i) { load_row(now, 0, i); });
+    mx_each<2>([&](auto i) { load_scales(0, i); });
+    mx_each<kRT + 1>([&](auto i) { load_row(next, 1, i); });
+    mx_each<3>([&](auto q) {
+      load_weight(0, q, integral_constant<int, 0>{});
+      load_weight(0, q, integral_constant<int, 1>{});
+    });
+    store_rows(ring, now);
+  }
+  store_rows(ring + kSlot, next);
+  mx_each<kRT + 1>([&](auto i) { load_row(next, 2, i); });
   lds_barrier();
   mx_each<kAhead>([&](auto i) { read_operand(ring, i); });
   mx_each<kRT>([&](auto i) { read_scale(ring, i); });
   const uint8_t* slot = ring;
-  const uint8_t* slot_next = ring + kMxSlot;
-  uint8_t* slot_free = ring + 2 * kMxSlot;
+  const uint8_t* slot_next = ring + kSlot;
+  uint8_t* slot_free = ring + 2 * kSlot;
   for (int step = 0; step < steps; ++step) {
     wsc[0] = __float_as_uint(wraw[0][0]) >> odd, wsc[1] = __float_as_uint(wraw[1][0]) >> odd;
     wsc[2] = __float_as_uint(wraw[0][1]) >> odd, wsc[3] = __float_as_uint(wraw[1][1]) >> odd;
@@ -627,7 +657,7 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
       constexpr int i = decltype(unit)::value, q = i / kRT, rt = i % kRT;
       if constexpr (i == kBarrier) {
         lds_barrier();
-        store_rows(slot_free);
+        store_rows(slot_free, next);
       }
       if constexpr (i + kAhead < kUnits)
         read_operand(slot, integral_constant<int, i + kAhead>{});
@@ -644,8 +674,8 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
         load_scales(step + 1, integral_constant<int, 0>{});
         load_scales(step + 1, integral_constant<int, 1>{});
       }
-      if constexpr (q == 2 && rt == kRT - 1) load_row(step + 3, integral_constant<int, kRT>{});
-      if constexpr (q == 3) load_row(step + 3, integral_constant<int, rt>{});
+      if constexpr (q == 2 && rt == kRT - 1) load_row(next, step + 3, integral_constant<int, kRT>{});
+      if constexpr (q == 3) load_row(next, step + 3, integral_constant<int, rt>{});
       acc[rt][0] = mfma_fp4_32<0, q>(wf[q][0], operand[i % 4], acc[rt][0], wsc[q], sb[rt]);
       acc[rt][1] = mfma_fp4_32<2, q>(wf[q][1], operand[i % 4], acc[rt][1], wsc[q], sb[rt]);
       __builtin_amdgcn_sched_barrier(0);
@@ -657,18 +687,19 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   }
   lds_barrier();
   if (rg >= g.row_groups) return;
-  // Every wave has left the ring: two areas of it a wave take turns.
+  // Every wave has left the ring: its areas a wave's own (two that take turns,
+  // where there is room).
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt)
-    mx_store32<kEpi>(g, acc[rt], rg, item, 32 * rt, count, targets, ring + (2 * wave + rt % 2) * kMxStoreArea);
+    mx_store32<kEpi>(g, acc[rt], rg, item, 32 * rt, count, targets, ring + (kMax > 2 ? 2 * wave + rt % 2 : wave) * kMxStoreArea);
 }
 
-template <int kEpi>
-__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2))) void mx_tiled_kernel(MxGemm g,
-                                                                                                      MxTiles tiles) {
-  __shared__ __attribute__((aligned(16))) uint8_t ring[3 * kMxSlot];
-  static_assert(2 * kMxWaves * kMxStoreArea <= 3 * kMxSlot, "the waves' store areas fit the ring");
-  __shared__ int32_t targets[kEpi == kMxHalf ? kMxTiledRows : 1];
+template <int kEpi, int kMax>
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(kMax > 2 ? 2 : 3))) void mx_tiled_kernel(
+    MxGemm g, MxTiles tiles) {
+  __shared__ __attribute__((aligned(16))) uint8_t ring[3 * mx_slot(kMax)];
+  static_assert((kMax > 2 ? 2 : 1) * kMxWaves * kMxStoreArea <= 3 * mx_slot(kMax), "the waves' store areas fit the ring");
+  __shared__ int32_t targets[kEpi == kMxHalf ? 32 * kMax : 1];
   // Runs of consecutive items go to the XCDs in turn (workgroup b runs on XCD
   // b % 8): a run's tiles share its rows, and an expert's consecutive items
   // its weights, in that XCD's L2.
@@ -683,14 +714,14 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(2)))
     mx_zero_rows(g, item, n_tile * kMxWaves * kMxRows, kMxWaves * kMxRows);
     return;
   }
-  if (item.z > 96)
-    mx_tiled_body<4, kEpi>(g, item, n_tile, ring, targets);
-  else if (item.z > 64)
-    mx_tiled_body<3, kEpi>(g, item, n_tile, ring, targets);
-  else if (item.z > 32)
-    mx_tiled_body<2, kEpi>(g, item, n_tile, ring, targets);
+  if constexpr (kMax > 2) {
+    if (item.z > 96) return mx_tiled_body<4, kEpi, kMax>(g, item, n_tile, ring, targets);
+    if (item.z > 64) return mx_tiled_body<3, kEpi, kMax>(g, item, n_tile, ring, targets);
+  }
+  if (item.z > 32)
+    mx_tiled_body<2, kEpi, kMax>(g, item, n_tile, ring, targets);
   else
-    mx_tiled_body<1, kEpi>(g, item, n_tile, ring, targets);
+    mx_tiled_body<1, kEpi, kMax>(g, item, n_tile, ring, targets);
 }
 
 // What a product needs first, in one launch: its rows quantised, and (by the
@@ -984,8 +1015,11 @@ void launch_gemm(const MxGemm& g, MxChoice c, int items, hipStream_t s) {
   if (c.tiled) {
     const MxTiles tiles{mx_ceil(g.row_groups, kMxWaves), 2, c.item_rows};
     const int runs = mx_ceil(items, kMxXcds * tiles.run) * kMxXcds;
-    hipLaunchKernelGGL(mx_tiled_kernel<kEpi>, dim3(static_cast<unsigned>(runs) * tiles.run * tiles.n_tiles),
-                       dim3(kMxThreads), 0, s, g, tiles);
+    const dim3 grid(static_cast<unsigned>(runs) * tiles.run * tiles.n_tiles), block(kMxThreads);
+    if (c.item_rows > 64)
+      hipLaunchKernelGGL((mx_tiled_kernel<kEpi, 4>), grid, block, 0, s, g, tiles);
+    else
+      hipLaunchKernelGGL((mx_tiled_kernel<kEpi, 2>), grid, block, 0, s, g, tiles);
   } else if constexpr (kEpi == kMxBf16) {
     if (c.item_rows <= 16)
       launch_stream<1, kEpi, true, kMxList>(g, items, s);
@@ -1206,7 +1240,7 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
   hipStream_t s = as_stream(stream);
   MxGemm g{};
   set_weight(g, w, ws, n, k);
-  g.a = p.q, g.as = p.qs, g.x = x, g.x_stride = x_row_stride, g.rows = static_cast<int>(rows);
+  g.a = p.q, g.as = p.qs, g.a_rows = rows, g.x = x, g.x_stride = x_row_stride, g.rows = static_cast<int>(rows);
   g.experts = num_experts, g.bounds = boundaries, g.zero_rest = zero_rest;
   g.out = out, g.out_stride = out_row_stride;
   if (p.walk) {
@@ -1224,7 +1258,7 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
       hipLaunchKernelGGL(mx_prepare_kernel<kMxBounds>, dim3(blocks + 1), dim3(kPrepareThreads), 0, s, prepare);
     else
       hipLaunchKernelGGL(mx_prepare_kernel<kMxRowsOnly>, dim3(blocks), dim3(kPrepareThreads), 0, s, prepare);
-    g.items = p.items, g.num_items = p.num_items;
+    g.items = p.items, g.num_items = p.num_items, g.max_items = p.max_items;
   }
   launch_gemm<kMxBf16>(g, p.how, p.max_items, s);
   D3_LAUNCHED("mxfp4_grouped");
@@ -1262,6 +1296,8 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   const MoePlan p = plan_moe(workspace, rows, top_k, num_experts, hidden, intermediate);
   D3_REQUIRE(workspace_bytes >= p.bytes, "mxfp4_moe: workspace of %lld bytes < required %lld",
              static_cast<long long>(workspace_bytes), static_cast<long long>(p.bytes));
+  D3_SUPPORTED(rows * mx_ceil(hidden, kMxStep) * kMxOperandCodes < static_cast<int64_t>(kMxNowhere),
+               "mxfp4_moe: more than 4 GiB of quantised rows");
   D3_SUPPORTED(static_cast<int64_t>(p.max_items) * (mx_ceil(2 * static_cast<int64_t>(intermediate), kMxRows) +
                                                     mx_ceil(hidden, kMxRows)) < (int64_t{1} << 31),
                "mxfp4_moe: more than 2^31 workgroups");
@@ -1269,12 +1305,12 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   const int i64 = ids_dtype == D3_DTYPE_I64, f32 = weights_dtype == D3_DTYPE_F32;
   MxGemm up{}, down{};  // the two products
   set_weight(up, w13, s13, 2 * intermediate, hidden);
-  up.x = x, up.x_stride = x_row_stride, up.a = p.q, up.as = p.qs;
+  up.x = x, up.x_stride = x_row_stride, up.a = p.q, up.as = p.qs, up.a_rows = rows;
   up.out = p.act, up.out_stride = intermediate, up.out_scales = p.acts;
   set_weight(down, w2, s2, hidden, intermediate);
   down.a = p.act, down.as = p.acts, down.out_stride = hidden;
   for (MxGemm* g : {&up, &down}) {
-    g->items = p.items, g->num_items = p.num_items, g->sorted = p.sorted, g->top_k = top_k;
+    g->items = p.items, g->num_items = p.num_items, g->max_items = p.max_items, g->sorted = p.sorted, g->top_k = top_k;
     g->ids = ids, g->ids_i64 = i64, g->experts = num_experts;
   }
   if (p.few) {
