@@ -129,6 +129,7 @@ __device__ __forceinline__ uint32_t mx_max_finite(uint32_t amax, float v) {
 // accesses at any address, so odd row strides cost no narrow path.
 struct __attribute__((packed, aligned(2))) MxWords4 { uint32_t w[4]; };
 struct __attribute__((packed, aligned(1))) MxWord { uint32_t w; };
+typedef uint32_t MxVector4 __attribute__((ext_vector_type(4), aligned(2)));
 
 // Rows -> codes: a lane takes 8 consecutive elements, four lanes a block of
 // 32.  The block's largest magnitude is an integer maximum of the values' bits
@@ -151,7 +152,8 @@ __device__ __forceinline__ uint32_t mx_quad_max(uint32_t v) {
   return MaxU32::apply(v, dpp_move<kDppQuad2301>(v, 0u));
 }
 
-template <bool kF32, bool kOperand, int kThreads>
+// kOnce: the rows are larger than the caches and loaded non-temporally.
+template <bool kF32, bool kOperand, int kThreads, bool kOnce = false>
 __device__ __forceinline__ void mx_quantize_units(const MxQuantize& q, uint32_t block) {
   constexpr int kUnits = kMxQuantizeUnits;
   const uint64_t first = static_cast<uint64_t>(block) * (kThreads * kUnits) + threadIdx.x;
@@ -165,9 +167,12 @@ __device__ __forceinline__ void mx_quantize_units(const MxQuantize& q, uint32_t 
     row[j] = (at >> 32) == 0 ? static_cast<uint32_t>(at) / q.per_row : at / q.per_row;
     unit[j] = static_cast<uint32_t>(at - row[j] * q.per_row);
     const int64_t element = static_cast<int64_t>(row[j]) * q.stride + 8 * static_cast<int64_t>(unit[j]);
-    const MxWords4* p = reinterpret_cast<const MxWords4*>(static_cast<const uint8_t*>(q.x) + element * (kF32 ? 4 : 2));
+    const MxVector4* p = reinterpret_cast<const MxVector4*>(static_cast<const uint8_t*>(q.x) + element * (kF32 ? 4 : 2));
 #pragma unroll
-    for (int h = 0; h < (kF32 ? 2 : 1); ++h) raw[j][h] = p[h];
+    for (int h = 0; h < (kF32 ? 2 : 1); ++h) {
+      const MxVector4 v = kOnce ? __builtin_nontemporal_load(p + h) : p[h];
+      raw[j][h] = __builtin_bit_cast(MxWords4, v);
+    }
   }
 #pragma unroll
   for (int j = 0; j < kUnits; ++j) {

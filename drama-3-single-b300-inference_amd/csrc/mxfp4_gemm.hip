@@ -305,8 +305,10 @@ enum MxSource {
 template <int kRT, int kEpi, int kSplit, bool kDirect, int kSource>
 __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blocks) {
   constexpr int kGroups = kMxWaves / kSplit;
-  // One matrix is read by every item; an expert's mostly by one.
-  constexpr bool kOnce = !(kSource == kMxList && kEpi == kMxBf16);
+  // One matrix is read by every item; an expert's mostly by one (but a call of
+  // few pairs is short of latency, not of cache: non-temporal loads cost one
+  // token's gate and up product 5.5 -> 7.2 us where its experts are cached).
+  constexpr bool kOnce = kSource == kMxGroups || (kSource == kMxList && kEpi != kMxBf16);
   __shared__ floatx4 part[kSplit > 1 ? kMxWaves * kRT * 4 * kWave : 1];
   const int index = blockIdx.x / blocks, block = blockIdx.x - index * blocks;
   if constexpr (kSource == kMxGroups) {
@@ -1146,6 +1148,11 @@ unsigned prepare_blocks(const MxQuantize& q) {
   return static_cast<unsigned>((q.units + kPerBlock - 1) / kPerBlock);
 }
 
+template <int kWhat, int kBatch = 1>
+void launch_prepare(const MxPrepare& p, unsigned blocks, hipStream_t s) {
+  hipLaunchKernelGGL((mx_prepare_kernel<kWhat, kBatch>), dim3(blocks), dim3(kPrepareThreads), 0, s, p);
+}
+
 // Up to so many pairs each is an item of its own, whatever their experts:
 // E256 H2048 I512, 64 / 128 / 192 / 256 pairs 23.9 / 36.3 / 49.7 / 61.8 us
 // against 32.3 / 42.9 / 53.2 / 61.1 with the routes grouped; E128 I768, 64 /
@@ -1265,9 +1272,9 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
     prepare.items = p.items, prepare.num_items = p.num_items;
     const unsigned blocks = prepare_blocks(prepare.rows);
     if (boundaries != nullptr)
-      hipLaunchKernelGGL(mx_prepare_kernel<kMxBounds>, dim3(blocks + 1), dim3(kPrepareThreads), 0, s, prepare);
+      launch_prepare<kMxBounds>(prepare, blocks + 1, s);
     else
-      hipLaunchKernelGGL(mx_prepare_kernel<kMxRowsOnly>, dim3(blocks), dim3(kPrepareThreads), 0, s, prepare);
+      launch_prepare<kMxRowsOnly>(prepare, blocks, s);
     g.items = p.items, g.num_items = p.num_items, g.max_items = p.max_items;
   }
   launch_gemm<kMxBf16>(g, p.how, p.max_items, s);
@@ -1343,21 +1350,20 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
         p.max_items, p.num_items, nullptr, p.scratch, p.scratch_ints, stream);
     if (status != D3_OK) return status;
     if (blocks > 0)
-      hipLaunchKernelGGL(mx_prepare_kernel<kMxRowsOnly>, dim3(blocks), dim3(kPrepareThreads), 0, s, prepare);
+      launch_prepare<kMxRowsOnly>(prepare, blocks, s);
   } else {
     prepare.groups = num_experts, prepare.count = static_cast<int>(p.pairs);
     prepare.ids = ids, prepare.ids_i64 = i64, prepare.sorted = p.sorted;
     prepare.item_rows = p.how.item_rows, prepare.max_items = p.max_items;
     prepare.items = p.items, prepare.num_items = p.num_items;
     prepare.chunks = p.chunks, prepare.chunk_counts = p.counts, prepare.ranks = p.scratch;
-    const dim3 block(kPrepareThreads);
     if (p.chunks > 0) {
-      hipLaunchKernelGGL(mx_prepare_kernel<kMxRouteChunks>, dim3(blocks + p.chunks), block, 0, s, prepare);
-      hipLaunchKernelGGL(mx_place_kernel, dim3(p.chunks), block, 0, s, prepare);
+      launch_prepare<kMxRouteChunks>(prepare, blocks + p.chunks, s);
+      hipLaunchKernelGGL(mx_place_kernel, dim3(p.chunks), dim3(kPrepareThreads), 0, s, prepare);
     } else if (p.pairs <= kPrepareThreads) {
-      hipLaunchKernelGGL((mx_prepare_kernel<kMxRoutes, 1>), dim3(blocks + 1), block, 0, s, prepare);
+      launch_prepare<kMxRoutes, 1>(prepare, blocks + 1, s);
     } else {
-      hipLaunchKernelGGL((mx_prepare_kernel<kMxRoutes, 8>), dim3(blocks + 1), block, 0, s, prepare);
+      launch_prepare<kMxRoutes, 8>(prepare, blocks + 1, s);
     }
   }
   launch_gemm<kMxAct>(up, p.how, p.max_items, s);
