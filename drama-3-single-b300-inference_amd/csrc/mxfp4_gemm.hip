@@ -51,6 +51,7 @@ struct MxGemm {
   int zero_rest;
   void* out;
   int64_t out_stride;  // elements (kMxAct: the row's width)
+  bool out_past;  // kMxBf16, tiled: more than the L2s hold, stored past them
   uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout; kMxHalf: exponents [rows][row groups]
 };
 
@@ -93,9 +94,12 @@ __device__ __forceinline__ MxWords4 mx_pack8(const float* v) {
 }
 
 // Eight 16-bit values at columns f .. of a row of n.
-__device__ __forceinline__ void mx_store16(uint16_t* out, int f, int n, const MxWords4& v) {
+__device__ __forceinline__ void mx_store16(uint16_t* out, int f, int n, const MxWords4& v, bool past = false) {
   if (f + 8 <= n) {
-    *reinterpret_cast<MxWords4*>(out + f) = v;
+    if (past)  // uniform
+      __builtin_nontemporal_store(__builtin_bit_cast(MxVector4, v), reinterpret_cast<MxVector4*>(out + f));
+    else
+      *reinterpret_cast<MxWords4*>(out + f) = v;
     return;
   }
   uint64_t lo = v.w[0] | (static_cast<uint64_t>(v.w[1]) << 32), hi = v.w[2] | (static_cast<uint64_t>(v.w[3]) << 32);
@@ -513,7 +517,8 @@ __device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[
       if (first + r < count) {
         int64_t to = item.y + first + r;
         if constexpr (kEpi == kMxHalf) to = targets[first + r];
-        mx_store16(static_cast<uint16_t*>(g.out) + to * g.out_stride, kMxRows * rg + 8 * part, g.n, w);
+        mx_store16(static_cast<uint16_t*>(g.out) + to * g.out_stride, kMxRows * rg + 8 * part, g.n, w,
+                   kEpi == kMxBf16 && g.out_past);
       }
     }
   }
@@ -1260,6 +1265,8 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
   g.a = p.q, g.as = p.qs, g.a_rows = rows, g.x = x, g.x_stride = x_row_stride, g.rows = static_cast<int>(rows);
   g.experts = num_experts, g.bounds = boundaries, g.zero_rest = zero_rest;
   g.out = out, g.out_stride = out_row_stride;
+  // (8191 x 4096 x 4096 87.5 -> 84.4 us, 16384 rows over 256 experts 82.5 -> 81.0)
+  g.out_past = rows * static_cast<int64_t>(n) * 2 > (int64_t{1} << 25);
   if (p.walk) {
     launch_stream<2, kMxBf16, true, kMxGroups>(g, num_experts + 1, s);
     D3_LAUNCHED("mxfp4_grouped");
