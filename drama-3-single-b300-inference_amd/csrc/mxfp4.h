@@ -17,6 +17,8 @@ constexpr int kMxOperandCodes = kMxStep / 2;         // a quantised row's codes 
 constexpr int kMxOperandScales = kMxStep / kMxBlock;  // and scales
 constexpr int kMxLow = 4;  // the MFMA's format code of e2m1 operands
 
+inline bool mx_aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
 // Row orders of a packed weight: which row of W row m = 4 g + i (i < 4) of
 // tile t of a row group holds.  The MFMAs' output lanes hold rows 4 g + i of
 // every tile; with these orders a pair of tiles is eight consecutive columns.

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ c
   }
 }
 
-bool mx_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+constexpr int64_t kMaxUnits = int64_t{1} << 33;  // (a grid holds fewer than 2^32 threads)
 
 unsigned row_blocks(uint64_t units) {
   return static_cast<unsigned>((units + kRowThreads * kRowUnits - 1) / (kRowThreads * kRowUnits));
@@ -130,7 +130,7 @@ extern "C" int d3_mxfp4_quantize(const void* x, int32_t x_dtype, int64_t x_row_s
     return D3_OK;
   }
   const uint32_t per_row = static_cast<uint32_t>(width) / 8;
-  D3_SUPPORTED(rows <= (int64_t{1} << 40) / per_row, "mxfp4_quantize: more than 2^43 elements");
+  D3_SUPPORTED(rows <= kMaxUnits / per_row, "mxfp4_quantize: more than 2^36 elements");
   const uint64_t units = static_cast<uint64_t>(rows) * per_row;
   const MxQuantize q{x, x_row_stride, units, per_row, 0, codes, scales};
   const dim3 grid(row_blocks(units)), block(kRowThreads);
@@ -153,7 +153,7 @@ extern "C" int d3_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, 
     return D3_OK;
   }
   const uint32_t per_row = static_cast<uint32_t>(width) / 8;
-  D3_SUPPORTED(rows <= (int64_t{1} << 40) / per_row, "mxfp4_dequantize: more than 2^43 elements");
+  D3_SUPPORTED(rows <= kMaxUnits / per_row, "mxfp4_dequantize: more than 2^36 elements");
   const uint64_t units = static_cast<uint64_t>(rows) * per_row;
   const dim3 grid(row_blocks(units)), block(kRowThreads);
   const bool f32 = out_dtype == D3_DTYPE_F32;

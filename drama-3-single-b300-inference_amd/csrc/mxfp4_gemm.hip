@@ -997,8 +997,6 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint16_t* 
                  pack_bf16x2(acc[6], acc[7]));
 }
 
-bool mx_aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
-
 int mx_ceil(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
 template <int kRT, int kEpi, bool kDirect, int kSource>
@@ -1217,13 +1215,20 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
   return p;
 }
 
+// Widths whose offsets within a row group's weights and within an item's rows
+// stay far inside the 32 bits of a buffer view, and the workgroups of a launch:
+// a grid holds fewer than 2^32 threads.
+constexpr int kMxMaxWidth = 1 << 20, kMxMaxColumns = 1 << 24;
+constexpr int64_t kMxMaxWorkgroups = int64_t{1} << 24;
+
 bool grouped_shape(int64_t rows, int experts, int n, int k) {
-  return rows >= 0 && rows < (int64_t{1} << 30) && experts > 0 && experts <= (1 << 16) && n > 0 && k > 0 &&
-         k % kGroup == 0;
+  return rows >= 0 && rows < (int64_t{1} << 30) && experts > 0 && experts <= (1 << 16) && n > 0 &&
+         n <= kMxMaxColumns && k > 0 && k <= kMxMaxWidth && k % kGroup == 0;
 }
 bool moe_shape(int64_t rows, int top_k, int experts, int hidden, int inter) {
-  return rows >= 0 && top_k >= 1 && top_k <= 16 && rows * top_k < (int64_t{1} << 26) && experts >= 1 && experts <= 512 &&
-         hidden > 0 && inter > 0 && hidden % kGroup == 0 && inter % kGroup == 0;
+  return rows >= 0 && rows < (int64_t{1} << 26) && top_k >= 1 && top_k <= 16 && rows * top_k < (int64_t{1} << 26) &&
+         experts >= 1 && experts <= 512 && hidden > 0 && inter > 0 && hidden <= kMxMaxWidth && inter <= kMxMaxWidth &&
+         hidden % kGroup == 0 && inter % kGroup == 0;
 }
 
 }  // namespace
@@ -1242,8 +1247,9 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
                                 uint16_t* out, int64_t out_row_stride, int32_t zero_rest, void* workspace,
                                 int64_t workspace_bytes, void* stream) {
   D3_REQUIRE(k > 0 && k % kGroup == 0, "mxfp4_grouped: K=%d must be a multiple of %d", k, kGroup);
-  D3_REQUIRE(grouped_shape(rows, num_experts, n, k), "mxfp4_grouped: rows %lld, experts %d, N=%d",
-             static_cast<long long>(rows), num_experts, n);
+  D3_REQUIRE(grouped_shape(rows, num_experts, n, k),
+             "mxfp4_grouped: rows %lld (fewer than 2^30), experts %d (1 to 65536), N=%d (to 2^24), K=%d (to 2^20)",
+             static_cast<long long>(rows), num_experts, n, k);
   D3_REQUIRE(boundaries != nullptr || num_experts == 1, "mxfp4_grouped: several experts need boundaries");
   D3_REQUIRE(rows == 0 || (x && w && ws && out), "mxfp4_grouped: null pointer");
   D3_REQUIRE(rows <= 1 || (x_row_stride >= 0 && out_row_stride >= n), "mxfp4_grouped: row strides");
@@ -1258,7 +1264,7 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
              "mxfp4_grouped: workspace of %lld bytes < required %lld", static_cast<long long>(workspace_bytes),
              static_cast<long long>(p.bytes));
   const int64_t most = p.walk ? num_experts + 1 : p.max_items;
-  D3_SUPPORTED(most * mx_ceil(n, kMxRows) < (int64_t{1} << 31), "mxfp4_grouped: more than 2^31 workgroups");
+  D3_SUPPORTED(most * mx_ceil(n, kMxRows) < kMxMaxWorkgroups, "mxfp4_grouped: more than 2^24 workgroups");
   hipStream_t s = as_stream(stream);
   MxGemm g{};
   set_weight(g, w, ws, n, k);
@@ -1302,8 +1308,9 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   D3_REQUIRE(hidden > 0 && intermediate > 0 && hidden % kGroup == 0 && intermediate % kGroup == 0,
              "mxfp4_moe: hidden %d and intermediate %d must be multiples of %d", hidden, intermediate, kGroup);
   D3_REQUIRE(moe_shape(rows, top_k, num_experts, hidden, intermediate),
-             "mxfp4_moe: rows %lld, top_k %d (1 to 16), experts %d (1 to 512), fewer than 2^26 (row, rank) pairs",
-             static_cast<long long>(rows), top_k, num_experts);
+             "mxfp4_moe: rows %lld, top_k %d (1 to 16), experts %d (1 to 512), hidden %d and intermediate %d (to 2^20), "
+             "fewer than 2^26 (row, rank) pairs",
+             static_cast<long long>(rows), top_k, num_experts, hidden, intermediate);
   D3_REQUIRE(ids_dtype == D3_DTYPE_I32 || ids_dtype == D3_DTYPE_I64, "mxfp4_moe: ids must be int32 or int64");
   D3_REQUIRE(weights_dtype == D3_DTYPE_BF16 || weights_dtype == D3_DTYPE_F32, "mxfp4_moe: weights must be bf16 or f32");
   D3_REQUIRE(rows == 0 || (x && ids && weights && w13 && s13 && w2 && s2 && out && workspace), "mxfp4_moe: null pointer");
@@ -1322,9 +1329,10 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
              static_cast<long long>(workspace_bytes), static_cast<long long>(p.bytes));
   D3_SUPPORTED(rows * mx_ceil(hidden, kMxStep) * kMxOperandCodes < static_cast<int64_t>(kMxNowhere),
                "mxfp4_moe: more than 4 GiB of quantised rows");
-  D3_SUPPORTED(static_cast<int64_t>(p.max_items) * (mx_ceil(2 * static_cast<int64_t>(intermediate), kMxRows) +
-                                                    mx_ceil(hidden, kMxRows)) < (int64_t{1} << 31),
-               "mxfp4_moe: more than 2^31 workgroups");
+  const int64_t widest = 2 * static_cast<int64_t>(intermediate) > hidden ? 2 * static_cast<int64_t>(intermediate) : hidden;
+  D3_SUPPORTED(p.max_items * static_cast<int64_t>(mx_ceil(widest, kMxRows)) < kMxMaxWorkgroups &&
+                   rows * mx_ceil(hidden, kMxCombineColumns) < kMxMaxWorkgroups,
+               "mxfp4_moe: more than 2^24 workgroups");
   hipStream_t s = as_stream(stream);
   const int i64 = ids_dtype == D3_DTYPE_I64, f32 = weights_dtype == D3_DTYPE_F32;
   MxGemm up{}, down{};  // the two products
@@ -1341,7 +1349,7 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
     launch_stream<1, kMxAct, true, kMxPairs>(up, static_cast<int>(p.pairs), s);
     down.out = out;
     hipLaunchKernelGGL(mx_down_combine_kernel, dim3(static_cast<unsigned>(rows) * down.row_groups),
-                       dim3(kDownWaves * kWave), 0, s,                       down, weights, f32);
+                       dim3(kDownWaves * kWave), 0, s, down, weights, f32);
     D3_LAUNCHED("mxfp4_moe");
   }
   MxPrepare prepare{};
@@ -1379,10 +1387,10 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   const int slices = mx_ceil(hidden, kMxCombineColumns);
   const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
   if (top_k == 8)
-    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
-                       slices, out);
+    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k,
+                       num_experts, hidden, slices, out);
   else
-    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
-                       slices, out);
+    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k,
+                       num_experts, hidden, slices, out);
   D3_LAUNCHED("mxfp4_moe");
 }

@@ -786,7 +786,7 @@ int d3_requests_save(int64_t *last, int64_t *history, int64_t *metadata, int64_t
 /*
  * Rows of MXFP4 from bf16 or f32: x [rows, width] (row stride in elements,
  * unit column stride, aligned to its elements) -> codes [rows, width / 2],
- * scales [rows, width / 32].  width % 32 == 0.
+ * scales [rows, width / 32].  width % 32 == 0; up to 2^36 elements.
  */
 int d3_mxfp4_quantize(const void *x, int32_t x_dtype, int64_t x_row_stride, int64_t rows,
                       int32_t width, uint8_t *codes, uint8_t *scales, void *stream);
@@ -816,7 +816,8 @@ int64_t d3_mxfp4_packed_bytes(int32_t num_experts, int32_t n, int32_t k, int32_t
  * (order 0) transposed -> the same rows of out bf16 [rows, n] (fp32 sums, one
  * rounding).  boundaries int32 [num_experts + 1] on the device, ascending,
  * clamped to [0, rows]; NULL with one expert: every row.  Rows of no group
- * are zeroed with zero_rest, else left as they were.  workspace: at least
+ * are zeroed with zero_rest, else left as they were.  num_experts <= 65536,
+ * n <= 2^24, k <= 2^20; out does not overlap x.  workspace: at least
  * d3_mxfp4_grouped_workspace bytes (NULL where that is 0), 16-byte aligned,
  * this call's alone until it has run.
  */
@@ -838,10 +839,10 @@ int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bo
  *   out[t] = sum over r of weights[t, r] * (w2[e] (order 0) a)
  * in rank order, the sums fp32, rounded to bf16 once (above 128 pairs each
  * rank's row is first rounded to a scaled fp16, an eighth of bf16's step).
- * ids int32 or int64
- * [rows, top_k] (an id outside [0, num_experts) adds nothing), weights bf16 or
- * f32.  top_k <= 16, num_experts <= 512, hidden and intermediate multiples of
- * 128.  workspace: d3_mxfp4_moe_workspace bytes, as for d3_mxfp4_grouped.
+ * ids int32 or int64 [rows, top_k] (an id outside [0, num_experts) adds
+ * nothing), weights bf16 or f32.  top_k <= 16, num_experts <= 512, hidden and
+ * intermediate multiples of 128 up to 2^20, fewer than 2^26 pairs; out does not
+ * overlap x.  workspace: d3_mxfp4_moe_workspace bytes, as for d3_mxfp4_grouped.
  */
 int d3_mxfp4_moe(const uint16_t *x, int64_t x_row_stride, int64_t rows, const void *ids,
                  int32_t ids_dtype, const void *weights, int32_t weights_dtype, int32_t top_k,

@@ -120,6 +120,35 @@ def test_c_entries_refuse_before_launching(lib):
     assert lib_.d3_mxfp4_packed_bytes(3, 65, 384, 1) == 3 * 128 * 512 // 32
 
 
+def test_sizes_past_the_kernels_offsets_are_refused(lib):
+    """Widths past the 32-bit views and launches of more threads than a grid
+    holds: an error before anything is launched, whatever the pointers."""
+    call, lib_ = lib.call, lib.load()
+    huge = 1 << 62
+    with pytest.raises(ValueError, match="2.36 elements"):
+        call("d3_mxfp4_quantize", 16, 0, 0, (1 << 31) + 1, 32, 16, 16, None)
+    with pytest.raises(ValueError, match="2.36 elements"):
+        call("d3_mxfp4_dequantize", 16, 16, (1 << 31) + 1, 32, 16, 0, None)
+    for rows, n, k, match in ((4, 64, (1 << 20) + 128, "K=1048704"), (4, (1 << 24) + 1, 128, "N=16777217"),
+                              (1 << 30, 64, 128, "rows 1073741824"), ((1 << 30) - 1, 1 << 10, 128, "workgroups")):
+        with pytest.raises(ValueError, match=match):
+            call("d3_mxfp4_grouped", 16, k, rows, None, 1, 16, 16, n, k, 16, n, 0, 16, huge, None)
+    with pytest.raises(ValueError, match="workgroups"):  # groups walked by their own workgroups
+        call("d3_mxfp4_grouped", 16, 128, 1, 16, 1 << 16, 16, 16, 1 << 15, 128, 16, 1 << 15, 0, None, 0, None)
+
+    def moe(rows, top_k, hidden, inter):
+        call("d3_mxfp4_moe", 16, hidden, rows, 16, 3, 16, 0, top_k, 16, 16, 16, 16, 16, hidden, inter, 16, 16,
+             huge, None)
+
+    for args, match in (((4, 8, (1 << 20) + 128, 128), "hidden 1048704"), ((4, 8, 128, (1 << 20) + 128), "2.20"),
+                        (((1 << 23) + 1, 8, 128, 128), "pairs"), ((1 << 62, 8, 128, 128), "pairs"),
+                        ((1 << 24, 1, 128, 128), "workgroups"), ((1 << 23, 1, 1024, 128), "4 GiB")):
+        with pytest.raises(ValueError, match=match):
+            moe(*args)
+    assert lib_.d3_mxfp4_grouped_workspace(4, 8, 1, 64, (1 << 20) + 128) == -1
+    assert lib_.d3_mxfp4_moe_workspace(1 << 62, 8, 16, 256, 128) == -1
+
+
 def test_empty_calls_need_no_buffers(lib):
     lib.call("d3_mxfp4_quantize", None, 0, 64, 0, 64, None, None, None)
     lib.call("d3_mxfp4_dequantize", None, None, 0, 64, None, 0, None)
