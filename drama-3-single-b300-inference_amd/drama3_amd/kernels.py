@@ -322,9 +322,10 @@ def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start
     if mxfp4:  # bf16 routing weights whatever the router's type, as below
         ids = torch.empty((rows, TOP_K), dtype=torch.int32, device=x.device)
         weights = torch.empty((rows, TOP_K), dtype=torch.bfloat16, device=x.device)
-        call("d3_route", ptr(logits), dtype_code(logits.dtype), logits.stride(0), rows, e, TOP_K,
-             None, None, ptr(ids), None, ptr(weights), dtype_code(weights.dtype),
-             _lib.stream(x.device))
+        with torch.cuda.device(x.device):  # (the stream's own)
+            call("d3_route", ptr(logits), dtype_code(logits.dtype), logits.stride(0), rows, e, TOP_K,
+                 None, None, ptr(ids), None, ptr(weights), dtype_code(weights.dtype),
+                 _lib.stream(x.device))
         return mxfp4_moe(x, ids, weights, experts)
     if x.stride(0) % 8 or x.data_ptr() % 16:
         x = x.contiguous()

@@ -137,6 +137,15 @@ class Mxfp4Weight:
     k: int
     order: int = ORDER_ROWS
 
+    def __post_init__(self):
+        """The kernels take the sizes as given: they have to be the buffers'."""
+        require_cuda(self.codes, self.scales)
+        _same_device(self.codes, self.scales, "scales")
+        for t, scales in ((self.codes, 0), (self.scales, 1)):
+            if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != _entry("d3_mxfp4_packed_bytes")(
+                    self.experts, self.n, self.k, scales):
+                raise ValueError("packed codes and scales do not hold [experts, n, k]; make them with prepare_mxfp4")
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -148,6 +157,13 @@ class Mxfp4Experts:
 
     w13: Mxfp4Weight
     w2: Mxfp4Weight
+
+    def __post_init__(self):
+        w13, w2 = self.w13, self.w2
+        if w13.order != ORDER_GATE_UP or w2.order != ORDER_ROWS:
+            raise ValueError("experts must come from prepare_mxfp4_experts")
+        if (w13.experts, w13.n, w13.k) != (w2.experts, 2 * w2.k, w2.n) or w13.device != w2.device:
+            raise ValueError("expert weights must be w13 [E, 2I, H], w2 [E, H, I] on one device")
 
     @property
     def num_experts(self) -> int:
@@ -226,6 +242,22 @@ def quantize_experts_mxfp4(experts) -> Mxfp4Experts:
     return Mxfp4Experts(*packed)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether 2-D bf16 tensors of unit column stride may share an element:
+    their spans meet, and they are not different columns of rows of one stride."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    apart = (b.data_ptr() - a.data_ptr()) // 2
+    if apart >= (len(a) - 1) * a.stride(0) + a.shape[1]:
+        return False
+    stride = a.stride(0)
+    if stride != b.stride(0) or stride == 0:
+        return True
+    return apart % stride < a.shape[1] or apart % stride + b.shape[1] > stride
+
+
 def _product(x, boundaries, weight: Mxfp4Weight, out, zero_rest: bool) -> torch.Tensor:
     _check_rows(x)
     if weight.order != ORDER_ROWS:
@@ -261,7 +293,8 @@ def grouped_mxfp4(x: torch.Tensor, boundaries: torch.Tensor, weight: Mxfp4Weight
 
     ``boundaries`` int32 [E + 1], ascending, on the device (groups may be
     empty; values are clamped to [0, T]).  Rows of no group are zeros, or left
-    as they were in a given ``out`` (bf16 [T, N], unit column stride)."""
+    as they were in a given ``out`` (bf16 [T, N], unit column stride, apart from
+    ``x``)."""
     _check_rows(x)
     require_cuda(boundaries, out)
     if boundaries.dtype != torch.int32:
@@ -276,6 +309,8 @@ def grouped_mxfp4(x: torch.Tensor, boundaries: torch.Tensor, weight: Mxfp4Weight
                 len(x) > 1 and out.stride(0) < weight.n):
             raise ValueError(f"out must be [{len(x)}, {weight.n}] with unit column stride")
         _same_device(x, out, "out")
+        if _overlap(x, out):
+            raise ValueError("out must not overlap x")
     return _product(x, boundaries, weight, out, out is None)
 
 
@@ -302,8 +337,6 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
         raise ValueError(f"rows of width {x.shape[1]}, experts of hidden size {experts.hidden}")
     ids, weights = topk_ids.contiguous(), topk_weights.contiguous()
     w13, w2 = experts.w13, experts.w2
-    if w13.order != ORDER_GATE_UP or w2.order != ORDER_ROWS:
-        raise ValueError("experts must come from prepare_mxfp4_experts")
     _same_device(x, ids, "topk_ids")
     _same_device(x, weights, "topk_weights")
     _same_device(x, w13.codes, "experts")

@@ -154,6 +154,28 @@ def test_linear_of_the_projection(device, rows, k, n):
     within(mxfp4_linear(x.to(device), prepare_mxfp4(codes.to(device), scales.to(device))), *product(x, values))
 
 
+@pytest.mark.parametrize("rows, k, n", [
+    (600, 384, 1500),                                                                # streamed, 32 rows an item
+    (1000, 384, 1500), (831, 640, 1500),                                             # tiles of 32 rows
+    (2100, 384, 1500), (2049, 128, 1601), (2111, 256, 1500),                         # items of 64, the last of 52, 1, 63
+    (4200, 384, 1500), (4097, 128, 1537), (4136, 640, 1500), (4166, 1152, 1409)])    # of 128, the last of 104, 1, 40, 70
+def test_linear_of_many_rows(device, rows, k, n):
+    """Items of every size, their last ones in bodies of one to four tiles, K
+    an odd and an even number of half steps; every other row of a wider buffer."""
+    from drama3_amd.mxfp4 import mxfp4_linear, prepare_mxfp4
+
+    rng = np.random.default_rng(rows + k + n)
+    x = rows_of(rng, rows, k)
+    x[rows - 2, k - 1] = float("nan")
+    codes, scales, values = weight_of(rng, n, k)
+    weight = prepare_mxfp4(codes.to(device), scales.to(device))
+    wide = torch.zeros((2 * rows, k + 3), dtype=torch.bfloat16, device=device)
+    wide[::2, 1:k + 1] = x.to(device)
+    out = mxfp4_linear(x.to(device), weight)
+    within(out, *product(x, values))
+    assert torch.equal(mxfp4_linear(wide[::2, 1:k + 1], weight).nan_to_num(9), out.nan_to_num(9))
+
+
 def test_linear_takes_any_rows_and_keeps_nan_in_its_row(device):
     """Strided rows at odd addresses; a row with an infinity or a NaN is NaN,
     its neighbours are not (K an odd multiple of 128: the padded half step lies
@@ -250,6 +272,51 @@ def test_grouped_at_random(device, rows, experts, k, n):
     within(out, want, bound)
 
 
+RAGGED = {  # groups that fill one to four tiles of an item, whole items, a row more, none
+    300: [2, 2, 35, 100, 101, 165, 299],
+    2100: [3, 36, 36, 133, 262, 263, 2090],
+}
+
+
+@pytest.mark.parametrize("rows, k, n", [(300, 384, 6500), (300, 640, 8301), (2100, 256, 8301)])
+def test_grouped_over_many_columns(device, rows, k, n):
+    """Items of 64 and 128 rows of ragged groups; the last case's results are
+    more than the L2s hold.  Odd columns, into a column slice of a wider buffer."""
+    from drama3_amd.mxfp4 import grouped_mxfp4, prepare_mxfp4
+
+    rng = np.random.default_rng(rows + k + n)
+    bounds = RAGGED[rows]
+    x = rows_of(rng, rows, k)
+    codes, scales, values = weight_of(rng, 6, n, k)
+    weight = prepare_mxfp4(codes.to(device), scales.to(device))
+    boundaries = torch.tensor(bounds, dtype=torch.int32, device=device)
+    want, bound, live = grouped_oracle(x, bounds, values)
+    out = grouped_mxfp4(x.to(device), boundaries, weight)
+    within(out, want, bound)
+    live = torch.from_numpy(live).to(device)
+    assert not out[~live].any()
+    buffer = torch.full((rows, n + 10), -3.0, dtype=torch.bfloat16, device=device)
+    given = grouped_mxfp4(x.to(device), boundaries, weight, out=buffer[:, 5:5 + n])
+    assert torch.equal(given, torch.where(live[:, None], out, -3.0))
+    assert (buffer[:, :5] == -3).all() and (buffer[:, 5 + n:] == -3).all()
+
+
+@pytest.mark.parametrize("rows", [512, 513])
+def test_grouped_with_one_busy_group(device, rows):
+    """Most rows of many groups that one launch walks, and one row more."""
+    from drama3_amd.mxfp4 import grouped_mxfp4, prepare_mxfp4
+
+    rng = np.random.default_rng(rows)
+    x = rows_of(rng, rows, 384)
+    codes, scales, values = weight_of(rng, 100, 130, 384)
+    bounds = np.concatenate([np.minimum(np.arange(50), 20), np.full(51, rows - 7)])
+    bounds[60:] += np.minimum(np.arange(41), 6)
+    out = grouped_mxfp4(x.to(device), torch.from_numpy(bounds.astype(np.int32)).to(device),
+                        prepare_mxfp4(codes.to(device), scales.to(device)))
+    want, bound, _ = grouped_oracle(x, bounds, values)
+    within(out, want, bound)
+
+
 def test_grouped_weights_past_32_bit_offsets(device):
     """More than 4 GiB of packed codes: the last expert is found."""
     from drama3_amd.mxfp4 import grouped_mxfp4, prepare_mxfp4
@@ -302,6 +369,47 @@ def test_moe(device, rows, experts, hidden, inter, top_k, skew):
     weights = weights.to(torch.bfloat16)
     out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
     within(out, *om.moe(f64(x), ids.numpy(), f64(weights), v13, v2))
+
+
+@pytest.mark.parametrize("rows, hidden, inter, skew", [(150, 640, 1152, 0.5), (320, 384, 1024, 0.0),
+                                                       (330, 256, 1152, 1.0)])
+def test_moe_in_large_items(device, rows, hidden, inter, skew):
+    """Items of 64 and of 128 rows in both products, their last ones of any
+    size; widths of whole and half steps; rows that are NaN keep to themselves."""
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    rng = np.random.default_rng(rows + hidden)
+    packed, v13, v2 = make_experts(rng, 8, hidden, inter, device)
+    x = rows_of(rng, rows, hidden)
+    ids, weights = make_routes(rng, rows, 8, 8, skew)
+    ids[rng.random(ids.shape) < 0.3] = 8  # no expert: groups of different sizes
+    ids, weights = ids.to(torch.int32), weights.to(torch.bfloat16)
+    clean = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
+    within(clean, *om.moe(f64(x), ids.numpy(), f64(weights), v13, v2))
+    ids[7, 0] = ids[rows - 1, 3] = 1
+    x[7, 1], x[rows - 1, hidden - 1] = float("inf"), float("nan")
+    out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
+    assert out[7].isnan().all() and out[-1].isnan().all()
+    keep = [r for r in range(rows - 1) if r != 7]
+    assert torch.equal(out[keep], clean[keep])
+
+
+def test_moe_rows_past_32_bit_offsets(device):
+    """Gathered rows whose offsets pass 2^31, routes' rows past 2^32 elements."""
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    rng = np.random.default_rng(25)
+    rows, hidden = 4_500_001, 1024
+    packed, v13, v2 = make_experts(rng, 2, hidden, 128, device)
+    x = torch.zeros((rows, hidden), dtype=torch.bfloat16, device=device)
+    tail = rows_of(rng, 40, hidden)
+    x[-40:] = tail.to(device)
+    ids = torch.zeros((rows, 1), dtype=torch.int32, device=device)
+    ids[-25:] = 1
+    weights = torch.full((rows, 1), 0.5, device=device)
+    out = mxfp4_moe(x, ids, weights, packed)
+    assert not out[:-40].any()
+    within(out[-40:], *om.moe(f64(tail), ids[-40:].cpu().numpy(), f64(weights[-40:]), v13, v2))
 
 
 @pytest.mark.parametrize("id_type, weight_type", [(torch.int32, torch.float32), (torch.int64, torch.bfloat16)])
@@ -467,6 +575,14 @@ def test_refusals(device):
     refused(ValueError, "T rows", mx.mxfp4_moe, x, ids[:5], w[:5], packed)
     refused(ValueError, "hidden size 256", mx.mxfp4_moe, x[:, :128], ids, w, packed)
     refused(ValueError, "top_k 17", mx.mxfp4_moe, x, ids[:, :1].expand(6, 17), w[:, :1].expand(6, 17), packed)
+    buffer = torch.zeros((6, 400), dtype=torch.bfloat16, device=device)
+    refused(ValueError, "overlap", mx.grouped_mxfp4, buffer[:, :256], bounds, weight, out=buffer[:, 200:264])
+    mx.grouped_mxfp4(buffer[:, :256], bounds, weight, out=buffer[:, 256:320])
+    refused(ValueError, "prepare_mxfp4", mx.Mxfp4Weight, weight.codes, weight.scales, 5, 64, 256)
+    refused(ValueError, "prepare_mxfp4", mx.Mxfp4Weight, weight.codes, weight.scales[8:], 4, 64, 256)
+    refused(ValueError, "prepare_mxfp4_experts", mx.Mxfp4Experts, packed.w2, packed.w2)
+    other, *_ = make_experts(rng, 4, 128, 128, device)
+    refused(ValueError, "one device", mx.Mxfp4Experts, packed.w13, other.w2)
     # the refused calls left nothing behind
     assert torch.equal(mx.mxfp4_moe(x, ids, w, packed), mx.mxfp4_moe(x, ids, w, packed))
 
@@ -530,3 +646,79 @@ def test_together_captured_replayed_and_on_streams(device):
     for i, results in enumerate(got):
         for a, b in zip(results, want[i % 4]):
             assert torch.equal(a, b)
+
+
+def test_large_batches_captured_and_replayed(device):
+    """The kernels of many rows in one graph: tiles, boundaries to items, the
+    pairs grouped by chunks and by the route sort; replays with other inputs
+    and eager work between, each against the eager results."""
+    from drama3_amd import mxfp4 as mx
+
+    rng = np.random.default_rng(26)
+    packed, *_ = make_experts(rng, 24, 128, 128, device)
+    lc, ls, _ = weight_of(rng, 1500, 128)
+    linear = mx.prepare_mxfp4(lc.to(device), ls.to(device))
+    gc, gs, _ = weight_of(rng, 5, 200, 128)
+    groups = mx.prepare_mxfp4(gc.to(device), gs.to(device))
+
+    def inputs():
+        made = [rows_of(rng, 8300, 128).to(device)]
+        ids, weights = make_routes(rng, 8300, 24, 8, 0.5)
+        ids[rng.random(ids.shape) < 0.02] = -1
+        ends = sorted(rng.integers(0, 8301, 6).tolist())
+        return made + [ids.to(torch.int32).to(device), weights.to(torch.bfloat16).to(device),
+                       torch.tensor(ends, dtype=torch.int32, device=device)]
+
+    def step(x, ids, weights, bounds):
+        return (mx.mxfp4_linear(x, linear), mx.grouped_mxfp4(x, bounds, groups), mx.mxfp4_moe(x, ids, weights, packed),
+                mx.mxfp4_moe(x[:1500], ids[:1500], weights[:1500], packed),
+                mx.mxfp4_moe(x[:700], ids[:700], weights[:700], packed))
+
+    held = inputs()
+    side = torch.cuda.Stream(device)
+    side.wait_stream(torch.cuda.current_stream(device))
+    with torch.cuda.stream(side):
+        step(*held)
+    torch.cuda.current_stream(device).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        results = step(*held)
+    for _ in range(4):
+        new = inputs()
+        for to, value in zip(held, new):
+            to.copy_(value)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(results, step(*new)):
+            assert torch.equal(got, want)
+
+
+def test_calls_from_two_threads(device):
+    """Two host threads, a stream each, the same weights."""
+    import threading
+
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    rng = np.random.default_rng(27)
+    packed, *_ = make_experts(rng, 16, 256, 128, device)
+    jobs = []
+    for rows in (40, 500):
+        ids, weights = make_routes(rng, rows, 16, 8)
+        jobs.append((rows_of(rng, rows, 256).to(device), ids.to(device), weights.to(torch.bfloat16).to(device)))
+    want = [mxfp4_moe(*job, packed) for job in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.device(device), torch.cuda.stream(torch.cuda.Stream(device)):
+            for _ in range(20):
+                got[i].append(mxfp4_moe(*jobs[i], packed))
+            torch.cuda.current_stream(device).synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(2):
+        assert len(got[i]) == 20 and all(torch.equal(out, want[i]) for out in got[i])

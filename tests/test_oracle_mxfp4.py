@@ -166,3 +166,28 @@ def test_host_tensors_are_refused(lib):
                  lambda: mx.prepare_mxfp4(codes, scales)):
         with pytest.raises(ValueError, match="device tensors"):
             made()
+    with pytest.raises(ValueError, match="device tensors"):
+        mx.Mxfp4Weight(codes, scales, 1, 2, 128)
+
+
+def test_overlapping_rows_are_found():
+    from drama3_amd.mxfp4 import _overlap
+
+    flat = torch.zeros(4000, dtype=torch.bfloat16)
+    wide = flat[:2000].view(20, 100)
+
+    def shared(a, b):
+        """By the elements themselves."""
+        index = torch.arange(4000)
+        at = [set(torch.as_strided(index, t.shape, t.stride(), t.storage_offset()).flatten().tolist()) for t in (a, b)]
+        return bool(at[0] & at[1])
+
+    views = [wide, wide[:, :60], wide[:, 60:], wide[:, 59:], wide[3:9, 20:60], wide[::2, :60], wide[5:6], wide[6:7],
+             wide[5:6, 40:90], wide[12:, :60], wide[:0], torch.as_strided(flat, (20, 60), (100, 1), 80),
+             torch.as_strided(flat, (20, 30), (0, 1), 70), flat[2000:].view(20, 100)]
+    for a in views:
+        for b in views:
+            assert _overlap(a, b) == _overlap(b, a)
+            assert _overlap(a, b) or not shared(a, b)
+    assert not _overlap(wide[:, :60], wide[:, 60:]) and not _overlap(wide, flat[2000:].view(20, 100))
+    assert not _overlap(wide[5:6], wide[6:7]) and not _overlap(wide[:0], wide)
