@@ -7,7 +7,8 @@ native_moe, routed_moe, combine_experts*, add_norm, silu_mul), ``moe_input``
 ``packed_prefill`` (PackedLayout, row_metadata), ``runtime_state``
 (DeviceRequests).  The decode step over persistent slots is
 ``pipeline.DecodeStep``, the mixed decode + prefill step ``mixed.MixedStep``
-and one whole MoE layer ``moe_layer.MoELayer``.  All compute runs in the HIP
+and one whole MoE layer ``moe_layer.MoELayer``.  ``mxfp4`` holds experts and
+projections in 4 bits, which ``kernels``' MoE operators take as well.  All compute runs in the HIP
 library ``_lib/libdrama3_moe.so``; there is no CPU fallback.
 """
 
