@@ -37,8 +37,10 @@ _FLOAT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 _INT = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
 
-# The current stream's handle without building a torch.cuda.Stream (1.7 us of
-# the 6 us a call of one launch costs the host).
+# Where rows are few, what a call costs the host counts (6.5 us with one launch,
+# 3.4 of them the launch): sizes are given to torch.empty one by one (1.0 us; as
+# a tuple 1.35), a tensor's length is taken from its shape (len: 0.27), and the
+# current stream's handle without building a torch.cuda.Stream (1.7).
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 if _raw_stream is None:
     def _raw_stream(index: int) -> int:
@@ -102,8 +104,8 @@ def quantize_mxfp4(x: torch.Tensor):
     rows, width = x.shape
     if width == 0 or width % BLOCK:
         raise ValueError(f"row width {width} must be a multiple of {BLOCK}")
-    codes = torch.empty((rows, width // 2), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((rows, width // BLOCK), dtype=torch.uint8, device=x.device)
+    codes = torch.empty(rows, width // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(rows, width // BLOCK, dtype=torch.uint8, device=x.device)
     _call(x.device, "d3_mxfp4_quantize", ptr(x), _FLOAT[x.dtype], x.stride(0), rows, width,
           ptr(codes), ptr(scales))
     return codes, scales
@@ -118,8 +120,9 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
     if dtype not in _FLOAT:
         raise TypeError("dtype must be bfloat16 or float32")
     codes, scales = codes.contiguous(), scales.contiguous()
-    rows, width = len(codes), 2 * codes.shape[1]
-    out = torch.empty((rows, width), dtype=dtype, device=codes.device)
+    rows, half = codes.shape
+    width = 2 * half
+    out = torch.empty(rows, width, dtype=dtype, device=codes.device)
     _call(codes.device, "d3_mxfp4_dequantize", ptr(codes), ptr(scales), rows, width, ptr(out),
           _FLOAT[dtype])
     return out
@@ -267,7 +270,7 @@ def _product(x, boundaries, weight: Mxfp4Weight, out, zero_rest: bool) -> torch.
         raise ValueError(f"rows of width {k}, weight of K={weight.k}")
     _same_device(x, weight.codes, "weight")
     if out is None:
-        out = torch.empty((rows, weight.n), dtype=torch.bfloat16, device=x.device)
+        out = torch.empty(rows, weight.n, dtype=torch.bfloat16, device=x.device)
     size = _entry("d3_mxfp4_grouped_workspace")(rows, weight.experts, boundaries is not None,
                                                   weight.n, k)
     workspace, at = _workspace(size, x)
@@ -303,11 +306,12 @@ def grouped_mxfp4(x: torch.Tensor, boundaries: torch.Tensor, weight: Mxfp4Weight
         raise ValueError(f"boundaries must be contiguous [{weight.experts + 1}], one more than the experts")
     _same_device(x, boundaries, "boundaries")
     if out is not None:
+        rows = x.shape[0]
         if out.dtype != torch.bfloat16:
             raise TypeError("out must be bfloat16")
-        if out.shape != (len(x), weight.n) or (weight.n > 1 and out.stride(1) != 1) or (
-                len(x) > 1 and out.stride(0) < weight.n):
-            raise ValueError(f"out must be [{len(x)}, {weight.n}] with unit column stride")
+        if out.shape != (rows, weight.n) or (weight.n > 1 and out.stride(1) != 1) or (
+                rows > 1 and out.stride(0) < weight.n):
+            raise ValueError(f"out must be [{rows}, {weight.n}] with unit column stride")
         _same_device(x, out, "out")
         if _overlap(x, out):
             raise ValueError("out must not overlap x")
@@ -327,7 +331,7 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     adds nothing), ``topk_weights`` bf16 / f32 of the same shape."""
     _check_rows(x)
     require_cuda(topk_ids, topk_weights)
-    if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape or len(topk_ids) != len(x):
+    if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape or topk_ids.shape[0] != x.shape[0]:
         raise ValueError("topk_ids / topk_weights must be [T, k] for the T rows of x")
     if topk_ids.dtype not in _INT:
         raise TypeError("topk_ids must be int32 or int64")
@@ -341,7 +345,7 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     _same_device(x, weights, "topk_weights")
     _same_device(x, w13.codes, "experts")
     rows, top_k = ids.shape
-    out = torch.empty((rows, experts.hidden), dtype=torch.bfloat16, device=x.device)
+    out = torch.empty(rows, experts.hidden, dtype=torch.bfloat16, device=x.device)
     size = _entry("d3_mxfp4_moe_workspace")(rows, top_k, w13.experts, w13.k, w2.k)
     workspace, at = _workspace(size, x)
     _call(x.device, "d3_mxfp4_moe", ptr(x), x.stride(0), rows, ptr(ids), _INT[ids.dtype],
