@@ -44,7 +44,7 @@ struct MxGemm {
   int rows;
   const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxHalf);
   int top_k;              // nullptr: the identity
-  const void* ids;        // kMxPairs: expert of each (row, rank) pair
+  const void* ids;        // kMxPairs, kMxScan: expert of each (row, rank) pair (kMxScan: of `rows` pairs)
   int ids_i64;
   int experts;
   const int32_t* bounds;  // kMxGroups: the groups' boundaries
@@ -111,8 +111,8 @@ __device__ __forceinline__ void mx_store16(uint16_t* out, int f, int n, const Mx
   }
 }
 
-// The four tiles of one row of `a` (this lane's row `row` of the item's list,
-// live or not) for row group rg.
+// The four tiles of one row of `a` (this lane's row `row` of the item's list, or
+// the row itself without one, live or not) for row group rg.
 template <int kEpi>
 __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4], int rg, int row, bool live, int group) {
   if constexpr (kEpi == kMxBf16 || kEpi == kMxHalf) {
@@ -129,7 +129,7 @@ __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4],
       const uint32_t exponent = mx_half_exponent(amax);
       factor = mx_half_factor(exponent);
       if (live) {
-        to = g.sorted[row];
+        if (g.sorted != nullptr) to = g.sorted[row];  // uniform
         if (group == 0) g.out_scales[to * g.row_groups + rg] = static_cast<uint8_t>(exponent);
       }
     }
@@ -213,8 +213,11 @@ __device__ __forceinline__ int64_t mx_pair_expert(const MxGemm& g, int64_t pair)
 // its own, which pays up to two row tiles.
 // kOnce: weights that one item reads are loaded non-temporally (moe 64 rows E256
 // 78.8 -> 72.0 us, grouped 384 rows E128 38.9 -> 37.4).
-template <int kRT, int kEpi, int kSplit, bool kDirect, bool kOnce>
-__device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item, int block, floatx4* part) {
+// kListed: the item's rows are those that `list` names (pairs), and so are the
+// rows of what it stores.
+template <int kRT, int kEpi, int kSplit, bool kDirect, bool kOnce, bool kListed = false>
+__device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item, int block, floatx4* part,
+                                               const int32_t* list = nullptr) {
   constexpr int kGroups = kMxWaves / kSplit;
   const int lane = lane_id(), row16 = lane & 15, group = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -229,6 +232,7 @@ __device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item
 #pragma unroll
   for (int rt = 0; rt < kRT; ++rt) {
     int64_t row = item.y + min(16 * rt + row16, count - 1);
+    if constexpr (kListed) row = list[row];
     if constexpr (kEpi == kMxAct) row = (g.sorted ? g.sorted[row] : static_cast<int>(row)) / g.top_k;
     if constexpr (kDirect) {
       codes[rt] = reinterpret_cast<const uint8_t*>(g.x + row * g.x_stride);
@@ -240,6 +244,11 @@ __device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item
   const int64_t base = static_cast<int64_t>(item.x) * g.row_groups + rg_read;
   const int32x4* w = reinterpret_cast<const int32x4*>(g.w + base * g.steps * kMxStepCodes) + lane;
   const uint2* ws = reinterpret_cast<const uint2*>(g.ws + base * g.steps * kMxStepScales) + lane;
+
+  auto store_row = [&](int rt) {
+    const int at = item.y + 16 * rt + row16;
+    return kListed ? list[min(at, item.y + count - 1)] : at;
+  };
 
   floatx4 acc[kRT][4];
 #pragma unroll
@@ -295,13 +304,13 @@ __device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item
         for (int s = 1; s < kSplit; ++s) sum[t] += part[(((first + s) * kRT + rt) * 4 + t) * kWave + lane];
       }
       if (rg < g.row_groups)
-        mx_store<kEpi>(g, sum, rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
+        mx_store<kEpi>(g, sum, rg, store_row(rt), 16 * rt + row16 < count, group);
     }
   } else {
     if (rg >= g.row_groups) return;
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt)
-      mx_store<kEpi>(g, acc[rt], rg, item.y + 16 * rt + row16, 16 * rt + row16 < count, group);
+      mx_store<kEpi>(g, acc[rt], rg, store_row(rt), 16 * rt + row16 < count, group);
   }
 }
 
@@ -309,15 +318,98 @@ __device__ __forceinline__ void mx_stream_item(const MxGemm& g, const int4& item
 enum MxSource {
   kMxList,   // the work items (or the rows in order)
   kMxPairs,  // an item per (row, rank) pair: few pairs, no route sort
+  kMxScan,   // the pairs of an expert, found among all of them by its workgroups: no route sort either
   kMxGroups, // the groups of the boundaries, one or two row tiles at a time
 };
+
+// Routes without a sort: the workgroups of an expert find its pairs among all of
+// them, and multiply the first 16.  An expert with more has a workgroup of its
+// own for each further 16; there are as many of those as pairs can fill, at the
+// front of the grid, and each finds its place from the experts' counts.
+constexpr int kMxScanPairs = 5 * kMxThreads;
+constexpr int kMxScanRounds = kMxScanPairs / kMxThreads;
+constexpr int kMxMaxExperts = 512;
+struct MxScan {
+  int32_t list[kMxScanPairs];
+  int counts[kMxMaxExperts];
+  int tally[kMxScanRounds][kMxWaves];
+  int expert, tile;
+};
+// An expert of c pairs has (c - 1) / 16 further tiles.
+__host__ __device__ constexpr int mx_scan_extra(int pairs) { return pairs / 16; }
+
+// The pairs of `expert` in ascending order; returns how many.
+__device__ __forceinline__ int mx_scan_pairs(const MxGemm& g, int expert, MxScan& scan) {
+  const int wave = threadIdx.x / kWave, rounds = (g.rows + kMxThreads - 1) / kMxThreads;
+  int64_t id[kMxScanRounds];
+  uint64_t hit[kMxScanRounds];
+#pragma unroll
+  for (int j = 0; j < kMxScanRounds; ++j)
+    if (j < rounds) id[j] = mx_pair_expert(g, min(j * kMxThreads + static_cast<int>(threadIdx.x), g.rows - 1));
+#pragma unroll
+  for (int j = 0; j < kMxScanRounds; ++j)
+    if (j < rounds) {
+      hit[j] = __ballot(id[j] == expert && j * kMxThreads + static_cast<int>(threadIdx.x) < g.rows);
+      if (lane_id() == 0) scan.tally[j][wave] = __builtin_popcountll(hit[j]);
+    }
+  __syncthreads();
+  int total = 0;
+#pragma unroll
+  for (int j = 0; j < kMxScanRounds; ++j)
+    if (j < rounds) {
+      int before = total;
+#pragma unroll
+      for (int w = 0; w < kMxWaves; ++w) {
+        const int n = scan.tally[j][w];
+        before += w < wave ? n : 0;
+        total += n;
+      }
+      if (hit[j] >> lane_id() & 1)
+        scan.list[before + __builtin_popcountll(hit[j] & ((uint64_t{1} << lane_id()) - 1))] =
+            j * kMxThreads + static_cast<int>(threadIdx.x);
+    }
+  __syncthreads();
+  return total;
+}
+
+// Expert and tile (1, ..) of the further tile `index`, into `scan`; expert -1: there is none.
+__device__ __forceinline__ void mx_scan_further(const MxGemm& g, int index, MxScan& scan) {
+  static_assert(kMxMaxExperts == 2 * kMxThreads, "two experts a thread");
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  scan.counts[2 * tid] = scan.counts[2 * tid + 1] = 0;
+  if (tid == 0) scan.expert = -1;
+  __syncthreads();
+  for (int at = tid; at < g.rows; at += kMxThreads) {
+    const int64_t id = mx_pair_expert(g, at);
+    if (id >= 0 && id < g.experts) atomicAdd(&scan.counts[id], 1);
+  }
+  __syncthreads();
+  auto further = [&](int e) { return max((scan.counts[e] + 15) / 16 - 1, 0); };
+  const int n0 = further(2 * tid), n1 = further(2 * tid + 1);
+  int sum = n0 + n1;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int v = __shfl_up(sum, d);
+    if (lane >= d) sum += v;
+  }
+  if (lane == kWave - 1) scan.tally[0][wave] = sum;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) sum += scan.tally[0][w];
+  const int first = sum - n0 - n1;
+  if (index >= first && index < first + n0)
+    scan.expert = 2 * tid, scan.tile = 1 + index - first;
+  else if (index >= first + n0 && index < sum)
+    scan.expert = 2 * tid + 1, scan.tile = 1 + index - first - n0;
+  __syncthreads();
+}
 
 template <int kRT, int kEpi, int kSplit, bool kDirect, int kSource>
 __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blocks) {
   constexpr int kGroups = kMxWaves / kSplit;
   // One matrix is read by every item; an expert's mostly by one (but a call of
-  // few pairs is short of latency, not of cache: non-temporal loads cost one
-  // token's gate and up product 5.5 -> 7.2 us where its experts are cached).
+  // few pairs or workgroups is short of latency, not of cache: non-temporal
+  // loads cost one token's gate and up product 5.5 -> 7.2 us where its experts
+  // are cached, and kMxScan's 57 rows over 60 experts 18.5 -> 21.3).
   constexpr bool kOnce = kSource == kMxGroups || (kSource == kMxList && kEpi != kMxBf16);
   __shared__ floatx4 part[kSplit > 1 ? kMxWaves * kRT * 4 * kWave : 1];
   const int index = blockIdx.x / blocks, block = blockIdx.x - index * blocks;
@@ -339,6 +431,20 @@ __global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blo
         mx_stream_item<1, kEpi, kSplit, kDirect, kOnce>(g, item, block, part);
       if (kSplit > 1) __syncthreads();  // `part` is read before the next tiles write it
     }
+  } else if constexpr (kSource == kMxScan) {
+    __shared__ MxScan scan;
+    const int extra = mx_scan_extra(g.rows);
+    int expert = index - extra, tile = 0;
+    if (index < extra) {  // uniform
+      mx_scan_further(g, index, scan);
+      expert = scan.expert, tile = scan.tile;
+      if (expert < 0) return;
+    }
+    const int count = mx_scan_pairs(g, expert, scan) - 16 * kRT * tile;
+    static_assert(kRT == 1, "tiles of 16 pairs");
+    if (count > 0)  // uniform
+      mx_stream_item<kRT, kEpi, kSplit, kDirect, kOnce, true>(g, make_int4(expert, 16 * tile, min(16, count), 0), block,
+                                                              part, scan.list);
   } else {
     int4 item;
     if constexpr (kSource == kMxPairs) {
@@ -746,7 +852,6 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(kMax
 // first workgroup) its work items, from the groups' boundaries or from the
 // routes' ids.
 constexpr int kPrepareThreads = 1024;
-constexpr int kMxSortExperts = 512;
 enum MxPrepareWhat {
   kMxRowsOnly,
   kMxBounds,
@@ -861,7 +966,7 @@ __device__ __forceinline__ void mx_items_of_routes(const MxPrepare& p, int* curs
   };
   constexpr int kRound = kPrepareThreads * kBatch;
   const bool once = p.count <= kRound;  // uniform
-  if (tid < kMxSortExperts) cursor[tid] = 0;
+  if (tid < kMxMaxExperts) cursor[tid] = 0;
   load(0);
   __syncthreads();
   for (int from = 0; from < p.count; from += kRound) {
@@ -905,7 +1010,7 @@ __device__ __forceinline__ int mx_route_expert(const MxPrepare& p, int pair) {
 __device__ __forceinline__ void mx_count_chunk(const MxPrepare& p, int chunk, int* counts) {
   const int tid = threadIdx.x, first = chunk * kChunkPairs + tid;
   const int e0 = mx_route_expert(p, first), e1 = mx_route_expert(p, first + kPrepareThreads);
-  if (tid < kMxSortExperts) counts[tid] = 0;
+  if (tid < kMxMaxExperts) counts[tid] = 0;
   __syncthreads();
   if (e0 >= 0) p.ranks[first] = atomicAdd(&counts[e0], 1);
   if (e1 >= 0) p.ranks[first + kPrepareThreads] = atomicAdd(&counts[e1], 1);
@@ -914,7 +1019,7 @@ __device__ __forceinline__ void mx_count_chunk(const MxPrepare& p, int chunk, in
 }
 
 __global__ __launch_bounds__(kPrepareThreads) void mx_place_kernel(MxPrepare p) {
-  __shared__ int place[kMxSortExperts];
+  __shared__ int place[kMxMaxExperts];
   __shared__ int2 sums[kPrepareThreads / kWave];
   const int tid = threadIdx.x, first = blockIdx.x * kChunkPairs + tid;
   int expert[2], rank[2];
@@ -950,7 +1055,7 @@ template <int kWhat, int kBatch = 1>
 __global__ __launch_bounds__(kPrepareThreads) void mx_prepare_kernel(MxPrepare p) {
   uint32_t block = blockIdx.x;
   if constexpr (kWhat != kMxRowsOnly) {
-    __shared__ int cursor[kMxSortExperts];
+    __shared__ int cursor[kMxMaxExperts];
     __shared__ int2 sums[kPrepareThreads / kWave];
     const uint32_t others = kWhat == kMxRouteChunks ? p.chunks : 1;
     if (block < others) {
@@ -1106,6 +1211,20 @@ MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n, int64_t k) {
   return choose_tiled(pairs, partial, n);
 }
 
+// Routes that need no sort (three launches, not four): few enough pairs for each
+// workgroup to look through, and no more workgroups than four a CU, for they all
+// do.  Us, without / with the sort: E16 H1024 I256, 160 / 320 / 1184 pairs 17.0 /
+// 17.0 / 21.4 against 17.6 / 20.4 / 25.4; E60 H640 I512, 456 pairs 19.7 against
+// 21.6; E200 H512 I256, 800 pairs (988 workgroups) 19.9 against 22.6; but E16
+// H2048 I768, 560 pairs (1152) 29.0 against 26.0, E8 H1920 I512, 1280 pairs
+// (1328) 39.8 against 27.0, E256 H2048 I512, 512 pairs (4576) 73.7 against 72.5,
+// and E16 H1024 I256, 2000 pairs 28.7 against 24.2.
+bool choose_scan(int64_t pairs, int64_t experts, int hidden, int inter) {
+  if (pairs > kMxScanPairs) return false;
+  const int64_t up = stream_blocks(2 * static_cast<int64_t>(inter), hidden), down = stream_blocks(hidden, inter);
+  return (experts + mx_scan_extra(static_cast<int>(pairs))) * (up > down ? up : down) <= 4 * kMxCus;
+}
+
 // Byte arena of one call, carved in order at 256-byte boundaries.
 struct Arena {
   uint8_t* base;
@@ -1185,6 +1304,7 @@ constexpr int kMxFewPairs = 128;
 constexpr int kMxOnePairs = 8 * kPrepareThreads;
 struct MoePlan {
   bool few;   // no grouping, down product and combine in one launch
+  bool scan;  // no grouping: every expert's workgroups find its pairs
   int chunks;  // 0: one workgroup groups the pairs; above kMxMaxChunks: the route sort
   MxChoice how;
   int max_items;
@@ -1202,6 +1322,7 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
   p.pairs = rows * top_k;
   p.few = p.pairs <= kMxFewPairs;
   p.chunks = p.pairs <= kMxOnePairs ? 0 : mx_ceil(p.pairs, kChunkPairs);
+  p.scan = !p.few && choose_scan(p.pairs, experts, hidden, inter);
   p.how = choose_routed(p.pairs, experts, 2 * static_cast<int64_t>(inter), hidden);
   p.max_items = d3_max_items(static_cast<int32_t>(p.pairs), experts, p.how.item_rows);
   Arena a{static_cast<uint8_t*>(arena)};
@@ -1209,12 +1330,14 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
   p.act = a.take<uint8_t>(p.pairs * act_steps * kMxOperandCodes);
   p.acts = a.take<uint8_t>(p.pairs * act_steps * kMxOperandScales);
   if (!p.few) {
-    if (p.how.tiled) {
+    if (p.how.tiled && !p.scan) {
       p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
       p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
     }
     p.rows = a.take<uint16_t>(p.pairs * hidden);
     p.exponents = a.take<uint8_t>(p.pairs * (hidden / kMxRows));
+  }
+  if (!p.few && !p.scan) {
     p.sorted = a.take<int32_t>(p.pairs);
     p.items = a.take<int4>(p.max_items);
     p.num_items = a.take<int32_t>(1);
@@ -1364,13 +1487,28 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   down.a = p.act, down.as = p.acts, down.out_stride = hidden;
   for (MxGemm* g : {&up, &down}) {
     g->items = p.items, g->num_items = p.num_items, g->max_items = p.max_items, g->sorted = p.sorted, g->top_k = top_k;
-    g->ids = ids, g->ids_i64 = i64, g->experts = num_experts;
+    g->ids = ids, g->ids_i64 = i64, g->experts = num_experts, g->rows = static_cast<int>(p.pairs);
   }
   if (p.few) {
     launch_stream<1, kMxAct, true, kMxPairs>(up, static_cast<int>(p.pairs), s);
     down.out = out;
     hipLaunchKernelGGL(mx_down_combine_kernel, dim3(static_cast<unsigned>(rows) * down.row_groups),
                        dim3(kDownWaves * kWave), 0, s, down, weights, f32);
+    D3_LAUNCHED("mxfp4_moe");
+  }
+  const int slices = mx_ceil(hidden, kMxCombineColumns);
+  const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
+  auto combine = [&] {
+    auto kernel = top_k == 8 ? mx_combine_kernel<8> : mx_combine_kernel<0>;
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
+                       slices, out);
+  };
+  down.out = p.rows, down.out_scales = p.exponents;
+  if (p.scan) {
+    const int items = num_experts + mx_scan_extra(static_cast<int>(p.pairs));
+    launch_stream<1, kMxAct, true, kMxScan>(up, items, s);
+    launch_stream<1, kMxHalf, false, kMxScan>(down, items, s);
+    combine();
     D3_LAUNCHED("mxfp4_moe");
   }
   MxPrepare prepare{};
@@ -1403,15 +1541,7 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
     }
   }
   launch_gemm<kMxAct>(up, p.how, p.max_items, s);
-  down.out = p.rows, down.out_scales = p.exponents;
   launch_gemm<kMxHalf>(down, p.how, p.max_items, s);
-  const int slices = mx_ceil(hidden, kMxCombineColumns);
-  const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
-  if (top_k == 8)
-    hipLaunchKernelGGL(mx_combine_kernel<8>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k,
-                       num_experts, hidden, slices, out);
-  else
-    hipLaunchKernelGGL(mx_combine_kernel<0>, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k,
-                       num_experts, hidden, slices, out);
+  combine();
   D3_LAUNCHED("mxfp4_moe");
 }

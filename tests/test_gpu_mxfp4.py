@@ -371,6 +371,30 @@ def test_moe(device, rows, experts, hidden, inter, top_k, skew):
     within(out, *om.moe(f64(x), ids.numpy(), f64(weights), v13, v2))
 
 
+@pytest.mark.parametrize("rows, experts, top_k, inter, id_type", [
+    (129, 3, 1, 128, torch.int32), (43, 512, 3, 128, torch.int64), (320, 5, 4, 128, torch.int32),  # to 1280 pairs
+    (427, 5, 3, 128, torch.int64), (40, 200, 8, 640, torch.int32), (100, 200, 8, 640, torch.int64)])
+def test_moe_pairs_found_by_their_experts(device, rows, experts, top_k, inter, id_type):
+    """Batches without a sort and the first with one: all pairs of one expert (the
+    last of them), of two, every count around whole tiles, ids of no expert."""
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    rng = np.random.default_rng(rows + experts)
+    packed, v13, v2 = make_experts(rng, experts, 128, inter, device)
+    x = rows_of(rng, rows, 128)
+    pairs = rows * top_k
+    weights = torch.from_numpy(rng.random((rows, top_k))).to(torch.bfloat16)
+    last = experts - 1
+    patterns = [np.full(pairs, last), np.where(np.arange(pairs) < 65, last, 0), np.where(np.arange(pairs) % 17, last, 0),
+                np.repeat(np.arange(-1, pairs // 16 + 1), 17)[:pairs] % (experts + 1),
+                np.repeat(np.arange(pairs // 15 + 1), 16)[:pairs] % experts - 1, np.full(pairs, experts),
+                rng.integers(-2, experts + 2, pairs)]
+    for ids in patterns:
+        ids = torch.from_numpy(rng.permutation(ids).reshape(rows, top_k)).to(id_type)
+        out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
+        within(out, *om.moe(f64(x), ids.numpy(), f64(weights), v13, v2))
+
+
 @pytest.mark.parametrize("rows, hidden, inter, skew", [(150, 640, 1152, 0.5), (320, 384, 1024, 0.0),
                                                        (330, 256, 1152, 1.0)])
 def test_moe_in_large_items(device, rows, hidden, inter, skew):
