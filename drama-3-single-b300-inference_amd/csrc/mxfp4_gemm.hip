@@ -901,20 +901,23 @@ __device__ __forceinline__ int mx_scan(int2* v, int2* sums) {
 }
 
 // Every thread's group as items from `at` on (each of the workgroup's threads
-// comes here): its first by the thread, a busy group's others by the whole wave
-// (16054 rows of one group, K 896 N 70: 30.0 us by its thread alone, 18.2 so).
+// comes here): its first 16 by the thread, a busy group's others by the whole
+// wave (16054 rows of one group, K 896 N 70: 30.0 us by its thread alone, 18.2
+// so; but 1600 pairs over 60 experts, H384 I128: 31.2 us if only the first is the
+// thread's, 19.9 so).
+constexpr int kMxOwnItems = 16;
 __device__ __forceinline__ void mx_write_items(const MxPrepare& p, int at, int expert, int first, int count) {
   const int lane = lane_id();
   auto write = [&](int i, int to, int e, int from, int n) {
     if (i * p.item_rows < n && to + i < p.max_items)
       p.items[to + i] = make_int4(e, from + i * p.item_rows, min(p.item_rows, n - i * p.item_rows), 0);
   };
-  write(0, at, expert, first, count);
-  for (uint64_t busy = __ballot(count > p.item_rows); busy != 0; busy &= busy - 1) {
+  for (int i = 0; i < kMxOwnItems && i * p.item_rows < count; ++i) write(i, at, expert, first, count);
+  for (uint64_t busy = __ballot(count > kMxOwnItems * p.item_rows); busy != 0; busy &= busy - 1) {
     const int of = __builtin_ctzll(busy);
     const int to = __shfl(at, of), e = __shfl(expert, of), from = __shfl(first, of), n = __shfl(count, of);
     const int items = min((n + p.item_rows - 1) / p.item_rows, p.max_items - to);
-    for (int i = 1 + lane; i < items; i += kWave) write(i, to, e, from, n);
+    for (int i = kMxOwnItems + lane; i < items; i += kWave) write(i, to, e, from, n);
   }
 }
 
