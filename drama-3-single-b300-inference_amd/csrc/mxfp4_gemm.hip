@@ -1216,12 +1216,13 @@ MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n, int64_t k) {
 
 // Routes that need no sort (three launches, not four): few enough pairs for each
 // workgroup to look through, and no more workgroups than four a CU, for they all
-// do.  Us, without / with the sort: E16 H1024 I256, 160 / 320 / 1184 pairs 17.0 /
-// 17.0 / 21.4 against 17.6 / 20.4 / 25.4; E60 H640 I512, 456 pairs 19.7 against
-// 21.6; E200 H512 I256, 800 pairs (988 workgroups) 19.9 against 22.6; but E16
-// H2048 I768, 560 pairs (1152) 29.0 against 26.0, E8 H1920 I512, 1280 pairs
-// (1328) 39.8 against 27.0, E256 H2048 I512, 512 pairs (4576) 73.7 against 72.5,
-// and E16 H1024 I256, 2000 pairs 28.7 against 24.2.
+// do.  Us, without / with the sort: E16 H1024 I256, 160 / 480 / 1038 / 1184 pairs
+// 16.9 / 17.2 / 20.0 / 21.4 against 17.5 / 19.0 / 21.7 / 22.0; E16 H2048 I768, 320
+// pairs 24.6 against 27.5; E60 H640 I512, 456 pairs 19.3 against 21.6; E200 H512
+// I256, 800 pairs (992 workgroups) 19.2 against 21.2; but E16 H2048 I768, 560
+// pairs (1224) 28.0 against 24.6, E8 H1920 I512, 1280 pairs (1408) 40.0 against
+// 25.3, E256 H2048 I512, 512 pairs (4608) 79.1 against 72.3, and E8 H1024 I256,
+// 2000 pairs 25.9 against 21.3.
 bool choose_scan(int64_t pairs, int64_t experts, int hidden, int inter) {
   if (pairs > kMxScanPairs) return false;
   const int64_t up = stream_blocks(2 * static_cast<int64_t>(inter), hidden), down = stream_blocks(hidden, inter);
