@@ -1203,15 +1203,13 @@ MxChoice choose_linear(int64_t rows, int64_t n, int64_t k) {
   return choose_tiled(rows, 0, n);
 }
 
-// Rows grouped by expert.  Routed experts stream up to 8 rows an expert, or
-// while that is a few rounds of workgroups.  Us, streaming / tiled: E256 H2048
-// I512, 8 rows an expert 98.7 / 105, 16 rows 122 / 108; E16 H1024 I256, 32 rows
-// an expert 20.1 / 22.9, 96 rows 25.0 / 25.6, 128 rows 28.1 / 26.6.
-constexpr int kMxFewGroups = 832;
-MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n, int64_t k) {
+// Rows grouped by expert: up to 8 rows an expert they stream, for more than one
+// tile of 16 reads an expert's weights again.  Us, streaming / tiled: E256 H2048
+// I512, 8 rows an expert 98.7 / 105, 16 rows 122 / 108; E8 H1920 I256, 164 rows an
+// expert 28.5 / 24.4; E24 H128 I128, 500 rows an expert 31.6 / 26.6.
+MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n) {
   const int64_t partial = (pairs < experts ? pairs : experts) / 2;
-  if (pairs <= 8 * experts || (pairs / 16 + partial) * stream_blocks(n, k) <= kMxFewGroups) return {false, 16};
-  return choose_tiled(pairs, partial, n);
+  return pairs <= 8 * experts ? MxChoice{false, 16} : choose_tiled(pairs, partial, n);
 }
 
 // Routes that need no sort (three launches, not four): few enough pairs for each
@@ -1301,7 +1299,11 @@ void launch_prepare(const MxPrepare& p, unsigned blocks, hipStream_t s) {
 // Up to so many pairs each is an item of its own, whatever their experts:
 // E256 H2048 I512, 64 / 128 / 192 / 256 pairs 23.9 / 36.3 / 49.7 / 61.8 us
 // against 32.3 / 42.9 / 53.2 / 61.1 with the routes grouped; E128 I768, 64 /
-// 128 / 192 pairs 30.9 / 46.7 / 62.9 against 38.8 / 48.7 / 55.8.
+// 128 / 192 pairs 30.9 / 46.7 / 62.9 against 38.8 / 48.7 / 55.8.  A few experts'
+// pairs read the same weights again and again: past four workgroups a CU their
+// experts' workgroups find them instead, if those are few enough (E8 H1536 I640,
+// 32 / 64 / 128 pairs 14.9 / 17.4 / 22.3 us against 14.7-16.5 / 15.0-16.7 /
+// 15.7-17.0; E16 H1024 I256, 128 pairs 14.0 against 15.1).
 constexpr int kMxFewPairs = 128;
 // Up to so many pairs are grouped by one workgroup, up to kMxMaxChunks chunks by
 // a workgroup a chunk, more by the route sort over many workgroups.
@@ -1324,10 +1326,11 @@ struct MoePlan {
 MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, int inter) {
   MoePlan p{};
   p.pairs = rows * top_k;
-  p.few = p.pairs <= kMxFewPairs;
   p.chunks = p.pairs <= kMxOnePairs ? 0 : mx_ceil(p.pairs, kChunkPairs);
-  p.scan = !p.few && choose_scan(p.pairs, experts, hidden, inter);
-  p.how = choose_routed(p.pairs, experts, 2 * static_cast<int64_t>(inter), hidden);
+  p.scan = choose_scan(p.pairs, experts, hidden, inter);
+  p.few = p.pairs <= kMxFewPairs && (!p.scan || p.pairs * stream_blocks(2 * static_cast<int64_t>(inter), hidden) <= 4 * kMxCus);
+  p.scan = p.scan && !p.few;
+  p.how = choose_routed(p.pairs, experts, 2 * static_cast<int64_t>(inter));
   p.max_items = d3_max_items(static_cast<int32_t>(p.pairs), experts, p.how.item_rows);
   Arena a{static_cast<uint8_t*>(arena)};
   const int64_t x_steps = mx_ceil(hidden, kMxStep), act_steps = mx_ceil(inter, kMxStep);

@@ -372,11 +372,12 @@ def test_moe(device, rows, experts, hidden, inter, top_k, skew):
 
 
 @pytest.mark.parametrize("rows, experts, top_k, inter, id_type", [
-    (129, 3, 1, 128, torch.int32), (43, 512, 3, 128, torch.int64), (320, 5, 4, 128, torch.int32),  # to 1280 pairs
-    (427, 5, 3, 128, torch.int64), (40, 200, 8, 640, torch.int32), (100, 200, 8, 640, torch.int64)])
+    (32, 3, 4, 1152, torch.int32), (129, 3, 1, 128, torch.int32), (43, 512, 3, 128, torch.int64), (320, 5, 4, 128, torch.int32),
+    (427, 5, 3, 128, torch.int64), (40, 200, 8, 640, torch.int32), (150, 200, 8, 640, torch.int64)])
 def test_moe_pairs_found_by_their_experts(device, rows, experts, top_k, inter, id_type):
-    """Batches without a sort and the first with one: all pairs of one expert (the
-    last of them), of two, every count around whole tiles, ids of no expert."""
+    """Batches without a sort (up to 1280 pairs of few workgroups) and with one:
+    all pairs of one expert (the last of them), of two, every count around whole
+    tiles, ids of no expert."""
     from drama3_amd.mxfp4 import mxfp4_moe
 
     rng = np.random.default_rng(rows + experts)
