@@ -1245,11 +1245,15 @@ void set_weight(MxGemm& g, const uint8_t* w, const uint8_t* ws, int n, int k) {
 }
 
 // A grouped product takes one of three ways:
-//   walk     few rows over many groups: one launch that walks each group's row
-//            tiles and quantises them itself (no work items);
+//   walk     few rows, or few over many groups: one launch that walks each
+//            group's row tiles and quantises them itself (no work items);
 //   direct   few rows of one matrix: one launch that quantises them itself;
 //   else     quantised rows, work items from the boundaries, the product.
-constexpr int kMxWalkRows = 512;  // most rows of groups walked by their own workgroups: one busy group is walked alone
+// A group's workgroups walk its rows one tile after the other, so a busy group
+// must be short.  Us, walked / not: one group of 21 rows K 768 N 584 8.8 / 12.3,
+// of 48 K 2048 N 2048 10.6 / 11.9, of 64 13.9 / 12.0, of 160 28.2 / 12.1; 500
+// rows over 16 groups 9.3 / 11.8 and, most of them in a few, 309 rows 20.6 / 12.5.
+constexpr int kMxWalkRows = 512, kMxWalkAny = 48;
 struct GroupedPlan {
   bool walk;
   MxChoice how;
@@ -1262,7 +1266,7 @@ struct GroupedPlan {
 
 GroupedPlan plan_grouped(void* arena, int64_t rows, int experts, bool bounded, int n, int k) {
   GroupedPlan p{};
-  p.walk = bounded && rows <= kMxWalkRows && rows <= 16 * static_cast<int64_t>(experts);
+  p.walk = bounded && (rows <= kMxWalkAny || (rows <= kMxWalkRows && rows <= 16 * static_cast<int64_t>(experts)));
   if (p.walk) return p;
   const int64_t partial = rows < experts ? rows : experts;
   p.how = bounded ? choose_tiled(rows, partial / 2, n) : choose_linear(rows, n, k);

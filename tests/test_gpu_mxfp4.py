@@ -257,7 +257,8 @@ def test_grouped(device, bounds, k, n):
 
 
 @pytest.mark.parametrize("rows, experts, k, n", [(700, 3, 128, 1000), (3000, 16, 256, 64), (900, 100, 256, 130),
-                                                 (4000, 2000, 128, 40), (1, 5, 384, 65)])
+                                                 (4000, 2000, 128, 40), (1, 5, 384, 65),
+                                                 (48, 1, 384, 130), (49, 1, 384, 130)])
 def test_grouped_at_random(device, rows, experts, k, n):
     from drama3_amd.mxfp4 import grouped_mxfp4, prepare_mxfp4
 
