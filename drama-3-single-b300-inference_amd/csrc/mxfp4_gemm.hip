@@ -1055,7 +1055,7 @@ __global__ __launch_bounds__(kPrepareThreads) void mx_place_kernel(MxPrepare p) 
 }
 
 template <int kWhat, int kBatch = 1>
-__global__ __launch_bounds__(kPrepareThreads) void mx_prepare_kernel(MxPrepare p) {
+__global__ __launch_bounds__(kPrepareThreads) __attribute__((amdgpu_waves_per_eu(8))) void mx_prepare_kernel(MxPrepare p) {
   uint32_t block = blockIdx.x;
   if constexpr (kWhat != kMxRowsOnly) {
     __shared__ int cursor[kMxMaxExperts];
