@@ -403,8 +403,11 @@ __device__ __forceinline__ void mx_scan_further(const MxGemm& g, int index, MxSc
   __syncthreads();
 }
 
+// Two row tiles are held to four waves a SIMD (384 rows over 128 groups 37.7 ->
+// 34.8 us; to five, with spills, 45); one tile has them anyhow, and asked for more
+// loses in skewed batches what it gains in even ones.
 template <int kRT, int kEpi, int kSplit, bool kDirect, int kSource>
-__global__ __launch_bounds__(kMxThreads) void mx_stream_kernel(MxGemm g, int blocks) {
+__global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(kRT > 1 ? 4 : 1))) void mx_stream_kernel(MxGemm g, int blocks) {
   constexpr int kGroups = kMxWaves / kSplit;
   // One matrix is read by every item; an expert's mostly by one (but a call of
   // few pairs or workgroups is short of latency, not of cache: non-temporal
