@@ -130,6 +130,18 @@ def test_quantize_and_back_past_32_bit_offsets(device):
     assert not values[-6].any()
 
 
+def test_quantize_more_units_than_32_bits_count(device):
+    """2^32 runs of eight elements and a few more, the same row all along."""
+    from drama3_amd.mxfp4 import quantize_mxfp4
+
+    x = rows_of(np.random.default_rng(28), 1, 32)
+    rows = (1 << 30) + 5
+    codes, scales = quantize_mxfp4(x.to(device).expand(rows, 32))
+    want_codes, want_scales = om.quantize(f64(x))
+    for part in (slice(0, 3), slice((1 << 29) - 2, (1 << 29) + 2), slice(rows - 8, rows)):
+        assert (codes[part].cpu().numpy() == want_codes).all() and (scales[part].cpu().numpy() == want_scales).all()
+
+
 # ---------------------------------------------------------------------------
 @pytest.mark.parametrize("rows", [1, 15, 16, 17, 33, 64, 65, 127, 129, 300])
 @pytest.mark.parametrize("k, n", [(128, 1), (256, 64), (384, 33), (1152, 200)])
@@ -359,7 +371,7 @@ def make_routes(rng, rows, experts, top_k, skew=0.0):
 @pytest.mark.parametrize("rows, experts, hidden, inter, top_k, skew", [
     (1, 16, 256, 128, 8, 0), (1, 1, 128, 128, 1, 0), (5, 60, 384, 256, 8, 0), (40, 16, 256, 384, 4, 1.5),
     (130, 8, 512, 128, 2, 0), (64, 200, 256, 128, 8, 0), (300, 4, 128, 256, 1, 1.0), (17, 16, 640, 128, 16, 0),
-    (600, 8, 256, 256, 8, 0.8)])
+    (600, 8, 256, 256, 8, 0.8), (3, 4, 2304, 256, 2, 0), (40, 4, 2304, 128, 8, 0), (30, 512, 128, 128, 5, 0)])
 def test_moe(device, rows, experts, hidden, inter, top_k, skew):
     from drama3_amd.mxfp4 import mxfp4_moe
 
