@@ -225,7 +225,11 @@ def prepare_mxfp4_experts(w13_codes, w13_scales, w2_codes, w2_scales) -> Mxfp4Ex
 def quantize_experts_mxfp4(experts) -> Mxfp4Experts:
     """FP8 block-scaled experts (``w13_weight``, ``w13_scale_inv``,
     ``w2_weight``, ``w2_scale_inv``: the MoE operators' contract) rounded to
-    MXFP4, one expert at a time, at load time."""
+    MXFP4, one expert at a time, at load time.  They have to hold checkpoint
+    rows: not after ``prepare_experts(..., keep_reference=False)``."""
+    if any(getattr(experts, f"d3_{name}_fragment_only", False) for name in ("w13", "w2")):
+        raise ValueError("experts hold only fragment-major codes; quantise them before "
+                         "prepare_experts(keep_reference=False)")
     packed = []
     for weight, inverse, order in ((experts.w13_weight, experts.w13_scale_inv, ORDER_GATE_UP),
                                    (experts.w2_weight, experts.w2_scale_inv, ORDER_ROWS)):

@@ -558,6 +558,19 @@ def test_operators_take_mxfp4_experts(device):
     assert routed_moe(x[:0], router[:0], experts).shape == (0, 256)
 
 
+def test_fp8_experts_without_checkpoint_rows_are_refused(device):
+    from drama3_amd import workloads
+    from drama3_amd.expert_weights import prepare_experts
+    from drama3_amd.mxfp4 import quantize_experts_mxfp4
+
+    fp8 = workloads.make_experts(torch.Generator("cpu").manual_seed(4), 2, 256, 128).to(device)
+    want = quantize_experts_mxfp4(fp8)
+    kept = quantize_experts_mxfp4(prepare_experts(fp8))
+    assert torch.equal(kept.w13.codes, want.w13.codes) and torch.equal(kept.w2.scales, want.w2.scales)
+    with pytest.raises(ValueError, match="fragment-major"):
+        quantize_experts_mxfp4(prepare_experts(fp8, keep_reference=False))
+
+
 def test_empty_batches(device):
     from drama3_amd import mxfp4 as mx
 
