@@ -25,7 +25,6 @@ products are one padded batch each.
 
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -207,7 +206,6 @@ def _plain_moe(state):
 # ---------------------------------------------------------------------------
 # The framework's calls
 # ---------------------------------------------------------------------------
-@functools.cache  # imported once, as a user's program does
 def _package():
     path = str(Path(__file__).resolve().parents[1] / "drama-3-single-b300-inference_amd")
     if path not in sys.path:
