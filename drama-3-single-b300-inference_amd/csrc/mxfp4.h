@@ -103,30 +103,6 @@ __device__ __forceinline__ uint32_t mx_codes8_bf16(const uint32_t* w, float scal
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2, w[3]), scale, 3);
 }
 
-// Eight fp32 values as scaled fp16 and back: a route's down row is kept in 16
-// bits between the product and the combine, with one power of two per 64
-// columns that brings their largest finite magnitude into [2^14, 2^15).  Its
-// rounding (2^-11 relative, fp16's half step, down to 2^-29 of the largest) is
-// an eighth of the bf16 rounding of the result, and the rows' traffic, the
-// largest of a prefill's down product and combine, is halved.
-// `exponent`: of the largest finite magnitude, biased, 15 .. 254; the factor is
-// 2^(141 - exponent), its inverse 2^(exponent - 141).
-__device__ __forceinline__ uint32_t mx_half_exponent(uint32_t amax) {
-  const uint32_t e = amax >> 23;
-  return e < 15u ? 15u : e;
-}
-__device__ __forceinline__ float mx_half_factor(uint32_t exponent) { return __uint_as_float((268u - exponent) << 23); }
-__device__ __forceinline__ float mx_half_inverse(uint32_t exponent) { return __uint_as_float((exponent - 14u) << 23); }
-typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
-__device__ __forceinline__ uint32_t mx_pack_half(float lo, float hi) {
-  return __builtin_bit_cast(uint32_t, halfx2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
-}
-// The larger of two magnitudes' bits, leaving out infinities and NaN.
-__device__ __forceinline__ uint32_t mx_max_finite(uint32_t amax, float v) {
-  const uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
-  return MaxU32::apply(amax, bits < 0x7f800000u ? bits : 0u);
-}
-
 // Memory words at the alignment of their elements only: gfx950 takes wide
 // accesses at any address, so odd row strides cost no narrow path.
 struct __attribute__((packed, aligned(2))) MxWords4 { uint32_t w[4]; };

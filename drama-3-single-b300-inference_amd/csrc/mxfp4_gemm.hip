@@ -23,7 +23,7 @@ constexpr int kMxThreads = kMxWaves * kWave;
 enum MxEpilogue {
   kMxBf16,  // bf16 rows at the item's rows
   kMxAct,   // silu(gate) * up quantised to MXFP4 rows at the item's rows (gate-up order)
-  kMxHalf,  // scaled fp16 rows at sorted[row]
+  kMxF32,   // fp32 rows at sorted[row]
 };
 
 struct MxGemm {
@@ -42,7 +42,7 @@ struct MxGemm {
   const int32_t* num_items;
   int max_items;
   int rows;
-  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxHalf);
+  const int32_t* sorted;  // route list: row of a = sorted[row] / top_k (kMxAct), row of out = sorted[row] (kMxF32);
   int top_k;              // nullptr: the identity
   const void* ids;        // kMxPairs, kMxScan: expert of each (row, rank) pair (kMxScan: of `rows` pairs)
   int ids_i64;
@@ -52,7 +52,7 @@ struct MxGemm {
   void* out;
   int64_t out_stride;  // elements (kMxAct: the row's width)
   bool out_past;  // kMxBf16, tiled: more than the L2s hold, stored past them
-  uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout; kMxHalf: exponents [rows][row groups]
+  uint8_t* out_scales;  // kMxAct: out and out_scales in the operand layout
 };
 
 // One MFMA with the scales in byte SA of `sa` and byte SB of `sb`.
@@ -83,13 +83,10 @@ __device__ __forceinline__ int4 mx_item(const MxGemm& g, int index, int item_row
   return index < live ? item : make_int4(0, 0, 0, 0);
 }
 
-// Eight values as bf16, or as the fp16 of kMxHalf.
-template <int kEpi>
 __device__ __forceinline__ MxWords4 mx_pack8(const float* v) {
   MxWords4 w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w.w[i] = kEpi == kMxHalf ? mx_pack_half(v[2 * i], v[2 * i + 1]) : pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) w.w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
   return w;
 }
 
@@ -115,32 +112,23 @@ __device__ __forceinline__ void mx_store16(uint16_t* out, int f, int n, const Mx
 // the row itself without one, live or not) for row group rg.
 template <int kEpi>
 __device__ __forceinline__ void mx_store(const MxGemm& g, const floatx4 (&c)[4], int rg, int row, bool live, int group) {
-  if constexpr (kEpi == kMxBf16 || kEpi == kMxHalf) {
-    int64_t to = row;
-    float factor = 1.0f;
-    if constexpr (kEpi == kMxHalf) {
-      uint32_t amax = 0;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) amax = mx_max_finite(amax, c[t][i]);
-      amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16)));
-      amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
-      const uint32_t exponent = mx_half_exponent(amax);
-      factor = mx_half_factor(exponent);
-      if (live) {
-        if (g.sorted != nullptr) to = g.sorted[row];  // uniform
-        if (group == 0) g.out_scales[to * g.row_groups + rg] = static_cast<uint8_t>(exponent);
-      }
-    }
+  if constexpr (kEpi == kMxBf16 || kEpi == kMxF32) {
     if (!live) return;
-    uint16_t* out = static_cast<uint16_t*>(g.out) + to * g.out_stride;
+    int64_t to = row;
+    if (kEpi == kMxF32 && g.sorted != nullptr) to = g.sorted[row];  // uniform
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      float v[8];
+      const int f = kMxRows * rg + 32 * p + 8 * group;
+      if constexpr (kEpi == kMxF32) {  // whole row groups: n is a multiple of 128
+        floatx4* out = reinterpret_cast<floatx4*>(static_cast<float*>(g.out) + to * g.out_stride + f);
+        out[0] = c[2 * p];
+        out[1] = c[2 * p + 1];
+      } else {
+        float v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c[2 * p + i / 4][i % 4] * factor;
-      mx_store16(out, kMxRows * rg + 32 * p + 8 * group, g.n, mx_pack8<kEpi>(v));
+        for (int i = 0; i < 8; ++i) v[i] = c[2 * p + i / 4][i % 4];
+        mx_store16(static_cast<uint16_t*>(g.out) + to * g.out_stride, f, g.n, mx_pack8(v));
+      }
     }
   } else if constexpr (kEpi == kMxAct) {
     // Gate (tiles 0, 1) and up (tiles 2, 3) of columns 32 rg + 8 group + i;
@@ -565,7 +553,7 @@ __device__ __forceinline__ floatx16 mfma_fp4_32(const int32x4& a, const int32x4&
 // The sums of 32 rows for row group rg in the 32x32 output layout: lane half
 // hl holds rows 8 j + 4 hl + i (element 4 j + i) of each 32-row half u of the
 // group, columns 16 (j % 2) + 8 hl + 4 (j / 2) + i of it.
-// 16-bit rows pass through the wave's own LDS, 144 bytes a row, so that a store
+// Rows pass through the wave's own LDS, 144 bytes a row, so that a store
 // writes eight whole 128-byte pieces instead of 32 bytes of 32 rows: a quarter
 // of the lines to look up (4096 x 2048 x 1281, whose rows start anywhere in a
 // line: 17.8 -> 13.6 us).
@@ -600,41 +588,43 @@ __device__ __forceinline__ void mx_store32(const MxGemm& g, const floatx16 (&c)[
     *reinterpret_cast<uint32_t*>(codes) = lo;
     *reinterpret_cast<uint32_t*>(codes + 8) = hi;
     if (hl == 0) mx_operand_scale(g.out_scales + at * kMxOperandScales, rg, blocks, code);
-  } else {
-    float factor = 1.0f;
-    if constexpr (kEpi == kMxHalf) {
-      uint32_t amax = 0;
+  } else if constexpr (kEpi == kMxF32) {
+    // A half of the group's columns at a time: 128 bytes a row, as above.
+    const int part = lane & 7;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) amax = mx_max_finite(amax, c[u][i]);
-      amax = MaxU32::apply(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32)));
-      const uint32_t exponent = mx_half_exponent(amax);
-      factor = mx_half_factor(exponent);
-      if (live && hl == 0)
-        g.out_scales[static_cast<int64_t>(targets[first + col]) * g.row_groups + rg] = static_cast<uint8_t>(exponent);
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<floatx4*>(area + col * kMxStoreRow + 64 * (j % 2) + 32 * hl + 16 * (j / 2)) =
+            floatx4{c[u][4 * j], c[u][4 * j + 1], c[u][4 * j + 2], c[u][4 * j + 3]};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 8 * k + (lane >> 3);
+        const floatx4 w = *reinterpret_cast<const floatx4*>(area + r * kMxStoreRow + 16 * part);
+        if (first + r < count)
+          *reinterpret_cast<floatx4*>(static_cast<float*>(g.out) + static_cast<int64_t>(targets[first + r]) * g.out_stride +
+                                      kMxRows * rg + 32 * u + 4 * part) = w;
+      }
     }
+  } else {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c[u][4 * j + 8 * (i / 4) + i % 4] * factor;
+        for (int i = 0; i < 8; ++i) v[i] = c[u][4 * j + 8 * (i / 4) + i % 4];
         *reinterpret_cast<int32x4*>(area + col * kMxStoreRow + 64 * u + 32 * j + 16 * hl) =
-            __builtin_bit_cast(int32x4, mx_pack8<kEpi>(v));
+            __builtin_bit_cast(int32x4, mx_pack8(v));
       }
     const int part = lane & 7;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int r = 8 * k + (lane >> 3);
       const MxWords4 w = __builtin_bit_cast(MxWords4, *reinterpret_cast<const int32x4*>(area + r * kMxStoreRow + 16 * part));
-      if (first + r < count) {
-        int64_t to = item.y + first + r;
-        if constexpr (kEpi == kMxHalf) to = targets[first + r];
-        mx_store16(static_cast<uint16_t*>(g.out) + to * g.out_stride, kMxRows * rg + 8 * part, g.n, w,
-                   kEpi == kMxBf16 && g.out_past);
-      }
+      if (first + r < count)
+        mx_store16(static_cast<uint16_t*>(g.out) + static_cast<int64_t>(item.y + first + r) * g.out_stride,
+                   kMxRows * rg + 8 * part, g.n, w, g.out_past);
     }
   }
 }
@@ -731,7 +721,7 @@ __device__ __forceinline__ void mx_tiled_body(const MxGemm& g, const int4& item,
   };
 
   // Where the item's rows go, for the stores (written before the first barrier).
-  if constexpr (kEpi == kMxHalf)
+  if constexpr (kEpi == kMxF32)
     if (tid < 32 * kRT) targets[tid] = g.sorted[item.y + min(tid, count - 1)];
 
   floatx16 acc[kRT][2];
@@ -826,7 +816,7 @@ __global__ __launch_bounds__(kMxThreads) __attribute__((amdgpu_waves_per_eu(kMax
     MxGemm g, MxTiles tiles) {
   __shared__ __attribute__((aligned(16))) uint8_t ring[3 * mx_slot(kMax)];
   static_assert((kMax > 2 ? 2 : 1) * kMxWaves * kMxStoreArea <= 3 * mx_slot(kMax), "the waves' store areas fit the ring");
-  __shared__ int32_t targets[kEpi == kMxHalf ? 32 * kMax : 1];
+  __shared__ int32_t targets[kEpi == kMxF32 ? 32 * kMax : 1];
   // Runs of consecutive items go to the XCDs in turn (workgroup b runs on XCD
   // b % 8): a run's tiles share its rows, and an expert's consecutive items
   // its weights, in that XCD's L2.
@@ -1079,13 +1069,16 @@ __global__ __launch_bounds__(kPrepareThreads) __attribute__((amdgpu_waves_per_eu
 }
 
 // out[t, :] = sum over ranks r of weights[t, r] * down[t * top_k + r, :] in
-// rank order (fp32, one FMA a rank), rounded to bf16 once.  Ranks whose id
+// rank order (fp32, one FMA a rank), rounded to bf16 once.  The down rows are
+// fp32: they are summands that may cancel.  They are most of what the down
+// product of a large batch writes and all that this kernel reads (29,344 pairs
+// of 2048: 240 MB; as scaled fp16 the whole call took 182 us, so 222, but no
+// result was within fp32's error of the sum any more).  Ranks whose id
 // names no expert add nothing (their down rows were never written).  A thread
 // has eight columns; every rank's row piece is loaded before the first sum.
 constexpr int kMxCombineColumns = kMxThreads * 8;
 template <int kTopK>  // 0: any
-__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint16_t* __restrict__ down,
-                                                                const uint8_t* __restrict__ exponents,
+__global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ down,
                                                                 const void* __restrict__ ids, int ids_i64,
                                                                 const void* __restrict__ weights, int weights_f32,
                                                                 int any_top_k, int experts, int hidden, int slices,
@@ -1098,13 +1091,13 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint16_t* 
   constexpr int kBatch = kTopK ? kTopK : 4;
   float acc[8] = {};
   for (int r0 = 0; r0 < top_k; r0 += kBatch) {
-    int32x4 y[kBatch];
-    float scale[kBatch];
+    floatx4 y[kBatch][2];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int64_t pair = first + min(r0 + k, top_k - 1);
-      y[k] = __builtin_nontemporal_load(reinterpret_cast<const int32x4*>(down + pair * hidden + column));
-      scale[k] = mx_half_inverse(exponents[pair * (hidden / kMxRows) + column / kMxRows]);
+      const floatx4* p = reinterpret_cast<const floatx4*>(down + pair * hidden + column);
+      y[k][0] = __builtin_nontemporal_load(p);
+      y[k][1] = __builtin_nontemporal_load(p + 1);
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
@@ -1114,11 +1107,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const uint16_t* 
       const float w = route_weight(weights, weights_f32, pair);
       if (live) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int word = y[k][i / 2];  // (a bit_cast of the element itself reads the vector's first)
-          const halfx2 h = __builtin_bit_cast(halfx2, word);
-          acc[i] = fmaf(w, static_cast<float>(h[i % 2]) * scale[k], acc[i]);
-        }
+        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, y[k][i / 4][i % 4], acc[i]);
       }
     }
   }
@@ -1323,8 +1312,7 @@ struct MoePlan {
   int max_items;
   int64_t pairs, scratch_ints;
   uint8_t *q, *qs, *act, *acts;
-  uint16_t* rows;  // down rows
-  uint8_t* exponents;
+  float* rows;  // down rows
   int32_t *counts, *starts, *total, *sorted, *expert_ids, *num_items, *scratch;
   int4* items;
   int64_t bytes;
@@ -1348,8 +1336,7 @@ MoePlan plan_moe(void* arena, int64_t rows, int top_k, int experts, int hidden, 
       p.q = a.take<uint8_t>(rows * x_steps * kMxOperandCodes);
       p.qs = a.take<uint8_t>(rows * x_steps * kMxOperandScales);
     }
-    p.rows = a.take<uint16_t>(p.pairs * hidden);
-    p.exponents = a.take<uint8_t>(p.pairs * (hidden / kMxRows));
+    p.rows = a.take<float>(p.pairs * hidden);
   }
   if (!p.few && !p.scan) {
     p.sorted = a.take<int32_t>(p.pairs);
@@ -1514,14 +1501,14 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   const dim3 grid(static_cast<unsigned>(rows) * slices), block(kMxThreads);
   auto combine = [&] {
     auto kernel = top_k == 8 ? mx_combine_kernel<8> : mx_combine_kernel<0>;
-    hipLaunchKernelGGL(kernel, grid, block, 0, s, p.rows, p.exponents, ids, i64, weights, f32, top_k, num_experts, hidden,
+    hipLaunchKernelGGL(kernel, grid, block, 0, s, p.rows, ids, i64, weights, f32, top_k, num_experts, hidden,
                        slices, out);
   };
-  down.out = p.rows, down.out_scales = p.exponents;
+  down.out = p.rows;
   if (p.scan) {
     const int items = num_experts + mx_scan_extra(static_cast<int>(p.pairs));
     launch_stream<1, kMxAct, true, kMxScan>(up, items, s);
-    launch_stream<1, kMxHalf, false, kMxScan>(down, items, s);
+    launch_stream<1, kMxF32, false, kMxScan>(down, items, s);
     combine();
     D3_LAUNCHED("mxfp4_moe");
   }
@@ -1555,7 +1542,7 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
     }
   }
   launch_gemm<kMxAct>(up, p.how, p.max_items, s);
-  launch_gemm<kMxHalf>(down, p.how, p.max_items, s);
+  launch_gemm<kMxF32>(down, p.how, p.max_items, s);
   combine();
   D3_LAUNCHED("mxfp4_moe");
 }

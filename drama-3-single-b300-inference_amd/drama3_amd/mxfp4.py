@@ -327,9 +327,7 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     """Routed SwiGLU experts: for row t and rank r with expert e =
     ``topk_ids[t, r]``, ``a = silu(G_e x) * (U_e x)`` and ``out[t] = sum_r
     topk_weights[t, r] * W2_e a`` in rank order, with x and a quantised to
-    MXFP4 and fp32 sums, rounded to bf16 [T, H] once.  (Unless the pairs are few, the
-    ranks' rows are held as scaled fp16 in between, whose rounding is an
-    eighth of bf16's.)
+    MXFP4 and fp32 sums (the ranks' rows too), rounded to bf16 [T, H] once.
 
     ``topk_ids`` int32 / int64 [T, k], k <= 16 (an id that names no expert
     adds nothing), ``topk_weights`` bf16 / f32 of the same shape."""

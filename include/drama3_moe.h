@@ -837,8 +837,7 @@ int64_t d3_mxfp4_grouped_workspace(int64_t rows, int32_t num_experts, int32_t bo
  * expert e = ids[t, r], a = silu(G x) * (U x) with x quantised to MXFP4 and
  * [G; U] = w13[e] (order 1), a quantised to MXFP4 from its fp32 values, and
  *   out[t] = sum over r of weights[t, r] * (w2[e] (order 0) a)
- * in rank order, the sums fp32, rounded to bf16 once (unless the pairs are few,
- * each rank's row is first rounded to a scaled fp16, an eighth of bf16's step).
+ * in rank order, every sum fp32, rounded to bf16 once.
  * ids int32 or int64 [rows, top_k] (an id outside [0, num_experts) adds
  * nothing), weights bf16 or f32.  top_k <= 16, num_experts <= 512, hidden and
  * intermediate multiples of 128 up to 2^20, fewer than 2^26 pairs; out does not

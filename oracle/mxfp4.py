@@ -8,7 +8,6 @@ import numpy as np
 BLOCK = 32
 GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
 BF16_HALF_STEP = 2.0 ** -8  # relative, of one rounding to bf16
-F16_HALF_STEP = 2.0 ** -11
 F32_HALF_STEP = 2.0 ** -24
 
 
@@ -81,9 +80,7 @@ def requantize(v: np.ndarray, error: np.ndarray):
 def moe(x, ids, weights, w13, w2):
     """Routed SwiGLU experts on dequantised weights w13 [E, 2I, H], w2 [E, H,
     I]; x the bf16 rows as float64.  Returns (out, bound): float64 results and
-    how far an fp32 evaluation rounded to bf16 may be from them, whose routes'
-    rows are rounded to fp16 (scaled to at least 2^14 at their largest: below
-    its 2^-28th fp16's steps are 2^-24) before they are summed."""
+    how far an fp32 evaluation rounded to bf16 may be from them."""
     rows = dequantize(*quantize(x))
     out, bound = np.zeros((len(x), w2.shape[1])), np.zeros((len(x), w2.shape[1]))
     inter = w2.shape[2]
@@ -104,6 +101,5 @@ def moe(x, ids, weights, w13, w2):
             y_err = y_err * 1.01 + a_err @ np.abs(w2[e]).T
             w = float(weights[t, r])
             out[t] += w * y[0]
-            y_err = y_err[0] + F16_HALF_STEP * (np.abs(y[0]) + y_err[0]) + 2.0 ** -39 * np.abs(y).max()
-            bound[t] += np.abs(w) * (y_err + 2 * ids.shape[1] * F32_HALF_STEP * np.abs(y[0]))
+            bound[t] += np.abs(w) * (y_err[0] + 2 * ids.shape[1] * F32_HALF_STEP * np.abs(y[0]))
     return out, bound + BF16_HALF_STEP * (np.abs(out) + bound)

@@ -773,3 +773,50 @@ def test_calls_from_two_threads(device):
         t.join()
     for i in range(2):
         assert len(got[i]) == 20 and all(torch.equal(out, want[i]) for out in got[i])
+
+
+# ---------------------------------------------------------------------------
+def moe_path(rows, top_k, experts, hidden, inter):
+    """How a batch runs, told by its workspace: ``few`` keeps activations only,
+    ``scan`` the ranks' rows too, ``sorted`` and ``tiled`` also the route list
+    and its items, ``tiled`` the quantised rows besides."""
+    from drama3_amd import _lib
+
+    lib, pairs = _lib.load(), rows * top_k
+    size = lib.d3_mxfp4_moe_workspace(rows, top_k, experts, hidden, inter)
+    slack = 2048  # every array starts at a multiple of 256 bytes
+    size -= pairs * -(-inter // 256) * 136
+    if size <= slack:
+        return "few"
+    size -= 4 * pairs * hidden
+    if size <= slack:
+        return "scan"
+    size -= 4 * pairs + 16 * lib.d3_max_items(pairs, experts, 16)
+    return "sorted" if size <= slack else "tiled"
+
+
+@pytest.mark.parametrize("path, rows, experts, hidden, inter", [
+    ("few", 3, 4, 256, 128), ("scan", 600, 16, 256, 128), ("sorted", 600, 512, 256, 640),
+    ("tiled", 1500, 8, 256, 128), ("tiled", 1300, 8, 384, 640), ("tiled", 1320, 8, 256, 1152)])
+def test_moe_ranks_that_cancel_keep_fp32(device, path, rows, experts, hidden, inter):
+    """Two ranks' results of 6144 and a little more, weighted 1 and -1: every
+    product and sum is exact in fp32, so the difference has to be.  (In 16 bits
+    they lie 4 apart.)"""
+    from drama3_amd.mxfp4 import mxfp4_moe, prepare_mxfp4_experts
+
+    assert moe_path(rows, 2, experts, hidden, inter) == path
+    # act = silu(64 x) * (6 / 64) x = 6 x^2 in every column, x 1 or 2
+    w13 = np.zeros((experts, 2 * inter, hidden))
+    w13[:, :inter, 0], w13[:, inter:, 0] = 64, 6 / 64
+    w2 = np.zeros((experts, hidden, inter))
+    w2[:, :, 0] = 1024
+    little = om.GRID[np.arange(hidden) % 8]
+    w2[0, :, 40] = little
+    packed = prepare_mxfp4_experts(*(torch.from_numpy(t).to(device) for w in (w13, w2) for t in om.quantize(w)))
+    scale = np.where(np.arange(rows) % 3, 1.0, 2.0)
+    x = torch.zeros((rows, hidden), dtype=torch.bfloat16)
+    x[:, 0] = torch.from_numpy(scale)
+    ids = torch.tensor([0, 1], dtype=torch.int32).expand(rows, 2).contiguous()
+    weights = torch.tensor([1.0, -1.0]).expand(rows, 2).contiguous()
+    out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
+    assert np.array_equal(f64(out), 6 * little * scale[:, None] ** 2)
