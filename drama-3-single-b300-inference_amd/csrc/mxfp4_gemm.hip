@@ -869,6 +869,12 @@ struct MxPrepare {
   int32_t* num_items;
 };
 
+// Boundaries lie on the device, where nobody has seen whether they ascend.  If
+// they do not, groups share rows, and 65,536 of them may have more items than 31
+// bits count (8,389,608 rows each: 32,768 times 65,544): items are counted up to that,
+// which is past every list, instead of coming round to places before it.
+__device__ __forceinline__ int mx_add_items(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
+
 // Exclusive scan of the workgroup's pairs (rows, items) in place; returns the
 // items' sum.  `sums` is LDS of one pair a wave, free again at the end.
 __device__ __forceinline__ int mx_scan(int2* v, int2* sums) {
@@ -877,7 +883,7 @@ __device__ __forceinline__ int mx_scan(int2* v, int2* sums) {
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
     const int x = __shfl_up(scan.x, d), y = __shfl_up(scan.y, d);
-    if (lane >= d) scan.x += x, scan.y += y;
+    if (lane >= d) scan.x += x, scan.y = mx_add_items(scan.y, y);
   }
   if (lane == kWave - 1) sums[wave] = scan;
   __syncthreads();
@@ -885,11 +891,11 @@ __device__ __forceinline__ int mx_scan(int2* v, int2* sums) {
 #pragma unroll
   for (int w = 0; w < kPrepareThreads / kWave; ++w) {
     if (w == wave) before = all;
-    all.x += sums[w].x, all.y += sums[w].y;
+    all.x += sums[w].x, all.y = mx_add_items(all.y, sums[w].y);
   }
   __syncthreads();
   v->x = before.x + scan.x - v->x;
-  v->y = before.y + scan.y - v->y;
+  v->y = mx_add_items(before.y, scan.y) - v->y;
   return all.y;
 }
 
@@ -902,7 +908,7 @@ constexpr int kMxOwnItems = 16;
 __device__ __forceinline__ void mx_write_items(const MxPrepare& p, int at, int expert, int first, int count) {
   const int lane = lane_id();
   auto write = [&](int i, int to, int e, int from, int n) {
-    if (i * p.item_rows < n && to + i < p.max_items)
+    if (i * p.item_rows < n && i < p.max_items - to)
       p.items[to + i] = make_int4(e, from + i * p.item_rows, min(p.item_rows, n - i * p.item_rows), 0);
   };
   for (int i = 0; i < kMxOwnItems && i * p.item_rows < count; ++i) write(i, at, expert, first, count);
@@ -933,8 +939,8 @@ __device__ __forceinline__ void mx_items_of_bounds(const MxPrepare& p, int2* sum
     const int count = max(last - first, 0);
     int2 at = make_int2(0, (count + p.item_rows - 1) / p.item_rows);
     const int total = mx_scan(&at, sums);
-    mx_write_items(p, base + at.y, expert, first, count);
-    base += total;
+    mx_write_items(p, mx_add_items(base, at.y), expert, first, count);
+    base = mx_add_items(base, total);
   }
   if (threadIdx.x == 0) *p.num_items = min(base, p.max_items);
 }

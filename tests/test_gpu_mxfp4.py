@@ -820,3 +820,19 @@ def test_moe_ranks_that_cancel_keep_fp32(device, path, rows, experts, hidden, in
     weights = torch.tensor([1.0, -1.0]).expand(rows, 2).contiguous()
     out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
     assert np.array_equal(f64(out), 6 * little * scale[:, None] ** 2)
+
+
+def test_grouped_boundaries_that_do_not_ascend_stay_in_their_list(device):
+    """Half of 65,536 groups claim every row, more work items together than 31
+    bits count.  Which of them a row is multiplied by is not said; here all are
+    the same, so the rows are known."""
+    from drama3_amd.mxfp4 import grouped_mxfp4, mxfp4_linear, prepare_mxfp4
+
+    rng = np.random.default_rng(29)
+    rows, groups = (1 << 23) + 1000, 1 << 16
+    x = rows_of(rng, 1, 128).to(device)
+    codes, scales, _ = (t.to(device) if torch.is_tensor(t) else t for t in weight_of(rng, 1, 128))
+    weight = prepare_mxfp4(codes.expand(groups, 1, 64), scales.expand(groups, 1, 4))
+    bounds = torch.arange(groups + 1, dtype=torch.int32, device=device) % 2 * rows
+    out = grouped_mxfp4(x.expand(rows, 128), bounds, weight, out=torch.zeros(rows, 1, dtype=torch.bfloat16, device=device))
+    assert (out == mxfp4_linear(x, prepare_mxfp4(codes, scales))).all()
