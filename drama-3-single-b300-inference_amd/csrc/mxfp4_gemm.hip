@@ -1288,9 +1288,9 @@ MxQuantize operand_rows(const uint16_t* x, int64_t stride, int64_t rows, int k, 
   return {x, stride, static_cast<uint64_t>(rows) * per_row, per_row, mx_ceil(k, kMxStep), codes, scales};
 }
 
-unsigned prepare_blocks(const MxQuantize& q) {
+int64_t prepare_blocks(const MxQuantize& q) {
   constexpr uint64_t kPerBlock = kPrepareThreads * kMxQuantizeUnits;
-  return static_cast<unsigned>((q.units + kPerBlock - 1) / kPerBlock);
+  return static_cast<int64_t>((q.units + kPerBlock - 1) / kPerBlock);
 }
 
 template <int kWhat, int kBatch = 1>
@@ -1414,6 +1414,10 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
              static_cast<long long>(p.bytes));
   const int64_t most = p.walk ? num_experts + 1 : p.max_items;
   D3_SUPPORTED(most * mx_ceil(n, kMxRows) < kMxMaxWorkgroups, "mxfp4_grouped: more than 2^24 workgroups");
+  // (rows of stride 0 need little memory: 2^25 of K 4096 would be 2^32 threads)
+  D3_SUPPORTED(!p.how.tiled || prepare_blocks(operand_rows(x, x_row_stride, rows, k, p.q, p.qs)) + 1 <
+                                   kMxMaxWorkgroups * kMxThreads / kPrepareThreads,
+               "mxfp4_grouped: 2^37 elements of rows or more");
   hipStream_t s = as_stream(stream);
   MxGemm g{};
   set_weight(g, w, ws, n, k);
@@ -1434,7 +1438,7 @@ extern "C" int d3_mxfp4_grouped(const uint16_t* x, int64_t x_row_stride, int64_t
     prepare.bounds = boundaries, prepare.groups = num_experts, prepare.count = static_cast<int>(rows);
     prepare.zero_rest = zero_rest, prepare.item_rows = p.how.item_rows, prepare.max_items = p.max_items;
     prepare.items = p.items, prepare.num_items = p.num_items;
-    const unsigned blocks = prepare_blocks(prepare.rows);
+    const unsigned blocks = static_cast<unsigned>(prepare_blocks(prepare.rows));
     if (boundaries != nullptr)
       launch_prepare<kMxBounds>(prepare, blocks + 1, s);
     else
@@ -1522,7 +1526,7 @@ extern "C" int d3_mxfp4_moe(const uint16_t* x, int64_t x_row_stride, int64_t row
   unsigned blocks = 0;
   if (p.how.tiled) {
     prepare.rows = operand_rows(x, x_row_stride, rows, hidden, p.q, p.qs);
-    blocks = prepare_blocks(prepare.rows);
+    blocks = static_cast<unsigned>(prepare_blocks(prepare.rows));
   }
   if (p.chunks > kMxMaxChunks) {
     const int status = d3_sort_routes_wide(

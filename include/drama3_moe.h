@@ -817,7 +817,7 @@ int64_t d3_mxfp4_packed_bytes(int32_t num_experts, int32_t n, int32_t k, int32_t
  * rounding).  boundaries int32 [num_experts + 1] on the device, ascending,
  * clamped to [0, rows]; NULL with one expert: every row.  Rows of no group
  * are zeroed with zero_rest, else left as they were.  num_experts <= 65536,
- * n <= 2^24, k <= 2^20; out does not overlap x.  workspace: at least
+ * n <= 2^24, k <= 2^20, rows * k < 2^37; out does not overlap x.  workspace: at least
  * d3_mxfp4_grouped_workspace bytes (NULL where that is 0), 16-byte aligned,
  * this call's alone until it has run.
  */

@@ -191,3 +191,11 @@ def test_overlapping_rows_are_found():
             assert _overlap(a, b) or not shared(a, b)
     assert not _overlap(wide[:, :60], wide[:, 60:]) and not _overlap(wide, flat[2000:].view(20, 100))
     assert not _overlap(wide[5:6], wide[6:7]) and not _overlap(wide[:0], wide)
+
+
+def test_rows_of_more_threads_than_a_grid_are_refused(lib):
+    """Their quantisation is a launch of its own, whose size their products' does not bound."""
+    huge = 1 << 62
+    for boundaries, experts in ((None, 1), (16, 8)):
+        with pytest.raises(ValueError, match="2.37 elements"):
+            lib.call("d3_mxfp4_grouped", 16, 0, 1 << 25, boundaries, experts, 16, 16, 1, 4096, 16, 1, 0, 16, huge, None)
