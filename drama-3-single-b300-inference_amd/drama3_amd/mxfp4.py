@@ -35,6 +35,7 @@ BLOCK = 32  # elements per scale
 ORDER_ROWS, ORDER_GATE_UP = 0, 1  # row order of a packed weight
 _FLOAT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
 _INT = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
+_MOST = (1 << 31) - 1  # of an int32 argument: ctypes cuts more off without a word
 
 
 # Where rows are few, what a call costs the host counts (6.5 us with one launch,
@@ -102,8 +103,8 @@ def quantize_mxfp4(x: torch.Tensor):
     ``(codes uint8 [T, K / 2], scales uint8 [T, K / 32])``."""
     _check_rows(x, _FLOAT)
     rows, width = x.shape
-    if width == 0 or width % BLOCK:
-        raise ValueError(f"row width {width} must be a multiple of {BLOCK}")
+    if width == 0 or width % BLOCK or width > _MOST:
+        raise ValueError(f"row width {width} must be a multiple of {BLOCK} below 2^31")
     codes = torch.empty(rows, width // 2, dtype=torch.uint8, device=x.device)
     scales = torch.empty(rows, width // BLOCK, dtype=torch.uint8, device=x.device)
     _call(x.device, "d3_mxfp4_quantize", ptr(x), _FLOAT[x.dtype], x.stride(0), rows, width,
@@ -122,6 +123,8 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor,
     codes, scales = codes.contiguous(), scales.contiguous()
     rows, half = codes.shape
     width = 2 * half
+    if width > _MOST:
+        raise ValueError(f"row width {width} must be below 2^31")
     out = torch.empty(rows, width, dtype=dtype, device=codes.device)
     _call(codes.device, "d3_mxfp4_dequantize", ptr(codes), ptr(scales), rows, width, ptr(out),
           _FLOAT[dtype])
@@ -144,6 +147,8 @@ class Mxfp4Weight:
         """The kernels take the sizes as given: they have to be the buffers'."""
         require_cuda(self.codes, self.scales)
         _same_device(self.codes, self.scales, "scales")
+        if max(self.experts, self.n, self.k) > _MOST:
+            raise ValueError(f"packed weights of [{self.experts}, {self.n}, {self.k}]: each must be below 2^31")
         for t, scales in ((self.codes, 0), (self.scales, 1)):
             if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != _entry("d3_mxfp4_packed_bytes")(
                     self.experts, self.n, self.k, scales):
@@ -188,8 +193,8 @@ def _prepare(codes: torch.Tensor, scales: torch.Tensor, order: int) -> Mxfp4Weig
     if codes.dim() != 3 or 0 in codes.shape:
         raise ValueError("weights must be [N, K / 2] or [E, N, K / 2] codes")
     experts, n, k = codes.shape[0], codes.shape[1], 2 * codes.shape[2]
-    if k % 128:
-        raise ValueError(f"K={k} must be a multiple of 128")
+    if k % 128 or max(experts, n, k) > _MOST:
+        raise ValueError(f"K={k} must be a multiple of 128, and it, N={n} and the experts below 2^31")
     codes, scales = codes.contiguous(), scales.contiguous()
     if codes.data_ptr() % 16:
         codes = codes.clone()
@@ -335,6 +340,8 @@ def mxfp4_moe(x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tenso
     require_cuda(topk_ids, topk_weights)
     if topk_ids.dim() != 2 or topk_ids.shape != topk_weights.shape or topk_ids.shape[0] != x.shape[0]:
         raise ValueError("topk_ids / topk_weights must be [T, k] for the T rows of x")
+    if topk_ids.shape[1] > _MOST:
+        raise ValueError(f"top_k {topk_ids.shape[1]} (1 to 16)")
     if topk_ids.dtype not in _INT:
         raise TypeError("topk_ids must be int32 or int64")
     if topk_weights.dtype not in _FLOAT:

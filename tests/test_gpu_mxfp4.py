@@ -836,3 +836,27 @@ def test_grouped_boundaries_that_do_not_ascend_stay_in_their_list(device):
     bounds = torch.arange(groups + 1, dtype=torch.int32, device=device) % 2 * rows
     out = grouped_mxfp4(x.expand(rows, 128), bounds, weight, out=torch.zeros(rows, 1, dtype=torch.bfloat16, device=device))
     assert (out == mxfp4_linear(x, prepare_mxfp4(codes, scales))).all()
+
+
+def test_sizes_past_32_bits_are_refused(device):
+    """Sizes whose low 32 bits would be fine."""
+    from drama3_amd import mxfp4 as mx
+
+    def refused(match, f, *args):
+        with pytest.raises(ValueError, match=match):
+            f(*args)
+
+    u8 = dict(dtype=torch.uint8, device=device)
+    width = (1 << 32) + 128
+    refused("below 2.31", mx.quantize_mxfp4, torch.empty((1, width), dtype=torch.bfloat16, device=device))
+    codes, scales = torch.empty((1, width // 2), **u8), torch.empty((1, width // 32), **u8)
+    refused("below 2.31", mx.dequantize_mxfp4, codes, scales)
+    refused("below 2.31", mx.prepare_mxfp4, codes, scales)
+    rng = np.random.default_rng(30)
+    packed, *_ = make_experts(rng, 4, 256, 128, device)
+    w2 = packed.w2
+    refused("below 2.31", mx.Mxfp4Weight, w2.codes, w2.scales, 4 + (1 << 32), w2.n, w2.k)
+    refused("below 2.31", mx.Mxfp4Weight, w2.codes, w2.scales, 4, w2.n, w2.k + (1 << 32))
+    x = rows_of(rng, 1, 256).to(device)
+    ids = torch.zeros((1, 1), dtype=torch.int32, device=device).expand(1, (1 << 32) + 8)
+    refused("top_k 4294967304", mx.mxfp4_moe, x, ids, torch.ones((1, 1), device=device).expand(ids.shape), packed)
