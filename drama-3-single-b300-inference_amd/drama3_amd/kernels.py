@@ -10,11 +10,13 @@ for shape / device / contract violations, ``TypeError`` for dtypes.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 
 from . import _lib
 from ._lib import call, ptr
-from .mxfp4 import Mxfp4Experts, mxfp4_moe
+from .mxfp4 import Mxfp4Experts, _same_device, mxfp4_moe
 from .pipeline import (WIDE_SORT_PAIRS, MoEWorkspace, Shape, by_pair_suited,
                        dtype_code, fragment_weights, grouped_supported, require_cuda,
                        routed_suited, rows_in_view, small_suited)
@@ -301,8 +303,10 @@ def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start
     if (row_slots is None) != (padding_start is None):
         raise ValueError("Reserved padding routing requires both row_slots and padding_start")
     mxfp4 = isinstance(experts, Mxfp4Experts)
-    if mxfp4 and x.shape[1] != experts.hidden:
-        raise ValueError(f"expert hidden size {experts.hidden} != activation width {x.shape[1]}")
+    if mxfp4:
+        _same_device(x, router, "router")
+        if x.shape[1] != experts.hidden:
+            raise ValueError(f"expert hidden size {experts.hidden} != activation width {x.shape[1]}")
     e, h, i = ((experts.num_experts, experts.hidden, experts.intermediate) if mxfp4
                else check_experts(experts, x.shape[1]))
     if router.shape[1] != e:
@@ -317,8 +321,10 @@ def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start
         # applies the padding rule to the fp32 logits in its fused launch.
         from .moe_input import prepare_moe_input
 
-        _, _, logits = prepare_moe_input(x, router, row_slots=row_slots,
-                                         padding_start=padding_start)
+        # (MXFP4 experts may be on another device than the current one)
+        with torch.cuda.device(x.device) if mxfp4 else nullcontext():
+            _, _, logits = prepare_moe_input(x, router, row_slots=row_slots,
+                                             padding_start=padding_start)
     if mxfp4:  # bf16 routing weights whatever the router's type, as below
         ids = torch.empty((rows, TOP_K), dtype=torch.int32, device=x.device)
         weights = torch.empty((rows, TOP_K), dtype=torch.bfloat16, device=x.device)

@@ -860,3 +860,44 @@ def test_sizes_past_32_bits_are_refused(device):
     x = rows_of(rng, 1, 256).to(device)
     ids = torch.zeros((1, 1), dtype=torch.int32, device=device).expand(1, (1 << 32) + 8)
     refused("top_k 4294967304", mx.mxfp4_moe, x, ids, torch.ones((1, 1), device=device).expand(ids.shape), packed)
+
+
+def test_routed_on_the_device_of_its_rows(device, monkeypatch):
+    """Both launches before the experts run with the rows' device current, the
+    reserved-padding router's too; a router of another device is refused."""
+    from drama3_amd import kernels, moe_input
+
+    rng = np.random.default_rng(31)
+    packed, *_ = make_experts(rng, 16, 256, 128, device)
+    x = rows_of(rng, 30, 256).to(device)
+    router = torch.from_numpy(rng.standard_normal((30, 16))).to(torch.bfloat16).to(device)
+    slots = torch.arange(30, device=device)
+    want = kernels.routed_moe(x, router, packed, row_slots=slots, padding_start=20)
+    current, seen = [], []
+    real = torch.cuda.device
+
+    class Recorded(real):
+        def __enter__(self):
+            current.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *what):
+            current.pop()
+            return super().__exit__(*what)
+
+    monkeypatch.setattr(torch.cuda, "device", Recorded)
+    for module in (kernels, moe_input):
+        def recorded(name, *args, call=module.call):
+            seen.append((name, current[-1:]))
+            return call(name, *args)
+
+        monkeypatch.setattr(module, "call", recorded)
+    out = kernels.routed_moe(x, router, packed, row_slots=slots, padding_start=20)
+    assert seen == [("d3_prepare_moe_input", [device.index]), ("d3_route", [device.index])]
+    assert torch.equal(out, want)
+
+    class Elsewhere(torch.Tensor):
+        device = property(lambda self: torch.device("cuda:1"))
+
+    with pytest.raises(ValueError, match="router is on cuda:1"):
+        kernels.routed_moe(x, router.as_subclass(Elsewhere), packed)
