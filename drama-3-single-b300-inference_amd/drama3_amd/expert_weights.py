@@ -56,7 +56,7 @@ def prepare_experts(experts, stream=None, keep_reference: bool = True):
     for name in ("w13", "w2"):
         if getattr(experts, f"d3_{name}_fragment_only", False):
             continue  # already holds only the fragment-major codes
-        weight = getattr(experts, f"{name}_weight")
+        weight = _weight(experts, name)
         packed = pack_expert_weights(weight, stream)
         if not keep_reference:
             setattr(experts, f"{name}_weight", packed)
@@ -70,8 +70,16 @@ def _identity(weight: torch.Tensor):
     return (weight.data_ptr(), tuple(weight.shape), weight._version)
 
 
+def _weight(experts, name: str):
+    try:
+        return getattr(experts, f"{name}_weight")
+    except AttributeError:
+        raise TypeError(f"experts must hold FP8 weights ({name}_weight), not {type(experts).__name__}: MXFP4 experts "
+                        "run through routed_moe, small_batch_moe, native_moe and mxfp4_moe") from None
+
+
 def _operands(experts, name: str):
-    weight = getattr(experts, f"{name}_weight")
+    weight = _weight(experts, name)
     scales = getattr(experts, f"{name}_scale_inv")
     packed = getattr(experts, f"d3_{name}_packed", None)
     if packed is not None and getattr(experts, f"d3_{name}_source", None) == _identity(weight):

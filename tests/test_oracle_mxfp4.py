@@ -199,3 +199,14 @@ def test_rows_of_more_threads_than_a_grid_are_refused(lib):
     for boundaries, experts in ((None, 1), (16, 8)):
         with pytest.raises(ValueError, match="2.37 elements"):
             lib.call("d3_mxfp4_grouped", 16, 0, 1 << 25, boundaries, experts, 16, 16, 1, 4096, 16, 1, 0, 16, huge, None)
+
+
+def test_steps_of_fp8_experts_refuse_mxfp4_ones():
+    """The decode, mixed and layer steps read their experts through these."""
+    from drama3_amd.expert_weights import fc1_operands, fc2_operands, prepare_experts
+    from drama3_amd.mxfp4 import Mxfp4Experts
+
+    experts = object.__new__(Mxfp4Experts)
+    for step in (fc1_operands, fc2_operands, prepare_experts):
+        with pytest.raises(TypeError, match="FP8 weights .* not Mxfp4Experts"):
+            step(experts)
