@@ -901,3 +901,154 @@ def test_routed_on_the_device_of_its_rows(device, monkeypatch):
 
     with pytest.raises(ValueError, match="router is on cuda:1"):
         kernels.routed_moe(x, router.as_subclass(Elsewhere), packed)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bounds", [b + b[-1:] for b in GROUPS])
+@pytest.mark.parametrize("k, n", [(128, 300), (384, 50), (640, 129), (1152, 1), (1152, 200)])
+def test_grouped_walked(device, bounds, k, n):
+    """The one launch that walks each group's row tiles itself (no workspace):
+    one, two and four slices of the contraction, groups of one to four tiles,
+    rows of no group zeroed or, in a given column slice, left alone."""
+    from drama3_amd import _lib
+    from drama3_amd.mxfp4 import grouped_mxfp4, prepare_mxfp4
+
+    assert _lib.load().d3_mxfp4_grouped_workspace(100, 7, 1, n, k) == 0
+    rng = np.random.default_rng(sum(bounds) % 1000 + k + n)
+    x = rows_of(rng, 100, k + 3)[:, 2:k + 2]
+    codes, scales, values = weight_of(rng, 7, n, k)
+    weight = prepare_mxfp4(codes.to(device), scales.to(device))
+    boundaries = torch.tensor(bounds, dtype=torch.int32, device=device)
+    want, bound, live = grouped_oracle(x, bounds, values)
+    live = torch.from_numpy(live).to(device)
+    out = grouped_mxfp4(x.to(device), boundaries, weight)
+    within(out, want, bound)
+    assert not out[~live].any()
+    buffer = torch.full((200, n + 9), -3.0, dtype=torch.bfloat16, device=device)
+    given = grouped_mxfp4(x.to(device), boundaries, weight, out=buffer[::2, 5:5 + n])
+    assert torch.equal(given, torch.where(live[:, None], out, -3.0))
+    assert (buffer[:, :5] == -3).all() and (buffer[:, 5 + n:] == -3).all() and (buffer[1::2] == -3).all()
+
+
+@pytest.mark.parametrize("bounds", [[0, 48], [3, 40], [-7, 1000], [48, 48], [0, 0], [20, 37]])
+@pytest.mark.parametrize("k", [256, 896])
+def test_grouped_walked_by_one_group(device, bounds, k):
+    from drama3_amd import _lib
+    from drama3_amd.mxfp4 import grouped_mxfp4, prepare_mxfp4
+
+    assert _lib.load().d3_mxfp4_grouped_workspace(48, 1, 1, 130, k) == 0
+    rng = np.random.default_rng(32 + k)
+    x = rows_of(rng, 48, k)
+    codes, scales, values = weight_of(rng, 1, 130, k)
+    out = grouped_mxfp4(x.to(device), torch.tensor(bounds, dtype=torch.int32, device=device),
+                        prepare_mxfp4(codes.to(device), scales.to(device)))
+    want, bound, live = grouped_oracle(x, bounds, values)
+    within(out, want, bound)
+    assert not out[~torch.from_numpy(live).to(device)].any()
+
+
+def many_experts(rng, distinct, experts, hidden, inter, device):
+    """``make_experts`` of which expert e is a copy of expert e % distinct, and
+    the ids by which the oracle finds it among the distinct ones."""
+    from drama3_amd.mxfp4 import prepare_mxfp4_experts
+
+    c13, s13, v13 = weight_of(rng, distinct, 2 * inter, hidden)
+    c2, s2, v2 = weight_of(rng, distinct, hidden, inter)
+    which = torch.arange(experts, device=device) % distinct
+    packed = prepare_mxfp4_experts(*(t.to(device)[which] for t in (c13, s13, c2, s2)))
+
+    def found(ids):
+        ids = ids.numpy().astype(np.int64)
+        return np.where((ids >= 0) & (ids < experts), ids % distinct, -1)
+
+    return packed, v13, v2, found
+
+
+@pytest.mark.parametrize("rows, hidden, inter", [(40, 512, 1024), (40, 1152, 128), (50, 1152, 1024), (150, 512, 640),
+                                                 (17, 256, 640)])
+@pytest.mark.parametrize("id_type", [torch.int32, torch.int64])
+def test_moe_sorted_and_streamed(device, rows, hidden, inter, id_type):
+    """Routes sorted into items of 16 rows and streamed, the path of a full
+    decode bucket: one, two and four slices of either product, ids of no
+    expert, an expert of every row."""
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    assert moe_path(rows, 8, 200, hidden, inter) == "sorted"
+    rng = np.random.default_rng(rows + hidden + inter)
+    packed, v13, v2, found = many_experts(rng, 7, 200, hidden, inter, device)
+    x = rows_of(rng, rows, hidden + 5)[:, 3:hidden + 3]
+    ids, weights = make_routes(rng, rows, 200, 8)
+    ids[rng.random(ids.shape) < 0.1] = -1
+    ids[1], ids[2, 5] = 200, 2 ** 31 - 1
+    ids, weights = ids.to(id_type), weights.to(torch.bfloat16)
+    for skewed in (False, True):
+        if skewed:
+            ids[:, 3], ids[5:, 0] = 190, 190  # (twice in a row)
+        out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
+        within(out, *om.moe(f64(x), found(ids), f64(weights), v13, v2))
+
+
+@pytest.mark.parametrize("rows, experts, hidden, inter, top_k", [(5, 60, 384, 256, 11), (8, 16, 256, 640, 16),
+                                                                 (1, 20, 128, 128, 9), (9, 512, 1152, 128, 13)])
+def test_moe_of_few_pairs_and_many_ranks(device, rows, experts, hidden, inter, top_k):
+    """More ranks than the down product's workgroup has waves."""
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    assert moe_path(rows, top_k, experts, hidden, inter) == "few"
+    rng = np.random.default_rng(rows + top_k)
+    packed, v13, v2, found = many_experts(rng, 5, experts, hidden, inter, device)
+    x = rows_of(rng, rows, hidden)
+    ids, weights = make_routes(rng, rows, experts, top_k)
+    ids[0, 8], ids[rows - 1, 2] = experts, -1
+    weights[0, 8] = float("nan")  # of a rank that adds nothing
+    out = mxfp4_moe(x.to(device), ids.to(device), weights.to(torch.float32).to(device), packed)
+    within(out, *om.moe(f64(x), found(ids), f64(weights.to(torch.float32)), v13, v2))
+
+
+@pytest.mark.parametrize("rows, experts, top_k, id_type", [
+    (1100, 512, 8, torch.int32), (4100, 3, 4, torch.int64), (9001, 1, 1, torch.int32),  # grouped by chunks
+    (4500, 512, 16, torch.int64), (33000, 3, 2, torch.int32), (66001, 1, 1, torch.int64)])  # by the route sort
+def test_moe_many_pairs_of_few_and_many_experts(device, rows, experts, top_k, id_type):
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    assert moe_path(rows, top_k, experts, 128, 128) == "tiled"
+    rng = np.random.default_rng(rows)
+    packed, v13, v2, found = many_experts(rng, 9, experts, 128, 128, device)
+    x = rows_of(rng, rows, 128)
+    ids = torch.from_numpy(rng.integers(0, experts, (rows, top_k)))
+    ids[torch.from_numpy(rng.random((rows, top_k)) < 0.5)] = experts - 1  # half of them of one expert
+    none = torch.from_numpy(rng.random((rows, top_k)) < 0.02)
+    ids[none] = experts if id_type == torch.int32 else (1 << 32)  # (a low half that names one)
+    ids, weights = ids.to(id_type), torch.from_numpy(rng.random((rows, top_k))).to(torch.float32)
+    out = mxfp4_moe(x.to(device), ids.to(device), weights.to(device), packed)
+    pick = np.concatenate([rng.choice(rows, 100, replace=False), np.flatnonzero(none.any(1))[:30], [0, rows - 1]])
+    want, bound = om.moe(f64(x)[pick], found(ids)[pick], f64(weights)[pick], v13, v2)
+    within(out[torch.from_numpy(pick).to(device)], want, bound)
+
+
+@pytest.mark.parametrize("experts, hidden, inter, paths", [
+    (200, 1152, 128, {1: "few", 16: "few", 40: "sorted", 190: "sorted", 260: "tiled"}),
+    (16, 512, 256, {1: "few", 5: "few", 40: "scan", 150: "scan", 400: "tiled"})])
+def test_batches_of_every_path_agree(device, experts, hidden, inter, paths):
+    """The first rows of a batch alone and with others, one size a path.  What
+    may differ is the order of the fp32 sums, and with it a code of an
+    activation at a border: any two results lie within twice the bound that
+    either has to the definition."""
+    from drama3_amd.mxfp4 import mxfp4_moe
+
+    rng = np.random.default_rng(33 + experts)
+    packed, v13, v2, found = many_experts(rng, 6, experts, hidden, inter, device)
+    most = max(paths)
+    x = rows_of(rng, most, hidden)
+    ids, weights = make_routes(rng, most, experts, 8)
+    on = [t.to(device) for t in (x, ids, weights.to(torch.float32))]
+    results = {}
+    for rows, path in paths.items():
+        assert moe_path(rows, 8, experts, hidden, inter) == path
+        results[rows] = f64(mxfp4_moe(*(t[:rows] for t in on), packed))
+    few = min(r for r in paths if r > 1)
+    want, bound = om.moe(f64(x[:few]), found(ids[:few]), f64(on[2][:few]), v13, v2)
+    for a in results.values():
+        for b in results.values():
+            n = min(len(a), len(b), few)
+            assert (np.abs(a[:n] - b[:n]) <= 2 * bound[:n]).all()
