@@ -288,7 +288,9 @@ def routed_moe(x, router, experts, decode=True, *, row_slots=None, padding_start
 
     The reference dispatches three numerically different backends (Triton
     GEMV for <= 8 rows, Fish's sorted GEMM for native prefill, FlashInfer for
-    decode batches above 8 rows); here every batch runs the same MI355X path
+    decode batches above 8 rows); here every batch is the same computation
+    (batches of different sizes run different kernels and sum in fp32 in
+    different orders, for MXFP4 experts before their activations are rounded)
     with ``route_kernel``'s ranking rule (``kernels.py:364-368``).  ``decode``
     is accepted for the signature.  With ``row_slots`` / ``padding_start``
     (both or neither), rows whose slot is >= ``padding_start`` take row 0's

@@ -12,8 +12,12 @@ scale is ``2 ** (floor(log2(amax)) - 2)`` (at least 2 ** -127), its elements
 that holds an infinity or a NaN reads as NaN throughout.
 
 Weights are packed once (``prepare_mxfp4``, ``prepare_mxfp4_experts``); every
-product takes bf16 rows and quantises them itself, so a batch of any size has
-the same numerics: codes times codes summed in fp32, rounded to bf16 once.
+product takes bf16 rows and quantises them itself, to the same codes in a batch
+of any size; codes times codes are summed in fp32 and rounded to bf16 once.  The
+order of a sum does depend on the batch (how a product runs follows from its
+sizes), so a row's results may differ in their last bit, and those of the routed
+experts by what an activation on a border between two codes adds.  The same call
+gives the same bits.
 
 Every call allocates what it returns and its workspace from torch's allocator
 on the current stream: calls on different streams share nothing, and a
