@@ -2,12 +2,15 @@
 // the MXFP4 products.
 //
 // Both directions read and write every element once and are bound by HBM.
-// Tensors that no cache holds go past them, so that these keep what is smaller
-// (rows read from more than the L2s' 32 MiB on, values written from half of the
-// 256 MiB last-level cache on): 131072 x 768 fp32 rows (402 MB read, 53 MB
-// written) 100 -> 85 us, 5.3 TB/s, and back to bf16 (53 and 201 MB) 47 -> 37 us,
-// 6.9 TB/s.  Smaller ones do not, their producer's and consumer's caches hold
-// them: 3668 x 2048 bf16 rows take 5.2 us so, 5.7 us past the caches.
+// bf16 tensors that no cache holds go past them: rows read from seven eighths of
+// the 256 MiB last-level cache on, values written from half of it on.  Us, past /
+// through the caches: rows of 98 MB 24.2 / 20.8, 197 MB 43.0 / 43.0 (38.1 where
+// they are in the cache), 246 MB 52.5 / 57.2, 403 MB 82.9 / 90.9 (4.9 TB/s read,
+// 5.5 with the codes written); values of 98 MB 20.5 / 21.1, 197 MB 37.8 / 40.6,
+// 246 MB 46.4 / 57.7, 403 MB 74.1 / 91.4.
+// fp32 ones never do: a lane's eight elements are two accesses of half its 32
+// bytes, and past the caches nothing joins the halves of a line.  Rows of 49 MB
+// 14.0 / 11.1, 403 MB 89.5 / 87.0; values of 154 MB 62 / 27.5, 403 MB 171 / 119.
 #include "mxfp4.h"
 #include "status.h"
 
@@ -16,7 +19,7 @@ namespace {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowUnits = kMxQuantizeUnits;
-constexpr int64_t kCachedIn = int64_t{1} << 25, kCachedOut = int64_t{1} << 27;
+constexpr int64_t kCachedIn = int64_t{7} << 25, kCachedOut = int64_t{1} << 27;
 
 template <bool kF32, bool kOnce>
 __global__ __launch_bounds__(kRowThreads) void quantize_kernel(MxQuantize q) {
@@ -134,9 +137,8 @@ extern "C" int d3_mxfp4_quantize(const void* x, int32_t x_dtype, int64_t x_row_s
   const uint64_t units = static_cast<uint64_t>(rows) * per_row;
   const MxQuantize q{x, x_row_stride, units, per_row, 0, codes, scales};
   const dim3 grid(row_blocks(units)), block(kRowThreads);
-  const bool once = rows * static_cast<int64_t>(width) * (f32 ? 4 : 2) > kCachedIn;
-  auto kernel = f32 ? (once ? quantize_kernel<true, true> : quantize_kernel<true, false>)
-                    : (once ? quantize_kernel<false, true> : quantize_kernel<false, false>);
+  const bool once = rows * static_cast<int64_t>(width) * 2 > kCachedIn;
+  auto kernel = f32 ? quantize_kernel<true, false> : (once ? quantize_kernel<false, true> : quantize_kernel<false, false>);
   hipLaunchKernelGGL(kernel, grid, block, 0, as_stream(stream), q);
   D3_LAUNCHED("mxfp4_quantize");
 }
@@ -157,9 +159,9 @@ extern "C" int d3_mxfp4_dequantize(const uint8_t* codes, const uint8_t* scales, 
   const uint64_t units = static_cast<uint64_t>(rows) * per_row;
   const dim3 grid(row_blocks(units)), block(kRowThreads);
   const bool f32 = out_dtype == D3_DTYPE_F32;
-  const bool once = rows * static_cast<int64_t>(width) * (f32 ? 4 : 2) > kCachedOut;
-  auto kernel = f32 ? (once ? dequantize_kernel<true, true> : dequantize_kernel<true, false>)
-                    : (once ? dequantize_kernel<false, true> : dequantize_kernel<false, false>);
+  const bool once = rows * static_cast<int64_t>(width) * 2 > kCachedOut;
+  auto kernel =
+      f32 ? dequantize_kernel<true, false> : (once ? dequantize_kernel<false, true> : dequantize_kernel<false, false>);
   hipLaunchKernelGGL(kernel, grid, block, 0, as_stream(stream), codes, scales, units, out);
   D3_LAUNCHED("mxfp4_dequantize");
 }
