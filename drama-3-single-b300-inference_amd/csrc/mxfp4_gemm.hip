@@ -1078,11 +1078,12 @@ __global__ __launch_bounds__(kPrepareThreads) __attribute__((amdgpu_waves_per_eu
 // rank order (fp32, one FMA a rank), rounded to bf16 once.  The down rows are
 // fp32: they are summands that may cancel.  They are most of what the down
 // product of a large batch writes and all that this kernel reads (29,344 pairs
-// of 2048: 240 MB; as scaled fp16 the whole call took 182 us, so 222, but no
-// result was within fp32's error of the sum any more).  Ranks whose id
-// names no expert add nothing (their down rows were never written).  A thread
-// has eight columns; every rank's row piece is loaded before the first sum.
-constexpr int kMxCombineColumns = kMxThreads * 8;
+// of 2048: 240 MB, read once at 5.5 TB/s; as scaled fp16 the whole call took 195
+// us, so 222, but a result was no longer within fp32's error of its sum).  Ranks
+// whose id names no expert add nothing (their down rows were never written).  A
+// thread has four columns, so that a wave reads whole lines past the caches
+// (eight: 222 -> 230); every rank's row piece is loaded before the first sum.
+constexpr int kMxCombineColumns = kMxThreads * 4;
 template <int kTopK>  // 0: any
 __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __restrict__ down,
                                                                 const void* __restrict__ ids, int ids_i64,
@@ -1090,21 +1091,18 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __r
                                                                 int any_top_k, int experts, int hidden, int slices,
                                                                 uint16_t* __restrict__ out) {
   const int row = blockIdx.x / slices;
-  const int column = (blockIdx.x % slices) * kMxCombineColumns + threadIdx.x * 8;
+  const int column = (blockIdx.x % slices) * kMxCombineColumns + threadIdx.x * 4;
   if (column >= hidden) return;
   const int top_k = kTopK ? kTopK : any_top_k;
   const int64_t first = static_cast<int64_t>(row) * top_k;
   constexpr int kBatch = kTopK ? kTopK : 4;
-  float acc[8] = {};
+  floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int r0 = 0; r0 < top_k; r0 += kBatch) {
-    floatx4 y[kBatch][2];
+    floatx4 y[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int64_t pair = first + min(r0 + k, top_k - 1);
-      const floatx4* p = reinterpret_cast<const floatx4*>(down + pair * hidden + column);
-      y[k][0] = __builtin_nontemporal_load(p);
-      y[k][1] = __builtin_nontemporal_load(p + 1);
-    }
+    for (int k = 0; k < kBatch; ++k)
+      y[k] = __builtin_nontemporal_load(
+          reinterpret_cast<const floatx4*>(down + (first + min(r0 + k, top_k - 1)) * hidden + column));
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int64_t pair = first + min(r0 + k, top_k - 1);
@@ -1113,13 +1111,12 @@ __global__ __launch_bounds__(kMxThreads) void mx_combine_kernel(const float* __r
       const float w = route_weight(weights, weights_f32, pair);
       if (live) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, y[k][i / 4][i % 4], acc[i]);
+        for (int i = 0; i < 4; ++i) acc[i] = fmaf(w, y[k][i], acc[i]);
       }
     }
   }
-  *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * hidden + column) =
-      make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]), pack_bf16x2(acc[4], acc[5]),
-                 pack_bf16x2(acc[6], acc[7]));
+  *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row) * hidden + column) =
+      make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
 }
 
 int mx_ceil(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }

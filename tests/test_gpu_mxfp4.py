@@ -806,13 +806,14 @@ def test_moe_ranks_that_cancel_keep_fp32(device, path, rows, experts, hidden, in
 
     assert moe_path(rows, 2, experts, hidden, inter) == path
     # act = silu(64 x) * (6 / 64) x = 6 x^2 in every column, x 1 or 2
-    w13 = np.zeros((experts, 2 * inter, hidden))
+    w13 = np.zeros((2, 2 * inter, hidden))
     w13[:, :inter, 0], w13[:, inter:, 0] = 64, 6 / 64
-    w2 = np.zeros((experts, hidden, inter))
+    w2 = np.zeros((2, hidden, inter))
     w2[:, :, 0] = 1024
     little = om.GRID[np.arange(hidden) % 8]
     w2[0, :, 40] = little
-    packed = prepare_mxfp4_experts(*(torch.from_numpy(t).to(device) for w in (w13, w2) for t in om.quantize(w)))
+    which = (torch.arange(experts, device=device) > 0).long()  # expert 0, and copies of expert 1
+    packed = prepare_mxfp4_experts(*(torch.from_numpy(t).to(device)[which] for w in (w13, w2) for t in om.quantize(w)))
     scale = np.where(np.arange(rows) % 3, 1.0, 2.0)
     x = torch.zeros((rows, hidden), dtype=torch.bfloat16)
     x[:, 0] = torch.from_numpy(scale)
