@@ -1199,9 +1199,10 @@ MxChoice choose_linear(int64_t rows, int64_t n, int64_t k) {
 }
 
 // Rows grouped by expert: up to 8 rows an expert they stream, for more than one
-// tile of 16 reads an expert's weights again.  Us, streaming / tiled: E256 H2048
-// I512, 8 rows an expert 98.7 / 105, 16 rows 122 / 108; E8 H1920 I256, 164 rows an
-// expert 28.5 / 24.4; E24 H128 I128, 500 rows an expert 31.6 / 26.6.
+// tile of 16 reads an expert's weights again.  Us a call in a graph, streaming /
+// tiled: E256 H2048 I512, 8 rows an expert 90.8 / 100.2, 16 rows 127 / 108; E8
+// H1920 I256, 164 rows an expert 31.5 / 26.0; E24 H128 I128, 500 rows an expert
+// 33.7 / 26.8.
 MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n) {
   const int64_t partial = (pairs < experts ? pairs : experts) / 2;
   return pairs <= 8 * experts ? MxChoice{false, 16} : choose_tiled(pairs, partial, n);
@@ -1209,13 +1210,13 @@ MxChoice choose_routed(int64_t pairs, int64_t experts, int64_t n) {
 
 // Routes that need no sort (three launches, not four): few enough pairs for each
 // workgroup to look through, and no more workgroups than four a CU, for they all
-// do.  Us, without / with the sort: E16 H1024 I256, 160 / 480 / 1038 / 1184 pairs
-// 16.9 / 17.2 / 20.0 / 21.4 against 17.5 / 19.0 / 21.7 / 22.0; E16 H2048 I768, 320
-// pairs 24.6 against 27.5; E60 H640 I512, 456 pairs 19.3 against 21.6; E200 H512
-// I256, 800 pairs (992 workgroups) 19.2 against 21.2; but E16 H2048 I768, 560
-// pairs (1224) 28.0 against 24.6, E8 H1920 I512, 1280 pairs (1408) 40.0 against
-// 25.3, E256 H2048 I512, 512 pairs (4608) 79.1 against 72.3, and E8 H1024 I256,
-// 2000 pairs 25.9 against 21.3.
+// do.  Us a call in a graph, without / with the sort: E16 H1024 I256, 160 / 480 /
+// 1038 / 1184 pairs 11.6 / 15.7 / 20.1 / 21.4 against 15.6 / 17.8 / 20.0 / 20.7;
+// E60 H640 I512, 456 pairs 17.9 against 21.3; E200 H512 I256, 800 pairs (992
+// workgroups) 18.2 against 21.2; E16 H2048 I768, 320 pairs (1008) 25.0 against
+// 24.2; but 560 pairs of it (1224) 28.7 against 25.0, E8 H1920 I512, 1280 pairs
+// (1408) 41.1 against 26.9, and E256 H2048 I512, 512 pairs (4608) 80.5 against
+// 73.2.
 bool choose_scan(int64_t pairs, int64_t experts, int hidden, int inter) {
   if (pairs > kMxScanPairs) return false;
   const int64_t up = stream_blocks(2 * static_cast<int64_t>(inter), hidden), down = stream_blocks(hidden, inter);
@@ -1295,14 +1296,16 @@ void launch_prepare(const MxPrepare& p, unsigned blocks, hipStream_t s) {
   hipLaunchKernelGGL((mx_prepare_kernel<kWhat, kBatch>), dim3(blocks), dim3(kPrepareThreads), 0, s, p);
 }
 
-// Up to so many pairs each is an item of its own, whatever their experts:
-// E256 H2048 I512, 64 / 128 / 192 / 256 pairs 23.9 / 36.3 / 49.7 / 61.8 us
-// against 32.3 / 42.9 / 53.2 / 61.1 with the routes grouped; E128 I768, 64 /
-// 128 / 192 pairs 30.9 / 46.7 / 62.9 against 38.8 / 48.7 / 55.8.  A few experts'
-// pairs read the same weights again and again: past four workgroups a CU their
-// experts' workgroups find them instead, if those are few enough (E8 H1536 I640,
-// 32 / 64 / 128 pairs 14.9 / 17.4 / 22.3 us against 14.7-16.5 / 15.0-16.7 /
-// 15.7-17.0; E16 H1024 I256, 128 pairs 14.0 against 15.1).
+// Up to so many pairs each is an item of its own: us a call in a graph against
+// grouped routes, E256 H2048 I512, 64 / 128 / 192 / 256 pairs 22.3 / 37.9 / 52.3 /
+// 64.8 against 30.2 / 41.1 / 50.8 / 57.4; E128 I768, 64 / 128 / 192 pairs 31.2 /
+// 47.5 / 65.2 against 36.4 / 46.8 / 54.1.  A few experts' pairs read the same
+// weights again and again: past four workgroups a CU their experts' workgroups
+// find them instead, if those are few enough (E8 H1536 I640, 32 / 64 / 128 pairs
+// 14.6 / 17.4 / 22.8 against 13.7 / 14.2 / 15.2; E16 H1024 I256, 128 pairs 10.2
+// against 11.3).  Where they are not, few wide experts, every pair streams its
+// expert's weights for itself: by their bytes up to 16 times what E8 H4096 I14336
+// needs at 128 pairs, which is neither timed nor avoided.
 constexpr int kMxFewPairs = 128;
 // Up to so many pairs are grouped by one workgroup, up to kMxMaxChunks chunks by
 // a workgroup a chunk, more by the route sort over many workgroups.
