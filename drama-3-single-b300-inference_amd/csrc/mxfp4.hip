@@ -6,7 +6,7 @@
 // the 256 MiB last-level cache on, values written from half of it on.  Us, past /
 // through the caches: rows of 98 MB 24.2 / 20.8, 197 MB 43.0 / 43.0 (38.1 where
 // they are in the cache), 246 MB 52.5 / 57.2, 403 MB 82.9 / 90.9 (4.9 TB/s read,
-// 5.5 with the codes written); values of 98 MB 20.5 / 21.1, 197 MB 37.8 / 40.6,
+// 6.2 with the codes written); values of 98 MB 20.5 / 21.1, 197 MB 37.8 / 40.6,
 // 246 MB 46.4 / 57.7, 403 MB 74.1 / 91.4.
 // fp32 ones never do: a lane's eight elements are two accesses of half its 32
 // bytes, and past the caches nothing joins the halves of a line.  Rows of 49 MB
