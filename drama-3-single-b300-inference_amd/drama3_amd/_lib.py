@@ -27,11 +27,29 @@ DTYPE_BF16 = 0
 DTYPE_F32 = 1
 DTYPE_I32 = 2
 DTYPE_I64 = 3
+DTYPE_E4M3 = 4
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+
+
+class RopeStruct(ctypes.Structure):
+    """``d3_rope``"""
+
+    _fields_ = [("turns", _p), ("rotary_dim", _i32), ("interleaved", _i32), ("magnitude", _f32)]
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """``d3_paged_cache``"""
+
+    _fields_ = [("keys", _p), ("values", _p), ("dtype", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("page_size", _i32), ("pages", _i64), ("key_page_stride", _i64), ("key_head_stride", _i64),
+                ("key_token_stride", _i64), ("value_page_stride", _i64), ("value_head_stride", _i64),
+                ("value_token_stride", _i64), ("page_table", _p), ("table_stride", _i64), ("slots", _i32),
+                ("max_pages", _i32), ("key_scales", _p), ("value_scales", _p)]
+
 
 # name -> (restype, argtypes); mirrors include/drama3_moe.h
 SIGNATURES = {
@@ -119,6 +137,15 @@ SIGNATURES = {
         _i32, [_p, _i64, _i64, _p, _i32, _p, _i32, _i32, _p, _p, _p, _p, _i32, _i32, _i32, _p, _p,
                _i64, _p]),
     "d3_mxfp4_moe_workspace": (_i64, [_i64, _i32, _i32, _i32, _i32]),
+    "d3_rope_rows": (
+        _i32, [_p, _i32, _i64, _i64, _i64, _i32, _i32, _p, _i32, _p, _p, _i64, _i64, _p]),
+    "d3_paged_append": (
+        _i32, [_p, _p, _i64, _i64, _p, _i64, _i64, _i64, _p, _i32, _p, _i32, _p, _p, _i64, _i64, _i32,
+               _p, _i64, _i64, _p]),
+    "d3_paged_attention": (
+        _i32, [_p, _p, _i64, _i64, _i64, _i32, _p, _p, _i32, _p, _i32, _i32, _i32, _f32, _i64, _p,
+               _i64, _i64, _i32, _p, _i64, _p]),
+    "d3_paged_attention_workspace": (_i64, [_p, _i64, _i32, _i32, _i32]),
 }
 
 _lib = None

@@ -1,0 +1,373 @@
+"""Attention over packed rows and a paged cache: rotary positions, appending keys
+and values to the cache with the rotation on the way, and the attention of new
+tokens over the cached ones, single ones and chunks alike.
+
+What precedes the MoE step in the reference's attention layers
+(``src/drama3/model.py:55-141``: rotary positions, paged decode over 16-token
+pages, packed prefill), over the same packed rows, persistent slots and int64
+positions that ``packed_prefill.packed_row_metadata`` and
+``runtime_state.DeviceRequests.load`` give.  The reference calls libraries here:
+the semantics are this module's own.
+
+A step of one layer, eager or captured::
+
+    q = append_paged(cache, k, v, positions, row_slots, rope=rope, q=q)
+    out = paged_attention(q, cache, layout, lengths)
+
+``lengths`` counts a sequence's tokens with the new ones.  Every call allocates
+what it returns and its workspace from torch's allocator on the current stream:
+calls on different streams share nothing, and a captured graph keeps its own
+workspace.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass, field
+
+import torch
+
+from . import _lib
+from ._lib import ptr
+from .mxfp4 import _MOST, _call, _entry, _same_device
+from .packed_prefill import PackedLayout
+from .pipeline import require_cuda
+
+HEAD_DIMS = (64, 128, 256)  # of paged_attention
+SCALINGS = ("none", "linear", "base", "bands")
+_FLOAT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_CACHE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float8_e4m3fn: _lib.DTYPE_E4M3}
+_INT = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions
+# ---------------------------------------------------------------------------
+@dataclass(frozen=True)
+class Rope:
+    """Rotary positions (``prepare_rope``): ``turns`` fp64 [rotary_dim / 2] on
+    the device, revolutions of each pair a position; ``magnitude`` multiplies
+    what is rotated.  Pairs are columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1)
+    where ``interleaved``."""
+
+    turns: torch.Tensor
+    interleaved: bool = False
+    magnitude: float = 1.0
+    _struct: _lib.RopeStruct = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self):
+        require_cuda(self.turns)
+        if self.turns.dtype != torch.float64:
+            raise TypeError("turns must be float64")
+        if self.turns.dim() != 1 or not 0 < len(self.turns) <= 512 or not self.turns.is_contiguous():
+            raise ValueError("turns must be contiguous [rotary_dim / 2], at most 512")
+        object.__setattr__(self, "_struct", _lib.RopeStruct(
+            ptr(self.turns), 2 * len(self.turns), int(self.interleaved), self.magnitude))
+
+    @property
+    def rotary_dim(self) -> int:
+        return 2 * len(self.turns)
+
+
+def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                     original_length: int = 0, slow: float = 1.0, fast: float = 32.0) -> list[float]:
+    """Radians a position of each of the ``rotary_dim / 2`` pairs:
+    ``f_i = base ** (-2 i / rotary_dim)``, scaled for contexts ``factor`` times
+    as long as the ``original_length`` a model was trained on:
+
+    ``"linear"``  f / factor (positions are interpolated);
+    ``"base"``    the base grows to ``base * factor ** (R / (R - 2))``, so that the
+                  slowest pair turns as under "linear" and the fastest as before;
+    ``"bands"``   pairs that turn ``fast`` times and more within the original
+                  length stay, those that turn ``slow`` times and less are
+                  interpolated, in between by the share (YaRN, arXiv 2309.00071)."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary width {rotary_dim} must be even and positive")
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling {scaling!r} is none of {SCALINGS}")
+    if base <= 0 or factor <= 0:
+        raise ValueError("base and factor must be positive")
+    if scaling == "base" and rotary_dim > 2:
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    frequencies = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
+    if scaling == "linear":
+        return [f / factor for f in frequencies]
+    if scaling == "bands":
+        if original_length <= 0 or not slow < fast:
+            raise ValueError("bands need the original length, and slow < fast")
+        for i, f in enumerate(frequencies):
+            turns = original_length * f / (2 * math.pi)
+            kept = min(1.0, max(0.0, (turns - slow) / (fast - slow)))
+            frequencies[i] = kept * f + (1.0 - kept) * f / factor
+    return frequencies
+
+
+def prepare_rope(rotary_dim: int, base: float = 10000.0, interleaved: bool = False, scaling: str = "none",
+                 factor: float = 1.0, original_length: int = 0, slow: float = 1.0, fast: float = 32.0,
+                 magnitude: float | None = None, device="cuda") -> Rope:
+    """The rotary positions of a model, once at load time (``rope_frequencies``
+    says what the scalings are).  ``magnitude`` defaults to 1, with ``"bands"``
+    to ``0.1 ln(factor) + 1`` (above 1 only)."""
+    frequencies = rope_frequencies(rotary_dim, base, scaling, factor, original_length, slow, fast)
+    if magnitude is None:
+        magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "bands" and factor > 1 else 1.0
+    turns = torch.tensor([f / (2 * math.pi) for f in frequencies], dtype=torch.float64, device=device)
+    return Rope(turns, interleaved, magnitude)
+
+
+def _check_heads(x: torch.Tensor, name: str, dtypes=(torch.bfloat16,)) -> None:
+    require_cuda(x)
+    if x.dim() != 3 or 0 in x.shape[1:] or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise ValueError(f"{name} must be [T, heads, head_dim] with unit column stride")
+    if x.dtype not in dtypes:
+        raise TypeError(f"{name} must be " + " or ".join(str(d).removeprefix("torch.") for d in dtypes))
+    if max(x.shape[1:]) > _MOST:
+        raise ValueError(f"{name}: sizes must be below 2^31")
+
+
+def _check_index(t: torch.Tensor, name: str, count: int) -> None:
+    require_cuda(t)
+    if t.dtype not in _INT:
+        raise TypeError(f"{name} must be int32 or int64")
+    if t.shape != (count,) or (count > 1 and t.stride(0) != 1):
+        raise ValueError(f"{name} must be contiguous [{count}]")
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """First and last byte address a tensor may touch, and one more."""
+    if t.numel() == 0:
+        return 0, 0
+    size = t.element_size()
+    low = sum(min(0, (n - 1) * s) for n, s in zip(t.shape, t.stride()))
+    high = sum(max(0, (n - 1) * s) for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr() + low * size, t.data_ptr() + (high + 1) * size
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a1 <= b0 or b1 <= a0
+
+
+def _check_out(out: torch.Tensor, x: torch.Tensor, name: str, in_place: bool) -> None:
+    """``out`` of the rows' type and shape, each element its own, apart from ``x`` (or ``x`` itself)."""
+    require_cuda(out)
+    if out.dtype != x.dtype:
+        raise TypeError(f"{name} must be {str(x.dtype).removeprefix('torch.')}")
+    rows, heads, dim = x.shape
+    if out.shape != x.shape or (dim > 1 and out.stride(2) != 1):
+        raise ValueError(f"{name} must be {list(x.shape)} with unit column stride")
+    _same_device(x, out, name)
+    row, head = out.stride(0), out.stride(1)
+    if rows and ((heads > 1 and head < dim) or (rows > 1 and row < (heads - 1) * (head if heads > 1 else 0) + dim)):
+        raise ValueError(f"{name} must hold rows of heads one behind the other")
+    if in_place and out.data_ptr() == x.data_ptr() and out.stride() == x.stride():
+        return
+    if not _apart(out, x):
+        raise ValueError(f"{name} must not overlap the rows")
+
+
+def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotates ``x`` bf16 or f32 [T, heads, head_dim] (any row and head stride) by
+    its rows' ``positions`` (int32 or int64 [T], any value): the first
+    ``rope.rotary_dim`` columns of every head, the others stay.  Angles are taken
+    in 64 bits, one rounding.  ``out`` (the rows' shape and type) may be ``x``."""
+    _check_heads(x, "x", _FLOAT)
+    rows, heads, dim = x.shape
+    _check_index(positions, "positions", rows)
+    _same_device(x, positions, "positions")
+    _same_device(x, rope.turns, "rope")
+    if out is None:
+        out = torch.empty(rows, heads, dim, dtype=x.dtype, device=x.device)
+    else:
+        _check_out(out, x, "out", True)
+    _call(x.device, "d3_rope_rows", ptr(x), _FLOAT[x.dtype], x.stride(0), x.stride(1), rows, heads, dim,
+          ptr(positions), _INT[positions.dtype], ctypes.byref(rope._struct), ptr(out), out.stride(0), out.stride(1))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# The paged cache
+# ---------------------------------------------------------------------------
+@dataclass(frozen=True)
+class PagedCache:
+    """Keys and values of one layer in pages: ``keys`` / ``values``
+    [pages, kv_heads, page_size, head_dim], bf16 or float8_e4m3fn (any page, head
+    and token stride of whole 16 bytes: a [pages, page_size, kv_heads, head_dim]
+    buffer goes in as its ``transpose(1, 2)``), and ``page_table`` int32 [slots,
+    max_pages]: token t of a slot lies in page ``page_table[slot, t // page_size]``
+    at token ``t % page_size``.  Entries outside [0, pages) are unmapped: nothing
+    is written there, and nothing attends them.  page_size is a power of two.
+
+    e4m3 codes stand for code * scale of their head, ``k_scale`` / ``v_scale``
+    f32 [kv_heads] (None: 1).  Two slots may share pages that neither appends to.
+
+    The cache holds on to the tensors: what they hold may change at any time
+    (the page table between two replays of a graph, too), where they lie may not."""
+
+    keys: torch.Tensor
+    values: torch.Tensor
+    page_table: torch.Tensor
+    k_scale: torch.Tensor | None = None
+    v_scale: torch.Tensor | None = None
+    _struct: _lib.PagedCacheStruct = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self):
+        """The kernels take the sizes as given: they have to be the tensors'."""
+        keys, values, table = self.keys, self.values, self.page_table
+        require_cuda(keys, values, table, self.k_scale, self.v_scale)
+        if keys.dtype not in _CACHE or values.dtype != keys.dtype:
+            raise TypeError("keys and values must both be bfloat16 or float8_e4m3fn")
+        if keys.dim() != 4 or keys.shape != values.shape or 0 in keys.shape:
+            raise ValueError("keys and values must be [pages, kv_heads, page_size, head_dim] of one shape")
+        pages, kv_heads, page_size, head_dim = keys.shape
+        if page_size & (page_size - 1):
+            raise ValueError(f"page size {page_size} must be a power of two")
+        if table.dtype != torch.int32:
+            raise TypeError("page_table must be int32")
+        if table.dim() != 2 or 0 in table.shape or (table.shape[1] > 1 and table.stride(1) != 1) or (
+                table.shape[0] > 1 and table.stride(0) < table.shape[1]):
+            raise ValueError("page_table must be [slots, max_pages] with unit column stride")
+        if max(pages, kv_heads, head_dim, table.shape[0]) > _MOST or table.shape[1] * page_size > 1 << 30:
+            raise ValueError("pages, heads and slots must be below 2^31, a slot's tokens at most 2^30")
+        part = 16 // keys.element_size()
+        for t, name in ((keys, "keys"), (values, "values")):
+            strides = t.stride()
+            if strides[3] != 1 or head_dim % part or t.data_ptr() % 16 or any(
+                    n > 1 and (s < head_dim or s % part) for n, s in zip(t.shape[:3], strides)):
+                raise ValueError(f"{name}: rows of whole 16 bytes, 16-byte aligned, one behind the other")
+            ordered = sorted((s, n) for n, s in zip(t.shape[:3], strides) if n > 1)
+            if any(big < s * n for (s, n), (big, _) in zip(ordered, ordered[1:])):
+                raise ValueError(f"{name} must not overlap themselves")
+        if not _apart(keys, values) and keys.data_ptr() == values.data_ptr():
+            raise ValueError("keys and values must not be the same memory")
+        for t, name in ((values, "values"), (table, "page_table"), (self.k_scale, "k_scale"), (self.v_scale, "v_scale")):
+            if t is not None:
+                _same_device(keys, t, name)
+        for t, name in ((self.k_scale, "k_scale"), (self.v_scale, "v_scale")):
+            if t is None:
+                continue
+            if keys.dtype == torch.bfloat16:
+                raise ValueError(f"{name} goes with float8_e4m3fn caches")
+            if t.dtype != torch.float32:
+                raise TypeError(f"{name} must be float32")
+            if t.shape != (kv_heads,) or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous [{kv_heads}]")
+        stride = lambda t: [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride())]  # noqa: E731
+        (kp, kh, kt), (vp, vh, vt) = stride(keys), stride(values)
+        object.__setattr__(self, "_struct", _lib.PagedCacheStruct(
+            ptr(keys), ptr(values), _CACHE[keys.dtype], kv_heads, head_dim, page_size, pages, kp, kh, kt, vp, vh, vt,
+            ptr(table), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[0], table.shape[1],
+            ptr(self.k_scale), ptr(self.v_scale)))
+
+    @classmethod
+    def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int, max_pages: int,
+              dtype: torch.dtype = torch.bfloat16, device="cuda", k_scale=None, v_scale=None) -> PagedCache:
+        """A cache of ``pages`` pages, none of them mapped."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device),
+                   torch.full((slots, max_pages), -1, dtype=torch.int32, device=device), k_scale, v_scale)
+
+    @property
+    def device(self) -> torch.device:
+        return self.keys.device
+
+
+def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                 row_slots: torch.Tensor, rope: Rope | None = None, q: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Writes ``k`` and ``v`` bf16 [T, kv_heads, head_dim] of new tokens to the
+    cache, row r as token ``positions[r]`` of slot ``row_slots[r]`` (int32 or int64
+    [T] each, as ``packed_row_metadata`` gives them), keys rotated by ``rope`` on
+    the way.  With ``q`` bf16 [T, heads, head_dim], returns the rotated queries
+    (into ``out``, which may be ``q``).  The three are usually views of one
+    projection's rows.
+
+    Rows of a slot outside [0, slots), of a negative position or one past the
+    table, and of an unmapped page write nothing; their queries are rotated.  No
+    two rows may name the same token: which of them it would hold is not said."""
+    _check_heads(k, "k")
+    _check_heads(v, "v")
+    rows = k.shape[0]
+    _, kv_heads, _, head_dim = cache.keys.shape
+    if k.shape != (rows, kv_heads, head_dim) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [T, {kv_heads}, {head_dim}], as the cache's heads")
+    _check_index(positions, "positions", rows)
+    _check_index(row_slots, "row_slots", rows)
+    for t, name in ((v, "v"), (positions, "positions"), (row_slots, "row_slots"), (cache.keys, "cache")):
+        _same_device(k, t, name)
+    if rope is not None:
+        _same_device(k, rope.turns, "rope")
+        if rope.rotary_dim > head_dim:
+            raise ValueError(f"rotary width {rope.rotary_dim} above the head's {head_dim}")
+    q_args = (None, 0, 0, 0, None, 0, 0)
+    if q is not None:
+        _check_heads(q, "q")
+        if q.shape[0] != rows or q.shape[2] != head_dim:
+            raise ValueError(f"q must be [{rows}, heads, {head_dim}]")
+        _same_device(k, q, "q")
+        if out is None:
+            out = torch.empty(rows, q.shape[1], head_dim, dtype=q.dtype, device=q.device)
+        else:
+            _check_out(out, q, "out", True)
+            if out.data_ptr() != q.data_ptr() and not (_apart(out, k) and _apart(out, v)):
+                raise ValueError("out must not overlap k or v")
+        q_args = (ptr(q), q.stride(0), q.stride(1), q.shape[1], ptr(out), out.stride(0), out.stride(1))
+    elif out is not None:
+        raise ValueError("out goes with q")
+    _call(k.device, "d3_paged_append", ctypes.byref(cache._struct), ptr(k), k.stride(0), k.stride(1), ptr(v),
+          v.stride(0), v.stride(1), rows, ptr(positions), _INT[positions.dtype], ptr(row_slots),
+          _INT[row_slots.dtype], None if rope is None else ctypes.byref(rope._struct), *q_args)
+    return out
+
+
+def paged_attention(q: torch.Tensor, cache: PagedCache, layout: PackedLayout, lengths: torch.Tensor,
+                    scale: float | None = None, window: int | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new tokens' queries ``q`` bf16 [T, heads, head_dim] over
+    the cache -> bf16 [T, heads, head_dim].
+
+    Rows ``[layout.boundaries[i], layout.boundaries[i + 1])`` are the newest tokens
+    of sequence i, which slot ``layout.sequence_slots[i]`` holds ``lengths[i]`` tokens
+    of, theirs included (int32 or int64 [n]; append first).  Row j of its n_i, at
+    position ``p = lengths[i] - n_i + j``, attends the mapped tokens up to p, the
+    last ``window`` of them where one is given, with weights
+    ``softmax(scale * q . k)`` (``scale`` defaults to head_dim ** -0.5); query head h
+    reads kv head ``h // (heads / kv_heads)``.  Rows that attend nothing are zeros.
+
+    Rows of no sequence (before the first boundary, from the last on) are zeros, or
+    left as they were in a given ``out`` (apart from ``q``).  ``layout.max_length`` is the
+    longest n_i: 1 chooses the kernel for single tokens; any value computes all rows.
+    head_dim is 64, 128 or 256."""
+    _check_heads(q, "q")
+    rows, heads, dim = q.shape
+    boundaries, slots = layout.boundaries, layout.sequence_slots
+    require_cuda(boundaries)
+    if boundaries.dtype != torch.int32:
+        raise TypeError("boundaries must be int32")
+    if boundaries.dim() != 1 or len(boundaries) < 1 or not boundaries.is_contiguous():
+        raise ValueError("boundaries must be contiguous [n + 1]")
+    count = boundaries.shape[0] - 1
+    _check_index(slots, "sequence_slots", count)
+    _check_index(lengths, "lengths", count)
+    kv_heads = cache.keys.shape[1]
+    if dim != cache.keys.shape[3] or heads % kv_heads:
+        raise ValueError(f"q must be [T, heads, {cache.keys.shape[3]}], heads a multiple of {kv_heads}")
+    for t, name in ((boundaries, "boundaries"), (slots, "sequence_slots"), (lengths, "lengths"), (cache.keys, "cache")):
+        _same_device(q, t, name)
+    if window is not None and window < 1:
+        raise ValueError(f"window {window} must be positive (or None)")
+    zero_rest = out is None
+    if out is None:
+        out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
+    else:
+        _check_out(out, q, "out", False)
+    longest = max(0, min(int(layout.max_length), _MOST))
+    struct = ctypes.byref(cache._struct)
+    size = _entry("d3_paged_attention_workspace")(struct, rows, heads, count, longest)
+    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
+    _call(q.device, "d3_paged_attention", struct, ptr(q), q.stride(0), q.stride(1), rows, heads, ptr(boundaries),
+          ptr(slots), _INT[slots.dtype], ptr(lengths), _INT[lengths.dtype], count, longest,
+          dim ** -0.5 if scale is None else float(scale), 0 if window is None else min(int(window), 1 << 62), ptr(out),
+          out.stride(0), out.stride(1), zero_rest, ptr(workspace), max(size, 0))
+    return out

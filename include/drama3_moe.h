@@ -47,6 +47,7 @@ extern "C" {
 #define D3_DTYPE_F32 1
 #define D3_DTYPE_I32 2
 #define D3_DTYPE_I64 3
+#define D3_DTYPE_E4M3 4 /* of a paged cache's keys and values */
 
 /* Expert weight layouts accepted by the expert GEMM entry points. */
 #define D3_LAYOUT_REFERENCE 0 /* w [E, N, K] row-major, as the checkpoint stores it */
@@ -852,6 +853,114 @@ int d3_mxfp4_moe(const uint16_t *x, int64_t x_row_stride, int64_t rows, const vo
 /* Workspace bytes of d3_mxfp4_moe (host-side arithmetic only; -1: not supported). */
 int64_t d3_mxfp4_moe_workspace(int64_t rows, int32_t top_k, int32_t num_experts, int32_t hidden,
                                int32_t intermediate);
+
+/*
+ * Attention over packed rows and a paged cache: what precedes the MoE step in
+ * the reference's attention layers (model.py:55-141: rotary positions, paged
+ * decode over 16-token pages, packed prefill), over the same packed rows,
+ * persistent slots and int64 positions that d3_row_metadata and
+ * d3_requests_load give.  Own semantics (parity unpinned: the reference calls
+ * libraries here).
+ */
+
+/*
+ * Rotary positions (host struct).  Pair i of a row at position p turns by
+ * p * turns[i] revolutions, computed in 64 bits: (a, b) -> magnitude * (a cos -
+ * b sin, a sin + b cos).  turns: rotary_dim / 2 doubles on the device.  Pairs
+ * are columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved;
+ * columns from rotary_dim on stay as they are.
+ */
+typedef struct d3_rope {
+  const double *turns;
+  int32_t rotary_dim;  /* even, >= 2 */
+  int32_t interleaved;
+  float magnitude;
+} d3_rope;
+
+/*
+ * A paged cache (host struct): token t of slot s lies in page
+ * page_table[s * table_stride + t / page_size] at token t % page_size; entries
+ * outside [0, pages) are unmapped.  keys / values are indexed [page][head][token]
+ * [column] with the given strides (elements; multiples of 16 bytes, bases
+ * 16-byte aligned, columns contiguous).  dtype D3_DTYPE_BF16, or D3_DTYPE_E4M3:
+ * codes that stand for code * scale of their head (float [kv_heads], NULL: 1).
+ * page_size is a power of two, max_pages * page_size <= 2^30, head_dim 64, 128 or 256 for d3_paged_attention.
+ */
+typedef struct d3_paged_cache {
+  void *keys, *values;
+  int32_t dtype;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int64_t pages;
+  int64_t key_page_stride, key_head_stride, key_token_stride;
+  int64_t value_page_stride, value_head_stride, value_token_stride;
+  const int32_t *page_table;
+  int64_t table_stride;
+  int32_t slots;
+  int32_t max_pages;
+  const float *key_scales, *value_scales;
+} d3_paged_cache;
+
+/*
+ * Rotates rows x [rows, heads, head_dim] (bf16 or f32, any row and head stride,
+ * unit column stride) by positions (int32 or int64 [rows], any value) into out
+ * of the same type, one rounding.  out may be x itself (same strides); it does
+ * not overlap x otherwise.  heads * head_dim <= 2^16.
+ */
+int d3_rope_rows(const void *x, int32_t x_dtype, int64_t x_row_stride, int64_t x_head_stride,
+                 int64_t rows, int32_t heads, int32_t head_dim, const void *positions,
+                 int32_t positions_dtype, const d3_rope *rope, void *out, int64_t out_row_stride,
+                 int64_t out_head_stride, void *stream);
+
+/*
+ * Writes keys and values [rows, kv_heads, head_dim] bf16 of new tokens to their
+ * place in the cache: row r is token positions[r] of slot row_slots[r] (int32
+ * or int64 each).  Keys are rotated on the way (rope NULL: not), and with q the
+ * queries [rows, q_heads, head_dim] too, into q_out (q_out may be q itself).
+ * e4m3 caches hold round(clamp(x / scale, -448, 448)) of the unrounded x.  Rows
+ * of a slot outside [0, slots), a negative position, one past the table or an
+ * unmapped page write no key and no value (their queries are rotated).  No two
+ * rows name the same token.  (q_heads + 2 kv_heads) * head_dim <= 2^16.
+ */
+int d3_paged_append(const d3_paged_cache *cache, const uint16_t *k, int64_t k_row_stride,
+                    int64_t k_head_stride, const uint16_t *v, int64_t v_row_stride,
+                    int64_t v_head_stride, int64_t rows, const void *positions,
+                    int32_t positions_dtype, const void *row_slots, int32_t row_slots_dtype,
+                    const d3_rope *rope, const uint16_t *q, int64_t q_row_stride,
+                    int64_t q_head_stride, int32_t q_heads, uint16_t *q_out,
+                    int64_t q_out_row_stride, int64_t q_out_head_stride, void *stream);
+
+/*
+ * Attention of new tokens over the cache.  Rows [boundaries[i], boundaries[i +
+ * 1]) of q bf16 [rows, q_heads, head_dim] are the newest n_i tokens of sequence
+ * i, whose slot sequence_slots[i] holds lengths[i] tokens (theirs included: append
+ * first).  Row j of it, at position p = lengths[i] - n_i + j, attends the mapped
+ * tokens c with p - window < c <= p (window <= 0: all c <= p) of its head's
+ * kv head h / (q_heads / kv_heads):
+ *   out = sum_c w_c value_c / sum_c w_c,  w_c = exp(scale * q . key_c),
+ * fp32 sums, weights rounded to bf16 for the product, one bf16 rounding of out.
+ * Rows that attend nothing (no token, no slot) are zeros.  Rows of no sequence
+ * are zeroed with zero_rest, else left as they were.
+ * boundaries int32 [sequences + 1] on the device, ascending, clamped to [0,
+ * rows]; sequence_slots and lengths int32 or int64 [sequences].  max_length: the
+ * longest n_i, which only chooses the kernels (any value gives the same rows
+ * computed).  out does not overlap q.  workspace: at least
+ * d3_paged_attention_workspace bytes, 16-byte aligned, this call's alone until
+ * it has run.  rows * q_heads <= 2^23, sequences <= 65536.
+ */
+int d3_paged_attention(const d3_paged_cache *cache, const uint16_t *q, int64_t q_row_stride,
+                       int64_t q_head_stride, int64_t rows, int32_t q_heads,
+                       const int32_t *boundaries, const void *sequence_slots,
+                       int32_t sequence_slots_dtype, const void *lengths, int32_t lengths_dtype,
+                       int32_t sequences, int32_t max_length, float scale, int64_t window,
+                       uint16_t *out, int64_t out_row_stride, int64_t out_head_stride,
+                       int32_t zero_rest, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Workspace bytes of d3_paged_attention (host-side arithmetic only; 0: none is
+ * needed; -1: not supported). */
+int64_t d3_paged_attention_workspace(const d3_paged_cache *cache, int64_t rows, int32_t q_heads,
+                                     int32_t sequences, int32_t max_length);
 
 #ifdef __cplusplus
 }

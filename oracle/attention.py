@@ -1,0 +1,157 @@
+"""Rotary positions, the paged cache and the attention over it in 64 bits, and
+how the attention's kernels cut a call (numpy; test infrastructure)."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+
+BF16_HALF_STEP = 2.0 ** -8
+F32_HALF_STEP = 2.0 ** -24
+E4M3_MAX = 448.0
+
+
+def rope(x, positions, frequencies, magnitude=1.0, interleaved=False):
+    """x [T, H, D] (float64), radians a position [R / 2] -> rotated [T, H, D] and
+    the sum |a| + |b| of each column's pair (0 where nothing turns)."""
+    half = len(frequencies)
+    # The angle's whole turns go before sine and cosine see it; long double keeps far positions exact.
+    turns = np.longdouble(positions)[:, None] * (np.longdouble(frequencies) / (2 * np.longdouble(np.pi)))
+    angle = ((turns - np.rint(turns)) * 2 * np.longdouble(np.pi)).astype(np.float64)[:, None, :]
+    cos, sin = magnitude * np.cos(angle), magnitude * np.sin(angle)
+    first = np.arange(half) * 2 if interleaved else np.arange(half)
+    second = first + 1 if interleaved else first + half
+    a, b = x[..., first], x[..., second]
+    out, size = x.astype(np.float64).copy(), np.zeros(x.shape)
+    out[..., first], out[..., second] = a * cos - b * sin, a * sin + b * cos
+    size[..., first] = size[..., second] = magnitude * (np.abs(a) + np.abs(b))
+    return out, size
+
+
+def rope_error(size):
+    """What an fp32 rotation may be off by before its rounding, for pairs of that
+    size: the remaining turn rounded to fp32 (at most 2^-25 turns), sine and
+    cosine of it (two steps of 2^-23 near 1), their product with the magnitude,
+    two products and a sum."""
+    return size * (2 * math.pi * 2.0 ** -25 + 2 * 2.0 ** -23 + 4 * F32_HALF_STEP)
+
+
+def e4m3(x):
+    """The e4m3 values nearest to x, ties to the even code, magnitudes above 448 to 448."""
+    x = np.clip(x, -E4M3_MAX, E4M3_MAX)
+    exponent = np.floor(np.log2(np.maximum(np.abs(x), 2.0 ** -6)))
+    step = np.exp2(exponent - 3)
+    return np.rint(x / step) * step
+
+
+def places(table, slots, positions, page_size, pages):
+    """(page, token) of each row, page -1 where it goes nowhere."""
+    out = []
+    for slot, position in zip(slots, positions):
+        page = -1
+        if 0 <= slot < len(table) and 0 <= position < table.shape[1] * page_size:
+            page = int(table[slot, position // page_size])
+            page = page if 0 <= page < pages else -1
+        out.append((page, int(position) % page_size))
+    return out
+
+
+def attention(q, keys, values, table, boundaries, slots, lengths, scale, window=None):
+    """q [T, H, D], keys / values [pages, kv heads, P, D] (float64) -> (out, bound on
+    what an fp32 evaluation with weights rounded to bf16 may be off by before
+    its own rounding, rows that belong to a sequence)."""
+    pages, kv_heads, page_size, dim = keys.shape
+    group = q.shape[1] // kv_heads
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    owned = np.zeros(len(q), dtype=bool)
+    for i, slot in enumerate(slots):
+        first, end = (min(max(int(b), 0), len(q)) for b in boundaries[i:i + 2])
+        owned[first:end] = True
+        if not 0 <= slot < len(table):
+            continue
+        before = int(lengths[i]) - (end - first)
+        for row in range(first, end):
+            position = before + row - first
+            at = np.arange(max(0, position - window + 1) if window else 0,
+                           max(0, min(position + 1, table.shape[1] * page_size)))
+            page = table[slot, at // page_size]
+            at, page = at[(page >= 0) & (page < pages)], page[(page >= 0) & (page < pages)]
+            if len(at) == 0:
+                continue
+            for head in range(q.shape[1]):
+                k, v = (t[page, head // group, at % page_size] for t in (keys, values))
+                with np.errstate(invalid="ignore", over="ignore"):
+                    s = k @ q[row, head] * scale
+                    w = np.exp(s - s.max())
+                    out[row, head] = (w @ v) / w.sum()
+                    # Relative error of a weight: the score's fp32 sum (its terms' sizes, the
+                    # products by scale), the exponent's difference, 2^x itself; then of the sums
+                    # over keys and the rescalings at growing maxima (at most one per 16 keys);
+                    # each counted in numerator and denominator.  The weight's own rounding to bf16
+                    # is in the numerator alone.
+                    sizes = (np.abs(k) @ np.abs(q[row, head])).max() * abs(scale)
+                    rel = (dim + 8) * 2 * F32_HALF_STEP * sizes + 4 * F32_HALF_STEP * (s.max() - s.min()) + 2.0 ** -21
+                    rel += (len(at) + 64) * 2 * F32_HALF_STEP + (len(at) // 16 + 8) * 2.0 ** -21
+                    bound[row, head] = (w @ np.abs(v)) / w.sum() * (BF16_HALF_STEP + 2 * rel * (1 + BF16_HALF_STEP))
+    return out, bound, owned
+
+
+# ---------------------------------------------------------------------------
+# How a call is cut, as the kernels do it
+# ---------------------------------------------------------------------------
+BLOCK = 64
+CUS = 256
+
+
+def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, window=0):
+    """(units, bounds): every workgroup's (sequence, tile, split, partial index or
+    None, key range, first and last packed row), and the sizes that bound them."""
+    group = q_heads // kv_heads
+    decode = max_length <= 1
+    slices, tile_rows = -(-group // 16), 128
+    tile_tokens = 1 if decode else tile_rows // group + 2
+    count = len(lengths)
+    tiles_most = rows * slices if decode else rows * group // tile_rows + min(count, rows)
+    target = max(1, 2 * CUS // kv_heads)
+    least = 2 if decode else 4
+    split = -(-capacity // BLOCK) > least
+    if not split:
+        least = 1 << 30
+    sequences, work = [], np.float32(0)
+    for i in range(count):
+        b0, b1 = (min(max(int(b), 0), rows) for b in boundaries[i:i + 2])
+        tokens, length = max(b1 - b0, 0), max(int(lengths[i]), 0)
+        tiles = tokens * slices if decode else -(-tokens * group // tile_rows)
+        keys = min(length, capacity)
+        if window:
+            keys = min(keys, window + tile_tokens + BLOCK)
+        blocks = -(-keys // BLOCK)
+        sequences.append((b0, tokens, length, tiles, blocks))
+        work = np.float32(work + np.float32(tiles) * np.float32(blocks))
+    chunk = max(least, math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target)))
+    units, partial = [], 0
+    for i, (first, tokens, length, tiles, blocks) in enumerate(sequences):
+        splits = max(1, -(-blocks // chunk))
+        for tile in range(tiles):
+            if decode:
+                low_token = high_token = tile // slices
+                packed = (low_token * group + 16 * (tile % slices),
+                          low_token * group + min(16 * (tile % slices) + 16, group) - 1)
+            else:
+                packed = (tile * tile_rows, min((tile + 1) * tile_rows, tokens * group) - 1)
+                low_token, high_token = packed[0] // group, packed[1] // group
+            before = length - tokens
+            end = min(max(before + high_token + 1, 0), capacity)
+            seen = before + low_token - window + 1 if window else 0
+            start = min(max(seen, 0), end)
+            aligned = start & ~(BLOCK - 1)
+            each = -(-(-(-(end - aligned) // BLOCK)) // splits)
+            for s in range(splits):
+                low = min(max(aligned + s * each * BLOCK, start), end)
+                high = max(min(aligned + (s + 1) * each * BLOCK, end), low)
+                at = partial + tile * splits + s if splits > 1 else None
+                units.append((i, tile, s, at, (low, high), packed, (start, end)))
+        partial += tiles * splits if splits > 1 else 0
+    return units, {"units": tiles_most + (target if split else 0), "partials": 2 * target if split else 0,
+                   "split_tiles": min(tiles_most, target)}
