@@ -4,10 +4,17 @@
 //
 // A sequence's new rows times the heads that share a kv head are packed rows:
 // packed row m of kv head h is token m / group, query head h * group + m % group.
-// They are cut into tiles of kTileRows; the keys a tile attends are cut into
-// splits of whole 64-key blocks where one workgroup a tile would leave the card
-// idle.  Unit = (tile, split); a workgroup takes one unit of one kv head.
+// They are cut into tiles of kTileRows, a sequence's single token into one tile per
+// 16 heads of its group.
+//
+// Single tokens: the key blocks of all their tiles, one behind the other, are dealt
+// to as many workgroups as are resident at once, the same number to each; where a
+// workgroup's share ends inside a tile, the tile's parts are joined afterwards.
+// Tiles of many rows: a workgroup each, or several for those of more key blocks
+// than an even share.
 #pragma once
+
+#include <type_traits>
 
 #include "common.h"
 #include "expert_tile.h"
@@ -15,7 +22,11 @@
 
 namespace d3 {
 
-constexpr int kKeyBlock = 64;  // keys a split is cut at
+constexpr int kKeyBlock = 64;  // keys that tiles are cut at
+constexpr int kPagedWaves = 4;
+constexpr int kPagedThreads = kPagedWaves * kWave;
+constexpr int kTileRows = 32 * kPagedWaves;
+constexpr int kZeroGroups = 64;  // workgroups behind the units' that zero rows of no sequence
 
 struct PagedArgs {
   const uint16_t* q;
@@ -34,28 +45,37 @@ struct PagedArgs {
   const void *sequence_slots, *lengths;
   int slots_64, lengths_64;
   int sequences, rows, q_heads, kv_heads, group;
-  int slices;       // 16-row parts of a token's group, each a tile of its own (decode)
-  int tile_rows;    // packed rows of a tile, or 0: one token's slice (decode)
-  int tile_tokens;  // most tokens a tile spans
-  float scale;      // with log2(e) in it: weights are powers of two
-  int window;       // 0: none
-  int target;       // units a kv head that the splits aim at
-  int least;        // fewest key blocks worth a split
-  int max_units;    // of a kv head, bounds the grid
-  int zero_rest;
-  float* sums;      // partial rows [split unit][kv head][tile rows][D]
-  float2* stats;    // their (maximum, sum) [split unit][kv head][tile rows]
+  int slices;         // 16-row parts of a token's group, each a tile where tokens are taken singly
+  int all_single;     // every token is taken singly (else those of sequences of one)
+  int tile_tokens;    // most tokens a tile spans
+  float scale;        // with log2(e) in it: weights are powers of two
+  int window;         // 0: none
+  int share_shift;    // log2 of the keys in a block of single tokens' shares
+  int shares, least;  // workgroups a kv head that single tokens' blocks are dealt to, fewest blocks of one
+  int target;         // units a kv head that the splits of tiles aim at
+  int least_split;    // fewest key blocks worth one
+  int tile_units;     // most units of a kv head
+  // Partial rows [part][kv head][rows of a tile][D] and their (maximum, sum), of single
+  // tokens' tiles (16 rows) and of the others (kTileRows).
+  float *single_sums, *tile_sums;
+  float2 *single_stats, *tile_stats;
+  int single_parts, tile_parts;  // how many there are: boundaries that are not ascending must not lead past them
 };
 
-// One unit's place.
+// Where a workgroup's work lies.
 struct PagedUnit {
   bool live;
-  int sequence, tile, split, splits, partial;  // partial: first partial of the tile's splits, where splits > 1
-  int first_row, tokens, length;               // rows of the sequence, tokens it holds
+  int sequence, tile, splits;
+  int split;                      // of a tile: which of its splits
+  int from, blocks;               // of a single token's tile: blocks [from, from + blocks)
+  int part;                       // partial of this unit (of a tile to join: the first)
+  int first_row, tokens, length;  // rows of the sequence, tokens it holds
+  int slot;                       // [0, slots), or -1
 };
 
 struct PagedSequence {
-  int first_row, tokens, length, tiles, splits, blocks;
+  int first_row, tokens, length, slot, tiles, blocks;
+  bool single;
 };
 
 __device__ __forceinline__ int64_t paged_index(const void* p, int is_64, int64_t i) {
@@ -63,18 +83,25 @@ __device__ __forceinline__ int64_t paged_index(const void* p, int is_64, int64_t
 }
 
 __device__ __forceinline__ PagedSequence paged_sequence(const PagedArgs& a, int i) {
-  PagedSequence s = {};
-  if (i >= a.sequences) return s;
-  const int b0 = min(max(a.boundaries[i], 0), a.rows), b1 = min(max(a.boundaries[i + 1], 0), a.rows);
-  const int64_t length = paged_index(a.lengths, a.lengths_64, i);
+  // (loads of every lane at once, none behind another)
+  const int at = min(i, a.sequences - 1);
+  const int from = a.boundaries[at], to = a.boundaries[at + 1];
+  const int64_t length = paged_index(a.lengths, a.lengths_64, at);
+  const int64_t slot = paged_index(a.sequence_slots, a.slots_64, at);
+  const int b0 = min(max(from, 0), a.rows), b1 = min(max(to, 0), a.rows);
+  PagedSequence s;
   s.first_row = b0;
-  s.tokens = max(b1 - b0, 0);
+  s.tokens = i < a.sequences ? max(b1 - b0, 0) : 0;
   s.length = static_cast<int>(length < 0 ? 0 : (length < 0x7fffffff ? length : 0x7fffffff));
-  s.tiles = a.tile_rows ? (s.tokens * a.group + a.tile_rows - 1) / a.tile_rows : s.tokens * a.slices;
+  s.slot = slot >= 0 && slot < a.slots ? static_cast<int>(slot) : -1;
+  s.single = a.all_single || s.tokens == 1;
+  s.tiles = s.single ? s.tokens * a.slices : (s.tokens * a.group + kTileRows - 1) / kTileRows;
   // Key blocks of the longest tile: all the sequence's, or what a window over its tokens touches.
   int keys = min(s.length, a.capacity);
-  if (a.window > 0) keys = static_cast<int>(min(static_cast<int64_t>(keys), static_cast<int64_t>(a.window) + a.tile_tokens + kKeyBlock));
-  s.blocks = (keys + kKeyBlock - 1) / kKeyBlock;
+  const int shift = s.single ? a.share_shift : 6;
+  if (a.window > 0)
+    keys = static_cast<int>(min(static_cast<int64_t>(keys), static_cast<int64_t>(a.window) + a.tile_tokens + (1 << shift)));
+  s.blocks = max((keys + (1 << shift) - 1) >> shift, 1);
   return s;
 }
 
@@ -82,99 +109,170 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __uint_as_float(wave_reduce<SumF32>(__float_as_uint(v)));
 }
 
-// Inclusive prefix sum over the wave's lanes.
-__device__ __forceinline__ int wave_prefix(int v) {
-#pragma unroll
-  for (int d = 1; d < kWave; d <<= 1) {
-    const int up = __shfl_up(v, d, kWave);
-    if (lane_id() >= d) v += up;
-  }
-  return v;
+// Inclusive prefix sum over the wave's lanes, on DPP moves: within rows of 16, then rows' ends.
+__device__ __forceinline__ int wave_prefix(int value) {
+  uint32_t v = static_cast<uint32_t>(value);
+  v += dpp_move<0x111>(v, 0);  // row_shr 1, 2, 4, 8
+  v += dpp_move<0x112>(v, 0);
+  v += dpp_move<0x114>(v, 0);
+  v += dpp_move<0x118>(v, 0);
+  v += dpp_move<kDppRowBcast15, 0xa>(v, 0);
+  v += dpp_move<kDppRowBcast31, 0xc>(v, 0);
+  return static_cast<int>(v);
 }
 
-// Key blocks of a split: the batch's blocks over the units aimed at.  A little
-// more than their quotient, so that the units stay within tiles + target
-// whatever fp32 rounds off.
-__device__ __forceinline__ int paged_chunk(const PagedArgs& a) {
-  float work = 0.0f;
-  for (int i = lane_id(); i - lane_id() < a.sequences; i += kWave) {
-    const PagedSequence s = paged_sequence(a, i);
-    work += static_cast<float>(s.tiles) * static_cast<float>(s.blocks);
-  }
-  work = wave_sum(work);
-  const float chunk = ceilf(work * 1.001f / static_cast<float>(a.target));
-  return max(a.least, chunk < 1e9f ? static_cast<int>(chunk) : 1000000000);
+__device__ __forceinline__ int wave_total(int v) {
+  return static_cast<int>(wave_reduce<SumU32>(static_cast<uint32_t>(v)));
 }
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, kWave - 1); }
 
-// The unit with index `at`, found by every wave for itself (no barrier); with
-// kTiles, the tile with index `at` among those that are split.
+// A walk over the sequences, 64 at a time (a lane each), found by every wave for
+// itself, without a barrier.
+struct PagedWalk {
+  PagedSequence mine;  // this lane's of the sequences [base, base + 64)
+  int base;
+  __device__ void start(const PagedArgs& a) { base = 0, mine = paged_sequence(a, lane_id()); }
+  __device__ bool next(const PagedArgs& a) {
+    base += kWave;
+    if (base >= a.sequences) return false;
+    mine = paged_sequence(a, base + lane_id());
+    return true;
+  }
+  __device__ void take(int lane, PagedUnit& u) const {
+    u.live = true;
+    u.sequence = base + lane;
+    u.first_row = __builtin_amdgcn_readlane(mine.first_row, lane);
+    u.tokens = __builtin_amdgcn_readlane(mine.tokens, lane);
+    u.length = __builtin_amdgcn_readlane(mine.length, lane);
+    u.slot = __builtin_amdgcn_readlane(mine.slot, lane);
+  }
+};
+
+// Shares of single tokens' blocks: workgroup w of a kv head takes the blocks [w *
+// each, (w + 1) * each) of all tiles one behind the other.  Part w + t is what
+// workgroup w computes of tile t: no two are the same, a tile's follow one another.
+struct PagedShares {
+  PagedWalk walk;
+  int to, tiles_to;              // inclusive prefix sums over the walk's lanes
+  int before, tiles_before;      // blocks and tiles before the walk's sequences
+  int total, each;
+  __device__ int blocks_here() const { return walk.mine.single ? walk.mine.tiles * walk.mine.blocks : 0; }
+  __device__ int tiles_here() const { return walk.mine.single ? walk.mine.tiles : 0; }
+  __device__ void sums() { to = before + wave_prefix(blocks_here()), tiles_to = tiles_before + wave_prefix(tiles_here()); }
+  __device__ void start(const PagedArgs& a) {
+    walk.start(a);
+    before = tiles_before = 0;
+    sums();
+    total = last_lane(to);
+    if (a.sequences > kWave) {
+      while (walk.next(a)) total += wave_total(blocks_here());
+      walk.start(a);
+    }
+    each = max(a.least, static_cast<int>((static_cast<uint32_t>(total) + a.shares - 1) / static_cast<uint32_t>(a.shares)));
+  }
+  // The tile that holds block `at` < total, of those from the walk's place on; u.from
+  // is the block's place in it, u.blocks what it has from there, u.part its number.
+  __device__ PagedUnit find(const PagedArgs& a, int at) {
+    PagedUnit u = {};
+    for (;;) {
+      const uint64_t here = __ballot(at < to);
+      if (here != 0) {
+        const int lane = __builtin_ctzll(here);
+        walk.take(lane, u);
+        const int blocks = __builtin_amdgcn_readlane(walk.mine.blocks, lane), tiles = __builtin_amdgcn_readlane(walk.mine.tiles, lane);
+        const uint32_t rest = static_cast<uint32_t>(at - (__builtin_amdgcn_readlane(to, lane) - blocks * tiles));
+        u.tile = static_cast<int>(rest / static_cast<uint32_t>(blocks));
+        u.from = static_cast<int>(rest) - u.tile * blocks;
+        u.blocks = blocks - u.from;
+        u.part = __builtin_amdgcn_readlane(tiles_to, lane) - tiles + u.tile;
+        return u;
+      }
+      before = last_lane(to), tiles_before = last_lane(tiles_to);
+      if (!walk.next(a)) return u;
+      sums();
+    }
+  }
+};
+
+// The unit with index `at` of the tiles of many rows; with kTiles, the tile with
+// index `at` among those that are split.
 template <bool kTiles>
-__device__ __forceinline__ PagedUnit paged_unit(const PagedArgs& a, int at) {
-  const int chunk = paged_chunk(a);
-  int units_before = 0, partials_before = 0;
-  for (int base = 0; base < a.sequences; base += kWave) {
-    PagedSequence s = paged_sequence(a, base + lane_id());
-    s.splits = max(1, (s.blocks + chunk - 1) / chunk);
-    const int units = kTiles ? (s.splits > 1 ? s.tiles : 0) : s.tiles * s.splits;
-    const int partials = s.splits > 1 ? s.tiles * s.splits : 0;
+__device__ __forceinline__ PagedUnit paged_tile_unit(const PagedArgs& a, int at) {
+  PagedWalk walk;
+  walk.start(a);
+  auto tiles_here = [&] { return walk.mine.single ? 0 : walk.mine.tiles; };
+  // Key blocks of a split: the batch's blocks over the units aimed at.  A little
+  // more than their quotient, so that the units stay within tiles + target
+  // whatever fp32 rounds off.
+  float work = static_cast<float>(tiles_here()) * static_cast<float>(walk.mine.blocks);
+  if (a.sequences > kWave) {
+    while (walk.next(a)) work += static_cast<float>(tiles_here()) * static_cast<float>(walk.mine.blocks);
+    walk.start(a);
+  }
+  const float even = ceilf(wave_sum(work) * 1.001f / static_cast<float>(a.target));
+  const int chunk = max(a.least_split, even < 1e9f ? static_cast<int>(even) : 1000000000);
+  int units_before = 0, parts_before = 0;
+  PagedUnit u = {};
+  do {
+    const int tiles = tiles_here();
+    const int splits = static_cast<int>((static_cast<uint32_t>(walk.mine.blocks) + chunk - 1) / static_cast<uint32_t>(chunk));
+    const int units = kTiles ? (splits > 1 ? tiles : 0) : tiles * splits;
+    const int parts = splits > 1 ? tiles * splits : 0;
     const int units_to = units_before + wave_prefix(units);
-    const int partials_to = partials_before + wave_prefix(partials);
+    const int parts_to = parts_before + wave_prefix(parts);
     const uint64_t here = __ballot(at < units_to);
     if (here != 0) {
       const int lane = __builtin_ctzll(here);
-      PagedUnit u;
-      u.live = true;
-      u.sequence = base + lane;
-      u.splits = __builtin_amdgcn_readlane(s.splits, lane);
-      u.first_row = __builtin_amdgcn_readlane(s.first_row, lane);
-      u.tokens = __builtin_amdgcn_readlane(s.tokens, lane);
-      u.length = __builtin_amdgcn_readlane(s.length, lane);
-      const int tiles = __builtin_amdgcn_readlane(s.tiles, lane);
-      const int rest = at - (__builtin_amdgcn_readlane(units_to, lane) - __builtin_amdgcn_readlane(units, lane));
+      auto of = [&](int v) { return __builtin_amdgcn_readlane(v, lane); };
+      walk.take(lane, u);
+      u.splits = of(splits);
+      const uint32_t rest = static_cast<uint32_t>(at - (of(units_to) - of(units))), count = static_cast<uint32_t>(u.splits);
       // The last tile attends the most keys: it comes first.
-      u.tile = tiles - 1 - (kTiles ? rest : rest / u.splits);
-      u.split = kTiles ? 0 : rest % u.splits;
-      u.partial = __builtin_amdgcn_readlane(partials_to, lane) - __builtin_amdgcn_readlane(partials, lane) +
-                  u.tile * u.splits;
+      u.tile = of(tiles) - 1 - static_cast<int>(kTiles ? rest : rest / count);
+      u.split = kTiles ? 0 : static_cast<int>(rest % count);
+      u.part = of(parts_to) - of(parts) + u.tile * u.splits + u.split;
+      u.live = u.splits <= 1 || (u.part >= 0 && u.part <= a.tile_parts - (kTiles ? u.splits : 1));
       return u;
     }
-    units_before = __builtin_amdgcn_readlane(units_to, kWave - 1);
-    partials_before = __builtin_amdgcn_readlane(partials_to, kWave - 1);
-  }
-  PagedUnit none = {};
-  return none;
+    units_before = last_lane(units_to), parts_before = last_lane(parts_to);
+  } while (walk.next(a));
+  return u;
 }
 
-// Keys [low, high) that a split of a tile attends: of tokens [first, last] of
-// the sequence, in whole blocks from the tile's first key's block.
+// Keys [low, high) of blocks [from, from + blocks) of a tile: of what tokens
+// [first, last] of the sequence attend, counted from the first key's block.
 struct PagedKeys {
   int low, high;
 };
-__device__ __forceinline__ PagedKeys paged_keys(const PagedArgs& a, const PagedUnit& u, int first, int last) {
+struct PagedReach {
+  int start, end, aligned;  // keys [start, end), the first one's block's first key
+};
+__device__ __forceinline__ PagedReach paged_reach(const PagedArgs& a, const PagedUnit& u, int first, int last, int shift) {
   const int before = u.length - u.tokens;  // may be negative: rows with no place
-  const int end = min(max(before + last + 1, 0), a.capacity);
+  PagedReach r;
+  r.end = u.slot < 0 ? 0 : min(max(before + last + 1, 0), a.capacity);
   const int64_t seen = a.window > 0 ? static_cast<int64_t>(before) + first - a.window + 1 : 0;
-  const int start = static_cast<int>(seen > 0 ? (seen < end ? seen : end) : 0);
-  const int aligned = start & ~(kKeyBlock - 1);
-  const int blocks = (end - aligned + kKeyBlock - 1) / kKeyBlock;
-  const int each = (blocks + u.splits - 1) / u.splits;
+  r.start = static_cast<int>(seen > 0 ? (seen < r.end ? seen : r.end) : 0);
+  r.aligned = r.start >> shift << shift;
+  return r;
+}
+__device__ __forceinline__ PagedKeys paged_keys(const PagedReach& r, int from, int blocks, int shift) {
+  const int64_t low = r.aligned + (static_cast<int64_t>(from) << shift), high = low + (static_cast<int64_t>(blocks) << shift);
   PagedKeys k;
-  const int64_t from = aligned + static_cast<int64_t>(u.split) * each * kKeyBlock;
-  const int64_t to = from + static_cast<int64_t>(each) * kKeyBlock;
-  k.low = static_cast<int>(from > start ? (from < end ? from : end) : start);
-  k.high = static_cast<int>(to < end ? to : end);
+  k.low = static_cast<int>(low > r.start ? (low < r.end ? low : r.end) : r.start);
+  k.high = static_cast<int>(high < r.end ? high : r.end);
   if (k.high < k.low) k.high = k.low;
   return k;
 }
 
-// Rows before the first sequence and behind the last are zeroed, a row a workgroup.
-__device__ __forceinline__ void paged_zero_rest(const PagedArgs& a, int workgroup, int workgroups, int head_dim) {
+// Rows before the first sequence and behind the last are zeroed, by workgroups of their own.
+__device__ __forceinline__ void paged_zero_rest(const PagedArgs& a, int workgroup, int head_dim) {
   const int b0 = a.sequences > 0 ? min(max(a.boundaries[0], 0), a.rows) : a.rows;
   const int b1 = a.sequences > 0 ? max(min(max(a.boundaries[a.sequences], 0), a.rows), b0) : a.rows;
   const int rest = b0 + a.rows - b1;
-  for (int r = workgroup; r < rest; r += workgroups) {
+  for (int r = workgroup; r < rest; r += kZeroGroups) {
     uint16_t* row = a.out + (r < b0 ? r : b1 + r - b0) * a.out_row;
-    for (int i = static_cast<int>(threadIdx.x); i < a.q_heads * head_dim; i += static_cast<int>(blockDim.x))
+    for (int i = static_cast<int>(threadIdx.x); i < a.q_heads * head_dim; i += kPagedThreads)
       row[(i / head_dim) * a.out_head + i % head_dim] = 0;
   }
 }
@@ -208,6 +306,18 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// An address that another lane holds: of a lane known to the wave, and of any.
+__device__ __forceinline__ const uint8_t* lane_address(const uint8_t* mine, int lane) {
+  const uint64_t p = reinterpret_cast<uint64_t>(mine);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(p), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(p >> 32), lane);
+  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ const uint8_t* shuffled_address(const uint8_t* mine, int lane) {
+  const uint64_t p = reinterpret_cast<uint64_t>(mine);
+  const uint32_t lo = __shfl(static_cast<int>(p), lane, kWave), hi = __shfl(static_cast<int>(p >> 32), lane, kWave);
+  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // Maximum and sum with the lane 32 away, and with those 16 and 32 away, in every lane.
 __device__ __forceinline__ float max_across_32(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -226,6 +336,21 @@ __device__ __forceinline__ float sum_across_16(float v) {
   return sum_across_32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// What scores of a head are multiplied by, positive: a weight is 2^(score * size -
+// maximum), one instruction before the exponential, and a masked score of -inf stays
+// -inf.  A negative factor turns the query's signs instead, 0 is the least positive.
+struct ScoreScale {
+  float size;
+  uint32_t sign;  // of both halves of a word of queries
+};
+__device__ __forceinline__ ScoreScale score_scale(float c) {
+  return {c == 0.0f ? 1.17549435e-38f : fabsf(c), c < 0.0f ? 0x80008000u : 0u};
+}
+__device__ __forceinline__ bf16x8 load_query(const uint16_t* q, uint32_t sign) {
+  const RowVector4 w = *reinterpret_cast<const RowVector4*>(q);
+  return operand(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
+}
+
 // 2^x by the hardware's v_exp_f32; -inf gives 0.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -235,7 +360,11 @@ __device__ __forceinline__ void store_row4(uint16_t* out, floatx4 v) {
   *reinterpret_cast<RowVector2*>(out) = RowVector2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
 }
 
-void launch_paged_decode(const PagedArgs& a, int head_dim, bool e4m3, hipStream_t stream);
-void launch_paged_tiles(const PagedArgs& a, int head_dim, bool e4m3, hipStream_t stream);
+// A workgroup that no unit takes: the rows of no sequence, zeroed.
+inline unsigned paged_workgroups(const PagedArgs& a, bool zero_rest) {
+  return static_cast<unsigned>((a.tile_units + a.shares) * a.kv_heads + (zero_rest ? kZeroGroups : 0));
+}
+
+void launch_paged_decode(const PagedArgs& a, int head_dim, bool e4m3, bool zero_rest, hipStream_t stream);
 
 }  // namespace d3

@@ -88,12 +88,13 @@ def attention(q, keys, values, table, boundaries, slots, lengths, scale, window=
                     # Relative error of a weight: the score's fp32 sum (its terms' sizes, the
                     # products by scale), the exponent's difference, 2^x itself; then of the sums
                     # over keys and the rescalings at growing maxima (at most one per 16 keys);
-                    # each counted in numerator and denominator.  The weight's own rounding to bf16
-                    # is in the numerator alone.
+                    # each counted in numerator and denominator.  The weights' own rounding to bf16 may
+                    # be in both: sum w (1 + d) v / sum w (1 + d) is off by sum w d (v - out) / sum w (1 + d).
                     sizes = (np.abs(k) @ np.abs(q[row, head])).max() * abs(scale)
                     rel = (dim + 8) * 2 * F32_HALF_STEP * sizes + 4 * F32_HALF_STEP * (s.max() - s.min()) + 2.0 ** -21
                     rel += (len(at) + 64) * 2 * F32_HALF_STEP + (len(at) // 16 + 8) * 2.0 ** -21
-                    bound[row, head] = (w @ np.abs(v)) / w.sum() * (BF16_HALF_STEP + 2 * rel * (1 + BF16_HALF_STEP))
+                    size = (w @ np.abs(v)) / w.sum() + np.abs(out[row, head])
+                    bound[row, head] = size * (BF16_HALF_STEP / (1 - BF16_HALF_STEP) + 2 * rel * (1 + BF16_HALF_STEP))
     return out, bound, owned
 
 
@@ -102,56 +103,85 @@ def attention(q, keys, values, table, boundaries, slots, lengths, scale, window=
 # ---------------------------------------------------------------------------
 BLOCK = 64
 CUS = 256
+ALONE, LEAST, LEAST_SPLIT = 512, 4, 4
 
 
-def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, window=0):
-    """(units, bounds): every workgroup's (sequence, tile, split, partial index or
-    None, key range, first and last packed row), and the sizes that bound them."""
+def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=128, window=0):
+    """(units, bounds): every workgroup's (sequence, tile, single token or not, part
+    or None, key range, the tile's range, packed rows), in the order of its keys,
+    and the sizes that bound them."""
     group = q_heads // kv_heads
-    decode = max_length <= 1
-    slices, tile_rows = -(-group // 16), 128
-    tile_tokens = 1 if decode else tile_rows // group + 2
-    count = len(lengths)
-    tiles_most = rows * slices if decode else rows * group // tile_rows + min(count, rows)
+    all_single = max_length <= 1
+    slices, tile_rows, count = -(-group // 16), 128, len(lengths)
+    tile_tokens = 1 if all_single else tile_rows // group + 2
+    some = min(count, rows)
+    single_tiles = (rows if all_single else some) * slices
+    shift = 6
+    while capacity <= ALONE and capacity > 1 << shift:
+        shift += 1
+    most_blocks = ((capacity - 1) >> shift) + 1
+    least = LEAST if most_blocks > 1 else 1
+    shares = min(-(-single_tiles * most_blocks // least), max(1, (4 if dim == 64 else 2) * CUS // kv_heads)) if count else 0
     target = max(1, 2 * CUS // kv_heads)
-    least = 2 if decode else 4
-    split = -(-capacity // BLOCK) > least
-    if not split:
-        least = 1 << 30
-    sequences, work = [], np.float32(0)
+    tiles_most = 0 if all_single else rows * group // tile_rows + some
+    split_tiles = not all_single and -(-capacity // BLOCK) > LEAST_SPLIT
+    bounds = {"shares": shares, "single_parts": shares + single_tiles if shares > 1 and most_blocks > 1 else 0,
+              "tile_units": tiles_most + (target if split_tiles else 0), "tile_parts": 2 * target if split_tiles else 0,
+              "split_tiles": min(tiles_most, target) if split_tiles else 0}
+    sequences, work, total = [], np.float32(0), 0
     for i in range(count):
         b0, b1 = (min(max(int(b), 0), rows) for b in boundaries[i:i + 2])
         tokens, length = max(b1 - b0, 0), max(int(lengths[i]), 0)
-        tiles = tokens * slices if decode else -(-tokens * group // tile_rows)
+        single = all_single or tokens == 1
+        tiles = tokens * slices if single else -(-tokens * group // tile_rows)
+        size = shift if single else 6
         keys = min(length, capacity)
         if window:
-            keys = min(keys, window + tile_tokens + BLOCK)
-        blocks = -(-keys // BLOCK)
-        sequences.append((b0, tokens, length, tiles, blocks))
-        work = np.float32(work + np.float32(tiles) * np.float32(blocks))
-    chunk = max(least, math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target)))
-    units, partial = [], 0
-    for i, (first, tokens, length, tiles, blocks) in enumerate(sequences):
-        splits = max(1, -(-blocks // chunk))
+            keys = min(keys, window + tile_tokens + (1 << size))
+        blocks = max(1, -(-keys // (1 << size)))
+        sequences.append((tokens, length, single, tiles, blocks))
+        if single:
+            total += tiles * blocks
+        else:
+            work = np.float32(work + np.float32(tiles) * np.float32(blocks))
+    chunk = max(LEAST_SPLIT if split_tiles else 1 << 30, math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target)))
+    each = max(least, -(-total // max(shares, 1)))
+    units, part, ordinal, at = [], 0, 0, 0
+    for i, (tokens, length, single, tiles, blocks) in enumerate(sequences):
         for tile in range(tiles):
-            if decode:
+            if single:
                 low_token = high_token = tile // slices
-                packed = (low_token * group + 16 * (tile % slices),
-                          low_token * group + min(16 * (tile % slices) + 16, group) - 1)
+                first = low_token * group + 16 * (tile % slices)
+                packed = (first, min(first + 16, (low_token + 1) * group) - 1)
             else:
                 packed = (tile * tile_rows, min((tile + 1) * tile_rows, tokens * group) - 1)
                 low_token, high_token = packed[0] // group, packed[1] // group
             before = length - tokens
+            size = shift if single else 6
             end = min(max(before + high_token + 1, 0), capacity)
             seen = before + low_token - window + 1 if window else 0
             start = min(max(seen, 0), end)
-            aligned = start & ~(BLOCK - 1)
-            each = -(-(-(-(end - aligned) // BLOCK)) // splits)
-            for s in range(splits):
-                low = min(max(aligned + s * each * BLOCK, start), end)
-                high = max(min(aligned + (s + 1) * each * BLOCK, end), low)
-                at = partial + tile * splits + s if splits > 1 else None
-                units.append((i, tile, s, at, (low, high), packed, (start, end)))
-        partial += tiles * splits if splits > 1 else 0
-    return units, {"units": tiles_most + (target if split else 0), "partials": 2 * target if split else 0,
-                   "split_tiles": min(tiles_most, target)}
+            aligned = start >> size << size
+
+            def keys(low, high):
+                return min(max(low, start), end), max(min(high, end), min(max(low, start), end))
+
+            if single:
+                w = at // each
+                while w * each < at + blocks:
+                    low, high = max(w * each, at) - at, min((w + 1) * each, at + blocks) - at
+                    whole = high - low == blocks
+                    units.append((i, tile, True, None if whole else w + ordinal,
+                                  keys(aligned + (low << size), aligned + (high << size)), (start, end), packed))
+                    w += 1
+                at += blocks
+                ordinal += 1
+            else:
+                splits = -(-blocks // chunk)
+                step = -(-(-(-(end - aligned) // BLOCK)) // splits) * BLOCK
+                for s in range(splits):
+                    units.append((i, tile, False, None if splits == 1 else part + tile * splits + s,
+                                  keys(aligned + s * step, aligned + (s + 1) * step), (start, end), packed))
+        if not single and -(-blocks // chunk) > 1:
+            part += tiles * -(-blocks // chunk)
+    return units, bounds | {"each": each, "total": total}

@@ -110,22 +110,26 @@ def test_cut_covers_every_row_and_key_within_its_bounds(seed):
     lengths = tokens + (np.exp(rng.uniform(0, np.log(capacity + 1), count)) - 2).astype(int)
     window = int(rng.choice([0, 0, 1, 100, 1000]))
     group = q_heads // kv_heads
-    units, most = oa.cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, 1 if decode else int(tokens.max()), window)
-    assert len(units) <= most["units"]
-    partials = [u[3] for u in units if u[3] is not None]
-    assert sorted(partials) == list(range(len(partials))) and len(partials) <= most["partials"]
-    assert len({u[:2] for u in units if u[3] is not None}) <= most["split_tiles"]
+    dim = int(rng.choice([64, 128]))
+    units, most = oa.cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, 1 if decode else int(tokens.max()), dim, window)
+    tiles = [u for u in units if not u[2]]
+    assert len(tiles) <= most["tile_units"] and -(-most["total"] // most["each"]) <= most["shares"]
+    for name, mine in (("tile_parts", tiles), ("single_parts", [u for u in units if u[2]])):
+        parts = [u[3] for u in mine if u[3] is not None]
+        assert len(set(parts)) == len(parts) and all(0 <= p < most[name] for p in parts)
+    assert len({u[:2] for u in tiles if u[3] is not None}) <= most["split_tiles"]
     for i in range(count):
         seen = []
         for tile in {u[1] for u in units if u[0] == i}:
             mine = [u for u in units if u[:2] == (i, tile)]
-            start, end = mine[0][6]
+            start, end = mine[0][5]
             at = start
-            for u in mine:  # consecutive ranges, cut at whole blocks
+            for u in mine:  # consecutive ranges, cut at whole blocks, consecutive parts
                 low, high = u[4]
                 if low < high:
                     assert low == at and (low == start or low % oa.BLOCK == 0)
                     at = high
-            assert at == end
-            seen += range(mine[0][5][0], mine[0][5][1] + 1)
+                assert u[3] is None or u[3] == mine[0][3] + mine.index(u)
+            assert at == end and (len(mine) == 1) == (mine[0][3] is None)
+            seen += range(mine[0][6][0], mine[0][6][1] + 1)
         assert sorted(seen) == list(range(tokens[i] * group))
