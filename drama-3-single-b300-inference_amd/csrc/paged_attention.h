@@ -4,7 +4,7 @@
 //
 // A sequence's new rows times the heads that share a kv head are packed rows:
 // packed row m of kv head h is token m / group, query head h * group + m % group.
-// They are cut into tiles of kTileRows, a sequence's single token into one tile per
+// They are cut into tiles of 128 or 256, a sequence's single token into one tile per
 // 16 heads of its group.
 //
 // Single tokens: the key blocks of all their tiles, one behind the other, are dealt
@@ -23,9 +23,8 @@
 namespace d3 {
 
 constexpr int kKeyBlock = 64;  // keys that tiles are cut at
-constexpr int kPagedWaves = 4;
-constexpr int kPagedThreads = kPagedWaves * kWave;
-constexpr int kTileRows = 32 * kPagedWaves;
+constexpr int kLeastSplit = 4;   // fewest key blocks worth a split of a tile
+constexpr int kGroupRows = 128;  // packed rows that four waves of a tile take
 constexpr int kZeroGroups = 64;  // workgroups behind the units' that zero rows of no sequence
 
 struct PagedArgs {
@@ -34,7 +33,8 @@ struct PagedArgs {
   uint16_t* out;
   int64_t out_row, out_head;
   const uint8_t *keys, *values;
-  int64_t k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
+  uint32_t k_page, k_token, v_page, v_token;  // bytes: products with a page's number are one instruction
+  int64_t k_head, v_head;
   const int32_t* page_table;
   int64_t table_stride;
   uint32_t pages;
@@ -47,16 +47,17 @@ struct PagedArgs {
   int sequences, rows, q_heads, kv_heads, group;
   int slices;         // 16-row parts of a token's group, each a tile where tokens are taken singly
   int all_single;     // every token is taken singly (else those of sequences of one)
+  int tile_rows;      // packed rows of the other tiles
   int tile_tokens;    // most tokens a tile spans
   float scale;        // with log2(e) in it: weights are powers of two
   int window;         // 0: none
   int share_shift;    // log2 of the keys in a block of single tokens' shares
   int shares, least;  // workgroups a kv head that single tokens' blocks are dealt to, fewest blocks of one
   int target;         // units a kv head that the splits of tiles aim at
-  int least_split;    // fewest key blocks worth one
+  int splitting;      // whether they may be split
   int tile_units;     // most units of a kv head
   // Partial rows [part][kv head][rows of a tile][D] and their (maximum, sum), of single
-  // tokens' tiles (16 rows) and of the others (kTileRows).
+  // tokens' tiles (16 rows) and of the others (tile_rows).
   float *single_sums, *tile_sums;
   float2 *single_stats, *tile_stats;
   int single_parts, tile_parts;  // how many there are: boundaries that are not ascending must not lead past them
@@ -95,7 +96,7 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedArgs& a, int 
   s.length = static_cast<int>(length < 0 ? 0 : (length < 0x7fffffff ? length : 0x7fffffff));
   s.slot = slot >= 0 && slot < a.slots ? static_cast<int>(slot) : -1;
   s.single = a.all_single || s.tokens == 1;
-  s.tiles = s.single ? s.tokens * a.slices : (s.tokens * a.group + kTileRows - 1) / kTileRows;
+  s.tiles = s.single ? s.tokens * a.slices : static_cast<int>(static_cast<uint32_t>(s.tokens * a.group + a.tile_rows - 1) / static_cast<uint32_t>(a.tile_rows));
   // Key blocks of the longest tile: all the sequence's, or what a window over its tokens touches.
   int keys = min(s.length, a.capacity);
   const int shift = s.single ? a.share_shift : 6;
@@ -209,8 +210,11 @@ __device__ __forceinline__ PagedUnit paged_tile_unit(const PagedArgs& a, int at)
     while (walk.next(a)) work += static_cast<float>(tiles_here()) * static_cast<float>(walk.mine.blocks);
     walk.start(a);
   }
-  const float even = ceilf(wave_sum(work) * 1.001f / static_cast<float>(a.target));
-  const int chunk = max(a.least_split, even < 1e9f ? static_cast<int>(even) : 1000000000);
+  // Fewest blocks worth a split: kLeastSplit where the units are few, up to twice that
+  // where a quarter of them would do.
+  const float even = fminf(ceilf(wave_sum(work) * 1.001f / static_cast<float>(a.target)), 1e9f);
+  const int least = a.splitting ? min(max(static_cast<int>(fminf(4.0f * even, 1e9f)), kLeastSplit), 2 * kLeastSplit) : 1 << 30;
+  const int chunk = max(least, static_cast<int>(even));
   int units_before = 0, parts_before = 0;
   PagedUnit u = {};
   do {
@@ -272,7 +276,7 @@ __device__ __forceinline__ void paged_zero_rest(const PagedArgs& a, int workgrou
   const int rest = b0 + a.rows - b1;
   for (int r = workgroup; r < rest; r += kZeroGroups) {
     uint16_t* row = a.out + (r < b0 ? r : b1 + r - b0) * a.out_row;
-    for (int i = static_cast<int>(threadIdx.x); i < a.q_heads * head_dim; i += kPagedThreads)
+    for (int i = static_cast<int>(threadIdx.x); i < a.q_heads * head_dim; i += static_cast<int>(blockDim.x))
       row[(i / head_dim) * a.out_head + i % head_dim] = 0;
   }
 }

@@ -8,7 +8,7 @@
 // both operands.  Keys come from memory straight into operand registers; values
 // go through LDS, whose transposing reads give four keys of one column.
 //
-// Bound by HBM: every key and value is read once.  The four waves of a workgroup
+// Bound by HBM: every key and value is read once.  The waves of a workgroup
 // take steps of 32 keys in turn, each with its own running softmax and no
 // barrier until the end, where their rows are added in LDS; the next step's
 // keys and values are in flight while one is multiplied.
@@ -18,26 +18,24 @@
 
 namespace d3 {
 
-// Keys of a wave's step: what its registers hold twice (bf16 rows of 256 columns: half, for two waves a SIMD).
-constexpr int decode_keys(int dim, bool e4m3) { return dim == 256 && !e4m3 ? 16 : 32; }
+// Keys of a wave's step: what its registers hold twice (rows of 256 columns: half, for two waves a SIMD).
+constexpr int decode_keys(int dim, bool e4m3) { return dim == 256 ? 16 : 32; }
 
+// Keys and values are read once: past the caches' use for them (16 x 32768 e4m3 keys
+// 151 us, 171 as ordinary loads).
 __device__ __forceinline__ int32x4 load_once(const uint8_t* p) {
-#ifdef D3_NT
   return __builtin_nontemporal_load(reinterpret_cast<const int32x4*>(p));
-#else
-  return *reinterpret_cast<const int32x4*>(p);
-#endif
 }
 
-template <int D, bool kE4m3>
+template <int D, int kWaves>
 struct DecodeShared {
   // a wave's values, later its fp32 rows of 16 columns
-  __attribute__((aligned(16))) uint8_t values[kPagedWaves][16 * D * 4];
-  float2 stats[kPagedWaves][16];
+  __attribute__((aligned(16))) uint8_t values[kWaves][16 * D * 4];
+  float2 stats[kWaves][16];
 };
 
-template <int D, bool kE4m3>
-__device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit& u, int head, DecodeShared<D, kE4m3>& shared) {
+template <int D, bool kE4m3, int kWaves>
+__device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit& u, int head, DecodeShared<D, kWaves>& shared) {
   constexpr int kKeys = decode_keys(D, kE4m3), kKeyTiles = kKeys / 16;
   constexpr int kBytes = kE4m3 ? 1 : 2;
   constexpr int kRowParts = D * kBytes / 16;              // 16-byte parts of a cached row
@@ -90,8 +88,8 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
   int32x4 kr[kKeyLoads], vr[kValueLoads];
   // (a lane works out where its own key's rows begin, the loads take it from there)
   auto load_keys = [&](int key, int page) {
-    const int64_t token = (key + lane % kKeys) & in_page;
-    const uint8_t* row = page < 0 ? paged_nothing : keys + page * a.k_page + token * a.k_token;
+    const uint64_t token = (key + lane % kKeys) & in_page, p = static_cast<uint32_t>(page);
+    const uint8_t* row = page < 0 ? paged_nothing : keys + (p * a.k_page + token * a.k_token);
 #pragma unroll
     for (int t = 0; t < kKeyTiles; ++t) {
       const uint8_t* at = shuffled_address(row, 16 * t + column) + 16 * g;
@@ -101,8 +99,8 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
     }
   };
   auto load_rows = [&](int key, int page) {
-    const int64_t token = (key + lane % kKeys) & in_page;
-    const uint8_t* row = page < 0 ? paged_nothing : values + page * a.v_page + token * a.v_token;
+    const uint64_t token = (key + lane % kKeys) & in_page, p = static_cast<uint32_t>(page);
+    const uint8_t* row = page < 0 ? paged_nothing : values + (p * a.v_page + token * a.v_token);
 #pragma unroll
     for (int i = 0; i < kValueLoads; ++i)
       vr[i] = load_once(shuffled_address(row, kKeysALoad * i + lane / kRowParts) + 16 * (lane % kRowParts));
@@ -110,13 +108,13 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
 
   int key = first + wave * kKeys;
   int page = page_of(key, entry_of(key));
-  int entry = entry_of(key + kPagedWaves * kKeys);
+  int entry = entry_of(key + kWaves * kKeys);
   if (key < range.high) {
     load_keys(key, page);
     load_rows(key, page);
   }
   uint8_t* mine = shared.values[wave];
-  for (; key < range.high; key += kPagedWaves * kKeys) {
+  for (; key < range.high; key += kWaves * kKeys) {
     const uint32_t attended = static_cast<uint32_t>(__ballot(page >= 0)) & (kKeys == 32 ? 0xffffffffu : 0xffffu);
     // S^T of the step's 16-key tiles
     floatx4 s[kKeyTiles];
@@ -134,9 +132,9 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
         }
       }
     }
-    const int next = key + kPagedWaves * kKeys;
+    const int next = key + kWaves * kKeys;
     const int next_page = page_of(next, entry);
-    entry = entry_of(next + kPagedWaves * kKeys);
+    entry = entry_of(next + kWaves * kKeys);
     if (next < range.high) load_keys(next, next_page);
     // The running softmax, in powers of two
     if (attended != (kKeys == 32 ? 0xffffffffu : 0xffffu)) {
@@ -220,16 +218,16 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
   __syncthreads();
   constexpr int kParts = D / 4;
   const float value_scale = kE4m3 && a.v_scales != nullptr ? a.v_scales[head] : 1.0f;
-  for (int i = static_cast<int>(threadIdx.x); i < heads * kParts; i += kPagedThreads) {
+  for (int i = static_cast<int>(threadIdx.x); i < heads * kParts; i += kWaves * kWave) {
     const int c = i / kParts, d = 4 * (i % kParts);
     float highest = -__builtin_huge_valf();
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) highest = fmaxf(highest, shared.stats[w][c].x);
+    for (int w = 0; w < kWaves; ++w) highest = fmaxf(highest, shared.stats[w][c].x);
     const float base = highest == -__builtin_huge_valf() ? 0.0f : highest;
     float total = 0.0f;
     floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w) {
+    for (int w = 0; w < kWaves; ++w) {
       const float2 stat = shared.stats[w][c];
       const float weight = exp2_fast(stat.x - base);
       total += weight * stat.y;
@@ -251,8 +249,8 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
 }
 
 // A workgroup's share of the single tokens' blocks: parts of one tile or of several.
-template <int D, bool kE4m3>
-__device__ __forceinline__ void decode_share(const PagedArgs& a, int workgroup, int head, DecodeShared<D, kE4m3>& shared) {
+template <int D, bool kE4m3, int kWaves>
+__device__ __forceinline__ void decode_share(const PagedArgs& a, int workgroup, int head, DecodeShared<D, kWaves>& shared) {
   PagedShares shares;
   shares.start(a);
   const int64_t first = static_cast<int64_t>(workgroup) * shares.each;
@@ -267,7 +265,7 @@ __device__ __forceinline__ void decode_share(const PagedArgs& a, int workgroup, 
     u.splits = whole ? 1 : 2;
     u.part += workgroup;
     if (!whole && (u.part < 0 || u.part >= a.single_parts)) return;
-    decode_unit<D, kE4m3>(a, u, head, shared);
+    decode_unit<D, kE4m3, kWaves>(a, u, head, shared);
     at += u.blocks;
     if (at >= end) return;
     __syncthreads();  // (the rows in LDS have been read)

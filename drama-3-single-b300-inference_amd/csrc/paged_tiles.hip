@@ -1,6 +1,5 @@
-// Attention of chunks of new tokens over a paged cache: tiles of 128 packed
-// rows, one pass over the keys; a sequence's single token among them as
-// paged_decode.h takes it.
+// Attention of chunks of new tokens over a paged cache: tiles of packed rows, one
+// pass over the keys; a sequence's single token among them as paged_decode.h takes it.
 //
 // Wave w of a workgroup holds rows 32 w .. + 32 of the tile as columns of
 // mfma_f32_32x32x16_bf16 and multiplies them with the workgroup's key block (64
@@ -9,25 +8,27 @@
 // + 4 h + j % 4 for lane half h, element j, in both operands).  Values are read
 // from LDS transposed.
 //
-// Bound by the matrix cores and, as much, by the exponentials and the LDS reads:
-// a wave reads every key and value of the block for its 32 rows.
-#ifdef D3_TUNE
-#include <stdlib.h>
-#endif
+// Bound by the matrix cores and, as much, by the vector units: a block is 32
+// products of 32 cycles a wave (128 columns) and about as long in exponentials (four
+// times an ordinary instruction's time) and what goes with them.  Two ways to keep both
+// busy: two workgroups a CU of one group of four waves each (128 rows), or one of two
+// groups (256 rows) whose waves share a SIMD and take turns by barriers: while one
+// multiplies (values of the last block, keys of this one), the other computes weights.
 #include "paged_decode.h"
 
 namespace d3 {
 namespace {
 
 // Byte of 16-byte part c of LDS row r: keys are read 16 rows at a time at one
-// part, values in 32-byte pieces of 8 rows (D = 64: two rows share a bank row).
+// part, values in 64-byte pieces of 4 rows (D = 64: two rows share a bank row); no
+// two of them lie on one bank (measured: no conflicts).
 template <int D>
 __device__ __forceinline__ int key_part(int r, int c) {
   return r * (2 * D) + ((c ^ (D == 256 ? r & 7 : (D == 128 ? r & 15 : (r >> 1) & 7))) << 4);
 }
 template <int D>
 __device__ __forceinline__ int value_part(int r, int c) {
-  return r * (2 * D) + ((c ^ (2 * (D >= 128 ? r & 7 : (r >> 1) & 3))) << 4);
+  return r * (2 * D) + ((c ^ (D >= 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1))) << 4);
 }
 
 typedef uint16_t uint16x2 __attribute__((ext_vector_type(2)));
@@ -54,32 +55,36 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t w) {
   return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
 }
 
-constexpr int tile_keys(int dim) { return dim == 256 ? 32 : 64; }  // of a step: what registers and LDS hold twice
+constexpr int tile_keys(int dim) { return dim == 256 ? 32 : 64; }  // of a block
 
-template <int D>
+template <int D, int kGroups>
 struct TileShared {
-  // [buffer][keys, values], first: a load's place is 16 bits
-  __attribute__((aligned(16))) uint8_t block[2][2][tile_keys(D) * D * 2];
-  int infinite;  // the last block whose values held an infinity or a NaN
+  // A block's keys (and values) are loaded once the group that is last done with its
+  // buffer's block: two blocks before it where groups take turns, one where there is one.
+  static constexpr int kBytes = tile_keys(D) * D * 2;
+  __attribute__((aligned(16))) uint8_t keys[kGroups + 1][kBytes];
+  __attribute__((aligned(16))) uint8_t values[kGroups + 1][kBytes];
+  int infinite[kGroups + 1];  // the last block of each buffer whose values held an infinity or a NaN
 };
 
-template <int D, bool kE4m3>
-__device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u, int head, TileShared<D>& shared) {
+template <int D, bool kE4m3, int kGroups>
+__device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u, int head, TileShared<D, kGroups>& shared) {
+  constexpr int kWaves = 4 * kGroups, kThreads = kWaves * kWave, kBuffers = kGroups + 1;
+  constexpr int kTileRows = kGroupRows * kGroups;
   constexpr int kBytes = kE4m3 ? 1 : 2;
   constexpr int kRowParts = D * kBytes / 16;  // 16-byte parts of a cached row
-  constexpr int kKeys = tile_keys(D);
-  constexpr int kHalves = kKeys / 32;
-  constexpr int kLoads = kKeys * kRowParts / kPagedThreads;  // of keys, and of values, a thread
-  constexpr int kKeysALoad = kPagedThreads / kRowParts;
+  constexpr int kKeys = tile_keys(D), kHalves = kKeys / 32;
+  constexpr int kParts = kKeys * kRowParts;                               // of a block's keys, and of its values
+  constexpr int kLoads = kParts < kThreads ? 1 : kParts / kThreads;       // a thread
+  constexpr int kKeysALoad = kThreads / kRowParts, kWaveRows = kWave / kRowParts;
   constexpr int kSteps = D / 16, kColumns = D / 32;
-  constexpr int kBlockBytes = kKeys * D * 2;
-  auto& lds = shared.block;
-  int& infinite = shared.infinite;
+  constexpr int kAhead = 8;  // fragments in flight from LDS
 
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int column = lane & 31, half = lane >> 5;
+  const bool second = kGroups == 2 && wave >= 4;
   const int all_rows = u.tokens * a.group;  // packed rows of the sequence
   const int tile_row = u.tile * kTileRows;
   const int last_row = min(tile_row + kTileRows, all_rows) - 1;
@@ -93,7 +98,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   const int in_page = (1 << a.page_shift) - 1;
   const ScoreScale scale = score_scale(a.scale * (kE4m3 && a.k_scales != nullptr ? a.k_scales[head] : 1.0f));
 
-  // This lane's row, and the positions of the wave's.
+  // This lane's row, and the positions of the wave's and of the tile's.
   const int wave_row = tile_row + 32 * wave;
   const bool wave_live = wave_row <= last_row;
   const int my_row = min(wave_row + column, last_row);
@@ -102,9 +107,12 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   const int position = before + my_token;
   const int wave_low = before + min(wave_row, last_row) / a.group;
   const int wave_high = before + min(wave_row + 31, last_row) / a.group;
-  // Keys up to these are out of the windows of this lane's row, the wave's first and its last.
+  const int tile_low = before + tile_row / a.group;
+  // Keys up to these are out of the windows of this lane's row, the wave's first and
+  // its last, and the tile's last.
   auto behind = [&](int p) { return a.window > 0 ? static_cast<int>(max(static_cast<int64_t>(p) - a.window, int64_t{-1})) : -1; };
   const int oldest = behind(position), oldest_low = behind(wave_low), oldest_high = behind(wave_high);
+  const int tile_oldest = behind(before + last_row / a.group);
   bf16x8 qf[kSteps];
   {
     const uint16_t* q = a.q + static_cast<int64_t>(u.first_row + my_token) * a.q_row + my_head * a.q_head + 8 * half;
@@ -118,113 +126,113 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   for (int t = 0; t < kColumns; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-  // The weights' sums are one more row of values, all ones: the matrix cores have time
-  // to spare, the vector units none.
-  floatx16 sums;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) sums[i] = 0.0f;
-  const bf16x8 ones = operand(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  float top = -__builtin_huge_valf();
+  float top = -__builtin_huge_valf(), sum = 0.0f;
 
-  // Row of a transposing read, and the 16-byte part (its row's turn repeats every 8 rows).
-  const int value_row = 4 * half + ((lane & 15) >> 2), value_column = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-
-  // Staging.  bf16 blocks go from memory to LDS without registers: load i of wave w
-  // fills 1 KiB, a lane's 16 bytes at their swizzled place by reading the part that
-  // belongs there.  e4m3 ones are widened on the way.
-  constexpr int kParts = kE4m3 ? kRowParts : D / 8;  // (of an LDS row, where the loads go by that)
-  int32x4 kr[kE4m3 ? kLoads : 1], vr[kE4m3 ? kLoads : 1];
   // The page of a block's key `lane`: the table's entry, loaded a block before it is
   // looked at (a use waits for every load before it); then -1 where nothing is attended.
   auto attends = [&](int key) { return key + (lane & (kKeys - 1)) >= range.low && key + (lane & (kKeys - 1)) < range.high; };
   auto entry_of = [&](int key) { return pages[attends(key) ? (key + (lane & (kKeys - 1))) >> a.page_shift : 0]; };
   auto page_of = [&](int key, int entry) { return attends(key) && static_cast<uint32_t>(entry) < a.pages ? entry : -1; };
-  // A load's rows of one page, all attended: its address is the same for the wave but
-  // for the lane's place, which no load changes (kKeysALoad rows turn alike).
-  constexpr int kWaveRows = kWave / kRowParts;
-  const bool by_page = !kE4m3 && (1 << a.page_shift) >= kWaveRows && max(a.k_token, a.v_token) < 1 << 24;
-  const uint32_t lane_row = lane / kRowParts, lane_part = lane % kRowParts;
-  const uint32_t k_lane = static_cast<uint32_t>(lane_row * a.k_token) + key_part<D>(kWaveRows * wave + lane_row, lane_part) - (kWaveRows * wave + lane_row) * 2 * D;
-  const uint32_t v_lane = static_cast<uint32_t>(lane_row * a.v_token) + value_part<D>(kWaveRows * wave + lane_row, lane_part) - (kWaveRows * wave + lane_row) * 2 * D;
-  // Where the rows of a block's keys begin: a lane's own key, so that the 64-bit
-  // products are made once a block and a load reads its address from a lane.
-  struct Rows {
-    const uint8_t *key, *value;
+  // Where its row begins: the products are made once a block, loads take it from there.
+  auto row_of = [&](const uint8_t* base, uint32_t page_bytes, uint32_t token_bytes, int key, int page) {
+    const uint64_t token = (key + (lane & (kKeys - 1))) & in_page;
+    return page < 0 ? paged_nothing : base + (static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_bytes + token * token_bytes);
   };
-  auto rows_of = [&](int key, int page) {
-    const int64_t token = (key + (lane & (kKeys - 1))) & in_page;
-    Rows r;
-    r.key = page < 0 ? paged_nothing : keys + page * a.k_page + token * a.k_token;
-    r.value = page < 0 ? paged_nothing : values + page * a.v_page + token * a.v_token;
-    return r;
+
+  // Staging.  bf16 blocks go from memory to LDS without registers: load i of wave w
+  // fills 1 KiB, a lane's 16 bytes at their swizzled place by reading the part that
+  // belongs there.  Where a load's rows are of one page and all attended, its address
+  // is the wave's but for the lane's place, which no load changes (kKeysALoad rows turn
+  // alike).  e4m3 blocks are widened on the way.
+  const bool by_page = !kE4m3 && (1 << a.page_shift) >= kWaveRows && max(a.k_token, a.v_token) < 1u << 24;
+  const bool loading = kWaveRows * wave < kKeys;
+  const int lane_row = lane / kRowParts, lane_part = lane % kRowParts;
+  const int wave_first = kWaveRows * wave;  // of the wave's first load
+  const uint32_t k_lane = lane_row * a.k_token + key_part<D>(wave_first + lane_row, lane_part) - (wave_first + lane_row) * 2 * D;
+  const uint32_t v_lane = lane_row * a.v_token + value_part<D>(wave_first + lane_row, lane_part) - (wave_first + lane_row) * 2 * D;
+  int32x4 kr[kE4m3 ? kLoads : 1], vr[kE4m3 ? kLoads : 1];
+  auto load_piece = [&](const uint8_t* rows, uint32_t lane_place, uint8_t* to, int i) {
+    load_to_lds(lane_address(rows, i * kKeysALoad + wave_first), lane_place, to + (i * kWaves + wave) * 1024);
   };
-  // Load `piece` of a block whose loads go by pages: those of keys, then those of values.
-  auto load_piece = [&](const Rows& rows, int buffer, int piece) {
-    const int i = piece % kLoads, which = piece / kLoads;
-    load_to_lds(lane_address(which ? rows.value : rows.key, i * kKeysALoad + kWaveRows * wave), which ? v_lane : k_lane,
-                lds[buffer][which] + (i * kPagedWaves + wave) * 1024);
-  };
-  auto load_block = [&](const Rows& rows, int buffer) {
-    int thread = tid;
-    asm volatile("" : "+v"(thread));  // (its places are worked out anew, not held in registers)
-    const int my_part = thread % kParts, my_key = thread / kParts;
+  auto load_keys = [&](const uint8_t* rows, uint8_t* to) {
+    if (!loading) return;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = my_key + i * kKeysALoad;
-      const uint8_t *k = shuffled_address(rows.key, r), *v = shuffled_address(rows.value, r);
-      if constexpr (kE4m3) {
-        kr[i] = *reinterpret_cast<const int32x4*>(k + 16 * my_part);
-        vr[i] = *reinterpret_cast<const int32x4*>(v + 16 * my_part);
-      } else {  // (the part stored at place c of row r is c ^ the row's turn)
-        const int at = (i * kPagedWaves + wave) * 1024;
-        load_to_lds(k + (key_part<D>(r, my_part) - r * (2 * D)), lds[buffer][0] + at);
-        load_to_lds(v + (value_part<D>(r, my_part) - r * (2 * D)), lds[buffer][1] + at);
-      }
+      const int r = wave_first + lane_row + i * kKeysALoad;
+      const uint8_t* from = shuffled_address(rows, r);
+      if constexpr (kE4m3)
+        kr[i] = *reinterpret_cast<const int32x4*>(from + 16 * lane_part);
+      else  // (the part stored at place c of row r is c ^ the row's turn)
+        load_to_lds(from + (key_part<D>(r, lane_part) - r * (2 * D)), to + (i * kWaves + wave) * 1024);
     }
   };
-  auto store_block = [&](int buffer) {
-    if constexpr (kE4m3) {
-      int thread = tid;
-      asm volatile("" : "+v"(thread));
-      const int my_part = thread % kParts, my_key = thread / kParts;
-      uint8_t *k = lds[buffer][0], *v = lds[buffer][1];
+  auto load_values = [&](const uint8_t* rows, uint8_t* to) {
+    if (!loading) return;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int r = my_key + i * kKeysALoad;
-        *reinterpret_cast<bf16x8*>(k + key_part<D>(r, 2 * my_part)) = widen8(kr[i][0], kr[i][1]);
-        *reinterpret_cast<bf16x8*>(k + key_part<D>(r, 2 * my_part + 1)) = widen8(kr[i][2], kr[i][3]);
-        *reinterpret_cast<bf16x8*>(v + value_part<D>(r, 2 * my_part)) = widen8(vr[i][0], vr[i][1]);
-        *reinterpret_cast<bf16x8*>(v + value_part<D>(r, 2 * my_part + 1)) = widen8(vr[i][2], vr[i][3]);
-      }
-    } else {
-      wait_loads();
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = wave_first + lane_row + i * kKeysALoad;
+      const uint8_t* from = shuffled_address(rows, r);
+      if constexpr (kE4m3)
+        vr[i] = *reinterpret_cast<const int32x4*>(from + 16 * lane_part);
+      else
+        load_to_lds(from + (value_part<D>(r, lane_part) - r * (2 * D)), to + (i * kWaves + wave) * 1024);
+    }
+  };
+  auto store_keys = [&](uint8_t* to) {  // (e4m3)
+    if (!loading) return;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = wave_first + lane_row + i * kKeysALoad;
+      *reinterpret_cast<bf16x8*>(to + key_part<D>(r, 2 * lane_part)) = widen8(kr[i][0], kr[i][1]);
+      *reinterpret_cast<bf16x8*>(to + key_part<D>(r, 2 * lane_part + 1)) = widen8(kr[i][2], kr[i][3]);
+    }
+  };
+  auto store_values = [&](uint8_t* to) {
+    if (!loading) return;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = wave_first + lane_row + i * kKeysALoad;
+      *reinterpret_cast<bf16x8*>(to + value_part<D>(r, 2 * lane_part)) = widen8(vr[i][0], vr[i][1]);
+      *reinterpret_cast<bf16x8*>(to + value_part<D>(r, 2 * lane_part + 1)) = widen8(vr[i][2], vr[i][3]);
     }
   };
 
   // Where the rows of a block's tile do not all attend the same of its keys, a row must
   // take nothing of a value that it does not attend, and 0 times an infinity or a NaN
-  // is NaN: such blocks are searched for them, zeros put in their place for the
-  // product, and what rows do attend added after it.
-  auto zero_infinite = [&](int key, uint8_t* v) {
+  // is NaN: each wave searches what it loaded of such a block for them and puts zeros in
+  // their place for the product; what rows do attend is added after it.
+  auto tile_uneven = [&](int key) { return key + kKeys - 1 > tile_low || key <= tile_oldest; };
+  auto zero_infinite = [&](int key, uint8_t* v, int* flag) {
+    if (!loading) return;
     bool found = false;
-#pragma unroll
-    for (int i = 0; i < kBlockBytes / (16 * kPagedThreads); ++i) {
-      int32x4* at = reinterpret_cast<int32x4*>(v + 16 * (i * kPagedThreads + tid));
-      const int32x4 w = *at;
+    auto check = [&](uint8_t* at) {
+      int32x4* place = reinterpret_cast<int32x4*>(at);
+      const int32x4 w = *place;
       int32x4 f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = static_cast<int>(finite_of(w[j]));
-      if (f[0] != w[0] || f[1] != w[1] || f[2] != w[2] || f[3] != w[3]) *at = f, found = true;
+      if (f[0] != w[0] || f[1] != w[1] || f[2] != w[2] || f[3] != w[3]) *place = f, found = true;
+    };
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if constexpr (kE4m3) {
+        const int r = wave_first + lane_row + i * kKeysALoad;
+        check(v + value_part<D>(r, 2 * lane_part));
+        check(v + value_part<D>(r, 2 * lane_part + 1));
+      } else {
+        check(v + (i * kWaves + wave) * 1024 + 16 * lane);
+      }
     }
-    if (found) infinite = key;
+    if (found) *flag = key;
   };
-  auto add_infinite = [&](int key, int page) {
+  auto add_infinite = [&](int key) {
+    const int page = page_of(key, entry_of(key));
 #pragma unroll 1
     for (int c = 0; c < kKeys; ++c) {
       const int p = __shfl(page, c, kWave);
       if (p < 0) continue;
       const bool mine = key + c <= position && key + c > oldest;
-      const uint8_t* row = values + p * a.v_page + ((key + c) & in_page) * a.v_token + 4 * kBytes * half;
+      const uint8_t* row = values + static_cast<uint64_t>(p) * a.v_page + static_cast<uint64_t>((key + c) & in_page) * a.v_token + 4 * kBytes * half;
 #pragma unroll
       for (int t = 0; t < kColumns; ++t)
 #pragma unroll
@@ -248,140 +256,187 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
     }
   };
 
-  int key = range.low & ~(kKeys - 1);
-  int here = page_of(key, entry_of(key));  // pages of this block's keys
-  uint64_t attended = __ballot(here >= 0);
-  if (tid == 0) infinite = -1;
-  if (key < range.high) {
-    load_block(rows_of(key, here), 0);
-    store_block(0);
-  }
-  int entry = entry_of(key + kKeys);
-  const int tile_low = before + tile_row / a.group, tile_oldest = behind(before + last_row / a.group);
-  __syncthreads();
-  for (int buffer = 0; key < range.high; buffer ^= 1, key += kKeys) {
-    const bool more = key + kKeys < range.high;
-    const int page = page_of(key + kKeys, entry);
-    const uint64_t next_attended = __ballot(page >= 0);
-    entry = entry_of(key + 2 * kKeys);
-    // Loads wait for one another: those of a whole block go among the products.
-    const bool pieces = !kE4m3 && more && by_page && next_attended == ~uint64_t{0};
-    const Rows rows = rows_of(key + kKeys, page);
-    if (more && !pieces) load_block(rows, buffer ^ 1);
-    if (key + kKeys - 1 > tile_low || key <= tile_oldest) {
-      zero_infinite(key, lds[buffer][1]);
+  // Blocks of the unit; rows of the wave attend a block, or none does.
+  const int key0 = range.low & ~(kKeys - 1);
+  const int blocks = range.low < range.high ? (range.high - key0 + kKeys - 1) / kKeys : 0;
+  auto wave_attends = [&](int key) { return wave_live && key <= wave_high && key + kKeys - 1 > oldest_low; };
+  auto wave_uneven = [&](int key) { return key + kKeys - 1 > wave_low || key <= oldest_high; };
+
+  // Before the first: its keys and values and the second's keys.
+  int page1 = -1;  // of the next block's keys
+  int entry = 0;   // table's, of the one after
+  uint64_t attended = 0, attended1 = 0;
+  if (blocks > 0) {
+    const int page0 = page_of(key0, entry_of(key0));
+    page1 = page_of(key0 + kKeys, entry_of(key0 + kKeys));
+    entry = entry_of(key0 + 2 * kKeys);
+    attended = __ballot(page0 >= 0), attended1 = __ballot(page1 >= 0);
+    load_keys(row_of(keys, a.k_page, a.k_token, key0, page0), shared.keys[0]);
+    load_values(row_of(values, a.v_page, a.v_token, key0, page0), shared.values[0]);
+    if constexpr (kE4m3) store_keys(shared.keys[0]), store_values(shared.values[0]);
+    load_keys(row_of(keys, a.k_page, a.k_token, key0 + kKeys, page1), shared.keys[1]);
+    if constexpr (kE4m3) store_keys(shared.keys[1]);
+    wait_loads();
+    if (tid < kBuffers) shared.infinite[tid] = -1;
+    if (tile_uneven(key0)) {
       lds_barrier();
+      zero_infinite(key0, shared.values[0], &shared.infinite[0]);
     }
-    // Blocks that no row of the wave attends are only staged.
-    const bool mine = wave_live && key <= wave_high && key + kKeys - 1 > oldest_low;
-    if (!mine && pieces) {
+  }
+  lds_barrier();
+  if (second) lds_barrier();  // half a block behind the first group
+
+  // Row of a transposing read, and the 16-byte part (its row's turn repeats every 4 rows).
+  const int value_row = 4 * half + ((lane & 15) >> 2), value_column = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  floatx16 s[kHalves];
+  bf16x8 p[2 * kHalves];
+  int b0 = 0, b1 = 1, b2 = kBuffers - 1;  // buffers of this block, the next and the last
+  for (int block = 0;; ++block) {
+    const int key = key0 + block * kKeys;
+    // Products: scores of this block, then the values of the last at its weights.
+    // Parts of a row differ by an exclusive or of the lane's own: one instruction a
+    // read, where addresses held in registers would cost the kernel its second wave.
+    int key_at = key_part<D>(column, half), value_at = value_part<D>(value_row, value_column) + 8 * (lane & 1);
+    asm volatile("" : "+v"(key_at), "+v"(value_at));
+    const bool scores = block < blocks && wave_attends(key);
+    const bool weighted = block > 0 && wave_attends(key - kKeys);
+    constexpr int kProducts = kHalves * kSteps, kValueProducts = 2 * kHalves * kColumns;
+    const uint8_t *k = shared.keys[b0], *v = shared.values[b2];
+    const int after = kGroups == 2 ? b2 : b0;  // the buffer of the block after next
+    auto key_fragment = [&](int n) {
+      return *reinterpret_cast<const bf16x8*>(k + (key_at ^ (32 * (n % kSteps))) + 32 * (n / kSteps) * (2 * D));
+    };
+    auto value_fragment = [&](int n) {
+      const uint8_t* at = v + (value_at ^ (64 * (n % kColumns))) + 16 * (n / kColumns) * (2 * D);
+      const uint32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * (2 * D));
+      return operand(lo[0], lo[1], hi[0], hi[1]);
+    };
+    __builtin_amdgcn_s_setprio(1);
+    bf16x8 w[kAhead];
+    if (scores) {
 #pragma unroll
-      for (int i = 0; i < 2 * kLoads; ++i) load_piece(rows, buffer ^ 1, i);
-    }
-    if (mine) {
-      const uint8_t *k = lds[buffer][0], *v = lds[buffer][1];
-      // Parts of a row differ by an exclusive or of the lane's own: one instruction a
-      // read, where addresses held in registers would cost the kernel its second wave.
-      int key_at = key_part<D>(column, half), value_at = value_part<D>(value_row, value_column) + 8 * (lane & 1);
-      asm volatile("" : "+v"(key_at), "+v"(value_at));
-      floatx16 s[kHalves];
-      auto scores = [&](auto with_loads) {
-        constexpr int kEvery = kHalves * kSteps / (2 * kLoads);  // products a piece
-#pragma unroll
-        for (int b = 0; b < kHalves; ++b) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-#pragma unroll
-          for (int st = 0; st < kSteps; ++st) {
-            const bf16x8 w = *reinterpret_cast<const bf16x8*>(k + (key_at ^ (32 * st)) + 32 * b * (2 * D));
-            s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w, qf[st], s[b], 0, 0, 0);
-            if constexpr (decltype(with_loads)::value)
-              if ((b * kSteps + st) % kEvery == 0) load_piece(rows, buffer ^ 1, (b * kSteps + st) / kEvery);
-          }
-        }
-      };
-      if constexpr (kE4m3) {
-        scores(std::false_type{});
-      } else {
-        if (pieces)
-          scores(std::true_type{});
-        else
-          scores(std::false_type{});
-      }
+      for (int n = 0; n < kAhead; ++n) w[n] = key_fragment(n);
       __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[h][i] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < kProducts; ++n) {
+        s[n / kSteps] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[n % kAhead], qf[n % kSteps], s[n / kSteps], 0, 0, 0);
+        if (n + kAhead < kProducts) w[n % kAhead] = key_fragment(n + kAhead);
+      }
+    }
+    if (weighted) {
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) w[n] = value_fragment(n);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int n = 0; n < kValueProducts; ++n) {
+        const int e = n / kColumns, t = n % kColumns;
+        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[n % kAhead], p[e], o[t], 0, 0, 0);
+        if (n + kAhead < kValueProducts) w[n % kAhead] = value_fragment(n + kAhead);
+      }
+      if (wave_uneven(key - kKeys) && shared.infinite[b2] == key - kKeys) add_infinite(key - kKeys);
+    }
+    __builtin_amdgcn_s_setprio(0);
+    if (block >= blocks) break;
+    // What was loaded beside the last weights: this block's values, the next one's keys.
+    if (block > 0) {
+      if constexpr (kE4m3)
+        store_keys(shared.keys[b1]), store_values(shared.values[b0]);
+      else
+        wait_loads();
+      if (tile_uneven(key)) zero_infinite(key, shared.values[b0], &shared.infinite[b0]);
+    }
+    lds_barrier();
+
+    // Weights; loads of the keys after next and of the next values among them.
+    const int page2 = page_of(key + 2 * kKeys, entry);
+    entry = entry_of(key + 3 * kKeys);
+    const uint64_t attended2 = __ballot(page2 >= 0);
+    const uint8_t* key_rows = row_of(keys, a.k_page, a.k_token, key + 2 * kKeys, page2);
+    const uint8_t* value_rows = row_of(values, a.v_page, a.v_token, key + kKeys, page1);
+    const bool pieces = by_page && loading && attended2 == ~uint64_t{0} && attended1 == ~uint64_t{0};
+    if (!pieces) {
+      if (block + 2 < blocks) load_keys(key_rows, shared.keys[after]);
+      if (block + 1 < blocks) load_values(value_rows, shared.values[b1]);
+    }
+    auto piece = [&](int n) {
+      if constexpr (!kE4m3) {
+        if (n < kLoads)
+          load_piece(key_rows, k_lane, shared.keys[after], n);
+        else
+          load_piece(value_rows, v_lane, shared.values[b1], n - kLoads);
+      }
+    };
+    auto weigh = [&](auto with_loads, float base) {
+      constexpr int kEvery = kHalves * 16 / (2 * kLoads);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if constexpr (decltype(with_loads)::value)
+            if ((16 * h + i) % kEvery == 0) piece((16 * h + i) / kEvery);
+          s[h][i] = exp2_fast(fmaf(s[h][i], scale.size, -base));
+          sum += s[h][i];
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          p[2 * h + e] = operand(pack_bf16x2(s[h][8 * e], s[h][8 * e + 1]), pack_bf16x2(s[h][8 * e + 2], s[h][8 * e + 3]),
+                                 pack_bf16x2(s[h][8 * e + 4], s[h][8 * e + 5]), pack_bf16x2(s[h][8 * e + 6], s[h][8 * e + 7]));
+      }
+    };
+    if (scores) {
       // Rows of the wave attend different keys of the block, or none of some: bit c
       // of the lane's mask is key 4 half + c of the block.
-      const bool uneven = key + kKeys - 1 > wave_low || key <= oldest_high;
-      uint64_t mask = attended;
-      if (uneven) {
+      if (wave_uneven(key) || attended != ~uint64_t{0}) {
         const int newest = position - key, stale = oldest - key + 1;  // bits above and below them go
+        uint64_t mask = attended;
         mask &= newest < 0 ? 0 : ~uint64_t{0} >> (newest < 63 ? 63 - newest : 0);
         mask &= stale <= 0 ? ~uint64_t{0} : (stale < 64 ? ~uint64_t{0} << stale : 0);
-      }
-      mask >>= 4 * half;
-      uint32_t mask_lo = static_cast<uint32_t>(mask), mask_hi = static_cast<uint32_t>(mask >> 32);
-      auto seen = [&](int b, int i) { return ((b ? mask_hi : mask_lo) >> (8 * (i >> 2) + (i & 3)) & 1u) != 0; };
-      if (uneven || attended != ~uint64_t{0}) {
+        mask >>= 4 * half;
+        const uint32_t mask_lo = static_cast<uint32_t>(mask), mask_hi = static_cast<uint32_t>(mask >> 32);
 #pragma unroll
-        for (int b = 0; b < kHalves; ++b)
+        for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] = seen(b, i) ? s[b][i] : -__builtin_huge_valf();
+          for (int i = 0; i < 16; ++i)
+            s[h][i] = ((h ? mask_hi : mask_lo) >> (8 * (i >> 2) + (i & 3)) & 1u) != 0 ? s[h][i] : -__builtin_huge_valf();
       }
       float most = s[0][0];
 #pragma unroll
-      for (int b = 0; b < kHalves; ++b)
+      for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[b][i]);
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, s[h][i]);
       most = max_across_32(most) * scale.size;
       if (__any(most > top)) {
         const float higher = fmaxf(top, most);
         const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
         top = higher;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sums[i] *= shrink;
+        sum *= shrink;
 #pragma unroll
         for (int t = 0; t < kColumns; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
       }
       const float base = top == -__builtin_huge_valf() ? 0.0f : top;
-      bf16x8 p[2 * kHalves];
+      if (pieces)
+        weigh(std::true_type{}, base);
+      else
+        weigh(std::false_type{}, base);
+    } else if (pieces) {
 #pragma unroll
-      for (int b = 0; b < kHalves; ++b) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[b][i] = exp2_fast(fmaf(s[b][i], scale.size, -base));
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          p[2 * b + e] = operand(pack_bf16x2(s[b][8 * e], s[b][8 * e + 1]), pack_bf16x2(s[b][8 * e + 2], s[b][8 * e + 3]),
-                                 pack_bf16x2(s[b][8 * e + 4], s[b][8 * e + 5]), pack_bf16x2(s[b][8 * e + 6], s[b][8 * e + 7]));
-      }
-      auto value_operand = [&](int t, int step, uint32_t* w) {
-        const uint8_t* at = v + (value_at ^ (64 * t)) + 16 * step * (2 * D);
-        const uint32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * (2 * D));
-        w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
-      };
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int e = 0; e < 2 * kHalves; ++e) {
-        sums = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ones, p[e], sums, 0, 0, 0);
-#pragma unroll
-        for (int t = 0; t < kColumns; ++t) {
-          uint32_t w[4];
-          value_operand(t, e, w);
-          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(operand(w[0], w[1], w[2], w[3]), p[e], o[t], 0, 0, 0);
-        }
-      }
-      if (uneven && infinite == key) add_infinite(key, here);
+      for (int n = 0; n < 2 * kLoads; ++n) piece(n);
     }
-    if (more) store_block(buffer ^ 1);
-    here = page;
-    attended = next_attended;
-    __syncthreads();
+    page1 = page2;
+    attended = attended1, attended1 = attended2;
+    const int last = b0;
+    b0 = b1, b1 = kGroups == 2 ? b2 : last, b2 = last;
+    lds_barrier();
   }
+  if (kGroups == 2 && !second) lds_barrier();  // (as many as the second group)
 
-  const float sum = sums[0];
+  sum = sum_across_32(sum);
   if (!wave_live || wave_row + column > last_row) return;
   if (u.splits > 1) {
     const int64_t at = (static_cast<int64_t>(u.part) * a.kv_heads + head) * kTileRows + 32 * wave + column;
@@ -408,76 +463,38 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
     }
 }
 
-template <int D, bool kE4m3>
-__global__ __launch_bounds__(kPagedThreads, D == 256 ? 1 : 2) void paged_tile_kernel(PagedArgs a) {
+template <int D, bool kE4m3, int kGroups>
+__global__ __launch_bounds__(4 * kGroups * kWave, D == 256 ? 1 : (D == 64 ? 3 : 2)) void paged_tile_kernel(PagedArgs a) {
   __shared__ union Shared {
     __device__ Shared() {}
-    DecodeShared<D, kE4m3> decode;
-    TileShared<D> tile;
+    DecodeShared<D, 4 * kGroups> decode;
+    TileShared<D, kGroups> tile;
   } shared;
   const int unit = static_cast<int>(blockIdx.x) / a.kv_heads, head = static_cast<int>(blockIdx.x) % a.kv_heads;
   if (unit < a.shares) {
-    decode_share<D, kE4m3>(a, unit, head, shared.decode);
+    decode_share<D, kE4m3, 4 * kGroups>(a, unit, head, shared.decode);
   } else if (unit < a.shares + a.tile_units) {
     const PagedUnit u = paged_tile_unit<false>(a, unit - a.shares);
-    if (u.live) tile_unit<D, kE4m3>(a, u, head, shared.tile);
+    if (u.live) tile_unit<D, kE4m3, kGroups>(a, u, head, shared.tile);
   } else {
     paged_zero_rest(a, static_cast<int>(blockIdx.x) - (a.tile_units + a.shares) * a.kv_heads, D);
   }
 }
 
-// Adds the parts of a tile's rows at the weights of their maxima, in the order of
-// their keys; a thread takes four columns of one of 16 rows, eight parts in flight.
+// Adds the parts of a tile's row at the weights of their maxima, in the order of
+// their keys; a thread takes four columns, eight parts in flight.
 template <int D>
-__global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tiles, bool e4m3) {
+__device__ __forceinline__ void join_row(const float* sums, const float2* stats, int64_t at, int64_t step, int parts, int d,
+                                         float value_scale, uint16_t* out) {
   constexpr int kBatch = 8;
-  constexpr int kRowParts = kTileRows / 16;
-  const int r = static_cast<int>(threadIdx.x) / (D / 4), d = 4 * (static_cast<int>(threadIdx.x) % (D / 4));
-  PagedUnit u;
-  int head, token, member;
-  int64_t at, step;
-  const float* sums;
-  const float2* stats;
-  if (static_cast<int>(blockIdx.x) < tiles * a.kv_heads * kRowParts) {
-    const int part = static_cast<int>(blockIdx.x) % (a.kv_heads * kRowParts);
-    head = part % a.kv_heads;
-    u = paged_tile_unit<true>(a, static_cast<int>(blockIdx.x) / (a.kv_heads * kRowParts));
-    if (!u.live) return;
-    const int row = 16 * (part / a.kv_heads) + r, m = u.tile * kTileRows + row;
-    if (m >= u.tokens * a.group) return;
-    token = m / a.group, member = m - token * a.group;
-    at = (static_cast<int64_t>(u.part) * a.kv_heads + head) * kTileRows + row, step = a.kv_heads * kTileRows;
-    sums = a.tile_sums, stats = a.tile_stats;
-  } else {
-    // The tile that the share of workgroup w ends in, where it is the tile's first part.
-    const int group = static_cast<int>(blockIdx.x) - tiles * a.kv_heads * kRowParts;
-    const int w = group / a.kv_heads;
-    head = group % a.kv_heads;
-    PagedShares shares;
-    shares.start(a);
-    const int64_t end = static_cast<int64_t>(w + 1) * shares.each;
-    if (end >= shares.total) return;
-    u = shares.find(a, static_cast<int>(end));
-    if (!u.live || u.from == 0 || u.from > shares.each) return;
-    // (a share that began with the tile ends `each` into it, any other less)
-    const int tile_end = u.from + u.blocks;  // blocks of the tile
-    u.splits = 1 + (tile_end - u.from + shares.each - 1) / shares.each;
-    u.part += w;
-    if (u.part < 0 || u.part > a.single_parts - u.splits) return;
-    token = u.tile / a.slices, member = 16 * (u.tile % a.slices) + r;
-    if (member >= a.group) return;
-    at = (static_cast<int64_t>(u.part) * a.kv_heads + head) * 16 + r, step = a.kv_heads * 16;
-    sums = a.single_sums, stats = a.single_stats;
-  }
-  const float value_scale = e4m3 && a.v_scales != nullptr ? a.v_scales[head] : 1.0f;
   float highest = -__builtin_huge_valf(), total = 0.0f;
   floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < u.splits; s += kBatch) {
+  for (int s = 0; s < parts; s += kBatch) {
     float2 stat[kBatch];
     floatx4 w[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int64_t from = at + min(s + b, u.splits - 1) * step;
+      const int64_t from = at + min(s + b, parts - 1) * step;
       stat[b] = stats[from];
       w[b] = *reinterpret_cast<const floatx4*>(sums + from * D + d);
     }
@@ -491,7 +508,7 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
     for (int k = 0; k < 4; ++k) v[k] *= shrink;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      if (s + b >= u.splits) break;
+      if (s + b >= parts) break;
       const float weight = exp2_fast(stat[b].x - base);
       total += weight * stat[b].y;
 #pragma unroll
@@ -502,21 +519,67 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
   const float inverse = total == 0.0f ? 0.0f : value_scale / total;
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = total == 0.0f ? 0.0f : v[k] * inverse;
-  store_row4(a.out + static_cast<int64_t>(u.first_row + token) * a.out_row + (head * a.group + member) * a.out_head + d, v);
+  store_row4(out + d, v);
 }
 
-// How a call is cut, as far as the host knows its sizes.
-constexpr int kCus = 256;
+// Workgroups 0 .. tiles * kv heads * parts: 16 rows of every `tiles`-th tile that is
+// split; those behind them: the tile that a share of single tokens' blocks ends in.
+template <int D>
+__global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tiles, bool e4m3) {
+  const int row_parts = a.tile_rows / 16;
+  const int r = static_cast<int>(threadIdx.x) / (D / 4), d = 4 * (static_cast<int>(threadIdx.x) % (D / 4));
+  const int of_tiles = tiles * a.kv_heads * row_parts;
+  const bool single = static_cast<int>(blockIdx.x) >= of_tiles;
+  const int index = static_cast<int>(blockIdx.x) - (single ? of_tiles : 0);
+  const int head = index % a.kv_heads;
+  const float value_scale = e4m3 && a.v_scales != nullptr ? a.v_scales[head] : 1.0f;
+  auto out_of = [&](const PagedUnit& u, int token, int member) {
+    return a.out + static_cast<int64_t>(u.first_row + token) * a.out_row + (head * a.group + member) * a.out_head;
+  };
+  if (single) {
+    // Of the shares that end in a tile, the one that does so first.
+    const int w = index / a.kv_heads;
+    PagedShares shares;
+    shares.start(a);
+    const int64_t end = static_cast<int64_t>(w + 1) * shares.each;
+    if (end >= shares.total) return;
+    const PagedUnit u = shares.find(a, static_cast<int>(end));
+    if (!u.live || u.from == 0 || u.from > shares.each) return;
+    const int parts = 1 + (u.blocks + shares.each - 1) / shares.each, part = u.part + w;
+    const int member = 16 * (u.tile % a.slices) + r;
+    if (part < 0 || part > a.single_parts - parts || member >= a.group) return;
+    join_row<D>(a.single_sums, a.single_stats, (static_cast<int64_t>(part) * a.kv_heads + head) * 16 + r, a.kv_heads * 16,
+                parts, d, value_scale, out_of(u, u.tile / a.slices, member));
+    return;
+  }
+  const int row = 16 * (index / a.kv_heads % row_parts) + r;
+  for (int t = index / (a.kv_heads * row_parts);; t += tiles) {
+    const PagedUnit u = paged_tile_unit<true>(a, t);
+    if (!u.live) return;
+    const int m = u.tile * a.tile_rows + row;
+    if (m >= u.tokens * a.group) continue;
+    const int token = m / a.group;
+    join_row<D>(a.tile_sums, a.tile_stats, (static_cast<int64_t>(u.part) * a.kv_heads + head) * a.tile_rows + row,
+                a.kv_heads * a.tile_rows, u.splits, d, value_scale, out_of(u, token, m - token * a.group));
+  }
+}
 
-#ifdef D3_TUNE
-int tuned(const char* name, int v) { const char* e = getenv(name); return e ? atoi(e) : v; }
-#else
-constexpr int tuned(const char*, int v) { return v; }
-#endif
+// How a call is cut, as far as the host knows its sizes.  Measured (us):
+//   kAlone: a token's 333 keys by one workgroup a kv head 7.8, cut in three and joined 10.4;
+//   workgroups a CU for single tokens: 52 x 2048 keys of 256 columns 39.0 with one, 40.2
+//   with two, 47.5 with three; 16 x 32768 e4m3 keys 193, 140, 141 (four: 155); a mixed
+//   step, whose tiles take the other place, 37.9 with one, 38.3 with two;
+//   kLeastShare: those 52 tokens 40.2 with two blocks or four, 48 with eight;
+//   kTwoGroupRows: a prompt of 8192 (32768 packed rows) 300 with tiles of two groups, 334
+//   with one; eight of 1000 (4000) 102 and 104; sixteen of 512 (2048) 85 and 80.
+constexpr int kCus = 256;
+constexpr int kAlone = 512;          // keys that are not worth a second launch
+constexpr int kLeastShare = 4;       // fewest blocks of a share
+constexpr int kTwoGroupRows = 4096;  // packed rows of the longest sequence
 
 struct PagedPlan {
   bool all_single, split_tiles, split_shares;
-  int slices, tile_tokens, share_shift, shares, least, target, least_split;
+  int slices, tile_rows, tile_tokens, share_shift, shares, least, target;
   int64_t tiles, tile_units, single_parts, tile_parts;
 };
 
@@ -527,28 +590,31 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
   const int64_t some = sequences < rows ? sequences : rows;
   p.all_single = max_length <= 1;
   p.slices = static_cast<int>((group + 15) / 16);
-  p.tile_tokens = p.all_single ? 1 : static_cast<int>(kTileRows / group + 2);
+  // Tiles of two groups where they alone fill the card.
+  const bool two_groups = c->head_dim == 128 && rows * q_heads >= int64_t{kCus} * 2 * kGroupRows &&
+                          max_length * group >= kTwoGroupRows;
+  p.tile_rows = two_groups ? 2 * kGroupRows : kGroupRows;
+  p.tile_tokens = p.all_single ? 1 : static_cast<int>(p.tile_rows / group + 2);
   // Single tokens: blocks of 64 keys; one block a tile where no slot holds more keys
   // than are worth a second launch; larger where all of them could be 2^30 and more.
   const int64_t single_tiles = (p.all_single ? rows : some) * p.slices;
   p.share_shift = 6;
-  while (capacity <= tuned("D3_ALONE", 512) && capacity > 1 << p.share_shift) ++p.share_shift;
+  while (capacity <= kAlone && capacity > 1 << p.share_shift) ++p.share_shift;
   while ((((capacity - 1) >> p.share_shift) + 1) * single_tiles >= int64_t{1} << 30) ++p.share_shift;
   const int64_t blocks = ((capacity - 1) >> p.share_shift) + 1;
-  const int resident = (p.all_single ? tuned("D3_PER_CU", c->head_dim == 64 ? 4 : 2) : tuned("D3_MIXED", 1)) * kCus / c->kv_heads;
-  p.least = blocks > 1 ? tuned("D3_LEAST", 4) : 1;
+  const int resident = (!p.all_single ? 1 : (c->head_dim == 64 ? 4 : 2)) * kCus / c->kv_heads;
+  p.least = blocks > 1 ? kLeastShare : 1;
   // No more workgroups than the blocks can give work to.
   const int64_t useful = (single_tiles * blocks + p.least - 1) / p.least;
   p.shares = sequences == 0 ? 0 : static_cast<int>(useful < resident ? useful : (resident > 0 ? resident : 1));
   p.split_shares = p.shares > 1 && blocks > 1;
   p.single_parts = p.split_shares ? p.shares + single_tiles : 0;
   // Tiles of more rows.
-  p.target = tuned("D3_TARGET", 2) * kCus / c->kv_heads;
+  p.target = (two_groups ? 1 : 2) * kCus / c->kv_heads;
   if (p.target < 1) p.target = 1;
-  p.least_split = tuned("D3_SPLIT", 8);
   if (!p.all_single && sequences > 0) {
-    p.tiles = rows * group / kTileRows + some;
-    p.split_tiles = (capacity + kKeyBlock - 1) / kKeyBlock > p.least_split;
+    p.tiles = rows * group / p.tile_rows + some;
+    p.split_tiles = (capacity + kKeyBlock - 1) / kKeyBlock > kLeastSplit;
     p.tile_units = p.tiles + (p.split_tiles ? p.target : 0);
     p.tile_parts = p.split_tiles ? 2 * static_cast<int64_t>(p.target) : 0;
   }
@@ -556,7 +622,7 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
 }
 
 int64_t workspace_rows(const PagedPlan& p, const d3_paged_cache* c) {
-  return (p.single_parts * 16 + p.tile_parts * kTileRows) * c->kv_heads;
+  return (p.single_parts * 16 + p.tile_parts * p.tile_rows) * c->kv_heads;
 }
 
 bool attention_suited(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int32_t sequences) {
@@ -566,13 +632,17 @@ bool attention_suited(const d3_paged_cache* c, int64_t rows, int32_t q_heads, in
 
 void launch_paged_tiles(const PagedArgs& a, int head_dim, bool e4m3, bool zero_rest, hipStream_t stream) {
   const unsigned workgroups = paged_workgroups(a, zero_rest);
-  auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(kPagedThreads), 0, stream, a); };
+  auto run = [&](auto kernel, int groups) {
+    hipLaunchKernelGGL(kernel, dim3(workgroups), dim3(4 * groups * kWave), 0, stream, a);
+  };
   if (head_dim == 64)
-    e4m3 ? run(paged_tile_kernel<64, true>) : run(paged_tile_kernel<64, false>);
-  else if (head_dim == 128)
-    e4m3 ? run(paged_tile_kernel<128, true>) : run(paged_tile_kernel<128, false>);
+    e4m3 ? run(paged_tile_kernel<64, true, 1>, 1) : run(paged_tile_kernel<64, false, 1>, 1);
+  else if (head_dim == 256)
+    e4m3 ? run(paged_tile_kernel<256, true, 1>, 1) : run(paged_tile_kernel<256, false, 1>, 1);
+  else if (a.tile_rows == kGroupRows)
+    e4m3 ? run(paged_tile_kernel<128, true, 1>, 1) : run(paged_tile_kernel<128, false, 1>, 1);
   else
-    e4m3 ? run(paged_tile_kernel<256, true>) : run(paged_tile_kernel<256, false>);
+    e4m3 ? run(paged_tile_kernel<128, true, 2>, 2) : run(paged_tile_kernel<128, false, 2>, 2);
 }
 
 }  // namespace
@@ -625,9 +695,9 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   a.q = q, a.q_row = q_row_stride, a.q_head = q_head_stride;
   a.out = out, a.out_row = out_row_stride, a.out_head = out_head_stride;
   a.keys = static_cast<const uint8_t*>(cache->keys), a.values = static_cast<const uint8_t*>(cache->values);
-  a.k_page = cache->key_page_stride * size, a.k_token = cache->key_token_stride * size;
+  a.k_page = static_cast<uint32_t>(cache->key_page_stride * size), a.k_token = static_cast<uint32_t>(cache->key_token_stride * size);
   a.k_head = cache->key_head_stride * size;
-  a.v_page = cache->value_page_stride * size, a.v_token = cache->value_token_stride * size;
+  a.v_page = static_cast<uint32_t>(cache->value_page_stride * size), a.v_token = static_cast<uint32_t>(cache->value_token_stride * size);
   a.v_head = cache->value_head_stride * size;
   a.page_table = cache->page_table, a.table_stride = cache->table_stride;
   a.pages = static_cast<uint32_t>(cache->pages), a.slots = cache->slots;
@@ -639,11 +709,11 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   a.lengths = lengths, a.lengths_64 = lengths_dtype == D3_DTYPE_I64;
   a.sequences = sequences, a.rows = static_cast<int>(rows);
   a.q_heads = q_heads, a.kv_heads = cache->kv_heads, a.group = q_heads / cache->kv_heads;
-  a.slices = p.slices, a.all_single = p.all_single, a.tile_tokens = p.tile_tokens;
+  a.slices = p.slices, a.all_single = p.all_single, a.tile_rows = p.tile_rows, a.tile_tokens = p.tile_tokens;
   a.scale = scale * 1.4426950408889634f;
   a.window = static_cast<int>(window < 0 ? 0 : (window < 0x7fffffff ? window : 0x7fffffff));
   a.share_shift = p.share_shift, a.shares = p.shares, a.least = p.least;
-  a.target = p.target, a.least_split = p.split_tiles ? p.least_split : 1 << 30;
+  a.target = p.target, a.splitting = p.split_tiles;
   a.tile_units = static_cast<int>(p.tile_units);
   a.single_parts = static_cast<int>(p.single_parts), a.tile_parts = static_cast<int>(p.tile_parts);
   const int64_t single_rows = p.single_parts * 16 * cache->kv_heads;
@@ -659,9 +729,10 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
     const hipError_t status = hipGetLastError();
     if (status != hipSuccess)
       return set_error(D3_ERR_HIP, "paged_attention launch failed: %s", hipGetErrorString(status));
-    const int tiles = p.split_tiles ? static_cast<int>(p.tiles < p.target ? p.tiles : p.target) : 0;
+    const int few = p.target < 4 ? 1 : p.target / 4;  // (of the tiles, up to p.target are split)
+    const int tiles = p.split_tiles ? static_cast<int>(p.tiles < few ? p.tiles : few) : 0;
     const int ends = p.split_shares ? p.shares - 1 : 0;
-    const dim3 grid(static_cast<unsigned>((tiles * (kTileRows / 16) + ends) * cache->kv_heads)), block(4 * cache->head_dim);
+    const dim3 grid(static_cast<unsigned>((tiles * (p.tile_rows / 16) + ends) * cache->kv_heads)), block(4 * cache->head_dim);
     auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, as_stream(stream), a, tiles, e4m3); };
     if (cache->head_dim == 64)
       run(paged_join_kernel<64>);

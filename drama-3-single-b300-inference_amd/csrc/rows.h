@@ -51,6 +51,9 @@ inline int check_paged_cache(const char* name, const d3_paged_cache* c) {
   D3_SUPPORTED(c->pages < (int64_t{1} << 31), "%s: more than 2^31 pages", name);
   D3_SUPPORTED(static_cast<int64_t>(c->max_pages) * c->page_size <= (int64_t{1} << 30),
                "%s: slots of more than 2^30 tokens", name);
+  for (const int64_t stride : {c->key_page_stride, c->key_head_stride, c->key_token_stride, c->value_page_stride,
+                               c->value_head_stride, c->value_token_stride})
+    D3_SUPPORTED(stride >= 0 && stride < (int64_t{1} << 31), "%s: a stride of 2^31 elements and more", name);
   D3_REQUIRE(c->keys && c->values && c->page_table, "%s: null cache pointer", name);
   const int64_t part = c->dtype == D3_DTYPE_BF16 ? 8 : 16;
   D3_REQUIRE(aligned_to(c->keys, 16) && aligned_to(c->values, 16), "%s: cache alignment", name);

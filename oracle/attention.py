@@ -112,7 +112,8 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     and the sizes that bound them."""
     group = q_heads // kv_heads
     all_single = max_length <= 1
-    slices, tile_rows, count = -(-group // 16), 128, len(lengths)
+    slices, count = -(-group // 16), len(lengths)
+    tile_rows = 256 if dim == 128 and rows * q_heads >= 512 * 128 and max_length * group >= 4096 else 128
     tile_tokens = 1 if all_single else tile_rows // group + 2
     some = min(count, rows)
     single_tiles = (rows if all_single else some) * slices
@@ -122,7 +123,7 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     most_blocks = ((capacity - 1) >> shift) + 1
     least = LEAST if most_blocks > 1 else 1
     shares = min(-(-single_tiles * most_blocks // least), max(1, (4 if dim == 64 else 2) * CUS // kv_heads)) if count else 0
-    target = max(1, 2 * CUS // kv_heads)
+    target = max(1, (1 if tile_rows == 256 else 2) * CUS // kv_heads)
     tiles_most = 0 if all_single else rows * group // tile_rows + some
     split_tiles = not all_single and -(-capacity // BLOCK) > LEAST_SPLIT
     bounds = {"shares": shares, "single_parts": shares + single_tiles if shares > 1 and most_blocks > 1 else 0,
@@ -144,7 +145,8 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
             total += tiles * blocks
         else:
             work = np.float32(work + np.float32(tiles) * np.float32(blocks))
-    chunk = max(LEAST_SPLIT if split_tiles else 1 << 30, math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target)))
+    even = math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target))
+    chunk = max(even, min(max(4 * even, LEAST_SPLIT), 2 * LEAST_SPLIT) if split_tiles else 1 << 30)
     each = max(least, -(-total // max(shares, 1)))
     units, part, ordinal, at = [], 0, 0, 0
     for i, (tokens, length, single, tiles, blocks) in enumerate(sequences):

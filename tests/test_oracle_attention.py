@@ -97,7 +97,7 @@ def test_cut_covers_every_row_and_key_within_its_bounds(seed):
     """The unit list that the kernels derive: as many as the grid holds, partials
     within the workspace, every tile's keys partitioned by its splits."""
     rng = np.random.default_rng(seed)
-    kv_heads = int(rng.choice([1, 2, 4, 8, 16]))
+    kv_heads = int(rng.choice([1, 2, 4, 8, 16, 96]))
     q_heads = kv_heads * int(rng.choice([1, 2, 3, 5, 8, 16, 17, 24, 40]))
     count = int(rng.integers(1, 70))
     decode = seed % 2 == 0
@@ -110,7 +110,7 @@ def test_cut_covers_every_row_and_key_within_its_bounds(seed):
     lengths = tokens + (np.exp(rng.uniform(0, np.log(capacity + 1), count)) - 2).astype(int)
     window = int(rng.choice([0, 0, 1, 100, 1000]))
     group = q_heads // kv_heads
-    dim = int(rng.choice([64, 128]))
+    dim = int(rng.choice([64, 128, 256]))
     units, most = oa.cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, 1 if decode else int(tokens.max()), dim, window)
     tiles = [u for u in units if not u[2]]
     assert len(tiles) <= most["tile_units"] and -(-most["total"] // most["each"]) <= most["shares"]
