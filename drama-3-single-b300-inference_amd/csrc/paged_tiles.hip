@@ -672,6 +672,7 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   D3_REQUIRE(rows >= 0 && sequences >= 0, "paged_attention: shape");
   D3_REQUIRE(q_heads > 0 && q_heads % cache->kv_heads == 0, "paged_attention: %d query heads, %d kv heads", q_heads,
              cache->kv_heads);
+  D3_REQUIRE(__builtin_isfinite(scale), "paged_attention: scale must be finite");
   D3_REQUIRE((sequence_slots_dtype == D3_DTYPE_I32 || sequence_slots_dtype == D3_DTYPE_I64) &&
                  (lengths_dtype == D3_DTYPE_I32 || lengths_dtype == D3_DTYPE_I64),
              "paged_attention: slots and lengths must be int32 or int64");

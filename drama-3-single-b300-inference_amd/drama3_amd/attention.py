@@ -23,6 +23,7 @@ workspace.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from dataclasses import dataclass, field
 
@@ -30,13 +31,14 @@ import torch
 
 from . import _lib
 from ._lib import ptr
-from .mxfp4 import _MOST, _call, _entry, _same_device
+from .mxfp4 import _MOST, _entry, _raw_stream, _same_device
 from .packed_prefill import PackedLayout
 from .pipeline import require_cuda
 
 HEAD_DIMS = (64, 128, 256)  # of paged_attention
 SCALINGS = ("none", "linear", "base", "bands")
 _FLOAT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float32: _lib.DTYPE_F32}
+_ROWS = {torch.bfloat16: _lib.DTYPE_BF16}
 _CACHE = {torch.bfloat16: _lib.DTYPE_BF16, torch.float8_e4m3fn: _lib.DTYPE_E4M3}
 _INT = {torch.int32: _lib.DTYPE_I32, torch.int64: _lib.DTYPE_I64}
 
@@ -55,6 +57,7 @@ class Rope:
     interleaved: bool = False
     magnitude: float = 1.0
     _struct: _lib.RopeStruct = field(init=False, repr=False, compare=False)
+    _ref: object = field(init=False, repr=False, compare=False)
 
     def __post_init__(self):
         require_cuda(self.turns)
@@ -64,6 +67,7 @@ class Rope:
             raise ValueError("turns must be contiguous [rotary_dim / 2], at most 512")
         object.__setattr__(self, "_struct", _lib.RopeStruct(
             ptr(self.turns), 2 * len(self.turns), int(self.interleaved), self.magnitude))
+        object.__setattr__(self, "_ref", ctypes.byref(self._struct))
 
     @property
     def rotary_dim(self) -> int:
@@ -116,22 +120,62 @@ def prepare_rope(rotary_dim: int, base: float = 10000.0, interleaved: bool = Fal
     return Rope(turns, interleaved, magnitude)
 
 
-def _check_heads(x: torch.Tensor, name: str, dtypes=(torch.bfloat16,)) -> None:
-    require_cuda(x)
-    if x.dim() != 3 or 0 in x.shape[1:] or (x.shape[2] > 1 and x.stride(2) != 1):
+# What a call costs the host counts where its rows are few: each tensor's shape,
+# strides and device number are asked for once (a torch.device costs 0.2 us, its
+# number 0.05).
+def _heads(x: torch.Tensor, name: str, dtypes=_ROWS):
+    """(rows, heads, head_dim, row stride, head stride, device number) of [T, heads, head_dim]."""
+    index = x.get_device()
+    if index < 0:
+        require_cuda(x)
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [T, heads, head_dim] with unit column stride")
+    rows, heads, dim = x.shape
+    row, head, unit = x.stride()
+    if not heads or not dim or (unit != 1 and dim > 1):
         raise ValueError(f"{name} must be [T, heads, head_dim] with unit column stride")
     if x.dtype not in dtypes:
         raise TypeError(f"{name} must be " + " or ".join(str(d).removeprefix("torch.") for d in dtypes))
-    if max(x.shape[1:]) > _MOST:
+    if heads > _MOST or dim > _MOST:
         raise ValueError(f"{name}: sizes must be below 2^31")
+    return rows, heads, dim, row, head, index
 
 
-def _check_index(t: torch.Tensor, name: str, count: int) -> None:
-    require_cuda(t)
-    if t.dtype not in _INT:
+def _indices(t: torch.Tensor, name: str, count: int, x: torch.Tensor, index: int) -> int:
+    """The type code of int32 or int64 [count] on the rows' device."""
+    code = _INT.get(t.dtype)
+    if code is None:
         raise TypeError(f"{name} must be int32 or int64")
-    if t.shape != (count,) or (count > 1 and t.stride(0) != 1):
+    if t.dim() != 1 or t.shape[0] != count or (count > 1 and t.stride(0) != 1):
         raise ValueError(f"{name} must be contiguous [{count}]")
+    if t.get_device() != index:
+        _elsewhere(x, t, name)
+    return code
+
+
+def _elsewhere(x: torch.Tensor, t: torch.Tensor, name: str) -> None:
+    require_cuda(t)
+    _same_device(x, t, name)
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """``mxfp4._call`` by the device's number."""
+    if index == torch.cuda.current_device():
+        status = _entry(name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = _entry(name)(*args, _raw_stream(index))
+    if status:
+        _lib.fail(status)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(sizes: tuple, rows: int, heads: int, count: int, longest: int) -> int:
+    """Of ``paged_attention``, for a cache of the given sizes (arithmetic alone)."""
+    dtype, kv_heads, head_dim, page_size, max_pages = sizes
+    part = 1 << 20  # (any address and stride: they have no part in it)
+    struct = _lib.PagedCacheStruct(part, part, dtype, kv_heads, head_dim, page_size, 1, 0, 0, 0, 0, 0, 0, part, 0, 1, max_pages)
+    return _entry("d3_paged_attention_workspace")(ctypes.byref(struct), rows, heads, count, longest)
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -172,17 +216,18 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, out: torch.
     its rows' ``positions`` (int32 or int64 [T], any value): the first
     ``rope.rotary_dim`` columns of every head, the others stay.  Angles are taken
     in 64 bits, one rounding.  ``out`` (the rows' shape and type) may be ``x``."""
-    _check_heads(x, "x", _FLOAT)
-    rows, heads, dim = x.shape
-    _check_index(positions, "positions", rows)
-    _same_device(x, positions, "positions")
-    _same_device(x, rope.turns, "rope")
+    rows, heads, dim, row, head, index = _heads(x, "x", _FLOAT)
+    code = _indices(positions, "positions", rows, x, index)
+    if rope.turns.get_device() != index:
+        _elsewhere(x, rope.turns, "rope")
     if out is None:
         out = torch.empty(rows, heads, dim, dtype=x.dtype, device=x.device)
+        out_row, out_head = heads * dim, dim
     else:
         _check_out(out, x, "out", True)
-    _call(x.device, "d3_rope_rows", ptr(x), _FLOAT[x.dtype], x.stride(0), x.stride(1), rows, heads, dim,
-          ptr(positions), _INT[positions.dtype], ctypes.byref(rope._struct), ptr(out), out.stride(0), out.stride(1))
+        out_row, out_head, _ = out.stride()
+    _launch(index, "d3_rope_rows", x.data_ptr(), _FLOAT[x.dtype], row, head, rows, heads, dim, positions.data_ptr(), code,
+            rope._ref, out.data_ptr(), out_row, out_head)
     return out
 
 
@@ -211,6 +256,8 @@ class PagedCache:
     k_scale: torch.Tensor | None = None
     v_scale: torch.Tensor | None = None
     _struct: _lib.PagedCacheStruct = field(init=False, repr=False, compare=False)
+    _ref: object = field(init=False, repr=False, compare=False)
+    _sizes: tuple = field(init=False, repr=False, compare=False)
 
     def __post_init__(self):
         """The kernels take the sizes as given: they have to be the tensors'."""
@@ -259,6 +306,8 @@ class PagedCache:
             ptr(keys), ptr(values), _CACHE[keys.dtype], kv_heads, head_dim, page_size, pages, kp, kh, kt, vp, vh, vt,
             ptr(table), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[0], table.shape[1],
             ptr(self.k_scale), ptr(self.v_scale)))
+        object.__setattr__(self, "_ref", ctypes.byref(self._struct))
+        object.__setattr__(self, "_sizes", (_CACHE[keys.dtype], kv_heads, head_dim, page_size, table.shape[1]))
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, slots: int, max_pages: int,
@@ -286,38 +335,44 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions:
     Rows of a slot outside [0, slots), of a negative position or one past the
     table, and of an unmapped page write nothing; their queries are rotated.  No
     two rows may name the same token: which of them it would hold is not said."""
-    _check_heads(k, "k")
-    _check_heads(v, "v")
-    rows = k.shape[0]
-    _, kv_heads, _, head_dim = cache.keys.shape
-    if k.shape != (rows, kv_heads, head_dim) or v.shape != k.shape:
-        raise ValueError(f"k and v must be [T, {kv_heads}, {head_dim}], as the cache's heads")
-    _check_index(positions, "positions", rows)
-    _check_index(row_slots, "row_slots", rows)
-    for t, name in ((v, "v"), (positions, "positions"), (row_slots, "row_slots"), (cache.keys, "cache")):
-        _same_device(k, t, name)
+    rows, kv_heads, dim, k_row, k_head, index = _heads(k, "k")
+    v_rows, v_heads, v_dim, v_row, v_head, v_index = _heads(v, "v")
+    _, cache_heads, head_dim, _, _ = cache._sizes
+    if kv_heads != cache_heads or dim != head_dim or (v_rows, v_heads, v_dim) != (rows, kv_heads, dim):
+        raise ValueError(f"k and v must be [T, {cache_heads}, {head_dim}], as the cache's heads")
+    if v_index != index:
+        _elsewhere(k, v, "v")
+    if cache.keys.get_device() != index:
+        _elsewhere(k, cache.keys, "cache")
+    position_code = _indices(positions, "positions", rows, k, index)
+    slot_code = _indices(row_slots, "row_slots", rows, k, index)
+    rope_ref = None
     if rope is not None:
-        _same_device(k, rope.turns, "rope")
+        rope_ref = rope._ref
+        if rope.turns.get_device() != index:
+            _elsewhere(k, rope.turns, "rope")
         if rope.rotary_dim > head_dim:
             raise ValueError(f"rotary width {rope.rotary_dim} above the head's {head_dim}")
     q_args = (None, 0, 0, 0, None, 0, 0)
     if q is not None:
-        _check_heads(q, "q")
-        if q.shape[0] != rows or q.shape[2] != head_dim:
+        q_rows, heads, q_dim, q_row, q_head, q_index = _heads(q, "q")
+        if q_rows != rows or q_dim != head_dim:
             raise ValueError(f"q must be [{rows}, heads, {head_dim}]")
-        _same_device(k, q, "q")
+        if q_index != index:
+            _elsewhere(k, q, "q")
         if out is None:
-            out = torch.empty(rows, q.shape[1], head_dim, dtype=q.dtype, device=q.device)
+            out = torch.empty(rows, heads, head_dim, dtype=q.dtype, device=q.device)
+            out_row, out_head = heads * head_dim, head_dim
         else:
             _check_out(out, q, "out", True)
             if out.data_ptr() != q.data_ptr() and not (_apart(out, k) and _apart(out, v)):
                 raise ValueError("out must not overlap k or v")
-        q_args = (ptr(q), q.stride(0), q.stride(1), q.shape[1], ptr(out), out.stride(0), out.stride(1))
+            out_row, out_head, _ = out.stride()
+        q_args = (q.data_ptr(), q_row, q_head, heads, out.data_ptr(), out_row, out_head)
     elif out is not None:
         raise ValueError("out goes with q")
-    _call(k.device, "d3_paged_append", ctypes.byref(cache._struct), ptr(k), k.stride(0), k.stride(1), ptr(v),
-          v.stride(0), v.stride(1), rows, ptr(positions), _INT[positions.dtype], ptr(row_slots),
-          _INT[row_slots.dtype], None if rope is None else ctypes.byref(rope._struct), *q_args)
+    _launch(index, "d3_paged_append", cache._ref, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows,
+            positions.data_ptr(), position_code, row_slots.data_ptr(), slot_code, rope_ref, *q_args)
     return out
 
 
@@ -339,35 +394,42 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, layout: PackedLayout, le
     left as they were in a given ``out`` (apart from ``q``).  ``layout.max_length`` is the
     longest n_i: 1 chooses the kernel for single tokens; any value computes all rows.
     head_dim is 64, 128 or 256."""
-    _check_heads(q, "q")
-    rows, heads, dim = q.shape
+    rows, heads, dim, q_row, q_head, index = _heads(q, "q")
     boundaries, slots = layout.boundaries, layout.sequence_slots
-    require_cuda(boundaries)
     if boundaries.dtype != torch.int32:
         raise TypeError("boundaries must be int32")
-    if boundaries.dim() != 1 or len(boundaries) < 1 or not boundaries.is_contiguous():
+    if boundaries.dim() != 1 or not boundaries.shape[0] or (boundaries.shape[0] > 1 and boundaries.stride(0) != 1):
         raise ValueError("boundaries must be contiguous [n + 1]")
+    if boundaries.get_device() != index:
+        _elsewhere(q, boundaries, "boundaries")
     count = boundaries.shape[0] - 1
-    _check_index(slots, "sequence_slots", count)
-    _check_index(lengths, "lengths", count)
-    kv_heads = cache.keys.shape[1]
-    if dim != cache.keys.shape[3] or heads % kv_heads:
-        raise ValueError(f"q must be [T, heads, {cache.keys.shape[3]}], heads a multiple of {kv_heads}")
-    for t, name in ((boundaries, "boundaries"), (slots, "sequence_slots"), (lengths, "lengths"), (cache.keys, "cache")):
-        _same_device(q, t, name)
+    slot_code = _indices(slots, "sequence_slots", count, q, index)
+    length_code = _indices(lengths, "lengths", count, q, index)
+    sizes = cache._sizes
+    if dim != sizes[2] or heads % sizes[1]:
+        raise ValueError(f"q must be [T, heads, {sizes[2]}], heads a multiple of {sizes[1]}")
+    if cache.keys.get_device() != index:
+        _elsewhere(q, cache.keys, "cache")
     if window is not None and window < 1:
         raise ValueError(f"window {window} must be positive (or None)")
+    if scale is None:
+        scale = dim ** -0.5
+    elif not math.isfinite(scale):
+        raise ValueError(f"scale {scale} must be finite")
     zero_rest = out is None
-    if out is None:
+    if zero_rest:
         out = torch.empty(rows, heads, dim, dtype=q.dtype, device=q.device)
+        out_row, out_head = heads * dim, dim
     else:
         _check_out(out, q, "out", False)
+        out_row, out_head, _ = out.stride()
     longest = max(0, min(int(layout.max_length), _MOST))
-    struct = ctypes.byref(cache._struct)
-    size = _entry("d3_paged_attention_workspace")(struct, rows, heads, count, longest)
-    workspace = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
-    _call(q.device, "d3_paged_attention", struct, ptr(q), q.stride(0), q.stride(1), rows, heads, ptr(boundaries),
-          ptr(slots), _INT[slots.dtype], ptr(lengths), _INT[lengths.dtype], count, longest,
-          dim ** -0.5 if scale is None else float(scale), 0 if window is None else min(int(window), 1 << 62), ptr(out),
-          out.stride(0), out.stride(1), zero_rest, ptr(workspace), max(size, 0))
+    size = _workspace_bytes(sizes, rows, heads, count, longest)
+    workspace, at = None, None
+    if size > 0:
+        workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+        at = workspace.data_ptr()
+    _launch(index, "d3_paged_attention", cache._ref, q.data_ptr(), q_row, q_head, rows, heads, boundaries.data_ptr(),
+            slots.data_ptr(), slot_code, lengths.data_ptr(), length_code, count, longest, scale,
+            0 if window is None else min(int(window), 1 << 62), out.data_ptr(), out_row, out_head, zero_rest, at, max(size, 0))
     return out
