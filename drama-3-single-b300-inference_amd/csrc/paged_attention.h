@@ -173,15 +173,23 @@ struct PagedShares {
   }
   // The tile that holds block `at` < total, of those from the walk's place on; u.from
   // is the block's place in it, u.blocks what it has from there, u.part its number.
+  // kTiles: the tile with number `at`; u.from is its first block.
+  template <bool kTiles = false>
   __device__ PagedUnit find(const PagedArgs& a, int at) {
     PagedUnit u = {};
     for (;;) {
-      const uint64_t here = __ballot(at < to);
+      const uint64_t here = __ballot(at < (kTiles ? tiles_to : to));
       if (here != 0) {
         const int lane = __builtin_ctzll(here);
         walk.take(lane, u);
         const int blocks = __builtin_amdgcn_readlane(walk.mine.blocks, lane), tiles = __builtin_amdgcn_readlane(walk.mine.tiles, lane);
-        const uint32_t rest = static_cast<uint32_t>(at - (__builtin_amdgcn_readlane(to, lane) - blocks * tiles));
+        const int first = __builtin_amdgcn_readlane(to, lane) - blocks * tiles;
+        if constexpr (kTiles) {
+          u.tile = at - (__builtin_amdgcn_readlane(tiles_to, lane) - tiles);
+          u.from = first + u.tile * blocks, u.blocks = blocks, u.part = at;
+          return u;
+        }
+        const uint32_t rest = static_cast<uint32_t>(at - first);
         u.tile = static_cast<int>(rest / static_cast<uint32_t>(blocks));
         u.from = static_cast<int>(rest) - u.tile * blocks;
         u.blocks = blocks - u.from;

@@ -337,7 +337,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[n % kAhead], p[e], o[t], 0, 0, 0);
         if (n + kAhead < kValueProducts) w[n % kAhead] = value_fragment(n + kAhead);
       }
-      if (wave_uneven(key - kKeys) && shared.infinite[b2] == key - kKeys) add_infinite(key - kKeys);
+      if (tile_uneven(key - kKeys) && shared.infinite[b2] == key - kKeys) add_infinite(key - kKeys);
     }
     __builtin_amdgcn_s_setprio(0);
     if (block >= blocks) break;
@@ -481,75 +481,114 @@ __global__ __launch_bounds__(4 * kGroups * kWave, D == 256 ? 1 : (D == 64 ? 3 : 
   }
 }
 
-// Adds the parts of a tile's row at the weights of their maxima, in the order of
-// their keys; a thread takes four columns, eight parts in flight.
-template <int D>
-__device__ __forceinline__ void join_row(const float* sums, const float2* stats, int64_t at, int64_t step, int parts, int d,
-                                         float value_scale, uint16_t* out) {
-  constexpr int kBatch = 8;
-  float highest = -__builtin_huge_valf(), total = 0.0f;
-  floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < parts; s += kBatch) {
-    float2 stat[kBatch];
-    floatx4 w[kBatch];
+// A row's parts, added at the weights of their maxima: four columns of a thread.
+struct Joined {
+  float highest, total;
+  floatx4 sum;
+  __device__ void add(float top, float weights, const floatx4& part, float base) {
+    const float weight = exp2_fast(top - base);
+    total += weight * weights;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int64_t from = at + min(s + b, parts - 1) * step;
-      stat[b] = stats[from];
-      w[b] = *reinterpret_cast<const floatx4*>(sums + from * D + d);
-    }
-    float higher = highest;
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) higher = fmaxf(higher, stat[b].x);
+    for (int k = 0; k < 4; ++k) sum[k] = fmaf(weight, part[k], sum[k]);
+  }
+  // Before parts of a maximum `higher`; what their weights are powers of two above.
+  __device__ float raise(float higher) {
     const float base = higher == -__builtin_huge_valf() ? 0.0f : higher;
     const float shrink = highest == higher ? 1.0f : exp2_fast(highest - base);
     total *= shrink;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] *= shrink;
+    for (int k = 0; k < 4; ++k) sum[k] *= shrink;
+    highest = higher;
+    return base;
+  }
+  __device__ void store(uint16_t* out, float value_scale) {
+    const float inverse = total == 0.0f ? 0.0f : value_scale / total;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum[k] = total == 0.0f ? 0.0f : sum[k] * inverse;
+    store_row4(out, sum);
+  }
+};
+
+// Every `stride`-th of the parts from `first` on, in the order of their keys, eight in flight.
+template <int D>
+__device__ __forceinline__ Joined join_parts(const float* sums, const float2* stats, int64_t at, int64_t step, int first,
+                                             int stride, int parts, int d) {
+  constexpr int kBatch = 8;
+  Joined row = {-__builtin_huge_valf(), 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+  for (int s = first; s < parts; s += kBatch * stride) {
+    float2 stat[kBatch];
+    floatx4 w[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      if (s + b >= parts) break;
-      const float weight = exp2_fast(stat[b].x - base);
-      total += weight * stat[b].y;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = fmaf(weight, w[b][k], v[k]);
+      const int64_t from = at + min(s + b * stride, parts - 1) * step;
+      stat[b] = stats[from];
+      w[b] = *reinterpret_cast<const floatx4*>(sums + from * D + d);
     }
-    highest = higher;
-  }
-  const float inverse = total == 0.0f ? 0.0f : value_scale / total;
+    float higher = row.highest;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) v[k] = total == 0.0f ? 0.0f : v[k] * inverse;
-  store_row4(out + d, v);
+    for (int b = 0; b < kBatch; ++b) higher = s + b * stride < parts ? fmaxf(higher, stat[b].x) : higher;
+    const float base = row.raise(higher);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (s + b * stride < parts) row.add(stat[b].x, stat[b].y, w[b], base);
+  }
+  return row;
 }
 
-// Workgroups 0 .. tiles * kv heads * parts: 16 rows of every `tiles`-th tile that is
-// split; those behind them: the tile that a share of single tokens' blocks ends in.
+// Workgroups 0 .. tiles * kv heads * (16-row parts): 16 rows of every `tiles`-th tile
+// that is split.  Those behind them, of single tokens' tiles: `lanes` workgroups a
+// tile, each 16 / lanes of its rows, a row's parts among `lanes` groups of threads
+// (few tiles have many parts: a token's 60000 keys 78 us with one); or (lanes 0) one
+// for each share that ends in a tile.
 template <int D>
-__global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tiles, bool e4m3) {
+__global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tiles, int lanes, bool e4m3) {
+  __shared__ Joined joined[4 * D];
   const int row_parts = a.tile_rows / 16;
-  const int r = static_cast<int>(threadIdx.x) / (D / 4), d = 4 * (static_cast<int>(threadIdx.x) % (D / 4));
+  const int d = 4 * (static_cast<int>(threadIdx.x) % (D / 4)), r = static_cast<int>(threadIdx.x) / (D / 4);
   const int of_tiles = tiles * a.kv_heads * row_parts;
   const bool single = static_cast<int>(blockIdx.x) >= of_tiles;
   const int index = static_cast<int>(blockIdx.x) - (single ? of_tiles : 0);
   const int head = index % a.kv_heads;
   const float value_scale = e4m3 && a.v_scales != nullptr ? a.v_scales[head] : 1.0f;
   auto out_of = [&](const PagedUnit& u, int token, int member) {
-    return a.out + static_cast<int64_t>(u.first_row + token) * a.out_row + (head * a.group + member) * a.out_head;
+    return a.out + static_cast<int64_t>(u.first_row + token) * a.out_row + (head * a.group + member) * a.out_head + d;
   };
   if (single) {
-    // Of the shares that end in a tile, the one that does so first.
-    const int w = index / a.kv_heads;
     PagedShares shares;
     shares.start(a);
-    const int64_t end = static_cast<int64_t>(w + 1) * shares.each;
-    if (end >= shares.total) return;
-    const PagedUnit u = shares.find(a, static_cast<int>(end));
-    if (!u.live || u.from == 0 || u.from > shares.each) return;
-    const int parts = 1 + (u.blocks + shares.each - 1) / shares.each, part = u.part + w;
-    const int member = 16 * (u.tile % a.slices) + r;
-    if (part < 0 || part > a.single_parts - parts || member >= a.group) return;
-    join_row<D>(a.single_sums, a.single_stats, (static_cast<int64_t>(part) * a.kv_heads + head) * 16 + r, a.kv_heads * 16,
-                parts, d, value_scale, out_of(u, u.tile / a.slices, member));
+    PagedUnit u;
+    int first, parts;  // workgroup of the tile's first part
+    if (lanes > 0) {
+      u = shares.find<true>(a, index / a.kv_heads / lanes);
+      if (!u.live) return;
+      first = u.from / shares.each, parts = (u.from + u.blocks - 1) / shares.each - first + 1;
+    } else {
+      // Of the shares that end in a tile, the one that does so first.
+      first = index / a.kv_heads;
+      const int64_t end = static_cast<int64_t>(first + 1) * shares.each;
+      if (end >= shares.total) return;
+      u = shares.find(a, static_cast<int>(end));
+      if (!u.live || u.from == 0 || u.from > shares.each) return;
+      parts = 1 + (u.blocks + shares.each - 1) / shares.each;
+    }
+    const int part = u.part + first, rows = lanes > 0 ? 16 / lanes : 16;
+    if (parts == 1 || part < 0 || part > a.single_parts - parts) return;
+    const int mine = r % rows + (lanes > 0 ? rows * (index / a.kv_heads % lanes) : 0), group = r / rows;
+    const int member = 16 * (u.tile % a.slices) + mine;
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * 16;
+    Joined row = join_parts<D>(a.single_sums, a.single_stats, part * step + head * 16 + mine, step, group, lanes > 0 ? lanes : 1,
+                               parts, d);
+    if (lanes > 1) {
+      joined[threadIdx.x] = row;
+      __syncthreads();
+      if (group > 0) return;
+      for (int g = 1; g < lanes; ++g) {
+        const Joined& other = joined[threadIdx.x + g * rows * (D / 4)];
+        const float base = row.raise(fmaxf(row.highest, other.highest));
+        row.add(other.highest, other.total, other.sum, base);
+      }
+    }
+    if (member < a.group) row.store(out_of(u, u.tile / a.slices, member), value_scale);
     return;
   }
   const int row = 16 * (index / a.kv_heads % row_parts) + r;
@@ -559,8 +598,9 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
     const int m = u.tile * a.tile_rows + row;
     if (m >= u.tokens * a.group) continue;
     const int token = m / a.group;
-    join_row<D>(a.tile_sums, a.tile_stats, (static_cast<int64_t>(u.part) * a.kv_heads + head) * a.tile_rows + row,
-                a.kv_heads * a.tile_rows, u.splits, d, value_scale, out_of(u, token, m - token * a.group));
+    const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile_rows;
+    join_parts<D>(a.tile_sums, a.tile_stats, u.part * step + head * a.tile_rows + row, step, 0, 1, u.splits, d)
+        .store(out_of(u, token, m - token * a.group), value_scale);
   }
 }
 
@@ -580,7 +620,7 @@ constexpr int kTwoGroupRows = 4096;  // packed rows of the longest sequence
 struct PagedPlan {
   bool all_single, split_tiles, split_shares;
   int slices, tile_rows, tile_tokens, share_shift, shares, least, target;
-  int64_t tiles, tile_units, single_parts, tile_parts;
+  int64_t single_tiles, tiles, tile_units, single_parts, tile_parts;
 };
 
 PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int32_t sequences, int32_t max_length) {
@@ -597,7 +637,7 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
   p.tile_tokens = p.all_single ? 1 : static_cast<int>(p.tile_rows / group + 2);
   // Single tokens: blocks of 64 keys; one block a tile where no slot holds more keys
   // than are worth a second launch; larger where all of them could be 2^30 and more.
-  const int64_t single_tiles = (p.all_single ? rows : some) * p.slices;
+  const int64_t single_tiles = p.single_tiles = (p.all_single ? rows : some) * p.slices;
   p.share_shift = 6;
   while (capacity <= kAlone && capacity > 1 << p.share_shift) ++p.share_shift;
   while ((((capacity - 1) >> p.share_shift) + 1) * single_tiles >= int64_t{1} << 30) ++p.share_shift;
@@ -730,11 +770,18 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
     const hipError_t status = hipGetLastError();
     if (status != hipSuccess)
       return set_error(D3_ERR_HIP, "paged_attention launch failed: %s", hipGetErrorString(status));
-    const int few = p.target < 4 ? 1 : p.target / 4;  // (of the tiles, up to p.target are split)
+    const int few = p.target < 8 ? 1 : p.target / 8;  // (of the tiles, up to p.target are split)
     const int tiles = p.split_tiles ? static_cast<int>(p.tiles < few ? p.tiles : few) : 0;
-    const int ends = p.split_shares ? p.shares - 1 : 0;
-    const dim3 grid(static_cast<unsigned>((tiles * (p.tile_rows / 16) + ends) * cache->kv_heads)), block(4 * cache->head_dim);
-    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, as_stream(stream), a, tiles, e4m3); };
+    // Single tokens' tiles: by their number where they are fewer than the shares.
+    int lanes = 0;
+    int64_t singles = p.split_shares ? p.shares - 1 : 0;
+    if (p.split_shares && p.single_tiles <= p.shares) {
+      lanes = 1;
+      while (lanes < 16 && p.single_tiles * lanes * 8 < p.shares) lanes *= 2;  // (a thread's parts in one batch)
+      singles = p.single_tiles * lanes;
+    }
+    const dim3 grid(static_cast<unsigned>((tiles * (p.tile_rows / 16) + singles) * cache->kv_heads)), block(4 * cache->head_dim);
+    auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, as_stream(stream), a, tiles, lanes, e4m3); };
     if (cache->head_dim == 64)
       run(paged_join_kernel<64>);
     else if (cache->head_dim == 128)

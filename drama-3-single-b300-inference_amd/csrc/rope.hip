@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kMaxRowsHere = 8;     // rows of a workgroup
+constexpr int64_t kCachedBytes = int64_t{32} << 20;  // the L2s together
 constexpr int kMaxPairsHere = 512;  // sines and cosines in LDS
 constexpr int kMaxColumns = 1 << 16;  // of a row: unit counts stay below what the division below is exact for
 
@@ -66,7 +67,7 @@ __device__ __forceinline__ void load_values(const void* p, float* v) {
 }
 
 // V values to fp32, bf16 or (kE4m3) codes of x / scale.
-template <int V, typename T, bool kE4m3>
+template <int V, typename T, bool kE4m3, bool kOnce>
 __device__ __forceinline__ void store_values(void* p, const float* v, float scale) {
   if constexpr (kE4m3) {
     uint8_t* at = static_cast<uint8_t*>(p);
@@ -83,7 +84,7 @@ __device__ __forceinline__ void store_values(void* p, const float* v, float scal
         at[i] = static_cast<uint8_t>(__builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamped(v[i], scale), 0.0f, 0, false));
     }
   } else if constexpr (sizeof(T) == 2) {
-    store_bf16<V>(p, v);
+    store_bf16<V, kOnce>(p, v);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) static_cast<float*>(p)[i] = v[i];
@@ -92,7 +93,7 @@ __device__ __forceinline__ void store_values(void* p, const float* v, float scal
 
 // One unit of a head: V pairs turned, or 2 V columns (the last unit perhaps V)
 // that stay.  V columns are one access.
-template <int V, typename T, bool kInterleaved, bool kE4m3>
+template <int V, typename T, bool kInterleaved, bool kE4m3, bool kOnce>
 __device__ __forceinline__ void rope_unit(const RopeArgs& a, const T* in, void* out, int unit, bool turned,
                                           const float2* turn, float scale) {
   constexpr int kOut = kE4m3 ? 1 : static_cast<int>(sizeof(T));
@@ -110,8 +111,8 @@ __device__ __forceinline__ void rope_unit(const RopeArgs& a, const T* in, void* 
       y[ia] = x[ia] * t.x - x[ib] * t.y;
       y[ib] = x[ia] * t.y + x[ib] * t.x;
     }
-    store_values<V, T, kE4m3>(to + first * kOut, y, scale);
-    store_values<V, T, kE4m3>(to + second * kOut, y + V, scale);
+    store_values<V, T, kE4m3, kOnce>(to + first * kOut, y, scale);
+    store_values<V, T, kE4m3, kOnce>(to + second * kOut, y + V, scale);
     return;
   }
   const int first = turned ? 2 * a.half + 2 * V * (unit - a.rotary_units) : 2 * V * unit;
@@ -119,15 +120,15 @@ __device__ __forceinline__ void rope_unit(const RopeArgs& a, const T* in, void* 
   if (first >= a.head_dim) return;
   load_values<V, T>(in + first, x);
   if (both) load_values<V, T>(in + first + V, x + V);
-  store_values<V, T, kE4m3>(to + first * kOut, x, scale);
-  if (both) store_values<V, T, kE4m3>(to + (first + V) * kOut, x + V, scale);
+  store_values<V, T, kE4m3, kOnce>(to + first * kOut, x, scale);
+  if (both) store_values<V, T, kE4m3, kOnce>(to + (first + V) * kOut, x + V, scale);
 }
 
 __device__ __forceinline__ int64_t index_at(const void* p, int is_64, int64_t i) {
   return is_64 ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
 }
 
-template <int V, typename T, bool kInterleaved, bool kE4m3, bool kAppend>
+template <int V, typename T, bool kInterleaved, bool kE4m3, bool kAppend, bool kOnce>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
   __shared__ float2 turn[kMaxPairsHere];
   __shared__ int64_t place[kMaxRowsHere];  // page * page size + token, or -1
@@ -164,7 +165,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
       int head = a.head_units == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), a.head_units_inverse));
       const int unit = i - head * a.head_units;
       if (head < a.q.heads) {
-        rope_unit<V, T, kInterleaved, false>(
+        rope_unit<V, T, kInterleaved, false, kOnce>(
             a, static_cast<const T*>(a.q.in) + row * a.q.in_row + head * a.q.in_head,
             static_cast<T*>(a.q.out) + row * a.q.out_row + head * a.q.out_head, unit, true, t, 1.0f);
         continue;
@@ -180,7 +181,7 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a) {
         const int64_t to =
             page * (key ? a.k_page : a.v_page) + token * (key ? a.k_token : a.v_token) + head * x.out_head;
         const float* scales = key ? a.k_scales : a.v_scales;
-        rope_unit<V, T, kInterleaved, kE4m3>(
+        rope_unit<V, T, kInterleaved, kE4m3, kOnce>(
             a, static_cast<const T*>(x.in) + row * x.in_row + head * x.in_head,
             static_cast<uint8_t*>(x.out) + to * (kE4m3 ? 1 : static_cast<int>(sizeof(T))), unit, key, t,
             kE4m3 && scales != nullptr ? scales[head] : 1.0f);
@@ -206,10 +207,17 @@ void launch_rope(RopeArgs a, int interleaved, hipStream_t stream) {
   if (all_units > a.head_units) a.head_units = all_units;
   a.head_units_inverse = static_cast<uint32_t>((uint64_t{1} << 32) / a.head_units + 1);
   const int64_t units = static_cast<int64_t>(a.q.heads + a.k.heads + a.v.heads) * a.head_units;
-  // About one sine and cosine a thread, and no more rows a workgroup than leave
-  // every CU four workgroups; a few rows spread their units over more of them.
+  // Rows of a workgroup: about one sine and cosine a thread at most, three units a
+  // thread (rope of 8191 x 40 x 128 31.7 us so, 33.0 with twice the rows; an e4m3
+  // append of 8192 x 48 39.9 and 43.1; 3668 x 20 10.4 with three rows, 11.2 with one),
+  // and no more than leave every CU four workgroups; few rows spread their units.
   int here = a.half ? kRopeThreads / a.half : kMaxRowsHere;
+  const int64_t enough = (3 * kRopeThreads + units / 2) / units;
+  if (here > enough) here = static_cast<int>(enough);
   if (here > a.rows / 1024) here = static_cast<int>(a.rows / 1024);
+  // What the L2s cannot hold until its next reader is stored past them (38.2 -> 33.0 us
+  // for those 8191 rows, 84 MB; smaller results stay).
+  const bool once = v == kWide && sizeof(T) == 2 && a.rows * units * 2 * v * static_cast<int64_t>(sizeof(T)) > kCachedBytes;
   a.rows_here = here < 1 ? 1 : (here > kMaxRowsHere ? kMaxRowsHere : here);
   const int64_t groups = (a.rows + a.rows_here - 1) / a.rows_here;
   int64_t slices = groups >= 512 ? 1 : 512 / groups;
@@ -217,19 +225,23 @@ void launch_rope(RopeArgs a, int interleaved, hipStream_t stream) {
   a.slices = static_cast<int>(slices < most ? slices : most);
   const dim3 grid(static_cast<unsigned>(groups * a.slices)), block(kRopeThreads);
   auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, a); };
-  auto with = [&](auto width) {
+  auto with = [&](auto width, auto past) {
     constexpr int V = decltype(width)::value;
+    constexpr bool kOnce = decltype(past)::value;
     if (interleaved)
-      run(rope_kernel<V, T, true, kE4m3, kAppend>);
+      run(rope_kernel<V, T, true, kE4m3, kAppend, kOnce>);
     else
-      run(rope_kernel<V, T, false, kE4m3, kAppend>);
+      run(rope_kernel<V, T, false, kE4m3, kAppend, kOnce>);
   };
-  if (v == kWide)
-    with(std::integral_constant<int, kWide>{});
-  else if (v == 2)
-    with(std::integral_constant<int, 2>{});
-  else
-    with(std::integral_constant<int, 1>{});
+  if (once) {
+    if constexpr (sizeof(T) == 2) with(std::integral_constant<int, kWide>{}, std::true_type{});
+  } else if (v == kWide) {
+    with(std::integral_constant<int, kWide>{}, std::false_type{});
+  } else if (v == 2) {
+    with(std::integral_constant<int, 2>{}, std::false_type{});
+  } else {
+    with(std::integral_constant<int, 1>{}, std::false_type{});
+  }
 }
 
 int check_rope(const char* name, const d3_rope* rope, int32_t head_dim) {

@@ -28,11 +28,15 @@ __device__ __forceinline__ void load_bf16(const void* p, float* v) {
     v[0] = bf16_to_f32(*static_cast<const uint16_t*>(p));
   }
 }
-template <int N>
+// (kOnce: eight values past the L2s.)
+template <int N, bool kOnce = false>
 __device__ __forceinline__ void store_bf16(void* p, const float* v) {
   if constexpr (N == 8) {
-    *static_cast<RowVector4*>(p) =
-        RowVector4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    const RowVector4 w = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    if constexpr (kOnce)
+      __builtin_nontemporal_store(w, static_cast<RowVector4*>(p));
+    else
+      *static_cast<RowVector4*>(p) = w;
   } else if constexpr (N == 2) {
     *static_cast<RowWord*>(p) = pack_bf16x2(v[0], v[1]);
   } else {

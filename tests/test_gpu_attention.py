@@ -462,6 +462,164 @@ def test_pages_past_32_bit_offsets(device, dtype):
 
 
 # ---------------------------------------------------------------------------
+# Many rows: tiles of two groups of waves, results larger than the L2s
+# ---------------------------------------------------------------------------
+def reference(q, keys, values, table, boundaries, slots, lengths, scale, window=None):
+    """The oracle's ``attention`` in torch float64 on the device, whole sequences at a time
+    (q, keys, values there; table and the rest as in the oracle): (out, bound)."""
+    pages, kv_heads, page_size, dim = keys.shape
+    group = q.shape[1] // kv_heads
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    for first, end, slot, length in zip(boundaries, boundaries[1:], slots, lengths):
+        if first == end:
+            continue
+        at = np.arange(min(int(length), table.shape[1] * page_size))
+        page = table[slot, at // page_size]
+        kept = (page >= 0) & (page < pages)
+        at, page = (torch.from_numpy(x[kept]).to(q.device) for x in (at, page))
+        position = torch.arange(int(length) - int(end - first), int(length), device=q.device)[:, None]
+        hidden = at > position
+        if window:
+            hidden |= at <= position - window
+        none = hidden.all(1)
+        count = len(at)
+        for head in range(q.shape[1]):
+            k, v = (t[page.long(), head // group, at % page_size] for t in (keys, values))
+            mine = q[first:end, head]
+            s = (mine @ k.T * scale).masked_fill(hidden, -torch.inf)
+            low, top = s.masked_fill(hidden, torch.inf).amin(1), s.amax(1)
+            w = torch.exp(s - top.masked_fill(none, 0)[:, None])
+            total = w.sum(1).masked_fill(none, 1)[:, None]
+            # (a value that a row does not attend takes no part, whatever it is)
+            bad = ~torch.isfinite(v)
+            clean = v.masked_fill(bad, 0)
+            o = w @ clean / total
+            if bad.any():
+                for t in bad.any(1).nonzero().squeeze(1).tolist():
+                    o[~hidden[:, t]] += torch.where(bad[t], v[t], 0.0)
+            sizes = (mine.abs() @ k.abs().T).masked_fill(hidden, 0).nan_to_num(0).amax(1) * abs(scale)
+            rel = (dim + 8) * 2 * oa.F32_HALF_STEP * sizes + 4 * oa.F32_HALF_STEP * (top - low) + 2.0 ** -21
+            rel = (rel + (count + 64) * 2 * oa.F32_HALF_STEP + (count // 16 + 8) * 2.0 ** -21).masked_fill(none, 0)[:, None]
+            share = oa.BF16_HALF_STEP / (1 - oa.BF16_HALF_STEP) + 2 * rel * (1 + oa.BF16_HALF_STEP)
+            out[first:end, head] = o.masked_fill(none[:, None], 0)
+            bound[first:end, head] = (w @ clean.abs() / total + o.abs().nan_to_num(0, 0, 0)) * share
+    return out, bound
+
+
+def test_the_device_reference_is_the_oracle(device):
+    rng = np.random.default_rng(20)
+    new, lengths = [20, 1, 0, 9], [60, 33, 5, 4]
+    table, slots, pages = tables_for(rng, lengths, 8)
+    table[slots[0], 2] = -1
+    _, keys, values = cache_of(rng, device, pages, 8, 2, 64, table)
+    boundaries = np.concatenate([[0], np.cumsum(new)])
+    q = randn(rng, boundaries[-1], 4, 64)
+    values[table[slots[0], 6], 1, 5, 7] = np.inf
+    want, bound, _ = oa.attention(f64(q), keys, values, table, boundaries, slots, lengths, 0.2, 25)
+    got, sizes = reference(q.double().to(device), *(torch.from_numpy(t).to(device) for t in (keys, values)), table, boundaries,
+                           slots, lengths, 0.2, 25)
+    within(got, want, 1e-12 * (1 + np.abs(np.nan_to_num(want, posinf=0))))
+    fine = np.isfinite(want)
+    assert np.allclose(f64(sizes)[fine], bound[fine], rtol=0.01)
+
+
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+@pytest.mark.parametrize("new, lengths, window, page_size", [
+    ([2100], [2400], None, 16), ([2049, 1, 33, 1, 0, 7], [2049, 900, 40, 3, 5, 700], None, 64),
+    ([2300, 1], [2500, 600], 300, 1), ([2150], [2150], 64, 128)])
+def test_many_rows(device, new, lengths, window, page_size, dtype):
+    from drama3_amd.attention import paged_attention
+
+    rng = np.random.default_rng(sum(new) + page_size)
+    table, slots, pages = tables_for(rng, lengths, page_size)
+    table[slots[0], len(table[0]) // 3] = -1
+    cache, keys, values = cache_of(rng, device, pages, page_size, 8, 128, table, dtype)
+    boundaries = np.concatenate([[0], np.cumsum(new)])
+    q = randn(rng, boundaries[-1] + 3, 32, 128)
+    out = paged_attention(q.to(device), cache, layout_of(device, boundaries, slots, max(new)),
+                          torch.tensor(lengths, device=device), window=window)
+    want, bound = reference(q.double().to(device), *(torch.from_numpy(t).to(device) for t in (keys, values)), table, boundaries,
+                            slots, lengths, 128 ** -0.5, window)
+    want, bound = f64(want), f64(bound)
+    within(out, want, bound + oa.BF16_HALF_STEP * (np.abs(want) + bound))
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("rows, heads, kv_heads, dim, window", [
+    (2100, 32, 8, 128, None), (600, 4, 2, 128, 150), (700, 4, 2, 64, None), (300, 8, 8, 64, 100), (300, 4, 2, 256, None)])
+def test_many_rows_do_not_feel_newer_values(device, rows, heads, kv_heads, dim, window, bad):
+    """An infinity or a NaN among the values: in a block that some rows of a tile attend,
+    others in part and others not at all, each row as if it were alone."""
+    from drama3_amd.attention import paged_attention
+
+    rng = np.random.default_rng(21 + rows)
+    lengths = [rows + 200]
+    table, slots, pages = tables_for(rng, lengths, 16)
+    cache, keys, values = cache_of(rng, device, pages, 16, kv_heads, dim, table)
+    for position in (rows + 199, rows - 3, rows - 2, rows // 2, 250, 201, 200, 199):
+        page, token, head = table[slots[0], position // 16], position % 16, int(rng.integers(0, kv_heads))
+        column = int(rng.integers(0, dim))
+        cache.values[page, head, token, column] = bad
+        values[page, head, token, column] = bad
+    q = randn(rng, rows, heads, dim)
+    out = paged_attention(q.to(device), cache, layout_of(device, [0, rows], slots, rows), torch.tensor(lengths, device=device),
+                          window=window)
+    want, bound = reference(q.double().to(device), *(torch.from_numpy(t).to(device) for t in (keys, values)), table, [0, rows],
+                            slots, lengths, dim ** -0.5, window)
+    assert (~torch.isfinite(want)).any(2).any(1).sum() > 50 and torch.isfinite(want).any(2).any(1).all()
+    want, bound = f64(want), f64(bound)
+    within(out, want, bound + oa.BF16_HALF_STEP * (np.abs(np.nan_to_num(want, nan=0, posinf=0, neginf=0)) + bound))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rows_past_the_caches(device, interleaved):
+    """Results of more than 32 MB: rope and append, against fp64 on the device."""
+    from drama3_amd.attention import PagedCache, append_paged, apply_rope, prepare_rope, rope_frequencies
+
+    rng = np.random.default_rng(22)
+    rows, heads, kv_heads, dim = 8300, 16, 2, 128
+    qkv = randn(rng, rows, heads + 2 * kv_heads, dim).to(device)
+    positions = torch.from_numpy(rng.permutation(rows)).to(device)
+    rope = prepare_rope(dim, interleaved=interleaved, device=device)
+    angle = positions.double()[:, None] * torch.tensor(rope_frequencies(dim), dtype=torch.float64, device=device)
+    cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+    x = qkv.double()
+    a, b = (x[..., 0::2], x[..., 1::2]) if interleaved else (x[..., :64], x[..., 64:])
+    want = (a * cos - b * sin, a * sin + b * cos)
+    want = torch.stack(want, -1).flatten(-2) if interleaved else torch.cat(want, -1)
+    size = a.abs() + b.abs()
+    size = size.repeat_interleave(2, -1) if interleaved else torch.cat((size, size), -1)
+    err = oa.rope_error(size) + size * 1e-9  # (the angle's own 64 bits at 8300 positions)
+    allowed = err + oa.BF16_HALF_STEP * (want.abs() + err)
+    assert ((apply_rope(qkv, positions, rope).double() - want).abs() <= allowed).all()
+    cache = PagedCache.empty(520, 16, kv_heads, dim, 2, 520, device=device)
+    order = torch.randperm(520, device=device)
+    cache.page_table[1] = order.int()
+    q, k, v = qkv.split((heads, kv_heads, kv_heads), 1)
+    out = append_paged(cache, k, v, positions, torch.ones_like(positions), rope=rope, q=q)
+    assert ((out.double() - want[:, :heads]).abs() <= allowed[:, :heads]).all()
+    at = order[positions // 16], positions % 16
+    assert ((cache.keys[at[0], :, at[1]].double() - want[:, heads:heads + kv_heads]).abs() <= allowed[:, heads:heads + kv_heads]).all()
+    assert torch.equal(cache.values[at[0], :, at[1]], v)
+
+
+@pytest.mark.parametrize("scale, k_sign", [(-0.1, 1.0), (0.0, 1.0), (0.1, -1.0)])
+def test_scales_of_any_sign(device, scale, k_sign):
+    from drama3_amd.attention import PagedCache, paged_attention
+
+    rng = np.random.default_rng(23)
+    new, lengths = [1, 40], [90, 70]
+    table, slots, pages = tables_for(rng, lengths, 16)
+    cache, keys, values = cache_of(rng, device, pages, 16, 2, 64, table, E4M3)
+    cache = PagedCache(cache.keys, cache.values, cache.page_table, cache.k_scale * k_sign, cache.v_scale * -1)
+    q = randn(rng, 41, 4, 64)
+    for hint in (1, 40):
+        out = paged_attention(q.to(device), cache, layout_of(device, [0, 1, 41], slots, hint), torch.tensor(lengths, device=device),
+                              scale=scale)
+        check(out, q, keys * k_sign, -values, table, [0, 1, 41], slots, lengths, scale)
+
+
+# ---------------------------------------------------------------------------
 # Used together
 # ---------------------------------------------------------------------------
 def test_prefill_then_decode_equals_attention_of_the_whole(device):
@@ -664,6 +822,7 @@ def test_call_refusals(device):
             type(layout)(layout.boundaries.long(), layout.sequence_slots, 5), lengths)
     refused(ValueError, "sequence_slots must be", paged_attention, x, cache, layout_of(device, [0, 2, 5], [0], 3), lengths)
     refused(TypeError, "lengths must be", paged_attention, x, cache, layout, lengths.float())
+    refused(ValueError, "finite", paged_attention, x, cache, layout, lengths, scale=float("nan"))
     refused(ValueError, "window", paged_attention, x, cache, layout, lengths, window=0)
     refused(ValueError, "overlap", paged_attention, x, cache, layout, lengths, out=x)
     narrow = PagedCache.empty(4, 16, 2, 32, 3, 5, device=device)
