@@ -55,7 +55,19 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t w) {
   return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) | ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
 }
 
+// What a row's weights are powers of two above need not be its highest score: it is
+// raised where a score is 2^8 times above it, and weights and sums reach 2^8 times
+// more.  (Raised at every new maximum, a prompt of
+// 8192 304 us, a chunk of 4096 over 20480 1478: so 290 and 1440.)
+constexpr float kSlack = 8.0f;
+
 constexpr int tile_keys(int dim) { return dim == 256 ? 32 : 64; }  // of a block
+
+// A score, or minus infinity where the bit of the mask is 0.
+__device__ __forceinline__ float attended_or_nothing(float score, uint32_t mask, int bit) {
+  const uint32_t keep = static_cast<uint32_t>(__builtin_amdgcn_sbfe(static_cast<int>(mask), bit, 1));
+  return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, score) & keep) | (0xff800000u & ~keep));
+}
 
 template <int D, int kGroups>
 struct TileShared {
@@ -204,26 +216,34 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   auto tile_uneven = [&](int key) { return key + kKeys - 1 > tile_low || key <= tile_oldest; };
   auto zero_infinite = [&](int key, uint8_t* v, int* flag) {
     if (!loading) return;
-    bool found = false;
-    auto check = [&](uint8_t* at) {
+    auto pieces_of = [&](auto visit) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if constexpr (kE4m3) {
+          const int r = wave_first + lane_row + i * kKeysALoad;
+          visit(v + value_part<D>(r, 2 * lane_part));
+          visit(v + value_part<D>(r, 2 * lane_part + 1));
+        } else {
+          visit(v + (i * kWaves + wave) * 1024 + 16 * lane);
+        }
+      }
+    };
+    uint16x2 largest = {0, 0};  // (first only whether there is any: 16 windowed prompts 64 us without)
+    pieces_of([&](const uint8_t* at) {
+      const int32x4 w = *reinterpret_cast<const int32x4*>(at);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) largest = __builtin_elementwise_max(largest, __builtin_bit_cast(uint16x2, w[j] & 0x7fff7fff));
+    });
+    if (max(largest.x, largest.y) < 0x7f80) return;
+    pieces_of([&](uint8_t* at) {
       int32x4* place = reinterpret_cast<int32x4*>(at);
       const int32x4 w = *place;
       int32x4 f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = static_cast<int>(finite_of(w[j]));
-      if (f[0] != w[0] || f[1] != w[1] || f[2] != w[2] || f[3] != w[3]) *place = f, found = true;
-    };
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      if constexpr (kE4m3) {
-        const int r = wave_first + lane_row + i * kKeysALoad;
-        check(v + value_part<D>(r, 2 * lane_part));
-        check(v + value_part<D>(r, 2 * lane_part + 1));
-      } else {
-        check(v + (i * kWaves + wave) * 1024 + 16 * lane);
-      }
-    }
-    if (found) *flag = key;
+      if (f[0] != w[0] || f[1] != w[1] || f[2] != w[2] || f[3] != w[3]) *place = f;
+    });
+    *flag = key;
   };
   auto add_infinite = [&](int key) {
     const int page = page_of(key, entry_of(key));
@@ -401,7 +421,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
         for (int h = 0; h < kHalves; ++h)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            s[h][i] = ((h ? mask_hi : mask_lo) >> (8 * (i >> 2) + (i & 3)) & 1u) != 0 ? s[h][i] : -__builtin_huge_valf();
+            s[h][i] = attended_or_nothing(s[h][i], h ? mask_hi : mask_lo, 8 * (i >> 2) + (i & 3));
       }
       float most = s[0][0];
 #pragma unroll
@@ -409,7 +429,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[h][i]);
       most = max_across_32(most) * scale.size;
-      if (__any(most > top)) {
+      if (__any(most > top + kSlack)) {
         const float higher = fmaxf(top, most);
         const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
         top = higher;
