@@ -60,7 +60,9 @@ struct PagedArgs {
   // tokens' tiles (16 rows) and of the others (tile_rows).
   float *single_sums, *tile_sums;
   float2 *single_stats, *tile_stats;
-  int single_parts, tile_parts;  // how many there are: boundaries that are not ascending must not lead past them
+  // A workgroup's share has two of the former at most: of the tile it begins within
+  // (2 * workgroup), of the one it ends within (2 * workgroup + 1).
+  int tile_parts;  // how many there are: boundaries that are not ascending must not lead past them
 };
 
 // Where a workgroup's work lies.
@@ -172,7 +174,7 @@ struct PagedShares {
     each = max(a.least, static_cast<int>((static_cast<uint32_t>(total) + a.shares - 1) / static_cast<uint32_t>(a.shares)));
   }
   // The tile that holds block `at` < total, of those from the walk's place on; u.from
-  // is the block's place in it, u.blocks what it has from there, u.part its number.
+  // is the block's place in it, u.blocks what it has from there.
   // kTiles: the tile with number `at`; u.from is its first block.
   template <bool kTiles = false>
   __device__ PagedUnit find(const PagedArgs& a, int at) {
@@ -186,14 +188,15 @@ struct PagedShares {
         const int first = __builtin_amdgcn_readlane(to, lane) - blocks * tiles;
         if constexpr (kTiles) {
           u.tile = at - (__builtin_amdgcn_readlane(tiles_to, lane) - tiles);
-          u.from = first + u.tile * blocks, u.blocks = blocks, u.part = at;
+          u.from = first + u.tile * blocks, u.blocks = blocks;
+          u.live = static_cast<uint32_t>(u.tile) < static_cast<uint32_t>(tiles);
           return u;
         }
         const uint32_t rest = static_cast<uint32_t>(at - first);
         u.tile = static_cast<int>(rest / static_cast<uint32_t>(blocks));
         u.from = static_cast<int>(rest) - u.tile * blocks;
         u.blocks = blocks - u.from;
-        u.part = __builtin_amdgcn_readlane(tiles_to, lane) - tiles + u.tile;
+        u.live = static_cast<uint32_t>(u.tile) < static_cast<uint32_t>(tiles);  // (sums of boundaries that do not ascend may wrap)
         return u;
       }
       before = last_lane(to), tiles_before = last_lane(tiles_to);
@@ -243,7 +246,8 @@ __device__ __forceinline__ PagedUnit paged_tile_unit(const PagedArgs& a, int at)
       u.tile = of(tiles) - 1 - static_cast<int>(kTiles ? rest : rest / count);
       u.split = kTiles ? 0 : static_cast<int>(rest % count);
       u.part = of(parts_to) - of(parts) + u.tile * u.splits + u.split;
-      u.live = u.splits <= 1 || (u.part >= 0 && u.part <= a.tile_parts - (kTiles ? u.splits : 1));
+      u.live = static_cast<uint32_t>(u.tile) < static_cast<uint32_t>(of(tiles)) &&
+               (u.splits <= 1 || (u.part >= 0 && u.part <= a.tile_parts - (kTiles ? u.splits : 1)));
       return u;
     }
     units_before = last_lane(units_to), parts_before = last_lane(parts_to);

@@ -263,8 +263,7 @@ __device__ __forceinline__ void decode_share(const PagedArgs& a, int workgroup, 
     const bool whole = u.from == 0 && u.blocks <= end - at;
     u.blocks = min(u.blocks, end - at);
     u.splits = whole ? 1 : 2;
-    u.part += workgroup;
-    if (!whole && (u.part < 0 || u.part >= a.single_parts)) return;
+    u.part = 2 * workgroup + (u.from == 0 ? 1 : 0);
     decode_unit<D, kE4m3, kWaves>(a, u, head, shared);
     at += u.blocks;
     if (at >= end) return;

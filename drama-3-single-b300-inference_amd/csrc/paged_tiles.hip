@@ -529,10 +529,11 @@ struct Joined {
   }
 };
 
-// Every `stride`-th of the parts from `first` on, in the order of their keys, eight in flight.
+// Every `stride`-th of the parts from `first` on, in the order of their keys, eight in
+// flight.  Part n is at + n * step, but for the first of all: `lead` behind.
 template <int D>
-__device__ __forceinline__ Joined join_parts(const float* sums, const float2* stats, int64_t at, int64_t step, int first,
-                                             int stride, int parts, int d) {
+__device__ __forceinline__ Joined join_parts(const float* sums, const float2* stats, int64_t at, int64_t step, int64_t lead,
+                                             int first, int stride, int parts, int d) {
   constexpr int kBatch = 8;
   Joined row = {-__builtin_huge_valf(), 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
   for (int s = first; s < parts; s += kBatch * stride) {
@@ -540,7 +541,8 @@ __device__ __forceinline__ Joined join_parts(const float* sums, const float2* st
     floatx4 w[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int64_t from = at + min(s + b * stride, parts - 1) * step;
+      const int n = min(s + b * stride, parts - 1);
+      const int64_t from = at + n * step + (n == 0 ? lead : 0);
       stat[b] = stats[from];
       w[b] = *reinterpret_cast<const floatx4*>(sums + from * D + d);
     }
@@ -591,13 +593,13 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
       if (!u.live || u.from == 0 || u.from > shares.each) return;
       parts = 1 + (u.blocks + shares.each - 1) / shares.each;
     }
-    const int part = u.part + first, rows = lanes > 0 ? 16 / lanes : 16;
-    if (parts == 1 || part < 0 || part > a.single_parts - parts) return;
+    const int rows = lanes > 0 ? 16 / lanes : 16;
+    if (parts == 1 || first < 0 || first > a.shares - parts) return;
     const int mine = r % rows + (lanes > 0 ? rows * (index / a.kv_heads % lanes) : 0), group = r / rows;
     const int member = 16 * (u.tile % a.slices) + mine;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * 16;
-    Joined row = join_parts<D>(a.single_sums, a.single_stats, part * step + head * 16 + mine, step, group, lanes > 0 ? lanes : 1,
-                               parts, d);
+    Joined row = join_parts<D>(a.single_sums, a.single_stats, 2 * first * step + head * 16 + mine, 2 * step, step, group,
+                               lanes > 0 ? lanes : 1, parts, d);
     if (lanes > 1) {
       joined[threadIdx.x] = row;
       __syncthreads();
@@ -619,7 +621,7 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
     if (m >= u.tokens * a.group) continue;
     const int token = m / a.group;
     const int64_t step = static_cast<int64_t>(a.kv_heads) * a.tile_rows;
-    join_parts<D>(a.tile_sums, a.tile_stats, u.part * step + head * a.tile_rows + row, step, 0, 1, u.splits, d)
+    join_parts<D>(a.tile_sums, a.tile_stats, u.part * step + head * a.tile_rows + row, step, 0, 0, 1, u.splits, d)
         .store(out_of(u, token, m - token * a.group), value_scale);
   }
 }
@@ -668,7 +670,7 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
   const int64_t useful = (single_tiles * blocks + p.least - 1) / p.least;
   p.shares = sequences == 0 ? 0 : static_cast<int>(useful < resident ? useful : (resident > 0 ? resident : 1));
   p.split_shares = p.shares > 1 && blocks > 1;
-  p.single_parts = p.split_shares ? p.shares + single_tiles : 0;
+  p.single_parts = p.split_shares ? 2 * static_cast<int64_t>(p.shares) : 0;
   // Tiles of more rows.
   p.target = (two_groups ? 1 : 2) * kCus / c->kv_heads;
   if (p.target < 1) p.target = 1;
@@ -776,7 +778,7 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   a.share_shift = p.share_shift, a.shares = p.shares, a.least = p.least;
   a.target = p.target, a.splitting = p.split_tiles;
   a.tile_units = static_cast<int>(p.tile_units);
-  a.single_parts = static_cast<int>(p.single_parts), a.tile_parts = static_cast<int>(p.tile_parts);
+  a.tile_parts = static_cast<int>(p.tile_parts);
   const int64_t single_rows = p.single_parts * 16 * cache->kv_heads;
   a.single_sums = static_cast<float*>(workspace);
   a.tile_sums = a.single_sums + single_rows * cache->head_dim;

@@ -126,7 +126,7 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     target = max(1, (1 if tile_rows == 256 else 2) * CUS // kv_heads)
     tiles_most = 0 if all_single else rows * group // tile_rows + some
     split_tiles = not all_single and -(-capacity // BLOCK) > LEAST_SPLIT
-    bounds = {"shares": shares, "single_parts": shares + single_tiles if shares > 1 and most_blocks > 1 else 0,
+    bounds = {"shares": shares, "single_parts": 2 * shares if shares > 1 and most_blocks > 1 else 0,
               "tile_units": tiles_most + (target if split_tiles else 0), "tile_parts": 2 * target if split_tiles else 0,
               "split_tiles": min(tiles_most, target) if split_tiles else 0}
     sequences, work, total = [], np.float32(0), 0
@@ -148,7 +148,7 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     even = math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target))
     chunk = max(even, min(max(4 * even, LEAST_SPLIT), 2 * LEAST_SPLIT) if split_tiles else 1 << 30)
     each = max(least, -(-total // max(shares, 1)))
-    units, part, ordinal, at = [], 0, 0, 0
+    units, part, at = [], 0, 0
     for i, (tokens, length, single, tiles, blocks) in enumerate(sequences):
         for tile in range(tiles):
             if single:
@@ -173,11 +173,10 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
                 while w * each < at + blocks:
                     low, high = max(w * each, at) - at, min((w + 1) * each, at + blocks) - at
                     whole = high - low == blocks
-                    units.append((i, tile, True, None if whole else w + ordinal,
+                    units.append((i, tile, True, None if whole else 2 * w + (low == 0),
                                   keys(aligned + (low << size), aligned + (high << size)), (start, end), packed))
                     w += 1
                 at += blocks
-                ordinal += 1
             else:
                 splits = -(-blocks // chunk)
                 step = -(-(-(-(end - aligned) // BLOCK)) // splits) * BLOCK

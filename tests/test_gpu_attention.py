@@ -391,6 +391,68 @@ def test_large_scores(device):
         check(out, q, keys, values, table, boundaries, slots, lengths, 1.0)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("step", [0.5, 7.0, 7.9, 8.1, 40.0, -7.9])
+def test_scores_that_climb_block_by_block(device, dim, step):
+    """Scores `step` powers of two higher every 32 keys, up and down in turns of five, with
+    values of up to 2^90: under the rise of a row's base, at it and above it."""
+    from drama3_amd.attention import paged_attention
+
+    rng = np.random.default_rng(31)
+    lengths = [700, 333]
+    table, slots, pages = tables_for(rng, lengths, 16)
+    cache, keys, values = cache_of(rng, device, pages, 16, 1, dim, table)
+    for store, mine in ((cache.keys, keys), (cache.values, values)):
+        rows = torch.from_numpy(mine).to(BF16)
+        if mine is values:
+            rows *= 2.0 ** 90
+        else:
+            rows[...] = 0
+            for slot, length in zip(slots, lengths):
+                for t in range(length):
+                    block = t // 32
+                    # (the sum of dim equal products is the score)
+                    rows[table[slot, t // 16], 0, t % 16] = step * (5 - abs(block % 10 - 5)) / dim
+        store.copy_(rows.to(device))
+        mine[...] = f64(rows)
+    for new in ([1, 1], [140, 30]):
+        boundaries = np.concatenate([[0], np.cumsum(new)])
+        q = torch.ones(boundaries[-1], 2, dim, dtype=BF16) * torch.tensor([1.0, 0.5]).to(BF16)[:, None]
+        out = paged_attention(q.to(device), cache, layout_of(device, boundaries, slots, max(new)),
+                              torch.tensor(lengths, device=device), scale=float(np.log(2)))
+        check(out, q, keys, values, table, boundaries, slots, lengths, float(np.log(2)))
+
+
+def test_graphs_replayed_at_once(device):
+    """Two captured calls, each with parts of its own, replayed on two streams at the same time."""
+    from drama3_amd.attention import paged_attention
+
+    rng = np.random.default_rng(32)
+    lengths = [5000, 3000, 64]
+    table, slots, pages = tables_for(rng, lengths, 16)
+    cache, _, _ = cache_of(rng, device, pages, 16, 2, 128, table)
+    told = torch.tensor(lengths, device=device)
+    calls, wants, graphs = [], [], []
+    for new in ([1, 1, 1], [40, 1, 20]):
+        layout = layout_of(device, np.concatenate([[0], np.cumsum(new)]), slots, max(new))
+        q = randn(rng, sum(new), 16, 128).to(device)
+        wants.append(paged_attention(q, cache, layout, told))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged_attention(q, cache, layout, told)
+        calls.append((q, layout, out)), graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for _, _, out in calls:
+            out.zero_()
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for (_, _, out), want in zip(calls, wants))
+
+
 @pytest.mark.parametrize("hint", [0, 1, 2, 100000])
 def test_longest_sequence_only_chooses_the_kernels(device, hint):
     from drama3_amd.attention import paged_attention

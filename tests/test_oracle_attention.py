@@ -124,12 +124,13 @@ def test_cut_covers_every_row_and_key_within_its_bounds(seed):
             mine = [u for u in units if u[:2] == (i, tile)]
             start, end = mine[0][5]
             at = start
-            for u in mine:  # consecutive ranges, cut at whole blocks, consecutive parts
+            for u in mine:  # consecutive ranges, cut at whole blocks, parts where the join looks for them
                 low, high = u[4]
                 if low < high:
                     assert low == at and (low == start or low % oa.BLOCK == 0)
                     at = high
-                assert u[3] is None or u[3] == mine[0][3] + mine.index(u)
+                n = mine.index(u)
+                assert u[3] is None or u[3] == mine[0][3] + (2 * n - (n > 0) if u[2] else n)
             assert at == end and (len(mine) == 1) == (mine[0][3] is None)
             seen += range(mine[0][6][0], mine[0][6][1] + 1)
         assert sorted(seen) == list(range(tokens[i] * group))
