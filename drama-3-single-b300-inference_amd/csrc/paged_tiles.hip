@@ -90,7 +90,9 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   constexpr int kLoads = kParts < kThreads ? 1 : kParts / kThreads;       // a thread
   constexpr int kKeysALoad = kThreads / kRowParts, kWaveRows = kWave / kRowParts;
   constexpr int kSteps = D / 16, kColumns = D / 32;
-  constexpr int kAhead = 8;  // fragments in flight from LDS
+  // Fragments in flight from LDS, in the order written here (4096 rows over 20480 keys:
+  // 1398 us, three 1407; eight 1475, and 1437 where the compiler orders them).
+  constexpr int kAhead = 4;
 
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = lane_id();
@@ -331,7 +333,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
       const uint32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * (2 * D));
       return operand(lo[0], lo[1], hi[0], hi[1]);
     };
-    if constexpr (kGroups == 2) __builtin_amdgcn_s_setprio(1);  // (the wave that multiplies goes first: 1458 -> 1442 us)
+    if constexpr (kGroups == 2) __builtin_amdgcn_s_setprio(1);  // (the wave that multiplies goes first: 1 %)
     bf16x8 w[kAhead];
     if (scores) {
 #pragma unroll
@@ -345,6 +347,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
       for (int n = 0; n < kProducts; ++n) {
         s[n / kSteps] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[n % kAhead], qf[n % kSteps], s[n / kSteps], 0, 0, 0);
         if (n + kAhead < kProducts) w[n % kAhead] = key_fragment(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (weighted) {
@@ -356,6 +359,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
         const int e = n / kColumns, t = n % kColumns;
         o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(w[n % kAhead], p[e], o[t], 0, 0, 0);
         if (n + kAhead < kValueProducts) w[n % kAhead] = value_fragment(n + kAhead);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (tile_uneven(key - kKeys) && shared.infinite[b2] == key - kKeys) add_infinite(key - kKeys);
     }
@@ -633,7 +637,8 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
 //   step, whose tiles take the other place, 37.9 with one, 38.3 with two;
 //   kLeastShare: those 52 tokens 40.2 with two blocks or four, 48 with eight;
 //   kTwoGroupRows: a prompt of 8192 (32768 packed rows) 300 with tiles of two groups, 334
-//   with one; eight of 1000 (4000) 102 and 104; sixteen of 512 (2048) 85 and 80.
+//   with one; eight of 1000 (4000) 102 and 104; sixteen of 512 (2048) 85 and 80 (all
+//   three are faster since, alike).
 constexpr int kCus = 256;
 constexpr int kAlone = 512;          // keys that are not worth a second launch
 constexpr int kLeastShare = 4;       // fewest blocks of a share
