@@ -14,6 +14,9 @@
 // busy: two workgroups a CU of one group of four waves each (128 rows), or one of two
 // groups (256 rows) whose waves share a SIMD and take turns by barriers: while one
 // multiplies (values of the last block, keys of this one), the other computes weights.
+// 4096 rows over 20480 keys of 128 columns 1400 us (1080 TFLOP/s; a product of 8192^3 by
+// the library 1390), a prompt of 8192 282 us; of 64 columns 680 TFLOP/s (half the products
+// a weight), of 256 510 (one wave a SIMD: nothing covers its weights).
 #include "paged_decode.h"
 
 namespace d3 {

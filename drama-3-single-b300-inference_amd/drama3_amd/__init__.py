@@ -8,7 +8,8 @@ native_moe, routed_moe, combine_experts*, add_norm, silu_mul), ``moe_input``
 (DeviceRequests).  The decode step over persistent slots is
 ``pipeline.DecodeStep``, the mixed decode + prefill step ``mixed.MixedStep``
 and one whole MoE layer ``moe_layer.MoELayer``.  ``mxfp4`` holds experts and
-projections in 4 bits, which ``kernels``' MoE operators take as well.  All compute runs in the HIP
+projections in 4 bits, which ``kernels``' MoE operators take as well, ``attention``
+rotary positions, a paged cache and the attention of packed rows over it.  All compute runs in the HIP
 library ``_lib/libdrama3_moe.so``; there is no CPU fallback.
 """
 

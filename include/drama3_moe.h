@@ -1,5 +1,6 @@
 /*
- * drama3_moe.h -- C ABI of the MI355X (gfx950) packed FP8 top-8 MoE step.
+ * drama3_moe.h -- C ABI of the MI355X (gfx950) packed FP8 top-8 MoE step and of
+ * the attention over a paged cache that precedes it in a layer.
  *
  * Every entry point takes raw device pointers, sizes and strides (in
  * elements) and a hipStream_t passed as `void *stream` (NULL = legacy default
