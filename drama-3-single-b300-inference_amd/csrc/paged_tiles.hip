@@ -45,11 +45,17 @@ __device__ __forceinline__ void load_to_lds(const uint8_t* from, const uint8_t* 
       static_cast<int>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)to)));
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from));
 }
-// The same from a wave's address and a lane's offset.
+// The same from a wave's address and a lane's offset.  The address comes out of a lane
+// (v_readlane), and a load may read an SGPR that a vector instruction wrote five wait
+// states later at the earliest, which the compiler does not see to in here: a scalar
+// copy, which waits by itself, is one.
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, uint32_t offset, const uint8_t* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane(
       static_cast<int>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)to)));
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(offset), "s"(from));
+  uint64_t address;
+  asm volatile("s_mov_b32 m0, %1\n\ts_mov_b64 %0, %3\n\tglobal_load_lds_dwordx4 %2, %0"
+               : "=&s"(address)
+               : "s"(at), "v"(offset), "s"(from));
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
