@@ -39,11 +39,12 @@ typedef uint16_t uint16x2 __attribute__((ext_vector_type(2)));
 // 16 bytes a lane from memory to LDS at `to` + 16 * lane (`to` of the wave, the
 // same in every lane).  As an instruction of its own: the compiler would wait for
 // it at the next LDS read of any buffer.  wait_loads() and a barrier come before
-// the first read of what it writes.  (m0 has no other use in the kernel.)
+// the first read of what it writes.  One wait state lies between the write of m0, which
+// has no other use in the kernel, and the load.
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, const uint8_t* to) {
   const uint32_t at = __builtin_amdgcn_readfirstlane(
       static_cast<int>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)to)));
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from));
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from));
 }
 // The same from a wave's address and a lane's offset.  The address comes out of a lane
 // (v_readlane), and a load may read an SGPR that a vector instruction wrote five wait

@@ -12,6 +12,7 @@ import pytest
 
 MAGIC = b"__CLANG_OFFLOAD_BUNDLE__"
 ADDRESS_STATES = 5  # a VALU instruction writes an SGPR, a memory instruction reads it
+M0_STATES = 1       # a scalar instruction writes m0, a load to LDS uses it
 
 
 def device_code(library):
@@ -51,6 +52,8 @@ def missing_waits(lines):
         states, j = 0, i - 1
         while j >= 0 and states < ADDRESS_STATES and code[j][0]:
             before, written = code[j]
+            if before.startswith("s_") and written[:1] == ["m0"] and states < M0_STATES:
+                found.append((code[j], code[i]))
             if before.startswith("v_"):
                 results = written[:2] if "_co_" in before or "div_scale" in before else written[:1]
                 if read & set().union(*map(registers, results)):
@@ -63,14 +66,15 @@ def missing_waits(lines):
 
 
 def test_missing_waits_are_seen():
-    load = "\tglobal_load_lds_dwordx4 v1, s[8:9]  // 000: 1"
+    load = ["\ts_mov_b32 m0, s4", "\tglobal_load_lds_dwordx4 v1, s[8:9]  // 000: 1"]
+    assert missing_waits(load)[1] and missing_waits([load[0], "\ts_nop 0", load[1]]) == (1, [])
     lane = "\tv_readlane_b32 s9, v2, s3"
-    assert missing_waits([lane, "\ts_nop 3", load])[1] and missing_waits([lane, "\ts_nop 4", load]) == (1, [])
-    assert missing_waits(["\tv_cmp_gt_i32 s[8:9], v2, v3", load])[1]
-    assert missing_waits([lane.replace("s9", "s7"), "\ts_mov_b64 s[8:9], s[6:7]", load]) == (1, [])
+    assert missing_waits([lane, "\ts_nop 3", load[1]])[1] and missing_waits([lane, "\ts_nop 4", load[1]]) == (1, [])
+    assert missing_waits(["\tv_cmp_gt_i32 s[8:9], v2, v3", load[1]])[1]
+    assert missing_waits([lane.replace("s9", "s7"), "\ts_mov_b64 s[8:9], s[6:7]", load[1]]) == (1, [])
 
 
-def test_loads_to_lds_wait_for_their_address():
+def test_loads_to_lds_wait_for_their_address_and_place():
     from drama3_amd import _lib
 
     objdump = shutil.which("llvm-objdump", path="/opt/rocm/llvm/bin")
