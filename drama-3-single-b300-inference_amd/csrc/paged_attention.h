@@ -367,6 +367,14 @@ __device__ __forceinline__ bf16x8 load_query(const uint16_t* q, uint32_t sign) {
   return operand(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
 }
 
+// Bases from which on (a step of 1) scores are multiplied and rounded before the base is
+// taken from them.  In one instruction the product is exact and the base, a product like
+// it, was rounded: the highest score's exponent is that rounding, which at bases of 2^32
+// is 2^8.  As products rounded alike, the highest weighs 1 and the others are off by half
+// a step of theirs, as the fp32 scores are themselves.
+constexpr float kCoarse = 8388608.0f;
+__device__ __forceinline__ bool any_coarse(float base) { return __any(fabsf(base) >= kCoarse); }
+
 // 2^x by the hardware's v_exp_f32; -inf gives 0.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -163,11 +163,19 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
         for (int i = 0; i < 4; ++i) o[t][i] *= shrink;
     }
     const float base = top == -__builtin_huge_valf() ? 0.0f : top;
+    float size = scale.size;
+    if (any_coarse(base)) {
+#pragma unroll
+      for (int t = 0; t < kKeyTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[t][i] *= size;
+      size = 1.0f;
+    }
 #pragma unroll
     for (int t = 0; t < kKeyTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[t][i] = exp2_fast(fmaf(s[t][i], scale.size, -base));
+        s[t][i] = exp2_fast(fmaf(s[t][i], size, -base));
         sum += s[t][i];
       }
     uint32_t p[2 * kKeyTiles];

@@ -404,7 +404,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
           load_piece(value_rows, v_lane, shared.values[b1], n - kLoads);
       }
     };
-    auto weigh = [&](auto with_loads, float base) {
+    auto weigh = [&](auto with_loads, float base, float size) {
       constexpr int kEvery = kHalves * 16 / (2 * kLoads);
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
@@ -412,7 +412,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
         for (int i = 0; i < 16; ++i) {
           if constexpr (decltype(with_loads)::value)
             if ((16 * h + i) % kEvery == 0) piece((16 * h + i) / kEvery);
-          s[h][i] = exp2_fast(fmaf(s[h][i], scale.size, -base));
+          s[h][i] = exp2_fast(fmaf(s[h][i], size, -base));
           sum += s[h][i];
         }
 #pragma unroll
@@ -443,7 +443,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[h][i]);
       most = max_across_32(most) * scale.size;
-      if (__any(most > top + kSlack)) {
+      if (__any(most - top > kSlack)) {
         const float higher = fmaxf(top, most);
         const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
         top = higher;
@@ -454,10 +454,18 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
           for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
       }
       const float base = top == -__builtin_huge_valf() ? 0.0f : top;
+      float size = scale.size;
+      if (any_coarse(base)) {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[h][i] *= size;
+        size = 1.0f;
+      }
       if (pieces)
-        weigh(std::true_type{}, base);
+        weigh(std::true_type{}, base, size);
       else
-        weigh(std::false_type{}, base);
+        weigh(std::false_type{}, base, size);
     } else if (pieces) {
 #pragma unroll
       for (int n = 0; n < 2 * kLoads; ++n) piece(n);

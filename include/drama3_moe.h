@@ -943,6 +943,8 @@ int d3_paged_append(const d3_paged_cache *cache, const uint16_t *k, int64_t k_ro
  * fp32 sums, weights rounded to bf16 for the product, one bf16 rounding of out.
  * Sums are divided at the end, and weights in them reach 2^8: values of magnitude
  * 2^96 and more may sum to infinity.
+ * Scores are fp32: finite ones of any magnitude are weighed by their differences, within
+ * what their own rounding leaves of those; past 2^127 (times log2 e) they are infinite.
  * Rows that attend nothing (no token, no slot) are zeros.  Rows of no sequence
  * are zeroed with zero_rest, else left as they were.
  * boundaries int32 [sequences + 1] on the device, ascending, clamped to [0,
