@@ -375,6 +375,12 @@ __device__ __forceinline__ bf16x8 load_query(const uint16_t* q, uint32_t sign) {
 constexpr float kCoarse = 8388608.0f;
 __device__ __forceinline__ bool any_coarse(float base) { return __any(fabsf(base) >= kCoarse); }
 
+// Of a row's scores the highest, scaled; no lower than the lowest number where it attends any key, so
+// that a base of minus infinity says of a row that it attends nothing (zeros), while one whose
+// scores are all minus infinity has weights of 0 / 0 (NaN).
+constexpr float kLowest = -3.402823466e38f;
+__device__ __forceinline__ float lowest_of(bool attends) { return attends ? kLowest : -__builtin_huge_valf(); }
+
 // 2^x by the hardware's v_exp_f32; -inf gives 0.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 

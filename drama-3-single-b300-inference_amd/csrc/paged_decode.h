@@ -151,7 +151,7 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
     for (int t = 0; t < kKeyTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][i]);
-    most = max_across_16(most) * scale.size;
+    most = fmaxf(max_across_16(most) * scale.size, lowest_of(attended != 0));
     if (__any(most > top)) {
       const float higher = fmaxf(top, most);
       const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
@@ -250,9 +250,10 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
       *reinterpret_cast<floatx4*>(a.single_sums + at * D + d) = v;
       if (d == 0) a.single_stats[at] = make_float2(highest, total);
     } else {
-      const float inverse = total == 0.0f ? 0.0f : value_scale / total;
+      const bool nothing = highest == -__builtin_huge_valf();
+      const float inverse = value_scale / total;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = total == 0.0f ? 0.0f : v[k] * inverse;
+      for (int k = 0; k < 4; ++k) v[k] = nothing ? 0.0f : v[k] * inverse;
       store_row4(a.out + row * a.out_row + (q_head0 + c) * a.out_head + d, v);
     }
   }

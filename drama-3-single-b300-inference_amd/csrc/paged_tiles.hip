@@ -422,6 +422,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
       }
     };
     if (scores) {
+      bool attends_any = true;
       // Rows of the wave attend different keys of the block, or none of some: bit c
       // of the lane's mask is key 4 half + c of the block.
       if (wave_uneven(key) || attended != ~uint64_t{0}) {
@@ -429,6 +430,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
         uint64_t mask = attended;
         mask &= newest < 0 ? 0 : ~uint64_t{0} >> (newest < 63 ? 63 - newest : 0);
         mask &= stale <= 0 ? ~uint64_t{0} : (stale < 64 ? ~uint64_t{0} << stale : 0);
+        attends_any = (kKeys == 32 ? mask & 0xffffffffu : mask) != 0;
         mask >>= 4 * half;
         const uint32_t mask_lo = static_cast<uint32_t>(mask), mask_hi = static_cast<uint32_t>(mask >> 32);
 #pragma unroll
@@ -442,7 +444,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
       for (int h = 0; h < kHalves; ++h)
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[h][i]);
-      most = max_across_32(most) * scale.size;
+      most = fmaxf(max_across_32(most) * scale.size, lowest_of(attends_any));
       if (__any(most - top > kSlack)) {
         const float higher = fmaxf(top, most);
         const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
@@ -492,7 +494,8 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
     return;
   }
   const float value_scale = kE4m3 && a.v_scales != nullptr ? a.v_scales[head] : 1.0f;
-  const float inverse = sum == 0.0f ? 0.0f : value_scale / sum;
+  const bool nothing = top == -__builtin_huge_valf();
+  const float inverse = value_scale / sum;
   uint16_t* out = a.out + static_cast<int64_t>(u.first_row + my_token) * a.out_row + my_head * a.out_head;
 #pragma unroll
   for (int t = 0; t < kColumns; ++t)
@@ -500,7 +503,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
     for (int i = 0; i < 4; ++i) {
       floatx4 w;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = sum == 0.0f ? 0.0f : o[t][4 * i + j] * inverse;
+      for (int j = 0; j < 4; ++j) w[j] = nothing ? 0.0f : o[t][4 * i + j] * inverse;
       store_row4(out + 32 * t + 8 * i + 4 * half, w);
     }
 }
@@ -544,9 +547,10 @@ struct Joined {
     return base;
   }
   __device__ void store(uint16_t* out, float value_scale) {
-    const float inverse = total == 0.0f ? 0.0f : value_scale / total;
+    const bool nothing = highest == -__builtin_huge_valf();
+    const float inverse = value_scale / total;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k] = total == 0.0f ? 0.0f : sum[k] * inverse;
+    for (int k = 0; k < 4; ++k) sum[k] = nothing ? 0.0f : sum[k] * inverse;
     store_row4(out, sum);
   }
 };

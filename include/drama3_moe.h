@@ -945,7 +945,8 @@ int d3_paged_append(const d3_paged_cache *cache, const uint16_t *k, int64_t k_ro
  * 2^96 and more may sum to infinity.
  * Scores are fp32: finite ones of any magnitude are weighed by their differences, within
  * what their own rounding leaves of those; past 2^127 (times log2 e) they are infinite.
- * Rows that attend nothing (no token, no slot) are zeros.  Rows of no sequence
+ * Rows that attend nothing (no token, no slot) are zeros; where all scores of a row
+ * are minus infinity, it is NaN.  Rows of no sequence
  * are zeroed with zero_rest, else left as they were.
  * boundaries int32 [sequences + 1] on the device, ascending, clamped to [0,
  * rows]; sequence_slots and lengths int32 or int64 [sequences].  max_length: the

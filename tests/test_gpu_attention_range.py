@@ -70,3 +70,38 @@ def test_high_level_scores_of_many_rows(device):
     count = np.arange(1, rows + 1)[:, None, None]
     want, sizes = np.cumsum(mine, 0) / count, np.cumsum(np.abs(mine), 0) / count
     within(out, want, of_equal_weights(want, sizes, rows, 24576.0 ** 2))
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [None, 30])
+@pytest.mark.parametrize("new, lengths", [([1, 1, 1, 1], [40, 700, 2100, 33]), ([1, 5, 140], [40, 300, 600])])
+def test_scores_of_minus_infinity(device, dim, window, new, lengths):
+    """Keys whose score is minus infinity weigh nothing; a row that attends only such has no softmax: NaN,
+    and not the zeros of a row that attends nothing."""
+    from drama3_amd.attention import paged_attention
+
+    rng = np.random.default_rng(dim + sum(lengths))
+    table, slots, pages = tables_for(rng, lengths, 1)  # (a token a page)
+    cache, keys, values = cache_of(rng, device, pages, 1, 2, dim, table)
+    spoiled = np.zeros(table.shape, dtype=bool)
+    spoiled[slots[0], :40] = True                # the first sequence has nothing else
+    spoiled[slots[1], 10:290] = True
+    spoiled[slots[2], :500] = True
+    table[slots[-1], lengths[-1] - 33:] = -1     # the last one's newest rows: under a window, nothing at all
+    spoiled &= table >= 0
+    for page in table[spoiled]:
+        keys[page, :, :, 7] = -np.inf
+    cache.keys.copy_(torch.from_numpy(keys).to(BF16).to(device))
+    cache.page_table.copy_(torch.from_numpy(table.astype(np.int32)).to(device))
+    boundaries = np.concatenate([[0], np.cumsum(new)])
+    q = randn(rng, boundaries[-1], 4, dim)
+    q[..., 7] = q[..., 7].abs() + 0.5
+    out = paged_attention(q.to(device), cache, layout_of(device, boundaries, slots, max(new)), torch.tensor(lengths, device=device),
+                          window=window)
+    call = lambda t: oa.attention(f64(q), keys, values, t, boundaries, slots, lengths, dim ** -0.5, window)  # noqa: E731
+    with np.errstate(all="ignore"):
+        nothing = np.isnan(call(table)[0])
+    want, bound, _ = call(np.where(spoiled, -1, table))
+    assert nothing[0].all() and not nothing[-1].any()
+    assert window is None or not want[-1].any()
+    within(out, np.where(nothing, np.nan, want), bound + oa.BF16_HALF_STEP * (np.abs(want) + bound))
