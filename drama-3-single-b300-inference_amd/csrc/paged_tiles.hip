@@ -679,9 +679,10 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
   const int64_t some = sequences < rows ? sequences : rows;
   p.all_single = max_length <= 1;
   p.slices = static_cast<int>((group + 15) / 16);
-  // Tiles of two groups where they alone fill the card.
+  // Tiles of two groups where they alone fill the card; a launch holds 2^32 threads, of which
+  // 512 for a sequence's and a kv head's last tile.
   const bool two_groups = c->head_dim == 128 && rows * q_heads >= int64_t{kCus} * 2 * kGroupRows &&
-                          max_length * group >= kTwoGroupRows;
+                          max_length * group >= kTwoGroupRows && some * c->kv_heads <= (int64_t{1} << 22);
   p.tile_rows = two_groups ? 2 * kGroupRows : kGroupRows;
   p.tile_tokens = p.all_single ? 1 : static_cast<int>(p.tile_rows / group + 2);
   // Single tokens: blocks of 64 keys; one block a tile where no slot holds more keys
@@ -715,8 +716,9 @@ int64_t workspace_rows(const PagedPlan& p, const d3_paged_cache* c) {
 }
 
 bool attention_suited(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int32_t sequences) {
+  // (so many heads that 256 threads of a tile and 1024 of a join's sixteen rows stay below 2^32)
   return (c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256) && rows * q_heads <= (int64_t{1} << 23) &&
-         sequences <= 65536;
+         sequences <= 65536 && c->kv_heads <= 65536;
 }
 
 void launch_paged_tiles(const PagedArgs& a, int head_dim, bool e4m3, bool zero_rest, hipStream_t stream) {
@@ -766,8 +768,8 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
                  (lengths_dtype == D3_DTYPE_I32 || lengths_dtype == D3_DTYPE_I64),
              "paged_attention: slots and lengths must be int32 or int64");
   D3_SUPPORTED(attention_suited(cache, rows, q_heads, sequences),
-               "paged_attention: head dim %d (64, 128 or 256), %lld rows of %d heads, %d sequences", cache->head_dim,
-               static_cast<long long>(rows), q_heads, sequences);
+               "paged_attention: head dim %d (64, 128 or 256), %lld rows of %d heads, %d kv heads, %d sequences", cache->head_dim,
+               static_cast<long long>(rows), q_heads, cache->kv_heads, sequences);
   D3_REQUIRE(rows == 0 || (q && out), "paged_attention: null pointer");
   D3_REQUIRE(rows == 0 || sequences == 0 || (boundaries && sequence_slots && lengths), "paged_attention: null pointer");
   if (rows == 0 || (sequences == 0 && !zero_rest)) {

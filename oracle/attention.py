@@ -113,9 +113,10 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     group = q_heads // kv_heads
     all_single = max_length <= 1
     slices, count = -(-group // 16), len(lengths)
-    tile_rows = 256 if dim == 128 and rows * q_heads >= 512 * 128 and max_length * group >= 4096 else 128
-    tile_tokens = 1 if all_single else tile_rows // group + 2
     some = min(count, rows)
+    tile_rows = 256 if (dim == 128 and rows * q_heads >= 512 * 128 and max_length * group >= 4096
+                        and some * kv_heads <= 1 << 22) else 128
+    tile_tokens = 1 if all_single else tile_rows // group + 2
     single_tiles = (rows if all_single else some) * slices
     shift = 6
     while capacity <= ALONE and capacity > 1 << shift:

@@ -177,3 +177,12 @@ def test_workspace_stays_bounded(lib, head_dim, kv_heads, q_heads, max_pages, ro
     for max_length in (0, 1, 7, rows, 1 << 30):
         need = lib.d3_paged_attention_workspace(at(kept), rows, q_heads, sequences, max_length)
         assert 0 <= need <= 160 << 20
+
+
+def test_attention_refuses_more_kv_heads_than_a_launch_holds(lib):
+    """(a join takes 8,192 threads of each kv head at most: 2^29 of 65,536)"""
+    wide = cache(kv_heads=65537, page_size=1, key_page_stride=65537 * 64, key_head_stride=64, value_page_stride=65537 * 64,
+                 value_head_stride=64)
+    with pytest.raises(ValueError, match="65537 kv heads"):
+        attend(wide, rows=1, q_heads=65537, sequences=1)
+    assert lib.d3_paged_attention_workspace(at(wide), 1, 65537, 1, 2) == -1
