@@ -193,6 +193,38 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a1 <= b0 or b1 <= a0
 
 
+def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors share memory: element by element where their strides are alike and each
+    steps over what the smaller ones reach (views of one buffer), else by their spans."""
+    if _apart(a, b):
+        return False
+    size = a.element_size()
+    offset = b.data_ptr() - a.data_ptr()
+    if a.dim() != b.dim() or b.element_size() != size or offset % size:
+        return True
+    dims = []
+    for n, m, s, t in zip(a.shape, b.shape, a.stride(), b.stride()):
+        if n > 1 and m > 1 and s != t:
+            return True
+        if n > 1 or m > 1:
+            dims.append((s if n > 1 else t, n, m))
+    dims.sort(reverse=True)
+    a_reach = b_reach = 1
+    for s, n, m in reversed(dims):
+        if s < max(a_reach, b_reach):
+            return True
+        a_reach, b_reach = a_reach + (n - 1) * s, b_reach + (m - 1) * s
+
+    def met(offset, level):  # differences of the indices from this dimension on that come to the offset
+        if level == len(dims):
+            return offset == 0
+        s, n, m = dims[level]
+        near = offset // s
+        return any(-m < d < n and met(offset - d * s, level + 1) for d in (near, near + 1))
+
+    return met(offset // size, 0)
+
+
 def _check_out(out: torch.Tensor, x: torch.Tensor, name: str, in_place: bool) -> None:
     """``out`` of the rows' type and shape, each element its own, apart from ``x`` (or ``x`` itself)."""
     require_cuda(out)
@@ -244,6 +276,7 @@ class PagedCache:
     at token ``t % page_size``.  Entries outside [0, pages) are unmapped: nothing
     is written there, and nothing attends them.  page_size is a power of two.
 
+    Keys and values share no memory (two parts of one buffer do not).
     e4m3 codes stand for code * scale of their head, ``k_scale`` / ``v_scale``
     f32 [kv_heads] (None: 1).  Two slots may share pages that neither appends to.
 
@@ -258,6 +291,7 @@ class PagedCache:
     _struct: _lib.PagedCacheStruct = field(init=False, repr=False, compare=False)
     _ref: object = field(init=False, repr=False, compare=False)
     _sizes: tuple = field(init=False, repr=False, compare=False)
+    _spans: tuple = field(init=False, repr=False, compare=False)
 
     def __post_init__(self):
         """The kernels take the sizes as given: they have to be the tensors'."""
@@ -286,8 +320,8 @@ class PagedCache:
             ordered = sorted((s, n) for n, s in zip(t.shape[:3], strides) if n > 1)
             if any(big < s * n for (s, n), (big, _) in zip(ordered, ordered[1:])):
                 raise ValueError(f"{name} must not overlap themselves")
-        if not _apart(keys, values) and keys.data_ptr() == values.data_ptr():
-            raise ValueError("keys and values must not be the same memory")
+        if _meet(keys, values):
+            raise ValueError("keys and values must not share the same memory")
         for t, name in ((values, "values"), (table, "page_table"), (self.k_scale, "k_scale"), (self.v_scale, "v_scale")):
             if t is not None:
                 _same_device(keys, t, name)
@@ -307,6 +341,8 @@ class PagedCache:
             ptr(table), table.stride(0) if table.shape[0] > 1 else table.shape[1], table.shape[0], table.shape[1],
             ptr(self.k_scale), ptr(self.v_scale)))
         object.__setattr__(self, "_ref", ctypes.byref(self._struct))
+        (k0, k1), (v0, v1) = _span(keys), _span(values)
+        object.__setattr__(self, "_spans", (min(k0, v0), max(k1, v1), k0, k1, v0, v1))
         object.__setattr__(self, "_sizes", (_CACHE[keys.dtype], kv_heads, head_dim, page_size, table.shape[1]))
 
     @classmethod
@@ -322,6 +358,13 @@ class PagedCache:
         return self.keys.device
 
 
+def _off_the_cache(cache: PagedCache, name: str, at: int, end: int) -> None:
+    """Refuses bytes [at, end) that lie where the keys or the values do."""
+    _, _, k0, k1, v0, v1 = cache._spans
+    if at < k1 and end > k0 or at < v1 and end > v0:
+        raise ValueError(f"{name} must not overlap the cache")
+
+
 def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
                  row_slots: torch.Tensor, rope: Rope | None = None, q: torch.Tensor | None = None,
                  out: torch.Tensor | None = None) -> torch.Tensor | None:
@@ -330,7 +373,7 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions:
     [T] each, as ``packed_row_metadata`` gives them), keys rotated by ``rope`` on
     the way.  With ``q`` bf16 [T, heads, head_dim], returns the rotated queries
     (into ``out``, which may be ``q``).  The three are usually views of one
-    projection's rows.
+    projection's rows; none of them lies in the cache.
 
     Rows of a slot outside [0, slots), of a negative position or one past the
     table, and of an unmapped page write nothing; their queries are rotated.  No
@@ -346,6 +389,13 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions:
         _elsewhere(k, cache.keys, "cache")
     position_code = _indices(positions, "positions", rows, k, index)
     slot_code = _indices(row_slots, "row_slots", rows, k, index)
+    # (what lies behind the cache needs no second look)
+    low, high = cache._spans[:2]
+    k_at, v_at = k.data_ptr(), v.data_ptr()
+    if k_at < high and (end := k_at + 2 * ((rows - 1) * k_row + (kv_heads - 1) * k_head + dim)) > low:
+        _off_the_cache(cache, "k", k_at, end)
+    if v_at < high and (end := v_at + 2 * ((rows - 1) * v_row + (kv_heads - 1) * v_head + dim)) > low:
+        _off_the_cache(cache, "v", v_at, end)
     rope_ref = None
     if rope is not None:
         rope_ref = rope._ref
@@ -360,18 +410,29 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions:
             raise ValueError(f"q must be [{rows}, heads, {head_dim}]")
         if q_index != index:
             _elsewhere(k, q, "q")
+        q_at = q.data_ptr()
+        if q_at < high and (end := q_at + 2 * ((rows - 1) * q_row + (heads - 1) * q_head + dim)) > low:
+            _off_the_cache(cache, "q", q_at, end)
         if out is None:
             out = torch.empty(rows, heads, head_dim, dtype=q.dtype, device=q.device)
             out_row, out_head = heads * head_dim, head_dim
         else:
             _check_out(out, q, "out", True)
-            if out.data_ptr() != q.data_ptr() and not (_apart(out, k) and _apart(out, v)):
-                raise ValueError("out must not overlap k or v")
+            if out.data_ptr() != q_at:
+                if not (_apart(out, k) and _apart(out, v)):
+                    raise ValueError("out must not overlap k or v")
+                _off_the_cache(cache, "out", *_span(out))
+            else:  # (in place: parts of one projection's rows, as a rule)
+                extent, step = 2 * ((heads - 1) * q_head + dim), 2 * q_row
+                for x, at, x_row, x_head in ((k, k_at, k_row, k_head), (v, v_at, v_row, v_head)):
+                    beside = x_row == q_row > 0 and extent <= (at - q_at) % step <= step - 2 * ((kv_heads - 1) * x_head + dim)
+                    if not beside and _meet(out, x):
+                        raise ValueError("out must not overlap k or v")
             out_row, out_head, _ = out.stride()
-        q_args = (q.data_ptr(), q_row, q_head, heads, out.data_ptr(), out_row, out_head)
+        q_args = (q_at, q_row, q_head, heads, out.data_ptr(), out_row, out_head)
     elif out is not None:
         raise ValueError("out goes with q")
-    _launch(index, "d3_paged_append", cache._ref, k.data_ptr(), k_row, k_head, v.data_ptr(), v_row, v_head, rows,
+    _launch(index, "d3_paged_append", cache._ref, k_at, k_row, k_head, v_at, v_row, v_head, rows,
             positions.data_ptr(), position_code, row_slots.data_ptr(), slot_code, rope_ref, *q_args)
     return out
 
@@ -422,6 +483,7 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, layout: PackedLayout, le
         out_row, out_head = heads * dim, dim
     else:
         _check_out(out, q, "out", False)
+        _off_the_cache(cache, "out", *_span(out))
         out_row, out_head, _ = out.stride()
     longest = max(0, min(int(layout.max_length), _MOST))
     size = _workspace_bytes(sizes, rows, heads, count, longest)
