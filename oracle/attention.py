@@ -121,13 +121,17 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     shift = 6
     while capacity <= ALONE and capacity > 1 << shift:
         shift += 1
+    while (((capacity - 1) >> shift) + 1) * single_tiles >= 1 << 30:
+        shift += 1
     most_blocks = ((capacity - 1) >> shift) + 1
     least = LEAST if most_blocks > 1 else 1
-    shares = min(-(-single_tiles * most_blocks // least), max(1, (4 if dim == 64 else 2) * CUS // kv_heads)) if count else 0
+    a_cu = 1 if not all_single else (4 if dim == 64 else 2)
+    shares = min(-(-single_tiles * most_blocks // least), max(1, a_cu * CUS // kv_heads)) if count else 0
     target = max(1, (1 if tile_rows == 256 else 2) * CUS // kv_heads)
-    tiles_most = 0 if all_single else rows * group // tile_rows + some
-    split_tiles = not all_single and -(-capacity // BLOCK) > LEAST_SPLIT
-    bounds = {"shares": shares, "single_parts": 2 * shares if shares > 1 and most_blocks > 1 else 0,
+    tiled = not all_single and count > 0
+    tiles_most = rows * group // tile_rows + some if tiled else 0
+    split_tiles = tiled and -(-capacity // BLOCK) > LEAST_SPLIT
+    bounds = {"shares": shares, "tile_rows": tile_rows, "single_parts": 2 * shares if shares > 1 and most_blocks > 1 else 0,
               "tile_units": tiles_most + (target if split_tiles else 0), "tile_parts": 2 * target if split_tiles else 0,
               "split_tiles": min(tiles_most, target) if split_tiles else 0}
     sequences, work, total = [], np.float32(0), 0

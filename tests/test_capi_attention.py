@@ -186,3 +186,26 @@ def test_attention_refuses_more_kv_heads_than_a_launch_holds(lib):
     with pytest.raises(ValueError, match="65537 kv heads"):
         attend(wide, rows=1, q_heads=65537, sequences=1)
     assert lib.d3_paged_attention_workspace(at(wide), 1, 65537, 1, 2) == -1
+
+
+@pytest.mark.parametrize("seed", range(200))
+def test_the_restated_plan_has_the_librarys_parts(lib, seed):
+    """``oracle.attention.cut`` says how many partial rows a call keeps: the workspace that the library asks for."""
+    import random
+
+    from oracle import attention as oa
+
+    rng = random.Random(seed)
+    spread = lambda low, high: round(low * (high / low) ** rng.random())  # noqa: E731
+    head_dim, kv_heads = rng.choice([64, 128, 256]), rng.choice([1, 2, 3, 8, 16, 96, 700])
+    q_heads = kv_heads * rng.choice([1, 2, 5, 8, 17, 40])
+    rows = min(spread(1, 40000), (1 << 23) // q_heads)
+    sequences = rng.choice([0, 1, spread(1, 200), spread(1, 65536)])
+    max_length = rng.choice([0, 1, 2, rows, spread(1, 100000)])
+    page_size = 1 << rng.randrange(9)
+    max_pages = spread(1, (1 << 30) // page_size)
+    kept = cache(head_dim=head_dim, kv_heads=kv_heads, page_size=page_size, max_pages=max_pages)
+    # (bounds hang on the sizes alone: no sequence has a row here)
+    _, most = oa.cut(rows, q_heads, kv_heads, [0] * (sequences + 1), [0] * sequences, page_size * max_pages, max_length, head_dim)
+    rows_kept = (most["single_parts"] * 16 + most["tile_parts"] * most["tile_rows"]) * kv_heads
+    assert lib.d3_paged_attention_workspace(at(kept), rows, q_heads, sequences, max_length) == rows_kept * (head_dim + 2) * 4
