@@ -54,6 +54,7 @@ struct PagedArgs {
   int share_shift;    // log2 of the keys in a block of single tokens' shares
   int shares, least;  // workgroups a kv head that single tokens' blocks are dealt to, fewest blocks of one
   int target;         // units a kv head that the splits of tiles aim at
+  int work_shift;     // log2 of the blocks in one of their sums, which stay below 2^31
   int splitting;      // whether they may be split
   int tile_units;     // most units of a kv head
   // Partial rows [part][kv head][rows of a tile][D] and their (maximum, sum), of single
@@ -213,19 +214,22 @@ __device__ __forceinline__ PagedUnit paged_tile_unit(const PagedArgs& a, int at)
   PagedWalk walk;
   walk.start(a);
   auto tiles_here = [&] { return walk.mine.single ? 0 : walk.mine.tiles; };
-  // Key blocks of a split: the batch's blocks over the units aimed at.  A little
-  // more than their quotient, so that the units stay within tiles + target
-  // whatever fp32 rounds off.
-  float work = static_cast<float>(tiles_here()) * static_cast<float>(walk.mine.blocks);
+  // Key blocks of a split: the batch's blocks over the units aimed at, so that the units
+  // stay within tiles + target.  In integers: the tiles and their join each find it for
+  // themselves, and have to find the same.
+  auto work_here = [&] {
+    return static_cast<uint32_t>(tiles_here()) * (static_cast<uint32_t>(walk.mine.blocks + (1 << a.work_shift) - 1) >> a.work_shift);
+  };
+  uint32_t work = wave_reduce<SumU32>(work_here());
   if (a.sequences > kWave) {
-    while (walk.next(a)) work += static_cast<float>(tiles_here()) * static_cast<float>(walk.mine.blocks);
+    while (walk.next(a)) work += wave_reduce<SumU32>(work_here());
     walk.start(a);
   }
-  // Fewest blocks worth a split: kLeastSplit where the units are few, up to twice that
-  // where a quarter of them would do.
-  const float even = fminf(ceilf(wave_sum(work) * 1.001f / static_cast<float>(a.target)), 1e9f);
-  const int least = a.splitting ? min(max(static_cast<int>(fminf(4.0f * even, 1e9f)), kLeastSplit), 2 * kLeastSplit) : 1 << 30;
-  const int chunk = max(least, static_cast<int>(even));
+  const uint32_t target = static_cast<uint32_t>(a.target);
+  const int even = static_cast<int>(min((work + target - 1) / target, (1u << 30) >> a.work_shift)) << a.work_shift;
+  // Fewest blocks worth a split: kLeastSplit where the units are few, else twice that.
+  const int least = !a.splitting ? 1 << 30 : (even > 1 ? 2 * kLeastSplit : kLeastSplit);
+  const int chunk = max(least, even);
   int units_before = 0, parts_before = 0;
   PagedUnit u = {};
   do {

@@ -668,7 +668,7 @@ constexpr int kTwoGroupRows = 4096;  // packed rows of the longest sequence
 
 struct PagedPlan {
   bool all_single, split_tiles, split_shares;
-  int slices, tile_rows, tile_tokens, share_shift, shares, least, target;
+  int slices, tile_rows, tile_tokens, share_shift, shares, least, target, work_shift;
   int64_t single_tiles, tiles, tile_units, single_parts, tile_parts;
 };
 
@@ -706,6 +706,8 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
     p.tiles = rows * group / p.tile_rows + some;
     p.split_tiles = (capacity + kKeyBlock - 1) / kKeyBlock > kLeastSplit;
     p.tile_units = p.tiles + (p.split_tiles ? p.target : 0);
+    const int64_t most = (capacity + kKeyBlock - 1) / kKeyBlock;
+    while (p.tiles * (((most - 1) >> p.work_shift) + 1) >= (int64_t{1} << 31) - p.target) ++p.work_shift;
     p.tile_parts = p.split_tiles ? 2 * static_cast<int64_t>(p.target) : 0;
   }
   return p;
@@ -805,7 +807,7 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   a.scale = scale * 1.4426950408889634f;
   a.window = static_cast<int>(window < 0 ? 0 : (window < 0x7fffffff ? window : 0x7fffffff));
   a.share_shift = p.share_shift, a.shares = p.shares, a.least = p.least;
-  a.target = p.target, a.splitting = p.split_tiles;
+  a.target = p.target, a.work_shift = p.work_shift, a.splitting = p.split_tiles;
   a.tile_units = static_cast<int>(p.tile_units);
   a.tile_parts = static_cast<int>(p.tile_parts);
   const int64_t single_rows = p.single_parts * 16 * cache->kv_heads;

@@ -134,7 +134,10 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
     bounds = {"shares": shares, "tile_rows": tile_rows, "single_parts": 2 * shares if shares > 1 and most_blocks > 1 else 0,
               "tile_units": tiles_most + (target if split_tiles else 0), "tile_parts": 2 * target if split_tiles else 0,
               "split_tiles": min(tiles_most, target) if split_tiles else 0}
-    sequences, work, total = [], np.float32(0), 0
+    most_tile_blocks, work_shift = -(-capacity // BLOCK), 0
+    while tiles_most * (((most_tile_blocks - 1) >> work_shift) + 1) >= (1 << 31) - target:
+        work_shift += 1
+    sequences, work, total = [], 0, 0
     for i in range(count):
         b0, b1 = (min(max(int(b), 0), rows) for b in boundaries[i:i + 2])
         tokens, length = max(b1 - b0, 0), max(int(lengths[i]), 0)
@@ -149,9 +152,10 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
         if single:
             total += tiles * blocks
         else:
-            work = np.float32(work + np.float32(tiles) * np.float32(blocks))
-    even = math.ceil(np.float32(work * np.float32(1.001)) / np.float32(target))
-    chunk = max(even, min(max(4 * even, LEAST_SPLIT), 2 * LEAST_SPLIT) if split_tiles else 1 << 30)
+            work += tiles * -(-blocks >> work_shift)
+    assert work < 1 << 31
+    even = min(-(-work // target), (1 << 30) >> work_shift) << work_shift
+    chunk = max(even, (2 * LEAST_SPLIT if even > 1 else LEAST_SPLIT) if split_tiles else 1 << 30)
     each = max(least, -(-total // max(shares, 1)))
     units, part, at = [], 0, 0
     for i, (tokens, length, single, tiles, blocks) in enumerate(sequences):

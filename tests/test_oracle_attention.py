@@ -134,3 +134,28 @@ def test_cut_covers_every_row_and_key_within_its_bounds(seed):
             assert at == end and (len(mine) == 1) == (mine[0][3] is None)
             seen += range(mine[0][6][0], mine[0][6][1] + 1)
         assert sorted(seen) == list(range(tokens[i] * group))
+
+
+def test_tiles_are_split_into_as_many_units_as_are_aimed_at():
+    """The blocks of a batch over the units aimed at, in integers: 8 tiles of 1,024 blocks are 512
+    units of 16, not 488 of 17 by a sum that rounds."""
+    units, most = oa.cut(1024, 1, 1, [0, 1024], [65536], 65536, 1024)
+    assert len(units) == most["tile_units"] - 1 - 8 == 512
+    assert {high - low for _, tile, _, _, (low, high), _, _ in units if tile == 7} == {1024}
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_cut_of_the_largest_tables_stays_within_its_bounds(seed):
+    """Sums of blocks past 32 bits: tables of 2^30 tokens."""
+    rng = np.random.default_rng(seed)
+    count = 3000
+    tokens = rng.integers(0, 4, count)
+    boundaries = np.concatenate([[0], tokens.cumsum()])
+    lengths = (1 << 30) - rng.integers(0, 1 << 28, count)
+    group = 40
+    units, most = oa.cut(int(boundaries[-1]), group, 1, boundaries, lengths, 1 << 30, 4, 128)
+    tiles = [u for u in units if not u[2]]
+    assert len(tiles) <= most["tile_units"]
+    parts = [u[3] for u in tiles if u[3] is not None]
+    assert len(set(parts)) == len(parts) and max(parts, default=-1) < most["tile_parts"]
+    assert len({u[:2] for u in tiles if u[3] is not None}) <= most["split_tiles"]
