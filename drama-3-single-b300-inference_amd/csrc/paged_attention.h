@@ -25,6 +25,7 @@ namespace d3 {
 constexpr int kKeyBlock = 64;  // keys that tiles are cut at
 constexpr int kLeastSplit = 4;   // fewest key blocks worth a split of a tile
 constexpr int kGroupRows = 128;  // packed rows that four waves of a tile take
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr int kZeroGroups = 64;  // workgroups behind the units' that zero rows of no sequence
 
 struct PagedArgs {

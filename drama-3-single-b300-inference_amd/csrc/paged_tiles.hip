@@ -765,7 +765,7 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   D3_REQUIRE(rows >= 0 && sequences >= 0, "paged_attention: shape");
   D3_REQUIRE(q_heads > 0 && q_heads % cache->kv_heads == 0, "paged_attention: %d query heads, %d kv heads", q_heads,
              cache->kv_heads);
-  D3_REQUIRE(__builtin_isfinite(scale), "paged_attention: scale must be finite");
+  D3_REQUIRE(__builtin_isfinite(scale * kLog2E), "paged_attention: scale times log2(e) must be finite");
   D3_REQUIRE((sequence_slots_dtype == D3_DTYPE_I32 || sequence_slots_dtype == D3_DTYPE_I64) &&
                  (lengths_dtype == D3_DTYPE_I32 || lengths_dtype == D3_DTYPE_I64),
              "paged_attention: slots and lengths must be int32 or int64");
@@ -804,7 +804,7 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   a.sequences = sequences, a.rows = static_cast<int>(rows);
   a.q_heads = q_heads, a.kv_heads = cache->kv_heads, a.group = q_heads / cache->kv_heads;
   a.slices = p.slices, a.all_single = p.all_single, a.tile_rows = p.tile_rows, a.tile_tokens = p.tile_tokens;
-  a.scale = scale * 1.4426950408889634f;
+  a.scale = scale * kLog2E;
   a.window = static_cast<int>(window < 0 ? 0 : (window < 0x7fffffff ? window : 0x7fffffff));
   a.share_shift = p.share_shift, a.shares = p.shares, a.least = p.least;
   a.target = p.target, a.work_shift = p.work_shift, a.splitting = p.split_tiles;

@@ -953,7 +953,7 @@ int d3_paged_append(const d3_paged_cache *cache, const uint16_t *k, int64_t k_ro
  * longest n_i, which only chooses the kernels (any value gives the same rows
  * computed).  out does not overlap q.  workspace: at least
  * d3_paged_attention_workspace bytes, 16-byte aligned, this call's alone until
- * it has run.  scale is finite, rows * q_heads <= 2^23, sequences and kv_heads <= 65536.
+ * it has run.  scale * log2(e) is finite, rows * q_heads <= 2^23, sequences and kv_heads <= 65536.
  */
 int d3_paged_attention(const d3_paged_cache *cache, const uint16_t *q, int64_t q_row_stride,
                        int64_t q_head_stride, int64_t rows, int32_t q_heads,

@@ -209,3 +209,10 @@ def test_the_restated_plan_has_the_librarys_parts(lib, seed):
     _, most = oa.cut(rows, q_heads, kv_heads, [0] * (sequences + 1), [0] * sequences, page_size * max_pages, max_length, head_dim)
     rows_kept = (most["single_parts"] * 16 + most["tile_parts"] * most["tile_rows"]) * kv_heads
     assert lib.d3_paged_attention_workspace(at(kept), rows, q_heads, sequences, max_length) == rows_kept * (head_dim + 2) * 4
+
+
+def test_attention_refuses_a_scale_that_powers_of_two_do_not_hold(lib):
+    """(scores are taken times log2 e: 3e38 of it is infinite)"""
+    for scale in (3e38, -3e38):
+        with pytest.raises(ValueError, match="finite"):
+            attend(cache(), scale=scale)
