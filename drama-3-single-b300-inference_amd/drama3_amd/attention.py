@@ -4,15 +4,24 @@ tokens over the cached ones, single ones and chunks alike.
 
 What precedes the MoE step in the reference's attention layers
 (``src/drama3/model.py:55-141``: rotary positions, paged decode over 16-token
-pages, packed prefill), over the same packed rows, persistent slots and int64
-positions that ``packed_prefill.packed_row_metadata`` and
-``runtime_state.DeviceRequests.load`` give.  The reference calls libraries here:
-the semantics are this module's own.
+pages, packed prefill), over the same packed rows and persistent slots.  The
+reference calls libraries here: the semantics are this module's own.
 
 A step of one layer, eager or captured::
 
     q = append_paged(cache, k, v, positions, row_slots, rope=rope, q=q)
     out = paged_attention(q, cache, layout, lengths)
+
+``positions`` are tokens of a slot, what it holds already counted:
+``runtime_state.DeviceRequests.load`` gives a single token's.
+``packed_prefill.packed_row_metadata`` counts every sequence's rows from 0, which
+is a whole prompt's, and gives rows behind the last boundary to the last sequence.
+Chunks on top of cached tokens, and batches with such rows, take from it::
+
+    packed_row_metadata(layout.boundaries, layout.sequence_slots, capacity, positions, row_slots)
+    new = layout.boundaries.diff()
+    positions[:rows] += torch.repeat_interleave(lengths - new, new, output_size=rows)
+    row_slots[rows:] = -1
 
 ``lengths`` counts a sequence's tokens with the new ones.  Every call allocates
 what it returns and its workspace from torch's allocator on the current stream:
@@ -370,8 +379,8 @@ def append_paged(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, positions:
                  out: torch.Tensor | None = None) -> torch.Tensor | None:
     """Writes ``k`` and ``v`` bf16 [T, kv_heads, head_dim] of new tokens to the
     cache, row r as token ``positions[r]`` of slot ``row_slots[r]`` (int32 or int64
-    [T] each, as ``packed_row_metadata`` gives them), keys rotated by ``rope`` on
-    the way.  With ``q`` bf16 [T, heads, head_dim], returns the rotated queries
+    [T] each; a chunk's positions count what its slot holds already, as above), keys
+    rotated by ``rope`` on the way.  With ``q`` bf16 [T, heads, head_dim], returns the rotated queries
     (into ``out``, which may be ``q``).  The three are usually views of one
     projection's rows; none of them lies in the cache.
 

@@ -858,9 +858,11 @@ int64_t d3_mxfp4_moe_workspace(int64_t rows, int32_t top_k, int32_t num_experts,
 /*
  * Attention over packed rows and a paged cache: what precedes the MoE step in
  * the reference's attention layers (model.py:55-141: rotary positions, paged
- * decode over 16-token pages, packed prefill), over the same packed rows,
- * persistent slots and int64 positions that d3_row_metadata and
- * d3_requests_load give.  Own semantics (parity unpinned: the reference calls
+ * decode over 16-token pages, packed prefill), over the same packed rows and
+ * persistent slots.  Positions are tokens of a slot: d3_requests_load gives a single
+ * token's, d3_row_metadata a whole prompt's (it counts each sequence's rows from 0,
+ * and rows behind the last boundary as the last sequence's: chunks on top of cached
+ * tokens add their number).  Own semantics (parity unpinned: the reference calls
  * libraries here).
  */
 
