@@ -55,6 +55,7 @@ struct PagedArgs {
   int share_shift;    // log2 of the keys in a block of single tokens' shares
   int shares, least;  // workgroups a kv head that single tokens' blocks are dealt to, fewest blocks of one
   int target;         // units a kv head that the splits of tiles aim at
+  uint32_t target_inverse;  // 2^32 / target, rounded up: a high product with it is the quotient or one more
   int work_shift;     // log2 of the blocks in one of their sums, which stay below 2^31
   int splitting;      // whether they may be split
   int tile_units;     // most units of a kv head
@@ -226,8 +227,8 @@ __device__ __forceinline__ PagedUnit paged_tile_unit(const PagedArgs& a, int at)
     while (walk.next(a)) work += wave_reduce<SumU32>(work_here());
     walk.start(a);
   }
-  const uint32_t target = static_cast<uint32_t>(a.target);
-  const int even = static_cast<int>(min((work + target - 1) / target, (1u << 30) >> a.work_shift)) << a.work_shift;
+  const uint32_t rounded_up = __umulhi(work + static_cast<uint32_t>(a.target) - (a.target > 1 ? 1 : 0), a.target_inverse);
+  const int even = static_cast<int>(min(rounded_up, (1u << 30) >> a.work_shift)) << a.work_shift;
   // Fewest blocks worth a split: kLeastSplit where the units are few, else twice that.
   const int least = !a.splitting ? 1 << 30 : (even > 1 ? 2 * kLeastSplit : kLeastSplit);
   const int chunk = max(least, even);
@@ -372,22 +373,20 @@ __device__ __forceinline__ bf16x8 load_query(const uint16_t* q, uint32_t sign) {
   return operand(w[0] ^ sign, w[1] ^ sign, w[2] ^ sign, w[3] ^ sign);
 }
 
-// Bases from which on (a step of 1) scores are multiplied and rounded before the base is
-// taken from them.  In one instruction the product is exact and the base, a product like
-// it, was rounded: the highest score's exponent is that rounding, which at bases of 2^32
-// is 2^8.  As products rounded alike, the highest weighs 1 and the others are off by half
-// a step of theirs, as the fp32 scores are themselves.
-constexpr float kCoarse = 8388608.0f;
-__device__ __forceinline__ bool any_coarse(float base) { return __any(fabsf(base) >= kCoarse); }
-
-// Of a row's scores the highest, scaled; no lower than the lowest number where it attends any key, so
-// that a base of minus infinity says of a row that it attends nothing (zeros), while one whose
-// scores are all minus infinity has weights of 0 / 0 (NaN).
-constexpr float kLowest = -3.402823466e38f;
-__device__ __forceinline__ float lowest_of(bool attends) { return attends ? kLowest : -__builtin_huge_valf(); }
-
 // 2^x by the hardware's v_exp_f32; -inf gives 0.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// A row's weights are 2^(score * size - base), the product exact within one instruction, base
+// the highest score times size, rounded.  The highest score's exponent is that rounding: at
+// bases of 2^32 up to 2^8.  From kCoarse on (a step of 1) scores are therefore multiplied
+// and rounded first, as the base was (and size is 1): the highest weighs 1, the others are
+// off by half a step of theirs, as the fp32 scores are themselves.
+//
+// All that an ordinary block needs is whether its highest score is within the row's limit: NaN,
+// which nothing is within, until the row attends a key; minus infinity where scores are
+// coarse.  A row whose scores are all minus infinity has the lowest number as its base and
+// weights of 0 / 0 (NaN); one that attends nothing keeps its limit (zeros).
+constexpr float kCoarse = 8388608.0f, kLowest = -3.402823466e38f;
 
 // Four consecutive columns of a row, rounded.
 typedef uint32_t RowVector2 __attribute__((ext_vector_type(2), aligned(2)));

@@ -78,7 +78,7 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
   floatx4 o[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  float top = -__builtin_huge_valf(), sum = 0.0f;
+  float base = 0.0f, limit = __builtin_nanf(""), size = scale.size, sum = 0.0f;
 
   // Blocks from the aligned one that holds the first key; wave w takes every fourth.
   const int first = range.low & ~(kKeys - 1);
@@ -151,25 +151,27 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
     for (int t = 0; t < kKeyTiles; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][i]);
-    most = fmaxf(max_across_16(most) * scale.size, lowest_of(attended != 0));
-    if (__any(most > top)) {
-      const float higher = fmaxf(top, most);
-      const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
-      top = higher;
+    most = max_across_16(most) * scale.size;
+    if (__any(!(most <= limit))) {
+      const bool fresh = limit != limit, attends = attended != 0;
+      const bool raise = fresh ? attends : most > base;
+      const float higher = raise ? fmaxf(most, kLowest) : base;
+      const float shrink = raise && !fresh ? exp2_fast(base - higher) : 1.0f;
+      base = higher;
       sum *= shrink;
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[t][i] *= shrink;
-    }
-    const float base = top == -__builtin_huge_valf() ? 0.0f : top;
-    float size = scale.size;
-    if (any_coarse(base)) {
+      const bool coarse = __any(fabsf(base) >= kCoarse);
+      if (!fresh || attends) limit = coarse ? -__builtin_huge_valf() : base;
+      size = coarse ? 1.0f : scale.size;
+      if (coarse) {
 #pragma unroll
-      for (int t = 0; t < kKeyTiles; ++t)
+        for (int t = 0; t < kKeyTiles; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][i] *= size;
-      size = 1.0f;
+          for (int i = 0; i < 4; ++i) s[t][i] *= scale.size;
+      }
     }
 #pragma unroll
     for (int t = 0; t < kKeyTiles; ++t)
@@ -220,7 +222,7 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
   // The waves' rows to LDS (fp32 [column][D], a wave's values' space), then one
   // pass adds them at the weights of their maxima.
   sum = sum_across_16(sum);
-  if (g == 0) shared.stats[wave][column] = make_float2(top, sum);
+  if (g == 0) shared.stats[wave][column] = make_float2(limit != limit ? -__builtin_huge_valf() : base, sum);
   float* sums = reinterpret_cast<float*>(mine);
 #pragma unroll
   for (int t = 0; t < kTiles; ++t)

@@ -130,7 +130,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   const int my_head = head * a.group + my_row - my_token * a.group;
   const int position = before + my_token;
   const int wave_low = before + min(wave_row, last_row) / a.group;
-  const int wave_high = before + min(wave_row + 31, last_row) / a.group;
+  const int wave_high = wave_live ? before + min(wave_row + 31, last_row) / a.group : -1;  // (-1: attends no block)
   const int tile_low = before + tile_row / a.group;
   // Keys up to these are out of the windows of this lane's row, the wave's first and
   // its last, and the tile's last.
@@ -150,7 +150,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   for (int t = 0; t < kColumns; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[t][i] = 0.0f;
-  float top = -__builtin_huge_valf(), sum = 0.0f;
+  float sum = 0.0f;
 
   // The page of a block's key `lane`: the table's entry, loaded a block before it is
   // looked at (a use waits for every load before it); then -1 where nothing is attended.
@@ -170,6 +170,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   // alike).  e4m3 blocks are widened on the way.
   const bool by_page = !kE4m3 && (1 << a.page_shift) >= kWaveRows && max(a.k_token, a.v_token) < 1u << 24;
   const bool loading = kWaveRows * wave < kKeys;
+  const int piecewise = __builtin_amdgcn_readfirstlane(by_page && loading);  // (a scalar register, where a condition is two)
   const int lane_row = lane / kRowParts, lane_part = lane % kRowParts;
   const int wave_first = kWaveRows * wave;  // of the wave's first load
   const uint32_t k_lane = lane_row * a.k_token + key_part<D>(wave_first + lane_row, lane_part) - (wave_first + lane_row) * 2 * D;
@@ -291,7 +292,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   // Blocks of the unit; rows of the wave attend a block, or none does.
   const int key0 = range.low & ~(kKeys - 1);
   const int blocks = range.low < range.high ? (range.high - key0 + kKeys - 1) / kKeys : 0;
-  auto wave_attends = [&](int key) { return wave_live && key <= wave_high && key + kKeys - 1 > oldest_low; };
+  auto wave_attends = [&](int key) { return key <= wave_high && key + kKeys - 1 > oldest_low; };
   auto wave_uneven = [&](int key) { return key + kKeys - 1 > wave_low || key <= oldest_high; };
 
   // Before the first: its keys and values and the second's keys.
@@ -323,6 +324,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   floatx16 s[kHalves];
   bf16x8 p[2 * kHalves];
   int b0 = 0, b1 = 1, b2 = kBuffers - 1;  // buffers of this block, the next and the last
+  float base = 0.0f, limit = __builtin_nanf(""), size = scale.size;
   for (int block = 0;; ++block) {
     const int key = key0 + block * kKeys;
     // Products: scores of this block, then the values of the last at its weights.
@@ -391,7 +393,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
     const uint64_t attended2 = __ballot(page2 >= 0);
     const uint8_t* key_rows = row_of(keys, a.k_page, a.k_token, key + 2 * kKeys, page2);
     const uint8_t* value_rows = row_of(values, a.v_page, a.v_token, key + kKeys, page1);
-    const bool pieces = by_page && loading && attended2 == ~uint64_t{0} && attended1 == ~uint64_t{0};
+    const bool pieces = piecewise && attended2 == ~uint64_t{0} && attended1 == ~uint64_t{0};
     if (!pieces) {
       if (block + 2 < blocks) load_keys(key_rows, shared.keys[after]);
       if (block + 1 < blocks) load_values(value_rows, shared.values[b1]);
@@ -404,15 +406,20 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
           load_piece(value_rows, v_lane, shared.values[b1], n - kLoads);
       }
     };
-    auto weigh = [&](auto with_loads, float base, float size) {
+    auto weigh = [&](auto with_loads) {
       constexpr int kEvery = kHalves * 16 / (2 * kLoads);
+      // (the packing of one copy is not the other's: made for both ahead of the branch, its results
+      // were moved to the products' registers, 3 % of a chunk)
+      if constexpr (decltype(with_loads)::value) {
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) asm volatile("" : "+v"(s[h]));
+      }
 #pragma unroll
       for (int h = 0; h < kHalves; ++h) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           if constexpr (decltype(with_loads)::value)
             if ((16 * h + i) % kEvery == 0) piece((16 * h + i) / kEvery);
-          s[h][i] = exp2_fast(fmaf(s[h][i], size, -base));
           sum += s[h][i];
         }
 #pragma unroll
@@ -422,16 +429,18 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
       }
     };
     if (scores) {
-      bool attends_any = true;
       // Rows of the wave attend different keys of the block, or none of some: bit c
-      // of the lane's mask is key 4 half + c of the block.
-      if (wave_uneven(key) || attended != ~uint64_t{0}) {
+      // of the lane's mask is key c of the block.
+      const bool uneven = wave_uneven(key) || attended != ~uint64_t{0};
+      auto mask_of_row = [&] {
         const int newest = position - key, stale = oldest - key + 1;  // bits above and below them go
-        uint64_t mask = attended;
+        uint64_t mask = kKeys == 32 ? attended & 0xffffffffu : attended;
         mask &= newest < 0 ? 0 : ~uint64_t{0} >> (newest < 63 ? 63 - newest : 0);
         mask &= stale <= 0 ? ~uint64_t{0} : (stale < 64 ? ~uint64_t{0} << stale : 0);
-        attends_any = (kKeys == 32 ? mask & 0xffffffffu : mask) != 0;
-        mask >>= 4 * half;
+        return mask;
+      };
+      if (uneven) {
+        const uint64_t mask = mask_of_row() >> (4 * half);
         const uint32_t mask_lo = static_cast<uint32_t>(mask), mask_hi = static_cast<uint32_t>(mask >> 32);
 #pragma unroll
         for (int h = 0; h < kHalves; ++h)
@@ -444,30 +453,37 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
       for (int h = 0; h < kHalves; ++h)
 #pragma unroll
         for (int i = 0; i < 16; ++i) most = fmaxf(most, s[h][i]);
-      most = fmaxf(max_across_32(most) * scale.size, lowest_of(attends_any));
-      if (__any(most - top > kSlack)) {
-        const float higher = fmaxf(top, most);
-        const float shrink = top == higher ? 1.0f : exp2_fast(top - higher);
-        top = higher;
+      most = max_across_32(most) * scale.size;
+      if (__any(!(most <= limit))) {
+        const bool fresh = limit != limit;
+        const bool attends = !uneven || mask_of_row() != 0;
+        const bool raise = fresh ? attends : most > base;
+        const float higher = raise ? fmaxf(most, kLowest) : base;
+        const float shrink = raise && !fresh ? exp2_fast(base - higher) : 1.0f;
+        base = higher;
         sum *= shrink;
 #pragma unroll
         for (int t = 0; t < kColumns; ++t)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[t][i] *= shrink;
-      }
-      const float base = top == -__builtin_huge_valf() ? 0.0f : top;
-      float size = scale.size;
-      if (any_coarse(base)) {
+        const bool coarse = __any(fabsf(base) >= kCoarse);
+        if (!fresh || attends) limit = coarse ? -__builtin_huge_valf() : base + kSlack;
+        size = coarse ? 1.0f : scale.size;
+        if (coarse) {
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
+          for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[h][i] *= size;
-        size = 1.0f;
+            for (int i = 0; i < 16; ++i) s[h][i] *= scale.size;
+        }
       }
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[h][i] = exp2_fast(fmaf(s[h][i], size, -base));
       if (pieces)
-        weigh(std::true_type{}, base, size);
+        weigh(std::true_type{});
       else
-        weigh(std::false_type{}, base, size);
+        weigh(std::false_type{});
     } else if (pieces) {
 #pragma unroll
       for (int n = 0; n < 2 * kLoads; ++n) piece(n);
@@ -481,6 +497,7 @@ __device__ __forceinline__ void tile_unit(const PagedArgs& a, const PagedUnit& u
   if (kGroups == 2 && !second) lds_barrier();  // (as many as the second group)
 
   sum = sum_across_32(sum);
+  const float top = limit != limit ? -__builtin_huge_valf() : base;  // (of a row that attends nothing)
   if (!wave_live || wave_row + column > last_row) return;
   if (u.splits > 1) {
     const int64_t at = (static_cast<int64_t>(u.part) * a.kv_heads + head) * kTileRows + 32 * wave + column;
@@ -707,7 +724,7 @@ PagedPlan paged_plan(const d3_paged_cache* c, int64_t rows, int32_t q_heads, int
     p.split_tiles = (capacity + kKeyBlock - 1) / kKeyBlock > kLeastSplit;
     p.tile_units = p.tiles + (p.split_tiles ? p.target : 0);
     const int64_t most = (capacity + kKeyBlock - 1) / kKeyBlock;
-    while (p.tiles * (((most - 1) >> p.work_shift) + 1) >= (int64_t{1} << 31) - p.target) ++p.work_shift;
+    while (p.tiles * (((most - 1) >> p.work_shift) + 1) >= (int64_t{1} << 31)) ++p.work_shift;
     p.tile_parts = p.split_tiles ? 2 * static_cast<int64_t>(p.target) : 0;
   }
   return p;
@@ -808,6 +825,7 @@ extern "C" int d3_paged_attention(const d3_paged_cache* cache, const uint16_t* q
   a.window = static_cast<int>(window < 0 ? 0 : (window < 0x7fffffff ? window : 0x7fffffff));
   a.share_shift = p.share_shift, a.shares = p.shares, a.least = p.least;
   a.target = p.target, a.work_shift = p.work_shift, a.splitting = p.split_tiles;
+  a.target_inverse = p.target > 1 ? static_cast<uint32_t>((uint64_t{1} << 32) / p.target + 1) : 0xffffffffu;
   a.tile_units = static_cast<int>(p.tile_units);
   a.tile_parts = static_cast<int>(p.tile_parts);
   const int64_t single_rows = p.single_parts * 16 * cache->kv_heads;

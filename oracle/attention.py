@@ -135,7 +135,7 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
               "tile_units": tiles_most + (target if split_tiles else 0), "tile_parts": 2 * target if split_tiles else 0,
               "split_tiles": min(tiles_most, target) if split_tiles else 0}
     most_tile_blocks, work_shift = -(-capacity // BLOCK), 0
-    while tiles_most * (((most_tile_blocks - 1) >> work_shift) + 1) >= (1 << 31) - target:
+    while tiles_most * (((most_tile_blocks - 1) >> work_shift) + 1) >= 1 << 31:
         work_shift += 1
     sequences, work, total = [], 0, 0
     for i in range(count):
@@ -154,7 +154,10 @@ def cut(rows, q_heads, kv_heads, boundaries, lengths, capacity, max_length, dim=
         else:
             work += tiles * -(-blocks >> work_shift)
     assert work < 1 << 31
-    even = min(-(-work // target), (1 << 30) >> work_shift) << work_shift
+    inverse = min((1 << 32) // target + 1, (1 << 32) - 1)
+    quotient = (work + target - (target > 1)) * inverse >> 32  # rounded up, or one more
+    assert -(-work // target) <= quotient <= -(-work // target) + 1
+    even = min(quotient, (1 << 30) >> work_shift) << work_shift
     chunk = max(even, (2 * LEAST_SPLIT if even > 1 else LEAST_SPLIT) if split_tiles else 1 << 30)
     each = max(least, -(-total // max(shares, 1)))
     units, part, at = [], 0, 0
