@@ -63,15 +63,14 @@ struct PagedArgs {
   // tokens' tiles (16 rows) and of the others (tile_rows).
   float *single_sums, *tile_sums;
   float2 *single_stats, *tile_stats;
-  // A workgroup's share has two of the former at most: of the tile it begins within
-  // (2 * workgroup), of the one it ends within (2 * workgroup + 1).
+  // A workgroup's share has two of the former at most (PagedShares).
   int tile_parts;  // how many there are: boundaries that are not ascending must not lead past them
 };
 
 // Where a workgroup's work lies.
 struct PagedUnit {
   bool live;
-  int sequence, tile, splits;
+  int tile, splits;
   int split;                      // of a tile: which of its splits
   int from, blocks;               // of a single token's tile: blocks [from, from + blocks)
   int part;                       // partial of this unit (of a tile to join: the first)
@@ -146,7 +145,6 @@ struct PagedWalk {
   }
   __device__ void take(int lane, PagedUnit& u) const {
     u.live = true;
-    u.sequence = base + lane;
     u.first_row = __builtin_amdgcn_readlane(mine.first_row, lane);
     u.tokens = __builtin_amdgcn_readlane(mine.tokens, lane);
     u.length = __builtin_amdgcn_readlane(mine.length, lane);
@@ -155,8 +153,10 @@ struct PagedWalk {
 };
 
 // Shares of single tokens' blocks: workgroup w of a kv head takes the blocks [w *
-// each, (w + 1) * each) of all tiles one behind the other.  Part w + t is what
-// workgroup w computes of tile t: no two are the same, a tile's follow one another.
+// each, (w + 1) * each) of all tiles one behind the other.  Part 2 w is what it
+// computes of a tile that the share begins within, 2 w + 1 of one that begins in the share
+// and ends behind it: a tile's first part is 2 w + 1 of its first workgroup, the others
+// follow as 2 (w + 1), 2 (w + 2) ...
 struct PagedShares {
   PagedWalk walk;
   int to, tiles_to;              // inclusive prefix sums over the walk's lanes

@@ -12,8 +12,8 @@
 // take steps of 32 keys in turn, each with its own running softmax and no
 // barrier until the end, where their rows are added in LDS; the next step's
 // keys and values are in flight while one is multiplied.  16 tokens over 32768 e4m3
-// keys 132 us (6.3 TB/s); 52 over 2048 keys of 256 columns 38.8 (33 and the join of the
-// parts); a token's 333 keys 7.8, a chain of dependent loads.
+// keys 134 us (6.2 TB/s); 52 over 2048 keys of 256 columns 39.0 (34 and the join of the
+// parts); a token's 333 keys 8.1: three dependent loads of the plan, then steps of 128 keys in turn.
 #pragma once
 
 #include "paged_attention.h"
@@ -21,7 +21,7 @@
 namespace d3 {
 
 // Keys of a wave's step: what its registers hold twice (rows of 256 columns: half, for two waves a SIMD).
-constexpr int decode_keys(int dim, bool e4m3) { return dim == 256 ? 16 : 32; }
+constexpr int decode_keys(int dim) { return dim == 256 ? 16 : 32; }
 
 // Keys and values are read once: past the caches' use for them (16 x 32768 e4m3 keys
 // 151 us, 171 as ordinary loads).
@@ -38,7 +38,7 @@ struct DecodeShared {
 
 template <int D, bool kE4m3, int kWaves>
 __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit& u, int head, DecodeShared<D, kWaves>& shared) {
-  constexpr int kKeys = decode_keys(D, kE4m3), kKeyTiles = kKeys / 16;
+  constexpr int kKeys = decode_keys(D), kKeyTiles = kKeys / 16;
   constexpr int kBytes = kE4m3 ? 1 : 2;
   constexpr int kRowParts = D * kBytes / 16;              // 16-byte parts of a cached row
   constexpr int kKeyLoads = kKeyTiles * (kRowParts / 4);  // a lane's: key lane % 16 of the tiles, every fourth part
@@ -80,7 +80,7 @@ __device__ __forceinline__ void decode_unit(const PagedArgs& a, const PagedUnit&
   for (int t = 0; t < kTiles; ++t) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   float base = 0.0f, limit = __builtin_nanf(""), size = scale.size, sum = 0.0f;
 
-  // Blocks from the aligned one that holds the first key; wave w takes every fourth.
+  // Steps from the aligned one that holds the first key; wave w takes every kWaves-th.
   const int first = range.low & ~(kKeys - 1);
   // The page of a step's key `lane`: the table's entry, loaded a step before it is
   // looked at (a use waits for every load before it); then -1 where nothing is attended.

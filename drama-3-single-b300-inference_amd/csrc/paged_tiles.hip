@@ -14,9 +14,11 @@
 // busy: two workgroups a CU of one group of four waves each (128 rows), or one of two
 // groups (256 rows) whose waves share a SIMD and take turns by barriers: while one
 // multiplies (values of the last block, keys of this one), the other computes weights.
-// 4096 rows over 20480 keys of 128 columns 1400 us (1080 TFLOP/s; a product of 8192^3 by
-// the library 1390), a prompt of 8192 282 us; of 64 columns 680 TFLOP/s (half the products
-// a weight), of 256 510 (one wave a SIMD: nothing covers its weights).
+// 4096 rows over 20480 keys of 128 columns 1375-1427 us by the card (1070-1110 TFLOP/s; a
+// product of 8192^3 by the library 1390), a prompt of 8192 281 us; 4096 rows over 4096 keys
+// 950 TFLOP/s, from e4m3 890 (a block is widened between its products and the barrier,
+// where the other group waits), of 64 columns 630 (half the products a weight, and nothing of
+// a wave's own beside its weights), of 256 500 (one wave a SIMD).
 #include "paged_decode.h"
 
 namespace d3 {
@@ -673,7 +675,8 @@ __global__ __launch_bounds__(4 * D) void paged_join_kernel(PagedArgs a, int tile
 //   kAlone: a token's 333 keys by one workgroup a kv head 7.8, cut in three and joined 10.4;
 //   workgroups a CU for single tokens: 52 x 2048 keys of 256 columns 39.0 with one, 40.2
 //   with two, 47.5 with three; 16 x 32768 e4m3 keys 193, 140, 141 (four: 155); a mixed
-//   step, whose tiles take the other place, 37.9 with one, 38.3 with two;
+//   step, whose tiles take the other place, 37.9 with one, 38.3 with two (over 2048 keys;
+//   with long contexts one is too few: those 16 with a prompt of 16 rows 164, alone 134);
 //   kLeastShare: those 52 tokens 40.2 with two blocks or four, 48 with eight;
 //   kTwoGroupRows: a prompt of 8192 (32768 packed rows) 300 with tiles of two groups, 334
 //   with one; eight of 1000 (4000) 102 and 104; sixteen of 512 (2048) 85 and 80 (all
