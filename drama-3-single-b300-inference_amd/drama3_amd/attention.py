@@ -94,7 +94,9 @@ def rope_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "non
                   slowest pair turns as under "linear" and the fastest as before;
     ``"bands"``   pairs that turn ``fast`` times and more within the original
                   length stay, those that turn ``slow`` times and less are
-                  interpolated, in between by the share (YaRN, arXiv 2309.00071)."""
+                  interpolated, in between by the share (YaRN, arXiv 2309.00071).
+                  Loaders that ramp over the pair's index instead have other
+                  frequencies in between: ``Rope(turns)`` takes any."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary width {rotary_dim} must be even and positive")
     if scaling not in SCALINGS:
@@ -458,7 +460,9 @@ def paged_attention(q: torch.Tensor, cache: PagedCache, layout: PackedLayout, le
     position ``p = lengths[i] - n_i + j``, attends the mapped tokens up to p, the
     last ``window`` of them where one is given, with weights
     ``softmax(scale * q . k)`` (``scale`` defaults to head_dim ** -0.5); query head h
-    reads kv head ``h // (heads / kv_heads)``.  Rows that attend nothing are zeros.
+    reads kv head ``h // (heads / kv_heads)``.  Rows that attend nothing are zeros; where
+    all scores of a row are minus infinity, it is NaN.  A row's last bits may change with
+    the rest of the batch, which how the call is cut follows.
 
     Rows of no sequence (before the first boundary, from the last on) are zeros, or
     left as they were in a given ``out`` (apart from ``q``).  ``layout.max_length`` is the
