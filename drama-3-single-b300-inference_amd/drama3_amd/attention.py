@@ -16,7 +16,8 @@ A step of one layer, eager or captured::
 ``runtime_state.DeviceRequests.load`` gives a single token's.
 ``packed_prefill.packed_row_metadata`` counts every sequence's rows from 0, which
 is a whole prompt's, and gives rows behind the last boundary to the last sequence.
-Chunks on top of cached tokens, and batches with such rows, take from it::
+Chunks on top of cached tokens, and batches with such rows (boundaries from 0 to
+``rows``), take from it::
 
     packed_row_metadata(layout.boundaries, layout.sequence_slots, capacity, positions, row_slots)
     new = layout.boundaries.diff()
